@@ -315,6 +315,94 @@ int nrs_attention_backward(float *dq, float *dk, float *dv, const float *dout, c
                            int64_t batch, int64_t heads, int64_t seq, int64_t d_head, int64_t ld,
                            float scale, float beta);
 
+/* --------------------------------------------------------- cross attention */
+/* attention_batch (src/cuda/nn/attention.rs:23-32) of a decoder's queries
+ * over an encoder's states, which the reference computes only where both have
+ * one length: no counterpart there. For every item b and query head h:
+ *   out = softmax(scale * q . k^T over the first key_len[b] keys) . v
+ * q [batch*seq_q, ld_q], out [batch*seq_q, ld_out], k and v [batch*seq_k,
+ * ld_kv], head h in columns [h*d_head, (h+1)*d_head) of q and out; query heads
+ * h*g .. h*g + g - 1, g = heads / kv_heads, share key head h. k and v may be
+ * the halves of one projection's rows. One query (a token being decoded) and
+ * one key are ordinary sizes; seq_q or seq_k 0 is allowed.
+ *   key_len (device, int32 [batch], or NULL: all seq_k) is taken as 0 below 0
+ * and as seq_k past it. Keys and values past it are never read. An item
+ * without live keys gets zeros.
+ *   stats ([batch*heads*seq_q*2], NULL when no backward follows) receives per
+ * query row the softmax in base 2 as nrs_attention_forward gives it: the
+ * maximum and the sum (both 0 without live keys).
+ * d_head is 1 to 128; strides are at most 2^20 floats; tensors may be longer
+ * than 4 GiB. nrs_cross_attention_supported says whether a shape is taken;
+ * one that is not is refused with NRS_ERR_ARG. Values of live keys and their
+ * queries must be finite and below 2^127 in magnitude: a row that meets
+ * another gets NaN or infinities, other rows are untouched by it.
+ *   work: NULL, or work_bytes of the caller's device memory (16-byte aligned)
+ * in place of the library's scratch, at least what
+ * nrs_cross_attention_workspace says for the call. A call under stream capture
+ * that needs scratch has to pass it, its own for every graph that may run at
+ * the same time as another.                                                  */
+int nrs_cross_attention_supported(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
+                                  int64_t seq_k, int64_t d_head, int64_t ld_q, int64_t ld_kv,
+                                  int64_t ld_out);
+int nrs_cross_attention_workspace(size_t *bytes, int64_t batch, int64_t heads, int64_t kv_heads,
+                                  int64_t seq_q, int64_t seq_k, int64_t d_head, int backward);
+int nrs_cross_attention_forward(float *out, float *stats, const float *q, const float *k,
+                                const float *v, const int32_t *key_len, int64_t batch,
+                                int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_k,
+                                int64_t d_head, int64_t ld_q, int64_t ld_kv, int64_t ld_out,
+                                float scale, void *work, size_t work_bytes);
+/* Its backward, from the forward's out and stats and the same key_len:
+ *   dq = beta_q * dq + dS . k,  dk = beta_kv * dk + dS^T . q,
+ *   dv = beta_kv * dv + P^T . dout,  dS = P * (dout . v^T - dout . out) * scale
+ * dk and dv add the query heads that share a key head. Their rows past
+ * key_len get a zero gradient: written as zeros with beta_kv 0, left as they
+ * are with 1. beta 0 never reads the old values. dq (strides of q), or dk and
+ * dv together (strides of k), may be NULL: not computed. dout has the strides
+ * of out. No output may overlap another or an input. Sums are taken in an
+ * order that depends on the sizes alone.                                     */
+int nrs_cross_attention_backward(float *dq, float *dk, float *dv, const float *dout,
+                                 const float *out, const float *q, const float *k, const float *v,
+                                 const float *stats, const int32_t *key_len, int64_t batch,
+                                 int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_k,
+                                 int64_t d_head, int64_t ld_q, int64_t ld_kv, int64_t ld_out,
+                                 float scale, float beta_q, float beta_kv, void *work,
+                                 size_t work_bytes);
+
+/* -------------------------------------------------- embedding and dropout */
+/* Token embedding (the reference's src/cuda/nn/embedding layer, with the
+ * scale of the table's rows folded in): out[i] = scale * table[ids[i]], out
+ * [count, dim], table [vocab, dim], ids int32 [count]. An id outside
+ * [0, vocab), -1 for padding say, gives a zero row. count and vocab are below
+ * 2^31 - 1, dim at most 2^20.                                                */
+int nrs_embedding_forward(float *out, const float *table, const int32_t *ids, int64_t count,
+                          int64_t vocab, int64_t dim, float scale);
+/* Its gradient: dtable[t] = beta * dtable[t] + scale * sum of grad[i] over the
+ * positions i with ids[i] = t, for every row of the table (beta 0 writes zeros
+ * into the rows of absent tokens; beta 1 leaves them as they are, unread). Ids
+ * outside the table add nothing. Added by sorted tokens, without atomics: the
+ * same ids give the same order of every sum. work as in
+ * nrs_cross_attention_forward.                                               */
+int nrs_embedding_workspace(size_t *bytes, int64_t count, int64_t vocab, int64_t dim);
+int nrs_embedding_backward(float *dtable, const float *grad, const int32_t *ids, int64_t count,
+                           int64_t vocab, int64_t dim, float scale, float beta, void *work,
+                           size_t work_bytes);
+/* Dropout (the reference's src/cuda/nn/dropout layer) whose mask is never
+ * stored: out = (kept ? x / (1 - p) : 0) (+ residual), rounded after the
+ * quotient and after the sum. Element i is kept when word i % 4 of the
+ * Philox4x32-10 block of counter (i / 4 in its low 64 bits, call + *step in
+ * its high ones) under the key `seed` is at least round(p * 2^32): the mask
+ * depends on i, p, seed and call + *step alone. A program counts `call` up
+ * for every dropout that it applies. step (device, or NULL: 0) is read when
+ * the launch runs: a captured graph's masks change between replays when its
+ * program changes *step. p is in [0, 1]; p = 1 drops everything. A dropped x
+ * may be infinite or NaN. out may be x or residual. residual may be NULL.    */
+int nrs_dropout_forward(float *out, const float *x, const float *residual, int64_t n, float p,
+                        uint64_t seed, uint64_t call, const uint64_t *step);
+/* Its backward with the same p, seed, call and step: gin = (kept ? grad /
+ * (1 - p) : 0) + beta * gin. (The residual's gradient is grad itself.)       */
+int nrs_dropout_backward(float *gin, const float *grad, int64_t n, float p, uint64_t seed,
+                         uint64_t call, const uint64_t *step, float beta);
+
 /* ---------------------------------------------------------------- conv2d */
 /* The five primitive launches of src/cuda/nn/conv.rs:161-236, same index
  * semantics (columns grouped by sample: col = ni*out_h*out_w + p).           */

@@ -20,6 +20,8 @@ EPI_NONE, EPI_BIAS_COL, EPI_BIAS_ROW, EPI_RELU = 0, 1, 2, 4
 _P = ctypes.c_void_p
 _I = ctypes.c_int64
 _F = ctypes.c_float
+_U = ctypes.c_uint64
+_S = ctypes.c_size_t
 
 GEMM_GROUP_MAX = 4
 
@@ -62,6 +64,15 @@ SIGNATURES = {
     "nrs_attention_supported": [_I, _I, _I, _I, _I],
     "nrs_attention_forward": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F],
     "nrs_attention_backward": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _F],
+    "nrs_cross_attention_supported": [_I] * 9,
+    "nrs_cross_attention_workspace": [ctypes.POINTER(_S)] + [_I] * 6 + [ctypes.c_int],
+    "nrs_cross_attention_forward": [_P] * 6 + [_I] * 9 + [_F, _P, _S],
+    "nrs_cross_attention_backward": [_P] * 10 + [_I] * 9 + [_F, _F, _F, _P, _S],
+    "nrs_embedding_forward": [_P, _P, _P, _I, _I, _I, _F],
+    "nrs_embedding_workspace": [ctypes.POINTER(_S), _I, _I, _I],
+    "nrs_embedding_backward": [_P, _P, _P, _I, _I, _I, _F, _F, _P, _S],
+    "nrs_dropout_forward": [_P, _P, _P, _I, _F, _U, _U, _P],
+    "nrs_dropout_backward": [_P, _P, _I, _F, _U, _U, _P, _F],
     "nrs_im2col": [_P, _P] + [_I] * 8,
     "nrs_col2out": [_P, _P, _P, _I, _I, _I, _I],
     "nrs_out2mm": [_P, _P, _I, _I, _I, _I],
@@ -248,6 +259,69 @@ def bmm_backward(layout, dA, dB, G, A, B, batch, m, k, n, beta=0.0):
     [k x n] for NN, B^T with B [n x k] for NT); dA or dB may be None."""
     call("nrs_bmm_backward", layout, _ptr(dA), _ptr(dB), _ptr(G), _ptr(A), _ptr(B),
          batch, m, k, n, beta)
+
+
+def _work(buf):
+    """The (work, work_bytes) arguments of an optional scratch buffer."""
+    if buf is None:
+        return None, 0
+    return _ptr(buf), buf.nbytes
+
+
+def cross_attention_workspace(batch, heads, kv_heads, seq_q, seq_k, d_head, backward=False):
+    """Bytes of scratch that a cross attention call of these sizes needs."""
+    n = ctypes.c_size_t()
+    call("nrs_cross_attention_workspace", ctypes.byref(n), batch, heads, kv_heads, seq_q, seq_k,
+         d_head, int(backward))
+    return n.value
+
+
+def cross_attention_forward(out, stats, q, k, v, key_len, batch, heads, kv_heads, seq_q, seq_k,
+                            d_head, ld_q, ld_kv, ld_out, scale, work=None):
+    """out = softmax(scale * q . k^T) . v of every head over each item's first
+    key_len keys (None: all); stats may be None when no backward follows."""
+    call("nrs_cross_attention_forward", _ptr(out), _ptr(stats), _ptr(q), _ptr(k), _ptr(v),
+         _ptr(key_len), batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv, ld_out, scale,
+         *_work(work))
+
+
+def cross_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, key_len, batch, heads,
+                             kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv, ld_out, scale,
+                             beta_q=0.0, beta_kv=0.0, work=None):
+    """dq, dk and dv (+ beta * old) from the forward's out and stats; dq, or dk
+    and dv, may be None."""
+    call("nrs_cross_attention_backward", _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dout), _ptr(out),
+         _ptr(q), _ptr(k), _ptr(v), _ptr(stats), _ptr(key_len), batch, heads, kv_heads, seq_q,
+         seq_k, d_head, ld_q, ld_kv, ld_out, scale, beta_q, beta_kv, *_work(work))
+
+
+def embedding_forward(out, table, ids, count, vocab, dim, scale=1.0):
+    """out[i] = scale * table[ids[i]] (int32 ids; zeros outside the table)."""
+    call("nrs_embedding_forward", _ptr(out), _ptr(table), _ptr(ids), count, vocab, dim, scale)
+
+
+def embedding_workspace(count, vocab, dim):
+    """Bytes of scratch that embedding_backward needs."""
+    n = ctypes.c_size_t()
+    call("nrs_embedding_workspace", ctypes.byref(n), count, vocab, dim)
+    return n.value
+
+
+def embedding_backward(dtable, grad, ids, count, vocab, dim, scale=1.0, beta=0.0, work=None):
+    """dtable[t] = beta * dtable[t] + scale * sum of grad[i] over ids[i] = t."""
+    call("nrs_embedding_backward", _ptr(dtable), _ptr(grad), _ptr(ids), count, vocab, dim, scale,
+         beta, *_work(work))
+
+
+def dropout_forward(out, x, residual, n, p, seed, number, step=None):
+    """out = x / (1 - p) where kept, else 0 (+ residual unless None); `number`
+    is the call's, step an optional device uint64 added to it."""
+    call("nrs_dropout_forward", _ptr(out), _ptr(x), _ptr(residual), n, p, seed, number, _ptr(step))
+
+
+def dropout_backward(gin, grad, n, p, seed, number, step=None, beta=0.0):
+    """gin = grad / (1 - p) where kept, else 0 (+ beta * gin)."""
+    call("nrs_dropout_backward", _ptr(gin), _ptr(grad), n, p, seed, number, _ptr(step), beta)
 
 
 def sync():

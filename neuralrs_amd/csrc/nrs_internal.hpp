@@ -27,7 +27,8 @@ int set_error(int code, const char* fmt, ...);
 //   3 reduction partials, 4 conv weights packed for LDS staging, 5 the conv
 //   output or its gradient around a fused pooling (not used by the conv
 //   entry points themselves, which the fused ones call), 6 the pooled
-//   gradient masked by a ReLU between conv and pooling.
+//   gradient masked by a ReLU between conv and pooling, 7 the scratch of the
+//   entry points that can also take the caller's (call_scratch).
 // Returns nullptr (and records an error) when the allocation fails.
 float* workspace(size_t bytes, int slot = 0);
 
@@ -36,6 +37,18 @@ float* workspace(size_t bytes, int slot = 0);
 // nullptr before nrs_init has run on the current device.
 constexpr size_t kNoAllocScratchBytes = size_t(14) << 20;
 float* noalloc_scratch();
+
+// The scratch of an entry point that takes an optional `work` buffer: the
+// caller's when given (device memory, 16-byte aligned, at least `need` bytes),
+// else the library's slot 7. A captured call has to bring its own: the
+// library's scratch moves when a later call needs more, which would leave the
+// graph with an address that is no longer allocated. `need` 0 gives a null
+// pointer.
+int call_scratch(float** p, size_t need, void* work, size_t work_bytes, const char* what);
+
+// Refuses a call made while another device than the library's is current: its
+// launches would go there.
+int check_device(const char* what);
 
 // Zero-fills device memory on the library stream with a kernel.
 int zero_fill(void* ptr, size_t bytes);

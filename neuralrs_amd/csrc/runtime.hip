@@ -13,7 +13,7 @@
 namespace nrs {
 namespace {
 
-constexpr int kSlots = 7;
+constexpr int kSlots = 8;
 
 // Scratch of the no-allocation entry points: one per GPU, held until the
 // process ends. In host code `scratch` names a host-side stand-in, so it is
@@ -152,6 +152,36 @@ float* workspace(size_t bytes, int slot) {
     g.ws[slot] = static_cast<float*>(p);
     g.ws_bytes[slot] = want;
     return g.ws[slot];
+}
+
+int call_scratch(float** p, size_t need, void* work, size_t work_bytes, const char* what) {
+    *p = nullptr;
+    NRS_ARG_CHECK(work || work_bytes == 0, "%s: work is null but work_bytes is %zu", what,
+                  work_bytes);
+    if (need == 0) return NRS_OK;
+    if (work) {
+        NRS_ARG_CHECK(((uintptr_t)work & 15) == 0, "%s: work must be 16-byte aligned", what);
+        NRS_ARG_CHECK(work_bytes >= need, "%s: work has %zu bytes, the call needs %zu", what,
+                      work_bytes, need);
+        *p = static_cast<float*>(work);
+        return NRS_OK;
+    }
+    if (g.stream) {
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        NRS_HIP_CHECK(hipStreamIsCapturing(g.stream, &status));
+        NRS_ARG_CHECK(status == hipStreamCaptureStatusNone,
+                      "%s: a captured call needs its own work buffer of %zu bytes", what, need);
+    }
+    *p = workspace(need, 7);
+    return *p ? NRS_OK : NRS_ERR_ALLOC;
+}
+
+int check_device(const char* what) {
+    int current = -1;
+    NRS_HIP_CHECK(hipGetDevice(&current));
+    NRS_ARG_CHECK(current == g.device, "%s: device %d is current, the library uses device %d",
+                  what, current, g.device);
+    return NRS_OK;
 }
 
 int zero_fill(void* ptr, size_t bytes) {

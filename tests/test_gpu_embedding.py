@@ -1,0 +1,144 @@
+"""nrs_embedding_forward / _backward against the definition in 64 bits.
+
+The forward rounds one product: exact against an f32 product. The gradient of
+a token that n positions hold is a sum of n floats in some fixed order, times
+the scale, plus beta times the old value: off by at most (n + 2) half steps
+(2^-24) of the sum of magnitudes, and one of the old value's product."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def make_ids(rng, count, vocab, how):
+    if how == "uniform":
+        return rng.integers(0, vocab, count).astype(np.int32)
+    if how == "one":
+        return np.full(count, vocab - 1, np.int32)
+    if how == "outside":  # every id beyond the table, at either side
+        return rng.choice([-1, vocab, -2 ** 31, 2 ** 31 - 1, -vocab], count).astype(np.int32)
+    # word frequencies fall off as one over their rank, with padding
+    rank = np.minimum((np.exp(rng.random(count) * np.log(vocab + 1.0)) - 1).astype(np.int64), vocab - 1)
+    ids = rng.permutation(vocab)[rank].astype(np.int32)
+    ids[rng.random(count) < 0.1] = -1
+    return ids
+
+
+def reference(ids, grad, vocab, scale):
+    """Sums, sums of magnitudes and counts per token, in 64 bits."""
+    keep = (ids >= 0) & (ids < vocab)
+    order = np.flatnonzero(keep)[np.argsort(ids[keep], kind="stable")]
+    total, size = np.zeros((vocab, grad.shape[1])), np.zeros((vocab, grad.shape[1]))
+    n = np.bincount(ids[keep], minlength=vocab)
+    if len(order):
+        starts = np.concatenate([[0], np.cumsum(n)])[:-1][n > 0]
+        g = grad[order].astype(np.float64)
+        total[n > 0] = np.add.reduceat(g, starts, axis=0)
+        size[n > 0] = np.add.reduceat(np.abs(g), starts, axis=0)
+    return scale * total, abs(scale) * size, n
+
+
+CASES = [
+    (1, 1, 1, "uniform"), (5, 3, 7, "uniform"), (64, 10, 16, "zipf"), (100, 1000, 33, "zipf"),
+    (257, 2, 256, "uniform"), (1000, 1, 12, "one"), (4096, 512, 260, "zipf"),
+    (3000, 70000, 64, "uniform"), (2000, 50021, 1000, "zipf"), (300, 40, 5, "outside"),
+    (20000, 259, 128, "zipf"), (9000, 100, 30, "one"), (70001, 33000, 9, "zipf"),
+    (513, 513, 2048, "zipf"), (63, 4000, 1027, "uniform"), (100000, 17, 3, "uniform"),
+]
+
+
+@pytest.mark.parametrize("count,vocab,dim,how", CASES)
+def test_forward_and_backward(hip, count, vocab, dim, how):
+    rng = np.random.default_rng(count + vocab)
+    ids = make_ids(rng, count, vocab, how)
+    table = rng.standard_normal((vocab, dim)).astype(np.float32)
+    grad = rng.standard_normal((count, dim)).astype(np.float32)
+    scale = np.float32(np.sqrt(dim))
+    print(f"embedding {count} of {vocab} x {dim} {how}", flush=True)
+    d_ids, d_table, d_grad = (hip.DeviceBuffer.from_host(x, x.dtype) for x in (ids, table, grad))
+    out = hip.DeviceBuffer.from_host(np.full((count, dim), np.nan, np.float32))
+    hip.embedding_forward(out, d_table, d_ids, count, vocab, dim, scale)
+    keep = ((ids >= 0) & (ids < vocab))[:, None]
+    want = np.where(keep, table[np.where(keep[:, 0], ids, 0)] * scale, np.float32(0))
+    assert np.array_equal(out.to_host((count, dim)), want)
+
+    value, size, n = reference(ids, grad, vocab, float(scale))
+    old = rng.standard_normal((vocab, dim)).astype(np.float32)
+    for beta in (0.0, 1.0, 0.5):
+        start = np.full_like(old, np.nan) if beta == 0.0 else old
+        dtable = hip.DeviceBuffer.from_host(start)
+        hip.embedding_backward(dtable, d_grad, d_ids, count, vocab, dim, scale, beta)
+        got = dtable.to_host((vocab, dim))
+        was = beta * old.astype(np.float64) if beta else np.zeros_like(value)
+        tol = (n[:, None] + 4) * U * (size + np.abs(was)) + 1e-37
+        bad = ~(np.abs(got - (value + was)) <= tol)
+        assert not bad.any(), (beta, np.argwhere(bad)[:3], bad.sum())
+        if beta == 1.0:
+            assert np.array_equal(got[n == 0], old[n == 0])
+        if beta == 0.0:
+            assert np.all(got[n == 0] == 0)
+        # the same bits again
+        hip.call("nrs_memcpy_htod", dtable.ptr, start.ctypes.data, start.nbytes)
+        hip.embedding_backward(dtable, d_grad, d_ids, count, vocab, dim, scale, beta)
+        assert np.array_equal(dtable.to_host((vocab, dim)), got)
+
+
+def test_integer_sums_are_exact(hip):
+    """Small integers add without rounding, in any order."""
+    rng = np.random.default_rng(2)
+    count, vocab, dim = 30011, 97, 40
+    ids = make_ids(rng, count, vocab, "zipf")
+    grad = rng.integers(-8, 9, (count, dim)).astype(np.float32)
+    value, _, _ = reference(ids, grad, vocab, 2.0)
+    dtable = hip.DeviceBuffer(vocab * dim)
+    hip.embedding_backward(dtable, hip.DeviceBuffer.from_host(grad),
+                           hip.DeviceBuffer.from_host(ids, np.int32), count, vocab, dim, 2.0)
+    assert np.array_equal(dtable.to_host((vocab, dim)), value.astype(np.float32))
+
+
+def test_no_tokens(hip):
+    old = np.arange(12, dtype=np.float32).reshape(4, 3)
+    for beta in (0.0, 1.0, 2.0):
+        dtable = hip.DeviceBuffer.from_host(old)
+        hip.embedding_backward(dtable, None, None, 0, 4, 3, 1.0, beta)
+        assert np.array_equal(dtable.to_host((4, 3)), beta * old)
+    hip.embedding_forward(None, None, None, 0, 4, 3)
+
+
+def test_unaligned_rows(hip):
+    """Buffers that start at any float."""
+    rng = np.random.default_rng(3)
+    count, vocab, dim = 200, 50, 36
+    ids = make_ids(rng, count, vocab, "zipf")
+    table, grad = (rng.standard_normal((n, dim)).astype(np.float32) for n in (vocab, count))
+    d_ids = hip.DeviceBuffer.from_host(np.concatenate([[7], ids]).astype(np.int32), np.int32)
+    d_table = hip.DeviceBuffer.from_host(np.concatenate([[1, 2, 3], table.ravel()]))
+    d_grad = hip.DeviceBuffer.from_host(np.concatenate([[1], grad.ravel()]))
+    out, dtable = hip.DeviceBuffer.zeros(count * dim + 2), hip.DeviceBuffer.zeros(vocab * dim + 3)
+    hip.embedding_forward(out.ptr + 4, d_table.ptr + 12, d_ids.ptr + 4, count, vocab, dim, 3.0)
+    got = out.to_host()
+    want = np.where((ids >= 0)[:, None], table[np.maximum(ids, 0)] * np.float32(3), np.float32(0))
+    assert np.array_equal(got[1:-1].reshape(count, dim), want) and got[0] == 0 and got[-1] == 0
+    hip.embedding_backward(dtable.ptr + 4, d_grad.ptr + 4, d_ids.ptr + 4, count, vocab, dim, 1.0)
+    got = dtable.to_host()
+    value, size, n = reference(ids, grad, vocab, 1.0)
+    assert np.all(np.abs(got[1:-2].reshape(vocab, dim) - value) <= (n[:, None] + 4) * U * size + 1e-37)
+    assert got[0] == 0 and np.all(got[-2:] == 0)
+
+
+def test_own_scratch(hip):
+    rng = np.random.default_rng(4)
+    for count, vocab, dim in ((5000, 300, 64), (33, 20000, 16), (40000, 2000, 100)):
+        ids = make_ids(rng, count, vocab, "zipf")
+        grad = hip.DeviceBuffer.from_host(rng.standard_normal((count, dim)).astype(np.float32))
+        d_ids = hip.DeviceBuffer.from_host(ids, np.int32)
+        a, b = hip.DeviceBuffer(vocab * dim), hip.DeviceBuffer(vocab * dim)
+        hip.embedding_backward(a, grad, d_ids, count, vocab, dim)
+        need = hip.embedding_workspace(count, vocab, dim)
+        fill = np.full((need + 3) // 4 + 64, np.float32(7))
+        work = hip.DeviceBuffer.from_host(fill)
+        hip.embedding_backward(b, grad, d_ids, count, vocab, dim, work=work)
+        assert np.array_equal(a.to_host(), b.to_host())
+        assert np.all(work.to_host()[(need + 3) // 4:] == 7)
