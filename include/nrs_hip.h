@@ -329,8 +329,9 @@ int nrs_attention_backward(float *dq, float *dk, float *dv, const float *dout, c
  * and as seq_k past it. Keys and values past it are never read. An item
  * without live keys gets zeros.
  *   stats ([batch*heads*seq_q*2], NULL when no backward follows) receives per
- * query row the softmax in base 2 as nrs_attention_forward gives it: the
- * maximum and the sum (both 0 without live keys).
+ * query row the softmax in base 2 for the backward: a reference exponent m, the
+ * row's maximum or at most 8 below it, and sum_j 2^(u_j - m) with u = scale *
+ * log2(e) * q . k^T (both 0 without live keys).
  * d_head is 1 to 128; strides are at most 2^20 floats; tensors may be longer
  * than 4 GiB. nrs_cross_attention_supported says whether a shape is taken;
  * one that is not is refused with NRS_ERR_ARG. Values of live keys and their

@@ -2,34 +2,17 @@
 // different lengths, several query heads to a key head, a length of live keys
 // for each batch item. Forward and backward, all f32.
 //
-// The query heads of one key head are further rows of the same product: with
-// group = heads / kv_heads, row r of (item, key head) is query r / group of
-// head kv_head * group + r % group, R = seq_q * group rows in all. Keys past
-// the item's length are never read (they stand for nothing, and may hold
-// anything); an item without live keys gets zeros.
-#include <algorithm>
+// Here: the forward of few rows (a token being decoded), the join of an item's
+// keys shared among workgroups, the backward, the plan and the entry points.
+#include "cross_attention.hpp"
 
-#include "buffer_ops.hpp"
+#include <algorithm>
 
 namespace nrs {
 namespace {
 
-struct CrossArgs {
-    const float *q, *k, *v, *dout, *o;
-    float *out, *stats;  // stats: [batch][heads][seq_q][2], base-2 max and sum
-    float *dq, *dk, *dv;
-    const int32_t* key_len;  // per item, null: all keys
-    int B, H, KV, G, Sq, Sk, D, ld_q, ld_kv, ld_out;
-    float scale, scale2;  // scale2 = scale * log2(e)
-    float beta_q, beta_kv;
-};
-
 __device__ __forceinline__ f32x4 mfma16(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
-
-__device__ __forceinline__ int live_keys(const CrossArgs& a, int b) {
-    return a.key_len ? max(0, min(a.key_len[b], a.Sk)) : a.Sk;
 }
 
 // 16 rows (rows, relative to `row0`, of this item and key head) of a tensor of
@@ -133,27 +116,43 @@ __device__ __forceinline__ void store_row(float* dst, const f32x4 (&acc)[NJ], fl
         }
 }
 
-__device__ __forceinline__ int64_t query_offset(const CrossArgs& a, int b, int kv, int r, int ld) {
-    return ((int64_t)b * a.Sq + r / a.G) * ld + (int64_t)(kv * a.G + r % a.G) * a.D;
-}
-
-__device__ __forceinline__ float* row_stats(const CrossArgs& a, int b, int kv, int r) {
-    return a.stats + (((int64_t)b * a.H + kv * a.G + r % a.G) * a.Sq + r / a.G) * 2;
-}
-
 __device__ __forceinline__ float across_groups(float x) {
     x += __shfl_xor(x, 16, 64);
     return x + __shfl_xor(x, 32, 64);
 }
 
-// One wave per 16 rows of an (item, key head), its keys 16 at a time.
+constexpr int kRowWaves = 4;
+
+// Few rows: K and V stream from HBM straight into registers, as operands of
+// v_mfma_f32_16x16x4_f32 (16 rows at 157 TFLOP/s keep pace with 8 TB/s of f32
+// keys and values). Waves of a workgroup take turns at tiles of 16 keys, each
+// with its next tile on the way, and are joined at the end; workgroups share
+// the keys of an item when there are few of them.
 template <int NJ>
-__global__ __launch_bounds__(64) void cross_fwd_kernel(CrossArgs a) {
-    const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
-    const int R = a.Sq * a.G, tiles = (R + 15) / 16;
-    const int item = blockIdx.x / tiles, r0 = (blockIdx.x - item * tiles) * 16;
+__global__ __launch_bounds__(64 * kRowWaves) void cross_rows_fwd_kernel(CrossArgs a) {
+    __shared__ float sums[kRowWaves][4 * NJ][64];
+    __shared__ float tops[kRowWaves][16], totals[kRowWaves][16];
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Sq * a.G, row_tiles = (R + 15) / 16, items = a.B * a.KV;
+    int rest = blockIdx.x;
+    const int r0 = rest % row_tiles * 16;
+    rest /= row_tiles;
+    const int item = rest % items, split_no = rest / items;
     const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
-    f32x4 qf[NJ], acc[NJ];
+    const int all = (L + 15) / 16;
+    const int t0 = (int)((int64_t)all * split_no / a.splits),
+              t1 = (int)((int64_t)all * (split_no + 1) / a.splits);
+    f32x4 qf[NJ], acc[NJ], kf[NJ];
+    float vf[4][NJ];
+    auto load = [&](int t) {
+        const int n = min(16, L - 16 * t);
+        Rows<false>(a, a.k, b, kv, a.ld_kv, 16 * t, n).template along<NJ>(kf, c, g);
+        const Rows<false> vs(a, a.v, b, kv, a.ld_kv, 16 * t, n);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vs.template across<NJ>(vf[r], 4 * g + r, c);
+    };
+    if (t0 + w < t1) load(t0 + w);
     Rows<true>(a, a.q, b, kv, a.ld_q, r0, min(16, R - r0)).template along<NJ>(qf, c, g);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
@@ -161,15 +160,18 @@ __global__ __launch_bounds__(64) void cross_fwd_kernel(CrossArgs a) {
         acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     float m = -INFINITY, l = 0.0f;
-    for (int k0 = 0; k0 < L; k0 += 16) {
-        const int n = min(16, L - k0);
-        f32x4 kf[NJ];
-        Rows<false>(a, a.k, b, kv, a.ld_kv, k0, n).template along<NJ>(kf, c, g);
+    for (int t = t0 + w; t < t1; t += kRowWaves) {
         f32x4 p = dot_rows<NJ>(kf, qf);
+        float vt[4][NJ];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) vt[r][j] = vf[r][j];
+        if (t + kRowWaves < t1) load(t + kRowWaves);
         float mt = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            if (4 * g + r >= n) p[r] = -INFINITY;
+            if (16 * t + 4 * g + r >= L) p[r] = -INFINITY;
             mt = fmaxf(mt, p[r]);
         }
         mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
@@ -179,122 +181,135 @@ __global__ __launch_bounds__(64) void cross_fwd_kernel(CrossArgs a) {
         m = top;
         l *= alpha;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            p[r] = 4 * g + r < n ? __builtin_amdgcn_exp2f(p[r] - m) : 0.0f;
-            l += p[r];
-        }
-#pragma unroll
         for (int j = 0; j < NJ; ++j) acc[j] = acc[j] * alpha;
-        add_rows<NJ>(acc, Rows<false>(a, a.v, b, kv, a.ld_kv, k0, n), p, c, g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            p[r] = 16 * t + 4 * g + r < L ? __builtin_amdgcn_exp2f(p[r] - m) : 0.0f;
+            l += p[r];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[j] = mfma16(vt[r][j], p[r], acc[j]);
+        }
     }
     l = across_groups(l);
-    if (r0 + c >= R) return;
-    store_row<NJ>(a.out + query_offset(a, b, kv, r0 + c, a.ld_out), acc, L > 0 ? 1.0f / l : 0.0f,
-                  0.0f, a.D, g);
-    if (a.stats && g == 0) {
-        float* st = row_stats(a, b, kv, r0 + c);
-        st[0] = L > 0 ? m : 0.0f;
-        st[1] = l;
+    if (g == 0) {
+        tops[w][c] = m;
+        totals[w][c] = l;
     }
-}
-
-// The gradient of the queries: the forward's walk over the keys again.
-template <int NJ>
-__global__ __launch_bounds__(64) void cross_dq_kernel(CrossArgs a) {
-    const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
-    const int R = a.Sq * a.G, tiles = (R + 15) / 16;
-    const int item = blockIdx.x / tiles, r0 = (blockIdx.x - item * tiles) * 16;
-    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b), nr = min(16, R - r0);
-    f32x4 qf[NJ], gf[NJ], of[NJ], acc[NJ];
-    Rows<true>(a, a.q, b, kv, a.ld_q, r0, nr).template along<NJ>(qf, c, g);
-    Rows<true>(a, a.dout, b, kv, a.ld_out, r0, nr).template along<NJ>(gf, c, g);
-    Rows<true>(a, a.o, b, kv, a.ld_out, r0, nr).template along<NJ>(of, c, g);
-    float delta = 0.0f;
+    __syncthreads();
+    float top = tops[0][c];
+#pragma unroll
+    for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, tops[i][c]);
+    // a wave without keys adds nothing; NaN must not be taken for that
+    const float f = m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) sums[w][r * NJ + j][lane] = acc[j][r] * f;
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kRowWaves; ++i) {
+        const float li = totals[i][c];
+        total += tops[i][c] == -INFINITY && li == 0.0f
+                     ? 0.0f
+                     : li * __builtin_amdgcn_exp2f(tops[i][c] - top);
+    }
+    __syncthreads();
+    if (r0 + c >= R) return;
+    // wave w adds the waves' register w: NJ neighbouring columns of row c
+    static_assert(kRowWaves == 4, "a register of an accumulator to each wave");
+    const bool whole = a.splits == 1;
+    const float scale = !whole ? 1.0f : L > 0 ? 1.0f / total : 0.0f;
+    const int64_t at = ((int64_t)split_no * items + item) * R + r0 + c;
+    float* dst = whole ? a.out + query_offset(a, b, kv, r0 + c, a.ld_out) : a.part + at * a.D;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        qf[j] = qf[j] * a.scale2;
-        acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float v = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) delta = fmaf(gf[j][e], of[j][e], delta);
+        for (int i = 0; i < kRowWaves; ++i) v += sums[i][w * NJ + j][lane];
+        const int d = (4 * g + w) * NJ + j;
+        if (d < a.D) dst[d] = v * scale;
     }
-    delta = across_groups(delta);
-    float m = 0.0f, rl = 0.0f;
-    if (c < nr && L > 0) {
-        const float* st = row_stats(a, b, kv, r0 + c);
-        m = st[0];
-        rl = 1.0f / st[1];
+    if (w == 0 && g == 0 && (!whole || a.stats)) {
+        float* st = whole ? row_stats(a, b, kv, r0 + c) : a.part_stats + 2 * at;
+        st[0] = whole && L == 0 ? 0.0f : top;
+        st[1] = total;
     }
-    for (int k0 = 0; k0 < L; k0 += 16) {
-        const int n = min(16, L - k0);
-        const Rows<false> keys(a, a.k, b, kv, a.ld_kv, k0, n);
-        f32x4 kf[NJ], vf[NJ];
-        keys.template along<NJ>(kf, c, g);
-        Rows<false>(a, a.v, b, kv, a.ld_kv, k0, n).template along<NJ>(vf, c, g);
-        f32x4 p = dot_rows<NJ>(kf, qf), dp = dot_rows<NJ>(vf, gf);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float w = 4 * g + r < n ? __builtin_amdgcn_exp2f(p[r] - m) * rl : 0.0f;
-            dp[r] = w * (dp[r] - delta) * a.scale;
-        }
-        add_rows<NJ>(acc, keys, dp, c, g);
-    }
-    if (c < nr)
-        store_row<NJ>(a.dq + query_offset(a, b, kv, r0 + c, a.ld_q), acc, 1.0f, a.beta_q, a.D, g);
 }
 
-// The gradients of 16 keys and values: one wave walks the rows of all heads
-// that share them.
-template <int NJ>
-__global__ __launch_bounds__(64) void cross_dkv_kernel(CrossArgs a) {
-    const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
-    const int tiles = (a.Sk + 15) / 16;
-    const int item = blockIdx.x / tiles, k0 = (blockIdx.x - item * tiles) * 16;
-    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
-    const int n = min(16, L - k0), R = n > 0 ? a.Sq * a.G : 0;  // dead keys: zeros
-    f32x4 kf[NJ], vf[NJ], acc_k[NJ], acc_v[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc_k[j] = acc_v[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (n > 0) {
-        Rows<false>(a, a.k, b, kv, a.ld_kv, k0, n).template along<NJ>(kf, c, g);
-        Rows<false>(a, a.v, b, kv, a.ld_kv, k0, n).template along<NJ>(vf, c, g);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) kf[j] = kf[j] * a.scale2;
+// Joins the splits of a row: out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M).
+// PER_ROW threads share a row, 32 (four columns each, d_head <= 128) or 256,
+// whose eight groups of 32 take turns at the splits and add up in LDS.
+template <int PER_ROW>
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
+    __shared__ float sums[256][5];
+    const int R = a.Sq * a.G, items = a.B * a.KV;
+    const int x = threadIdx.x % 32, turn = PER_ROW == 256 ? threadIdx.x / 32 : 0;
+    const int64_t at = (int64_t)blockIdx.x * (256 / PER_ROW) + threadIdx.x / PER_ROW;
+    const int64_t rows = (int64_t)items * R;
+    if (PER_ROW != 256 && at >= rows) return;
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_stats[2 * (s * rows + at)]);
+    float v[4] = {}, total = 0.0f;
+    const int live = max(0, min(4, a.D - 4 * x));
+    for (int s = turn; s < a.splits; s += PER_ROW / 32) {
+        const float m = a.part_stats[2 * (s * rows + at)], l = a.part_stats[2 * (s * rows + at) + 1];
+        if (m == -INFINITY && l == 0.0f) continue;  // no keys in this split
+        const float f = __builtin_amdgcn_exp2f(m - top);
+        total = fmaf(l, f, total);
+        const float* src = a.part + (s * rows + at) * a.D + 4 * x;
+        for (int e = 0; e < live; ++e) v[e] = fmaf(src[e], f, v[e]);
     }
-    for (int r0 = 0; r0 < R; r0 += 16) {
-        const int nr = min(16, R - r0);
-        const Rows<true> qs(a, a.q, b, kv, a.ld_q, r0, nr), gs(a, a.dout, b, kv, a.ld_out, r0, nr);
-        f32x4 qf[NJ], gf[NJ], of[NJ];
-        qs.template along<NJ>(qf, c, g);
-        gs.template along<NJ>(gf, c, g);
-        Rows<true>(a, a.o, b, kv, a.ld_out, r0, nr).template along<NJ>(of, c, g);
-        float delta = 0.0f, m = 0.0f, rl = 0.0f;
+    if constexpr (PER_ROW == 256) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int e = 0; e < 4; ++e) sums[threadIdx.x][e] = v[e];
+        sums[threadIdx.x][4] = total;
+        __syncthreads();
+        if (turn != 0) return;
+        for (int t = 1; t < 8; ++t) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) delta = fmaf(gf[j][e], of[j][e], delta);
-        delta = across_groups(delta);
-        if (c < nr) {
-            const float* st = row_stats(a, b, kv, r0 + c);
-            m = st[0];
-            rl = 1.0f / st[1];
+            for (int e = 0; e < 4; ++e) v[e] += sums[32 * t + x][e];
+            total += sums[32 * t + x][4];
         }
-        f32x4 p = dot_rows<NJ>(qf, kf), dp = dot_rows<NJ>(gf, vf);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            // the row of register r is 4g + r, whose values lane 4g + r holds
-            const float mr = __shfl(m, 4 * g + r, 64), lr = __shfl(rl, 4 * g + r, 64),
-                        dr = __shfl(delta, 4 * g + r, 64);
-            const bool live = 4 * g + r < nr && c < n;
-            p[r] = live ? __builtin_amdgcn_exp2f(p[r] - mr) * lr : 0.0f;
-            dp[r] = p[r] * (dp[r] - dr) * a.scale;
-        }
-        add_rows<NJ>(acc_v, gs, p, c, g);
-        add_rows<NJ>(acc_k, qs, dp, c, g);
     }
-    if (k0 + c >= a.Sk) return;
-    const int64_t at = ((int64_t)b * a.Sk + k0 + c) * a.ld_kv + (int64_t)kv * a.D;
-    store_row<NJ>(a.dk + at, acc_k, 1.0f, a.beta_kv, a.D, g);
-    store_row<NJ>(a.dv + at, acc_v, 1.0f, a.beta_kv, a.D, g);
+    const int item = (int)(at / R), r = (int)(at - (int64_t)item * R);
+    const int b = item / a.KV, kv = item - b * a.KV;
+    const bool any = live_keys(a, b) > 0;
+    const float scale = any ? 1.0f / total : 0.0f;
+    float* dst = a.out + query_offset(a, b, kv, r, a.ld_out) + 4 * x;
+    for (int e = 0; e < live; ++e) dst[e] = v[e] * scale;
+    if (a.stats && x == 0) {
+        float* st = row_stats(a, b, kv, r);
+        st[0] = any ? top : 0.0f;
+        st[1] = any ? total : 0.0f;
+    }
+}
+
+// Adds the shares of a gradient in order: dst = f * sum + beta * dst, 32
+// threads to a row of d_head. KEYS: rows are keys, dead ones without shares.
+template <bool KEYS>
+__global__ __launch_bounds__(256) void cross_sum_kernel(CrossArgs a) {
+    const int n = KEYS ? a.Sk : a.Sq * a.G, x = threadIdx.x % 32;
+    const int64_t at = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    const int64_t rows = (int64_t)a.B * a.KV * n;
+    if (at >= rows) return;
+    const int item = (int)(at / n), r = (int)(at - (int64_t)item * n);
+    const int b = item / a.KV, kv = item - b * a.KV;
+    const bool live = !KEYS || r < live_keys(a, b);
+    const float beta = KEYS ? a.beta_kv : a.beta_q;
+    if (!live && beta == 1.0f) return;
+    for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
+        const float* part = KEYS ? (which ? a.dv_part : a.dk_part) : a.dq_part;
+        float* dst = KEYS ? (which ? a.dv : a.dk) + key_offset(a, b, kv, r)
+                          : a.dq + query_offset(a, b, kv, r, a.ld_q);
+        const float f = which ? 1.0f : a.scale;
+        const int shares = KEYS ? a.kv_splits : a.q_splits;
+        for (int d = 4 * x; d < min(a.D, 4 * x + 4); ++d) {
+            float v = 0.0f;
+            if (live)
+                for (int s = 0; s < shares; ++s) v += part[(s * rows + at) * a.D + d];
+            dst[d] = beta != 0.0f ? v * f + beta * dst[d] : v * f;
+        }
+    }
 }
 
 template <class F>
@@ -309,7 +324,7 @@ void for_width(int d, F f) {
         f(std::integral_constant<int, 8>());
 }
 
-constexpr int64_t kMaxLd = 1 << 20, kMaxLen = 1 << 26;
+constexpr int64_t kMaxLd = 1 << 20, kMaxLen = 1 << 26, kMaxGroups = 1 << 22;
 
 const char* refusal(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_k,
                     int64_t d_head, int64_t ld_q, int64_t ld_kv, int64_t ld_out) {
@@ -322,10 +337,11 @@ const char* refusal(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_
         return "a row stride is shorter than its heads";
     if (ld_q > kMaxLd || ld_kv > kMaxLd || ld_out > kMaxLd) return "a row stride is past 2^20";
     if (seq_q > kMaxLen || seq_k > kMaxLen) return "a length is past 2^26";
+    // a launch has fewer than 2^32 threads, 256 for 16 rows or keys at most
     const int64_t rows = (seq_q * (heads / kv_heads) + 15) / 16, keys = (seq_k + 15) / 16;
-    if (seq_q * (heads / kv_heads) > INT32_MAX / 2 || batch > INT32_MAX / kv_heads ||
-        batch * kv_heads * std::max<int64_t>({rows, keys, 1}) > INT32_MAX)
-        return "too many rows for one launch";
+    if (batch > kMaxGroups ||
+        batch * kv_heads * std::max<int64_t>({rows, keys, 1}) > kMaxGroups)
+        return "more than 2^26 rows or keys (in groups of 16 of an item)";
     return nullptr;
 }
 
@@ -340,6 +356,85 @@ int check_shape(const char* what, int64_t batch, int64_t heads, int64_t kv_heads
                   (long long)seq_q, (long long)seq_k, (long long)d_head, (long long)ld_q,
                   (long long)ld_kv, (long long)ld_out);
     return NRS_OK;
+}
+
+struct ForwardPlan {
+    bool tiles;  // the kernel of many rows
+    int splits;
+    int64_t blocks;  // workgroups, splits included
+};
+
+// Rows of an item up to which the kernel of few rows takes the call.
+constexpr int64_t kFewRows = 32;
+
+ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
+                         int64_t seq_k, int64_t d_head) {
+    const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads, cus = num_cus();
+    ForwardPlan p{R > kFewRows, 1, 0};
+    if (items == 0 || R == 0) return p;
+    if (!p.tiles) {
+        // 16 waves to a compute unit, at least a tile of 16 keys for each
+        const int64_t base = items * ((R + 15) / 16);
+        const int64_t most = std::max<int64_t>(1, seq_k / (16 * kRowWaves));
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({4 * cus / base, most, 256}));
+        p.blocks = base * p.splits;
+    } else {
+        // one workgroup to a compute unit: the split with the least time, in
+        // key tiles, of the fullest one; a workgroup's beginning and end cost
+        // two tiles, a join four
+        const int rows = cross_forward_rows((int)R, (int)d_head);
+        const int64_t base = items * ((R + rows - 1) / rows);
+        const int64_t keys = cross_tile_keys((int)d_head), tiles = (seq_k + keys - 1) / keys;
+        int64_t best = INT64_MAX;
+        p.splits = 1;
+        for (int s = 1; s <= 16 && s <= std::max<int64_t>(1, tiles / 2); ++s) {
+            const int64_t turns = (base * s + cus - 1) / cus;
+            const int64_t cost = turns * ((tiles + s - 1) / s + 2) + (s > 1 ? 4 : 0);
+            if (cost < best) {
+                best = cost;
+                p.splits = s;
+            }
+        }
+        p.blocks = base * p.splits;
+    }
+    return p;
+}
+
+struct BackwardPlan {
+    int q_splits, kv_splits;
+    int64_t rows, keys;  // of all items
+    size_t prepared, q_part, kv_part;  // floats of each kind of scratch
+    size_t bytes() const { return sizeof(float) * (prepared + q_part + 2 * kv_part); }
+};
+
+// A workgroup to a compute unit: a walk that is longer than a compute unit's
+// even part of all the work is shared out. A step of dq is three products a
+// tile, one of dk and dv four. Asked for both gradients or not, the plan is
+// that of both: each has the same bits by itself.
+BackwardPlan plan_backward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
+                           int64_t seq_k, int64_t d_head) {
+    const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads, cus = num_cus();
+    BackwardPlan p{1, 1, items * R, items * seq_k, 0, 0, 0};
+    p.prepared = (size_t)((2 * p.rows + 3) / 4 * 4);  // needed without keys, too
+    if (p.rows == 0 || p.keys == 0) return p;
+    const int64_t tile = cross_tile_keys((int)d_head),
+                  own = cross_backward_rows((int)R, (int)seq_k, (int)d_head);
+    const int64_t q_len = (seq_k + tile - 1) / tile, kv_len = (R + tile - 1) / tile;
+    const int64_t q_groups = items * ((R + own - 1) / own),
+                  kv_groups = items * ((seq_k + own - 1) / own);
+    const int64_t even = std::max<int64_t>(8, (3 * q_groups * q_len + 4 * kv_groups * kv_len) / cus);
+    auto shares = [&](int64_t cost, int64_t len) {
+        return (int)std::max<int64_t>(1, std::min<int64_t>({(cost + even - 1) / even, len, 64}));
+    };
+    p.q_splits = shares(3 * q_len, q_len);
+    p.kv_splits = shares(4 * kv_len, kv_len);
+    if (p.q_splits > 1) p.q_part = (size_t)((p.q_splits * p.rows * d_head + 3) / 4 * 4);
+    if (p.kv_splits > 1) p.kv_part = (size_t)((p.kv_splits * p.keys * d_head + 3) / 4 * 4);
+    return p;
+}
+
+size_t forward_scratch(const ForwardPlan& p, int64_t rows, int64_t d_head) {
+    return p.splits > 1 ? sizeof(float) * (size_t)p.splits * rows * (d_head + 2) : 0;
 }
 
 }  // namespace
@@ -360,8 +455,11 @@ int nrs_cross_attention_workspace(size_t* bytes, int64_t batch, int64_t heads, i
                                   seq_k, d_head, heads * d_head, kv_heads * d_head,
                                   heads * d_head))
         return rc;
-    (void)backward;
-    *bytes = 0;
+    *bytes = backward
+                 ? nrs::plan_backward(batch, heads, kv_heads, seq_q, seq_k, d_head).bytes()
+                 : nrs::forward_scratch(
+                       nrs::plan_forward(batch, heads, kv_heads, seq_q, seq_k, d_head),
+                       batch * heads * seq_q, d_head);
     return NRS_OK;
 }
 
@@ -378,9 +476,16 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
     NRS_ARG_CHECK(out && q && ((k && v) || seq_k == 0), "%s: null pointer", what);
     NRS_REQUIRE_INIT();
     if (int rc = nrs::check_device(what)) return rc;
+    const auto plan = nrs::plan_forward(batch, heads, kv_heads, seq_q, seq_k, d_head);
+    const int64_t rows = batch * heads * seq_q;
     float* scratch = nullptr;
-    if (int rc = nrs::call_scratch(&scratch, 0, work, work_bytes, what)) return rc;
+    if (int rc = nrs::call_scratch(&scratch, nrs::forward_scratch(plan, rows, d_head), work,
+                                   work_bytes, what))
+        return rc;
     nrs::CrossArgs a{};
+    a.splits = plan.splits;
+    a.part = scratch;
+    a.part_stats = scratch ? scratch + plan.splits * rows * d_head : nullptr;
     a.q = q;
     a.k = k;
     a.v = v;
@@ -397,14 +502,26 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
     a.ld_q = (int)ld_q;
     a.ld_kv = (int)ld_kv;
     a.ld_out = (int)ld_out;
+    a.by_group = nrs::make_fastdiv((uint32_t)a.G);
     a.scale = scale;
     a.scale2 = scale * 1.4426950408889634f;
-    const int64_t tiles = (seq_q * a.G + 15) / 16;
-    nrs::for_width(a.D, [&](auto nj) {
-        hipLaunchKernelGGL(nrs::cross_fwd_kernel<decltype(nj)::value>,
-                           dim3((unsigned)(batch * kv_heads * tiles)), dim3(64), 0, nrs::stream(),
-                           a);
-    });
+    if (plan.tiles) {
+        nrs::cross_tile_forward(a);
+    } else {
+        nrs::for_width(a.D, [&](auto nj) {
+            hipLaunchKernelGGL(nrs::cross_rows_fwd_kernel<decltype(nj)::value>,
+                               dim3((unsigned)plan.blocks), dim3(64 * nrs::kRowWaves), 0,
+                               nrs::stream(), a);
+        });
+    }
+    NRS_LAUNCH_CHECK(what);
+    if (a.splits > 1) {
+        // many splits: a workgroup to a row
+        const bool wide = a.splits > 8;
+        auto join = wide ? nrs::cross_join_kernel<256> : nrs::cross_join_kernel<32>;
+        hipLaunchKernelGGL(join, dim3((unsigned)(wide ? rows : (rows + 7) / 8)), dim3(256), 0,
+                           nrs::stream(), a);
+    }
     NRS_LAUNCH_CHECK(what);
     return NRS_OK;
 }
@@ -427,8 +544,9 @@ int nrs_cross_attention_backward(float* dq, float* dk, float* dv, const float* d
                   "%s: null pointer", what);
     NRS_REQUIRE_INIT();
     if (int rc = nrs::check_device(what)) return rc;
+    const auto plan = nrs::plan_backward(batch, heads, kv_heads, seq_q, seq_k, d_head);
     float* scratch = nullptr;
-    if (int rc = nrs::call_scratch(&scratch, 0, work, work_bytes, what)) return rc;
+    if (int rc = nrs::call_scratch(&scratch, plan.bytes(), work, work_bytes, what)) return rc;
     nrs::CrossArgs a{};
     a.q = q;
     a.k = k;
@@ -450,21 +568,29 @@ int nrs_cross_attention_backward(float* dq, float* dk, float* dv, const float* d
     a.ld_q = (int)ld_q;
     a.ld_kv = (int)ld_kv;
     a.ld_out = (int)ld_out;
+    a.by_group = nrs::make_fastdiv((uint32_t)a.G);
     a.scale = scale;
     a.scale2 = scale * 1.4426950408889634f;  // as the forward computed it
     a.beta_q = beta_q;
     a.beta_kv = beta_kv;
-    const int64_t row_tiles = (seq_q * a.G + 15) / 16, key_tiles = (seq_k + 15) / 16;
-    nrs::for_width(a.D, [&](auto nj) {
-        if (dq && rows)
-            hipLaunchKernelGGL(nrs::cross_dq_kernel<decltype(nj)::value>,
-                               dim3((unsigned)(batch * kv_heads * row_tiles)), dim3(64), 0,
-                               nrs::stream(), a);
-        if (dk && keys)
-            hipLaunchKernelGGL(nrs::cross_dkv_kernel<decltype(nj)::value>,
-                               dim3((unsigned)(batch * kv_heads * key_tiles)), dim3(64), 0,
-                               nrs::stream(), a);
-    });
+    a.q_splits = plan.q_splits;
+    a.kv_splits = plan.kv_splits;
+    a.neg_lse = scratch;
+    a.neg_delta = scratch + plan.rows;
+    a.dq_part = scratch + plan.prepared;
+    a.dk_part = a.dq_part + plan.q_part;
+    a.dv_part = a.dk_part + plan.kv_part;
+    const int own = nrs::cross_backward_rows(a.Sq * a.G, a.Sk, a.D);
+    if (dq && rows)
+        a.q_blocks = (int)((a.Sq * a.G + own - 1) / own * batch * kv_heads * plan.q_splits);
+    if (!keys) a.dk = a.dv = nullptr;
+    nrs::cross_tile_backward(a);
+    if (dq && plan.q_splits > 1)
+        hipLaunchKernelGGL(nrs::cross_sum_kernel<false>, dim3((unsigned)((plan.rows + 7) / 8)),
+                           dim3(256), 0, nrs::stream(), a);
+    if (a.dk && plan.kv_splits > 1)
+        hipLaunchKernelGGL(nrs::cross_sum_kernel<true>, dim3((unsigned)((plan.keys + 7) / 8)),
+                           dim3(256), 0, nrs::stream(), a);
     NRS_LAUNCH_CHECK(what);
     return NRS_OK;
 }

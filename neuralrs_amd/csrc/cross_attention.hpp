@@ -1,0 +1,64 @@
+// Arguments and device helpers shared by the cross attention kernels
+// (cross_attention.hip: few rows, joins and sums, entry points;
+// cross_attention_tile.hip: many rows, the backward).
+//
+// The query heads of one key head are further rows of the same product: with
+// group = heads / kv_heads, row r of an item (batch item, key head) is query
+// r / group of head kv_head * group + r % group, R = seq_q * group rows in
+// all. Keys past the item's length are never read.
+#pragma once
+
+#include "buffer_ops.hpp"
+#include "fastdiv.hpp"
+
+namespace nrs {
+
+struct CrossArgs {
+    const float *q, *k, *v, *dout, *o;
+    float *out, *stats;  // stats: [batch][heads][seq_q][2], base-2 reference and sum
+    float *dq, *dk, *dv;
+    const int32_t* key_len;  // per batch item, null: all keys
+    int B, H, KV, G, Sq, Sk, D, ld_q, ld_kv, ld_out;
+    FastDiv by_group;     // division by G
+    float scale, scale2;  // scale2 = scale * log2(e)
+    float beta_q, beta_kv;
+    int splits;         // forward: workgroups that share an item's keys
+    float* part;        // splits > 1: [splits][items][R][D] sums, not yet divided
+    float* part_stats;  // and their [splits][items][R][2]
+    // backward
+    float *neg_lse, *neg_delta;  // [items][R]: -log2 sum 2^u and -dout . out
+    int q_splits, kv_splits;     // workgroups that share a dq (dk and dv) tile's walk
+    float *dq_part, *dk_part, *dv_part;  // [splits][items][rows][D] when shared
+    int q_blocks;                // workgroups of the dq part of the launch
+};
+
+__device__ __forceinline__ int live_keys(const CrossArgs& a, int b) {
+    return a.key_len ? max(0, min(a.key_len[b], a.Sk)) : a.Sk;
+}
+
+// Element offset of row r of (b, kv) in a tensor of queries.
+__device__ __forceinline__ int64_t query_offset(const CrossArgs& a, int b, int kv, int r, int ld) {
+    const int s = (int)fast_div((uint32_t)r, a.by_group);
+    return ((int64_t)b * a.Sq + s) * ld + (int64_t)(kv * a.G + (r - s * a.G)) * a.D;
+}
+
+__device__ __forceinline__ int64_t key_offset(const CrossArgs& a, int b, int kv, int r) {
+    return ((int64_t)b * a.Sk + r) * a.ld_kv + (int64_t)kv * a.D;
+}
+
+__device__ __forceinline__ float* row_stats(const CrossArgs& a, int b, int kv, int r) {
+    const int s = (int)fast_div((uint32_t)r, a.by_group);
+    return a.stats + (((int64_t)b * a.H + kv * a.G + (r - s * a.G)) * a.Sq + s) * 2;
+}
+
+// The kernels of cross_attention_tile.hip. Rows of a workgroup of the forward
+// (backward) and rows of K or of the queries it takes at a time, by which the
+// calls are planned.
+constexpr int cross_tile_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+constexpr int cross_tile_keys(int D) { return 4096 / cross_tile_width(D); }
+int cross_forward_rows(int R, int D);
+int cross_backward_rows(int R, int Sk, int D);
+void cross_tile_forward(const CrossArgs& a);
+void cross_tile_backward(const CrossArgs& a);
+
+}  // namespace nrs

@@ -1,0 +1,661 @@
+// Cross attention of many rows, forward and backward, on the bf16 matrix
+// cores.
+//
+// A float is the exact sum of three bf16 pieces, and the six largest of the
+// nine products of two floats' pieces give their product to 2^-24
+// (gemm_split.hpp tells why that is as good as f32): 2.7 times the rate of the
+// f32 matrix instructions.
+//
+// A workgroup of WAVES waves owns 32 * WAVES rows (or keys) of an item, 32 to
+// a wave, held as split operands in registers, and walks the item's keys (or
+// rows) in tiles through LDS. With "own" and "met" for the two sides, a wave
+// computes met . own^T on v_mfma_f32_32x32x16_bf16: lane (c, h) = (lane % 32,
+// lane / 32) gets 16 products of ONE of its own, c, with the met
+// 8 (i / 4) + 4h + i % 4 of a block of 32. So
+//   - the forward's softmax over the keys it meets is lane-local but for one
+//     exchange with lane c ^ 32;
+//   - registers 8u .. 8u + 7, split, are k-step u of the operand of
+//     acc^T[d][own] += met^T[d][met] . w[met][own] as they lie: O += V^T P,
+//     dQ += K^T dS (own rows), dV += dO^T P, dK += Q^T dS (own keys).
+// met^T is read from the same LDS copy as met, by transposing reads.
+//
+// Tiles are split once per workgroup, on their way into LDS, as three planes
+// of 16-byte units (one lane's operand): unit q of a row holds d = 4q .. 4q + 3
+// and D/2 + 4q .. D/2 + 4q + 3, so that a row's lanes load whole segments. The
+// next tile is loaded to registers while this one is multiplied, and stored to
+// the other of two buffers.
+//
+// The forward's softmax is online in base 2, against a reference m that
+// follows the running maximum only when that passes it by 2^8: sums of
+// probabilities up to 256 lose nothing in f32, and most tiles need no
+// rescaling of the accumulators. The products start from -m (in the backward
+// from -log2 of the row's sum, and from -dout . out), so neither needs a
+// subtraction.
+#include <algorithm>
+
+#include "cross_attention.hpp"
+
+namespace nrs {
+namespace {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct __attribute__((packed, aligned(4))) Quad {  // 128 bits at any float
+    f32x4 v;
+};
+
+// The three pieces of 8 floats: an operand of the matrix instructions each.
+__device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&p)[3]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const uint32_t w = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+            p[n][i] = w;
+            a -= __builtin_bit_cast(float, w << 16);
+            b -= __builtin_bit_cast(float, w & 0xffff0000u);
+        }
+        p[2][i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b),
+                                        __builtin_bit_cast(uint32_t, a), 0x07060302u);
+    }
+}
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// c += a . b from their pieces, the smallest products first.
+__device__ __forceinline__ f32x16 mfma_split(const u32x4 (&a)[3], const u32x4 (&b)[3], f32x16 c) {
+    c = mfma32(a[2], b[0], c);
+    c = mfma32(a[1], b[1], c);
+    c = mfma32(a[0], b[2], c);
+    c = mfma32(a[1], b[0], c);
+    c = mfma32(a[0], b[1], c);
+    return mfma32(a[0], b[0], c);
+}
+
+__device__ __forceinline__ f32x16 all16(float x) {
+    f32x16 v;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = x;
+    return v;
+}
+
+template <int D_, int WAVES_>
+struct TileCfg {
+    static constexpr int D = D_, WAVES = WAVES_, NT = 64 * WAVES;
+    static constexpr int KT = 4096 / D;       // rows of a tile
+    static constexpr int Q = D / 8;           // units of a row
+    static constexpr int PLANE = KT * Q;      // units of a plane
+    static constexpr int U = PLANE / NT;      // units a thread stages
+    static constexpr int SET = 3 * PLANE;     // units of a tensor's tile
+    static constexpr int NS = D / 16, NJ = D / 32, NB = KT / 32;
+    static_assert(U * NT == PLANE && KT % 32 == 0 && D % 32 == 0, "units");
+};
+
+// Unit q of row r in a plane: the 32 rows of a block are contiguous for the
+// operand reads; the exclusive or sends the units of a row, which neighbouring
+// lanes store, to different 16-byte columns, and units q and q + 2, which a
+// transposing read takes together, to different 64-byte ones.
+template <class C>
+__device__ __forceinline__ constexpr int mix(int q) {
+    return ((q ^ (q << 1)) * (C::Q < 8 ? 8 / C::Q : 1)) & 31;
+}
+template <class C>
+__device__ __forceinline__ int unit_at(int r, int q) {
+    return ((r >> 5) * C::Q + q) * 32 + ((r & 31) ^ mix<C>(q));
+}
+
+// A tile of a tensor on its way from global memory to LDS: thread t stages
+// unit i % Q of row i / Q, i = t + NT u.
+template <class C, bool FULL>
+struct Stage {
+    f32x4 x[C::U][2];
+
+    // Rows r0 .. r0 + n - 1 of an item's keys, or (QUERY) of its rows.
+    template <bool QUERY>
+    __device__ __forceinline__ void load(const CrossArgs& a, const float* base, int ld, int b,
+                                         int kv, int r0, int n) {
+        int first = r0;
+        int64_t at, floats;
+        if (QUERY) {
+            first = (int)fast_div((uint32_t)r0, a.by_group);
+            const int last = (int)fast_div((uint32_t)(r0 + n - 1), a.by_group);
+            at = ((int64_t)b * a.Sq + first) * ld + (int64_t)kv * a.G * a.D;
+            floats = (int64_t)(last - first) * ld + a.G * a.D;
+        } else {
+            at = key_offset(a, b, kv, r0);
+            floats = (int64_t)(n - 1) * ld + a.D;
+        }
+        const auto rs = buffer_rsrc(base + at, floats * 4);
+#pragma unroll
+        for (int u = 0; u < C::U; ++u) {
+            const int i = threadIdx.x + C::NT * u, row = i / C::Q, q = i % C::Q;
+            int off = row * ld;
+            if (QUERY) {
+                const int r = r0 + row, s = (int)fast_div((uint32_t)r, a.by_group);
+                off = (s - first) * ld + (r - s * a.G) * a.D;
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int d = 4 * q + s * (C::D / 2);
+                x[u][s] = buffer_load4(
+                    rs, row < n && (FULL || d < a.D) ? (off + d) * 4 : kOutOfRange);
+            }
+        }
+    }
+
+    __device__ __forceinline__ void store(const CrossArgs& a, u32x4* lds) const {
+#pragma unroll
+        for (int u = 0; u < C::U; ++u) {
+            const int i = threadIdx.x + C::NT * u, row = i / C::Q, q = i % C::Q;
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                f[e] = x[u][e / 4][e % 4];
+                // what follows the head in its row is not part of it
+                if (!FULL && 4 * q + e % 4 + (e / 4) * (C::D / 2) >= a.D) f[e] = 0.0f;
+            }
+            u32x4 p[3];
+            split8(f, p);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) lds[n * C::PLANE + unit_at<C>(row, q)] = p[n];
+        }
+    }
+};
+
+// The lane's operands of its own row at `src` (zeros unless live), times f.
+template <class C, bool FULL>
+__device__ __forceinline__ void own_pieces(u32x4 (&own)[C::NS][3], const CrossArgs& a,
+                                           const float* src, bool live, int h, float f) {
+#pragma unroll
+    for (int s = 0; s < C::NS; ++s) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int d = 4 * (2 * s + h) + e * (C::D / 2);
+            f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (live) {
+                if (FULL || d + 4 <= a.D) {
+                    v = reinterpret_cast<const Quad*>(src + d)->v;
+                } else {
+                    for (int i = 0; i < 4; ++i)
+                        if (d + i < a.D) v[i] = src[d + i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[4 * e + i] = v[i] * f;
+        }
+        split8(x, own[s]);
+    }
+}
+
+// start + met . own^T of block kb of a tile.
+template <class C>
+__device__ __forceinline__ f32x16 products(const u32x4* set, const u32x4 (&own)[C::NS][3], int kb,
+                                           f32x16 start, int c, int h) {
+#pragma unroll
+    for (int s = 0; s < C::NS; ++s) {
+        u32x4 met[3];
+        const int unit = unit_at<C>(kb * 32 + c, 2 * s + h);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) met[p] = set[p * C::PLANE + unit];
+        start = mfma_split(met, own[s], start);
+    }
+    return start;
+}
+
+// A transposing read: lanes 4e + x of a group of 16 give the places of four
+// 16-bit values each, x of row e; lane j gets values j of the four rows.
+__device__ __forceinline__ u32x2 read_transposed(const u32x2* p) {
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    return __builtin_bit_cast(
+        u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                   (lds_ptr)(__attribute__((address_space(3))) void*)const_cast<u32x2*>(p)));
+}
+
+// acc[j] += met^T . w for k-step u of block kb, w split. Of the 32 places m of
+// output block j, 16 tt + 4x + y is d = 4 (4j + 2 (x / 2) + tt) + (x % 2) D/2 + y:
+// each x a half of one unit.
+template <class C>
+__device__ __forceinline__ void add_transposed(f32x16 (&acc)[C::NJ], const u32x4* set, int kb,
+                                               int u, const u32x4 (&w)[3], int lane) {
+    const int x = lane & 3, e = (lane >> 2) & 3, tt = (lane >> 4) & 1, h = lane >> 5;
+    const int q0 = 2 * (x >> 1) + tt;
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) {
+        u32x4 met[3];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int unit = unit_at<C>(kb * 32 + 16 * u + 8 * half + 4 * h + e, 4 * j + q0);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                const u32x2 v = read_transposed(
+                    reinterpret_cast<const u32x2*>(set + p * C::PLANE + unit) + (x & 1));
+                met[p][2 * half] = v[0];
+                met[p][2 * half + 1] = v[1];
+            }
+        }
+        acc[j] = mfma_split(met, w, acc[j]);
+    }
+}
+
+// Stores a lane's acc * f (+ beta * old) into its own row of d_head floats.
+template <class C, bool FULL>
+__device__ __forceinline__ void store_own(float* dst, const f32x16 (&acc)[C::NJ], float f,
+                                          float beta, int D, int h) {
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = 4 * (4 * j + 2 * ((i / 4) % 2) + i / 8) + h * (C::D / 2);
+            f32x4 v = f32x4{acc[j][i], acc[j][i + 1], acc[j][i + 2], acc[j][i + 3]} * f;
+            if (FULL || d + 4 <= D) {
+                Quad* const to = reinterpret_cast<Quad*>(dst + d);
+                if (beta != 0.0f) v = v + beta * to->v;
+                to->v = v;
+            } else {
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < D) dst[d + e] = beta != 0.0f ? v[e] + beta * dst[d + e] : v[e];
+            }
+        }
+}
+
+// The part of `count` that share number `no` of `shares` walks.
+__device__ __forceinline__ void share(int count, int no, int shares, int& from, int& to) {
+    from = (int)((int64_t)count * no / shares);
+    to = (int)((int64_t)count * (no + 1) / shares);
+}
+
+template <int D, int WAVES, bool FULL>
+__global__ __launch_bounds__(64 * WAVES) void cross_tile_fwd_kernel(CrossArgs a) {
+    using C = TileCfg<D, WAVES>;
+    __shared__ u32x4 lds[2][2 * C::SET];
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Sq * a.G, tiles = (R + 32 * WAVES - 1) / (32 * WAVES);
+    const int items = a.B * a.KV;
+    int rest = blockIdx.x;
+    const int tile = rest % tiles;
+    rest /= tiles;
+    const int item = rest % items, split_no = rest / items;
+    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
+    const int row = (tile * WAVES + w) * 32 + c;
+    const bool wave_live = (tile * WAVES + w) * 32 < R, live = row < R;
+    int t0, t1;  // this split's key tiles of the item's
+    share((L + C::KT - 1) / C::KT, split_no, a.splits, t0, t1);
+
+    Stage<C, FULL> k, v;
+    auto load = [&](int t) {
+        const int n = min(C::KT, L - t * C::KT);
+        k.template load<false>(a, a.k, a.ld_kv, b, kv, t * C::KT, n);
+        v.template load<false>(a, a.v, a.ld_kv, b, kv, t * C::KT, n);
+    };
+    if (t0 < t1) load(t0);
+    u32x4 qf[C::NS][3];
+    own_pieces<C, FULL>(qf, a, a.q + (live ? query_offset(a, b, kv, row, a.ld_q) : 0), live, h,
+                        a.scale2);
+    f32x16 acc[C::NJ], start = all16(0.0f);  // start: -m, where the scores start
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) acc[j] = all16(0.0f);
+    float m = 0.0f, l = 0.0f;
+    if (t0 < t1) {
+        k.store(a, lds[0]);
+        v.store(a, lds[0] + C::SET);
+        if (t0 + 1 < t1) load(t0 + 1);
+        __syncthreads();
+    }
+    for (int t = t0; t < t1; ++t) {
+        const u32x4* const kl = lds[(t - t0) & 1];
+        const u32x4* const vl = kl + C::SET;
+        if (wave_live) {
+            const int n = L - t * C::KT;  // live keys of the tile, or more
+            f32x16 s[C::NB];
+#pragma unroll
+            for (int kb = 0; kb < C::NB; ++kb) s[kb] = products<C>(kl, qf, kb, start, c, h);
+            if (n < C::KT) {
+#pragma unroll
+                for (int kb = 0; kb < C::NB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (kb * 32 + 8 * (i / 4) + 4 * h + i % 4 >= n) s[kb][i] = -INFINITY;
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int kb = 0; kb < C::NB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const bool first = t == t0;
+            if (__any(first || top > 8.0f)) {
+                const float shift = first || top > 8.0f ? top : 0.0f;
+                const float alpha = first ? 0.0f : __builtin_amdgcn_exp2f(-shift);
+                m += shift;
+                l *= alpha;
+                start = all16(-m);
+#pragma unroll
+                for (int kb = 0; kb < C::NB; ++kb) s[kb] = s[kb] - shift;
+#pragma unroll
+                for (int j = 0; j < C::NJ; ++j) acc[j] = acc[j] * alpha;
+            }
+#pragma unroll
+            for (int kb = 0; kb < C::NB; ++kb)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = __builtin_amdgcn_exp2f(s[kb][8 * u + i]);
+                        l += x[i];
+                    }
+                    u32x4 p[3];
+                    split8(x, p);
+                    add_transposed<C>(acc, vl, kb, u, p, lane);
+                }
+        }
+        if (t + 1 < t1) {
+            // the other buffer was last read in step t - 1, which every wave
+            // had left before the barrier that ended it
+            k.store(a, lds[(t + 1 - t0) & 1]);
+            v.store(a, lds[(t + 1 - t0) & 1] + C::SET);
+            if (t + 2 < t1) load(t + 2);
+            __syncthreads();
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (!live) return;
+    if (a.splits > 1) {
+        const int64_t at = ((int64_t)split_no * items + item) * R + row;
+        store_own<C, FULL>(a.part + at * a.D, acc, 1.0f, 0.0f, a.D, h);
+        if (h == 0) {
+            a.part_stats[2 * at] = t0 < t1 ? m : -INFINITY;
+            a.part_stats[2 * at + 1] = l;
+        }
+        return;
+    }
+    store_own<C, FULL>(a.out + query_offset(a, b, kv, row, a.ld_out), acc,
+                       L > 0 ? 1.0f / l : 0.0f, 0.0f, a.D, h);
+    if (a.stats && h == 0) {
+        float* st = row_stats(a, b, kv, row);
+        st[0] = m;
+        st[1] = l;
+    }
+}
+
+// What the backward starts its products from: per row -log2 of its sum of
+// exponentials (-infinity where no key is live: no probability) and
+// -dout . out. 32 lanes to a row, four columns each.
+__global__ __launch_bounds__(256) void cross_rows_prepare_kernel(CrossArgs a) {
+    const int R = a.Sq * a.G, x = threadIdx.x % 32;
+    const int64_t at = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    if (at >= (int64_t)a.B * a.KV * R) return;
+    const int item = (int)(at / R), r = (int)(at - (int64_t)item * R);
+    const int b = item / a.KV, kv = item - b * a.KV;
+    const int64_t off = query_offset(a, b, kv, r, a.ld_out);
+    float dot = 0.0f;
+    for (int d = 4 * x; d < min(a.D, 4 * x + 4); ++d) dot = fmaf(a.dout[off + d], a.o[off + d], dot);
+#pragma unroll
+    for (int i = 1; i < 32; i *= 2) dot += __shfl_xor(dot, i, 64);
+    if (x == 0) {
+        const float* st = row_stats(a, b, kv, r);
+        a.neg_lse[at] = live_keys(a, b) > 0 ? -(st[0] + __builtin_amdgcn_logf(st[1])) : -INFINITY;
+        a.neg_delta[at] = -dot;
+    }
+}
+
+// dq of a workgroup's rows: P = 2^(k . q - lse), dS = P (v . dout - delta),
+// dQ = scale * K^T dS.
+template <int D, int WAVES, bool FULL>
+__device__ __forceinline__ void dq_walk(const CrossArgs& a, u32x4* lds, int block) {
+    using C = TileCfg<D, WAVES>;
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Sq * a.G, tiles = (R + 32 * WAVES - 1) / (32 * WAVES), items = a.B * a.KV;
+    const int tile = block % tiles, item = block / tiles % items, no = block / tiles / items;
+    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
+    const int row = (tile * WAVES + w) * 32 + c;
+    const bool wave_live = (tile * WAVES + w) * 32 < R, live = row < R;
+    int t0, t1;
+    share((L + C::KT - 1) / C::KT, no, a.q_splits, t0, t1);
+    Stage<C, FULL> k, v;
+    auto load = [&](int t) {
+        const int n = min(C::KT, L - t * C::KT);
+        k.template load<false>(a, a.k, a.ld_kv, b, kv, t * C::KT, n);
+        v.template load<false>(a, a.v, a.ld_kv, b, kv, t * C::KT, n);
+    };
+    if (t0 < t1) load(t0);
+    u32x4 qf[C::NS][3], gf[C::NS][3];
+    own_pieces<C, FULL>(qf, a, a.q + (live ? query_offset(a, b, kv, row, a.ld_q) : 0), live, h,
+                        a.scale2);
+    own_pieces<C, FULL>(gf, a, a.dout + (live ? query_offset(a, b, kv, row, a.ld_out) : 0), live, h,
+                        1.0f);
+    const float nl = live ? a.neg_lse[(int64_t)item * R + row] : -INFINITY;
+    const float nd = live ? a.neg_delta[(int64_t)item * R + row] : 0.0f;
+    f32x16 acc[C::NJ];
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) acc[j] = all16(0.0f);
+    if (t0 < t1) {
+        k.store(a, lds);
+        v.store(a, lds + C::SET);
+        if (t0 + 1 < t1) load(t0 + 1);
+        __syncthreads();
+    }
+    for (int t = t0; t < t1; ++t) {
+        u32x4* const kl = lds + ((t - t0) & 1) * 2 * C::SET;
+        if (wave_live) {
+            const int n = L - t * C::KT;
+#pragma unroll
+            for (int kb = 0; kb < C::NB; ++kb) {
+                f32x16 s = products<C>(kl, qf, kb, all16(nl), c, h);
+                const f32x16 dp = products<C>(kl + C::SET, gf, kb, all16(nd), c, h);
+                if (n < C::KT) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (kb * 32 + 8 * (i / 4) + 4 * h + i % 4 >= n) s[i] = -INFINITY;
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        x[i] = __builtin_amdgcn_exp2f(s[8 * u + i]) * dp[8 * u + i];
+                    u32x4 p[3];
+                    split8(x, p);
+                    add_transposed<C>(acc, kl, kb, u, p, lane);
+                }
+            }
+        }
+        if (t + 1 < t1) {
+            u32x4* const other = lds + ((t + 1 - t0) & 1) * 2 * C::SET;
+            k.store(a, other);
+            v.store(a, other + C::SET);
+            if (t + 2 < t1) load(t + 2);
+            __syncthreads();
+        }
+    }
+    if (!live) return;
+    if (a.q_splits > 1)
+        store_own<C, FULL>(a.dq_part + (((int64_t)no * items + item) * R + row) * a.D, acc, 1.0f,
+                           0.0f, a.D, h);
+    else
+        store_own<C, FULL>(a.dq + query_offset(a, b, kv, row, a.ld_q), acc, a.scale, a.beta_q, a.D,
+                           h);
+}
+
+// dk and dv of a workgroup's keys: the same P and dS with the rows met,
+// dV = dO^T P, dK = scale * Q^T dS.
+template <int D, int WAVES, bool FULL>
+__device__ __forceinline__ void dkv_walk(const CrossArgs& a, u32x4* lds, float* starts, int block) {
+    using C = TileCfg<D, WAVES>;
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Sq * a.G, tiles = (a.Sk + 32 * WAVES - 1) / (32 * WAVES), items = a.B * a.KV;
+    const int tile = block % tiles, item = block / tiles % items, no = block / tiles / items;
+    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
+    const int key = (tile * WAVES + w) * 32 + c;
+    const bool wave_live = (tile * WAVES + w) * 32 < L, live = key < L;
+    int t0, t1;
+    share((R + C::KT - 1) / C::KT, no, a.kv_splits, t0, t1);
+    if (tile * WAVES * 32 >= L) t1 = t0;  // no live key here
+    Stage<C, FULL> q, g;
+    float start[2];  // of threads below KT: -lse and -delta of a row of the tile
+    auto load = [&](int t) {
+        const int r0 = t * C::KT, n = min(C::KT, R - r0);
+        q.template load<true>(a, a.q, a.ld_q, b, kv, r0, n);
+        g.template load<true>(a, a.dout, a.ld_out, b, kv, r0, n);
+        start[0] = -INFINITY;
+        start[1] = 0.0f;
+        if ((int)threadIdx.x < n) {
+            start[0] = a.neg_lse[(int64_t)item * R + r0 + threadIdx.x];
+            start[1] = a.neg_delta[(int64_t)item * R + r0 + threadIdx.x];
+        }
+    };
+    auto store = [&](int buf) {
+        q.store(a, lds + buf * 2 * C::SET);
+        g.store(a, lds + buf * 2 * C::SET + C::SET);
+        if ((int)threadIdx.x < C::KT) {
+            starts[buf * 2 * C::KT + threadIdx.x] = start[0];
+            starts[buf * 2 * C::KT + C::KT + threadIdx.x] = start[1];
+        }
+    };
+    if (t0 < t1) load(t0);
+    u32x4 kf[C::NS][3], vf[C::NS][3];
+    own_pieces<C, FULL>(kf, a, a.k + (live ? key_offset(a, b, kv, key) : 0), live, h, a.scale2);
+    own_pieces<C, FULL>(vf, a, a.v + (live ? key_offset(a, b, kv, key) : 0), live, h, 1.0f);
+    f32x16 acc_k[C::NJ], acc_v[C::NJ];
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) acc_k[j] = acc_v[j] = all16(0.0f);
+    if (t0 < t1) {
+        store(0);
+        if (t0 + 1 < t1) load(t0 + 1);
+        __syncthreads();
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        u32x4* const ql = lds + buf * 2 * C::SET;
+        if (wave_live) {
+#pragma unroll
+            for (int rb = 0; rb < C::NB; ++rb) {
+                f32x16 s, dp;  // start at -lse and -delta of the 16 rows
+                const float* const st = starts + buf * 2 * C::KT + rb * 32 + 4 * h;
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[i + e] = st[2 * i + e];
+                        dp[i + e] = st[C::KT + 2 * i + e];
+                    }
+                s = products<C>(ql, kf, rb, s, c, h);
+                dp = products<C>(ql + C::SET, vf, rb, dp, c, h);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    float x[8], y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = __builtin_amdgcn_exp2f(s[8 * u + i]);
+                        y[i] = x[i] * dp[8 * u + i];
+                    }
+                    u32x4 p[3];
+                    split8(x, p);
+                    add_transposed<C>(acc_v, ql + C::SET, rb, u, p, lane);
+                    split8(y, p);
+                    add_transposed<C>(acc_k, ql, rb, u, p, lane);
+                }
+            }
+        }
+        if (t + 1 < t1) {
+            store(buf ^ 1);
+            if (t + 2 < t1) load(t + 2);
+            __syncthreads();
+        }
+    }
+    if (key >= a.Sk) return;
+    if (a.kv_splits > 1) {
+        if (!live) return;  // the sum takes dead keys as zeros
+        const int64_t at = (((int64_t)no * items + item) * a.Sk + key) * a.D;
+        store_own<C, FULL>(a.dk_part + at, acc_k, 1.0f, 0.0f, a.D, h);
+        store_own<C, FULL>(a.dv_part + at, acc_v, 1.0f, 0.0f, a.D, h);
+        return;
+    }
+    if (!live) {
+        if (a.beta_kv == 1.0f) return;
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j) acc_k[j] = acc_v[j] = all16(0.0f);
+    }
+    const int64_t at = key_offset(a, b, kv, key);
+    store_own<C, FULL>(a.dk + at, acc_k, a.scale, a.beta_kv, a.D, h);
+    store_own<C, FULL>(a.dv + at, acc_v, 1.0f, a.beta_kv, a.D, h);
+}
+
+// One launch for both: they need nothing of each other, and the workgroups of
+// one fill the compute units that the other leaves idle.
+template <int D, int WAVES, bool FULL>
+__global__ __launch_bounds__(64 * WAVES) void cross_tile_bwd_kernel(CrossArgs a) {
+    using C = TileCfg<D, WAVES>;
+    __shared__ u32x4 lds[4 * C::SET];
+    __shared__ float starts[4 * C::KT];
+    if ((int)blockIdx.x < a.q_blocks)
+        dq_walk<D, WAVES, FULL>(a, lds, blockIdx.x);
+    else
+        dkv_walk<D, WAVES, FULL>(a, lds, starts, blockIdx.x - a.q_blocks);
+}
+
+template <int D>
+void launch_forward(const CrossArgs& a) {
+    const int R = a.Sq * a.G, rows = cross_forward_rows(R, D);
+    const unsigned grid = (unsigned)(((R + rows - 1) / rows) * (int64_t)a.B * a.KV * a.splits);
+    const bool full = a.D == D;
+    auto kernel = rows == 256
+                      ? (full ? cross_tile_fwd_kernel<D, 8, true> : cross_tile_fwd_kernel<D, 8, false>)
+                      : (full ? cross_tile_fwd_kernel<D, 4, true> : cross_tile_fwd_kernel<D, 4, false>);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(2 * rows), 0, stream(), a);
+}
+
+template <int D, int WAVES>
+void launch_backward(const CrossArgs& a, unsigned grid) {
+    auto kernel = a.D == D ? cross_tile_bwd_kernel<D, WAVES, true> : cross_tile_bwd_kernel<D, WAVES, false>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * WAVES), 0, stream(), a);
+}
+
+}  // namespace
+
+int cross_forward_rows(int R, int) { return R > 128 ? 256 : 128; }
+
+// Wide heads' operands fill the registers of one wave to a SIMD.
+int cross_backward_rows(int R, int Sk, int D) { return D <= 64 && std::max(R, Sk) > 128 ? 256 : 128; }
+
+void cross_tile_forward(const CrossArgs& a) {
+    if (a.D <= 32)
+        launch_forward<32>(a);
+    else if (a.D <= 64)
+        launch_forward<64>(a);
+    else
+        launch_forward<128>(a);
+}
+
+void cross_tile_backward(const CrossArgs& a) {
+    const int R = a.Sq * a.G, rows = cross_backward_rows(R, a.Sk, a.D);
+    const int64_t items = (int64_t)a.B * a.KV;
+    if (R > 0) {
+        const int64_t n = items * R;
+        hipLaunchKernelGGL(cross_rows_prepare_kernel, dim3((unsigned)((n + 7) / 8)), dim3(256), 0,
+                           stream(), a);
+    }
+    const unsigned grid =
+        (unsigned)(a.q_blocks + (a.dk ? (a.Sk + rows - 1) / rows * items * a.kv_splits : 0));
+    if (grid == 0) return;
+    if (a.D <= 32)
+        rows == 256 ? launch_backward<32, 8>(a, grid) : launch_backward<32, 4>(a, grid);
+    else if (a.D <= 64)
+        rows == 256 ? launch_backward<64, 8>(a, grid) : launch_backward<64, 4>(a, grid);
+    else
+        launch_backward<128, 4>(a, grid);
+}
+
+}  // namespace nrs

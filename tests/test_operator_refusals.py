@@ -24,8 +24,9 @@ BAD = [
     (dict(d_head=0), "d_head"), (dict(d_head=129, ld_q=1024, ld_kv=1024, ld_out=1024), "d_head"),
     (dict(ld_q=127), "stride"), (dict(ld_kv=63), "stride"), (dict(ld_out=100), "stride"),
     (dict(ld_q=2 ** 20 + 1), "2\\^20"), (dict(ld_kv=2 ** 33), "2\\^20"), (dict(seq_k=2 ** 40), "2\\^26"),
-    (dict(seq_q=2 ** 27), "2\\^26"), (dict(batch=2 ** 40), "too many"),
-    (dict(batch=2 ** 20, seq_q=2 ** 20), "too many"),
+    (dict(seq_q=2 ** 27), "2\\^26"), (dict(batch=2 ** 40), "2\\^26"),
+    (dict(batch=2 ** 20, seq_q=2 ** 20), "2\\^26"), (dict(batch=2 ** 12, seq_k=2 ** 16), "2\\^26"),
+    (dict(seq_q=2 ** 26, heads=2 ** 14, kv_heads=1, ld_q=2 ** 19, ld_out=2 ** 19), "2\\^26"),
     (dict(heads=2 ** 62, kv_heads=1), "stride"),
 ]
 
@@ -116,6 +117,15 @@ def test_dropout_sizes_and_nulls():
             _abi.dropout_forward(*args, None, 8, 0.5, 1, 1)
         with pytest.raises(_abi.NrsError, match="null pointer"):
             _abi.dropout_backward(*args, 8, 0.5, 1, 1)
+
+
+def test_workspace_of_a_backward_without_keys_or_rows():
+    """The rows' statistics are written even where there is nothing to attend
+    to: two floats a row, in whole 16 bytes."""
+    assert _abi.cross_attention_workspace(2, 4, 2, 3, 0, 32, backward=True) >= 2 * 4 * 3 * 8
+    assert _abi.cross_attention_workspace(2, 4, 2, 0, 5, 32, backward=True) == 0
+    assert _abi.cross_attention_workspace(2, 4, 2, 0, 5, 32) == 0
+    assert _abi.cross_attention_workspace(0, 4, 2, 3, 5, 32) == 0
 
 
 def test_workspace_queries():
