@@ -4,8 +4,19 @@
 //   dtable[t] = scale * sum over ids[i] = t of grad[i] + beta * dtable[t]
 //                                              outside the table, no gradient)
 //
-// The gradient adds a token's rows in the order of their positions, by no
-// atomics: the same call gives the same bits.
+// The gradient takes three launches:
+//  1. sort: every workgroup owns a range of tokens, looks through all ids twice
+//     (they stay in the caches) and places its own tokens' positions, in order,
+//     behind those of lower tokens: a counting sort without a pass between
+//     workgroups. It also writes the rows of its tokens that do not occur, so
+//     the stores of a large table run beside the sort.
+//  2. sum: the sorted positions are cut into tiles of equal length, so that a
+//     token that holds a sixth of all places (a space, say) is as even as any.
+//     A wave adds a tile's rows, 256 columns of them, and writes the sums of
+//     the tokens that begin and end in it; the sum of a run that crosses the
+//     tile's beginning or end goes to scratch.
+//  3. join: adds the parts of every run that crosses tiles, in order.
+// No floating-point atomics: the order of a sum depends on the ids alone.
 #include <algorithm>
 
 #include "nrs_internal.hpp"
@@ -45,39 +56,257 @@ __global__ __launch_bounds__(kThreads) void embedding_forward_kernel(
     }
 }
 
-// One wave per table row and 256 columns: it looks through all ids and adds
-// the rows that are its token's.
-__global__ __launch_bounds__(64) void embedding_backward_kernel(
-    float* dtable, const float* grad, const int32_t* ids, int64_t count, int vocab, int dim,
-    float scale, float beta) {
-    const int t = blockIdx.x, d = blockIdx.y * 256 + threadIdx.x * 4;
-    const int live = max(0, min(4, dim - d));
-    float sum[4] = {};
-    bool any = false;
-    for (int64_t i0 = 0; i0 < count; i0 += 64) {
-        const int64_t i = i0 + threadIdx.x;
-        uint64_t hits = __ballot(i < count && ids[i] == t);
-        any |= hits != 0;
-        while (hits) {
-            const int64_t row = i0 + __builtin_ctzll(hits);
-            hits &= hits - 1;
-            for (int e = 0; e < live; ++e) sum[e] += grad[row * dim + d + e];
+constexpr int kSortWaves = 16, kSortThreads = 64 * kSortWaves;
+constexpr int kMaxBins = 1024;  // tokens of a sorting workgroup
+constexpr int kBatch = 8;       // rows a wave has in flight
+
+struct BackwardArgs {
+    float* dtable;
+    const float* grad;
+    const int32_t* ids;
+    int count, vocab, dim, bins, tile;
+    float scale, beta;
+    int32_t* sorted;  // [count] positions by token, then by position
+    int32_t* start;   // [vocab + 1] where each token's begin
+    float* part;      // [tiles][2][dim] sums of runs from before, and into after, a tile
+};
+
+struct __attribute__((packed, aligned(4))) IdQuad {
+    int32_t v[4];
+};
+
+__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(BackwardArgs a) {
+    __shared__ int hist[kSortWaves][kMaxBins];
+    __shared__ int totals[kMaxBins];
+    __shared__ int below[kSortWaves];
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lo = blockIdx.x * a.bins, bins = min(a.bins, a.vocab - lo);
+    // the wave's part of the ids
+    const int per = ((a.count + kSortWaves - 1) / kSortWaves + 255) & ~255;
+    const int i0 = (int)min((int64_t)a.count, (int64_t)w * per), i1 = (int)min((int64_t)a.count, (int64_t)i0 + per);
+    for (int i = threadIdx.x; i < kSortWaves * a.bins; i += kSortThreads)
+        hist[i / a.bins][i % a.bins] = 0;
+    __syncthreads();
+    int less = 0;  // this lane's ids of lower tokens
+    for (int i = i0 + 4 * lane; i < i1; i += 256) {
+        int id[4];
+        if (i + 4 <= i1) {
+            const IdQuad v = *reinterpret_cast<const IdQuad*>(a.ids + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) id[e] = v.v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) id[e] = i + e < i1 ? a.ids[i + e] : -1;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            less += (uint32_t)id[e] < (uint32_t)lo;
+            const uint32_t bin = (uint32_t)id[e] - (uint32_t)lo;
+            if (bin < (uint32_t)bins) atomicAdd(&hist[w][bin], 1);  // whole numbers: any order
         }
     }
-    float* dst = dtable + (int64_t)t * dim + d;
-    for (int e = 0; e < live; ++e) {
-        if (beta == 0.0f)
-            dst[e] = scale * sum[e];
-        else if (any || beta != 1.0f)
-            dst[e] = scale * sum[e] + beta * dst[e];
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) less += __shfl_xor(less, d, 64);
+    if (lane == 0) below[w] = less;
+    __syncthreads();
+    // a bin's total, then where each wave's places of each bin begin
+    const int t = threadIdx.x;
+    int total = 0;
+    if (t < bins)
+#pragma unroll
+        for (int i = 0; i < kSortWaves; ++i) total += hist[i][t];
+    int upto = total;  // inclusive over the bins of the wave
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int v = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += v;
+    }
+    if (t < kMaxBins) totals[t] = total;
+    __shared__ int wave_sum[kSortWaves];
+    if (lane == 63) wave_sum[w] = upto;
+    __syncthreads();
+    int at = upto - total;
+    for (int i = 0; i < kSortWaves; ++i) at += below[i] + (i < w ? wave_sum[i] : 0);
+    if (t < bins) {
+        a.start[lo + t] = at;
+#pragma unroll
+        for (int i = 0; i < kSortWaves; ++i) {
+            const int n = hist[i][t];
+            hist[i][t] = at;
+            at += n;
+        }
+        if (lo + t == a.vocab - 1) a.start[a.vocab] = at;
+    }
+    __syncthreads();
+    // the rows of absent tokens
+    if (a.beta != 1.0f) {
+        for (int bin = w; bin < bins; bin += kSortWaves) {
+            if (totals[bin] != 0) continue;
+            float* const row = a.dtable + (int64_t)(lo + bin) * a.dim;
+            for (int d = 4 * lane; d < a.dim; d += 256) {
+                if (d + 4 <= a.dim) {
+                    Quad* const to = reinterpret_cast<Quad*>(row + d);
+                    to->v = a.beta != 0.0f ? a.beta * to->v : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                } else {
+                    for (int e = d; e < a.dim; ++e) row[e] = a.beta != 0.0f ? a.beta * row[e] : 0.0f;
+                }
+            }
+        }
+    }
+    // place the positions: 64 ids at a time, in order. Only this wave uses its
+    // row of `hist` now; one lane writes what all read in the next turn.
+    volatile int* const places = hist[w];
+    for (int base = i0; base < i1; base += 256) {
+        int id[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = base + 64 * e + lane;
+            id[e] = i < i1 ? a.ids[i] : -1;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t bin = (uint32_t)id[e] - (uint32_t)lo;
+            uint64_t mine = __ballot(bin < (uint32_t)bins);
+            while (mine) {
+                const uint32_t one = __builtin_amdgcn_readlane(bin, __builtin_ctzll(mine));
+                const uint64_t same = __ballot(bin == one);
+                const int first = places[one];
+                if (bin == one)
+                    a.sorted[first + __popcll(same & ((1ull << lane) - 1))] = base + 64 * e + lane;
+                if (lane == 0) places[one] = first + __popcll(same);
+                mine &= ~same;
+            }
+        }
     }
 }
 
+// One wave per tile of sorted positions and 256 columns.
+__global__ __launch_bounds__(64) void embedding_sum_kernel(BackwardArgs a) {
+    const int lane = threadIdx.x, d = blockIdx.y * 256 + 4 * lane;
+    const int total = a.start[a.vocab];
+    const int64_t e0 = (int64_t)blockIdx.x * a.tile;
+    if (e0 >= total) return;
+    const int e1 = (int)min((int64_t)total, e0 + a.tile);
+    const bool whole = d + 4 <= a.dim;
+    const int live = max(0, min(4, a.dim - d));
+    f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c0 = (int)e0; c0 < e1; c0 += 64) {
+        // lane j looks up entry c0 + j: its position, its token and that one's run
+        const int n = min(64, e1 - c0);
+        int pos = 0, token = 0, begin = 0, end = 0;
+        if (lane < n) {
+            pos = a.sorted[c0 + lane];
+            token = a.ids[pos];
+            begin = a.start[token];
+            end = a.start[token + 1];
+        }
+        const uint64_t ends = __ballot(lane < n && (c0 + lane + 1 == end || c0 + lane + 1 == e1));
+        for (int i0 = 0; i0 < n; i0 += kBatch) {
+            f32x4 rows[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                rows[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (i0 + i < n) {
+                    const float* src =
+                        a.grad + (int64_t)__builtin_amdgcn_readlane(pos, i0 + i) * a.dim + d;
+                    if (whole)
+                        rows[i] = reinterpret_cast<const Quad*>(src)->v;
+                    else
+                        for (int k = 0; k < live; ++k) rows[i][k] = src[k];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                sum = sum + rows[i];
+                if (i0 + i >= n || !((ends >> (i0 + i)) & 1)) continue;
+                // the end of a run, or of the tile
+                const int e = c0 + i0 + i + 1, t = __builtin_amdgcn_readlane(token, i0 + i);
+                const bool head = __builtin_amdgcn_readlane(begin, i0 + i) < e0,
+                           tail = __builtin_amdgcn_readlane(end, i0 + i) > e;
+                const bool inside = !head && !tail;
+                float* dst = inside ? a.dtable + (int64_t)t * a.dim + d
+                                    : a.part + ((int64_t)blockIdx.x * 2 + (head ? 0 : 1)) * a.dim + d;
+                f32x4 v = sum;
+                sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (inside) v = v * a.scale;
+                const bool add = inside && a.beta != 0.0f;
+                if (whole) {
+                    Quad* const to = reinterpret_cast<Quad*>(dst);
+                    if (add) v = v + a.beta * to->v;
+                    to->v = v;
+                } else {
+                    for (int k = 0; k < live; ++k) dst[k] = add ? v[k] + a.beta * dst[k] : v[k];
+                }
+            }
+        }
+    }
+}
+
+// One wave per tile and 256 columns: the run that begins in the tile and goes
+// on past it, if there is one.
+__global__ __launch_bounds__(64) void embedding_join_kernel(BackwardArgs a) {
+    const int total = a.start[a.vocab];
+    const int64_t e0 = (int64_t)blockIdx.x * a.tile;
+    const int64_t e1 = e0 + a.tile;
+    if (e1 >= total) return;  // the last tile's runs end in it
+    const int token = a.ids[a.sorted[e1 - 1]];
+    const int begin = a.start[token], end = a.start[token + 1];
+    if (begin < e0 || end <= e1) return;
+    const int d = blockIdx.y * 256 + 4 * threadIdx.x, live = max(0, min(4, a.dim - d));
+    if (live == 0) return;
+    const int last = (int)((end - 1) / a.tile);
+    float sum[4] = {};
+    const float* src = a.part + ((int64_t)blockIdx.x * 2 + 1) * a.dim + d;
+    for (int e = 0; e < live; ++e) sum[e] = src[e];
+    src = a.part + (int64_t)(blockIdx.x + 1) * 2 * a.dim + d;
+    const int n = last - (int)blockIdx.x;
+    for (int i = 0; i < n; i += kBatch) {
+        float rows[kBatch][4];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                rows[k][e] = i + k < n && e < live ? src[(int64_t)(i + k) * 2 * a.dim + e] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] += rows[k][e];
+    }
+    float* dst = a.dtable + (int64_t)token * a.dim + d;
+    for (int e = 0; e < live; ++e)
+        dst[e] = a.beta != 0.0f ? a.scale * sum[e] + a.beta * dst[e] : a.scale * sum[e];
+}
+
+struct BackwardPlan {
+    int bins, tile;
+    int64_t groups, tiles;
+    size_t sorted, start, part;  // scratch, in 4-byte words
+    size_t bytes() const { return 4 * (sorted + start + part); }
+};
+
+BackwardPlan plan_backward(int64_t count, int64_t vocab, int64_t dim) {
+    BackwardPlan p;
+    const int64_t cus = num_cus();
+    p.bins = (int)std::min<int64_t>(kMaxBins, (vocab + cus - 1) / cus);
+    p.groups = (vocab + p.bins - 1) / p.bins;
+    // about four waves to a compute unit, a column block each; tiles of at least 16
+    const int64_t blocks = (dim + 255) / 256;
+    const int64_t even = count * blocks / (4 * cus);
+    p.tile = (int)std::max<int64_t>(16, std::min<int64_t>(256, (even + 15) / 16 * 16));
+    p.tiles = (count + p.tile - 1) / p.tile;
+    auto round4 = [](int64_t n) { return (size_t)((n + 3) / 4 * 4); };
+    p.sorted = round4(count);
+    p.start = round4(vocab + 1);
+    p.part = round4(p.tiles * 2 * dim);
+    return p;
+}
+
 int check_shape(const char* what, int64_t count, int64_t vocab, int64_t dim) {
-    NRS_ARG_CHECK(count >= 0 && count < INT32_MAX && vocab >= 1 && vocab < INT32_MAX && dim >= 1 &&
-                      dim <= (1 << 20),
-                  "%s: unsupported sizes (count %lld, vocab %lld, dim %lld): count and vocab are "
-                  "below 2^31 - 1, vocab and dim at least 1, dim at most 2^20",
+    NRS_ARG_CHECK(count >= 0 && count <= (1 << 30) && vocab >= 1 && vocab < INT32_MAX &&
+                      dim >= 1 && dim <= (1 << 20),
+                  "%s: unsupported sizes (count %lld, vocab %lld, dim %lld): count is at most 2^30, "
+                  "vocab below 2^31 - 1, dim at most 2^20, vocab and dim at least 1",
                   what, (long long)count, (long long)vocab, (long long)dim);
     return NRS_OK;
 }
@@ -108,7 +337,7 @@ int nrs_embedding_forward(float* out, const float* table, const int32_t* ids, in
 int nrs_embedding_workspace(size_t* bytes, int64_t count, int64_t vocab, int64_t dim) {
     NRS_ARG_CHECK(bytes, "embedding workspace: null pointer");
     if (int rc = nrs::check_shape("embedding workspace", count, vocab, dim)) return rc;
-    *bytes = 0;
+    *bytes = nrs::plan_backward(count, vocab, dim).bytes();
     return NRS_OK;
 }
 
@@ -119,11 +348,31 @@ int nrs_embedding_backward(float* dtable, const float* grad, const int32_t* ids,
     NRS_ARG_CHECK(dtable && ((grad && ids) || count == 0), "embedding backward: null pointer");
     NRS_REQUIRE_INIT();
     if (int rc = nrs::check_device("embedding backward")) return rc;
+    const auto plan = nrs::plan_backward(count, vocab, dim);
     float* scratch = nullptr;
-    if (int rc = nrs::call_scratch(&scratch, 0, work, work_bytes, "embedding backward")) return rc;
-    const dim3 grid((unsigned)vocab, (unsigned)((dim + 255) / 256));
-    hipLaunchKernelGGL(nrs::embedding_backward_kernel, grid, dim3(64), 0, nrs::stream(), dtable,
-                       grad, ids, count, (int)vocab, (int)dim, scale, beta);
+    if (int rc = nrs::call_scratch(&scratch, plan.bytes(), work, work_bytes, "embedding backward"))
+        return rc;
+    nrs::BackwardArgs a{};
+    a.dtable = dtable;
+    a.grad = grad;
+    a.ids = ids;
+    a.count = (int)count;
+    a.vocab = (int)vocab;
+    a.dim = (int)dim;
+    a.bins = plan.bins;
+    a.tile = plan.tile;
+    a.scale = scale;
+    a.beta = beta;
+    a.sorted = reinterpret_cast<int32_t*>(scratch);
+    a.start = a.sorted + plan.sorted;
+    a.part = scratch + plan.sorted + plan.start;
+    hipLaunchKernelGGL(nrs::embedding_sort_kernel, dim3((unsigned)plan.groups),
+                       dim3(nrs::kSortThreads), 0, nrs::stream(), a);
+    if (count > 0) {
+        const dim3 grid((unsigned)plan.tiles, (unsigned)((dim + 255) / 256));
+        hipLaunchKernelGGL(nrs::embedding_sum_kernel, grid, dim3(64), 0, nrs::stream(), a);
+        hipLaunchKernelGGL(nrs::embedding_join_kernel, grid, dim3(64), 0, nrs::stream(), a);
+    }
     NRS_LAUNCH_CHECK("embedding backward");
     return NRS_OK;
 }
