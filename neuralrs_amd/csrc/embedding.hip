@@ -8,8 +8,7 @@
 //  1. sort: every workgroup owns a range of tokens, looks through all ids twice
 //     (they stay in the caches) and places its own tokens' positions, in order,
 //     behind those of lower tokens: a counting sort without a pass between
-//     workgroups. It also writes the rows of its tokens that do not occur, so
-//     the stores of a large table run beside the sort.
+//     workgroups. Beside it, with beta 0, other workgroups clear the table.
 //  2. sum: the sorted positions are cut into tiles of equal length, so that a
 //     token that holds a sixth of all places (a space, say) is as even as any.
 //     A wave adds a tile's rows, 256 columns of them, and writes the sums of
@@ -19,38 +18,55 @@
 // No floating-point atomics: the order of a sum depends on the ids alone.
 #include <algorithm>
 
-#include "nrs_internal.hpp"
+#include "buffer_ops.hpp"
 
 namespace nrs {
 namespace {
 
 // Rows need not be 16-byte aligned: gfx950 loads 128 bits from any dword.
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 struct __attribute__((packed, aligned(4))) Quad {
     f32x4 v;
 };
 
 constexpr int kThreads = 256;
+constexpr int kRows = 4;  // rows a thread of the lookup has in flight
 
 // `lanes` threads (a power of two) share a row, four columns each at a time;
-// a row's last columns go one by one when dim is no multiple of four.
+// a row's last columns go one by one when dim is no multiple of four. The
+// rows' tokens, then the rows, are asked for together: a row by itself waits
+// for two loads, one after the other.
 __global__ __launch_bounds__(kThreads) void embedding_forward_kernel(
     float* out, const float* table, const int32_t* ids, int64_t count, int vocab, int dim,
     int lanes, float scale) {
     const int rows = kThreads / lanes, r = threadIdx.x / lanes, c = threadIdx.x % lanes;
     const int64_t stride = (int64_t)gridDim.x * rows;
-    for (int64_t i = (int64_t)blockIdx.x * rows + r; i < count; i += stride) {
-        const int id = ids[i];
-        const bool live = (uint32_t)id < (uint32_t)vocab;
-        const float* src = table + (int64_t)(live ? id : 0) * dim;
-        float* dst = out + i * dim;
+    for (int64_t i0 = (int64_t)blockIdx.x * rows + r; i0 < count; i0 += kRows * stride) {
+        int id[kRows];
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) id[k] = i0 + k * stride < count ? ids[i0 + k * stride] : -1;
         for (int d = 4 * c; d < dim; d += 4 * lanes) {
-            if (d + 4 <= dim) {
-                f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (live) v = reinterpret_cast<const Quad*>(src + d)->v * scale;
-                reinterpret_cast<Quad*>(dst + d)->v = v;
-            } else {
-                for (int e = d; e < dim; ++e) dst[e] = live ? src[e] * scale : 0.0f;
+            const int live = min(4, dim - d);
+            f32x4 v[kRows];
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) {
+                v[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if ((uint32_t)id[k] >= (uint32_t)vocab) continue;
+                const float* src = table + (int64_t)id[k] * dim + d;
+                if (live == 4)
+                    v[k] = reinterpret_cast<const Quad*>(src)->v;
+                else
+                    for (int e = 0; e < live; ++e) v[k][e] = src[e];
+            }
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) {
+                const int64_t i = i0 + k * stride;
+                if (i >= count) break;
+                const f32x4 x = (uint32_t)id[k] < (uint32_t)vocab ? v[k] * scale : v[k];
+                float* dst = out + i * dim + d;
+                if (live == 4)
+                    reinterpret_cast<Quad*>(dst)->v = x;
+                else
+                    for (int e = 0; e < live; ++e) dst[e] = x[e];
             }
         }
     }
@@ -58,22 +74,45 @@ __global__ __launch_bounds__(kThreads) void embedding_forward_kernel(
 
 constexpr int kSortWaves = 16, kSortThreads = 64 * kSortWaves;
 constexpr int kMaxBins = 1024;  // tokens of a sorting workgroup
+constexpr int kIds = 16;        // ids a lane has in flight
 constexpr int kBatch = 8;       // rows a wave has in flight
 
 struct BackwardArgs {
     float* dtable;
     const float* grad;
     const int32_t* ids;
-    int count, vocab, dim, bins, tile;
+    int count, vocab, dim, bins, tile, blocks;  // blocks: of 256 columns
+    int groups;  // sorting workgroups; any after them clear the table
     float scale, beta;
     int32_t* sorted;  // [count] positions by token, then by position
     int32_t* start;   // [vocab + 1] where each token's begin
     float* part;      // [tiles][2][dim] sums of runs from before, and into after, a tile
 };
 
-struct __attribute__((packed, aligned(4))) IdQuad {
-    int32_t v[4];
-};
+// Zeros over workgroup `no` of `shares`' part of the table.
+__device__ __forceinline__ void clear_table(const BackwardArgs& a, int no, int shares) {
+    const int64_t n = (int64_t)a.vocab * a.dim, quads = n / 4;
+    Quad* const to = reinterpret_cast<Quad*>(a.dtable);
+    for (int64_t i = (int64_t)no * kSortThreads + threadIdx.x; i < quads;
+         i += (int64_t)shares * kSortThreads)
+        to[i].v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (no == 0 && threadIdx.x < n - 4 * quads) a.dtable[4 * quads + threadIdx.x] = 0.0f;
+}
+
+// Ids base + 64 e + lane, -1 past the end: all asked for before any is used.
+__device__ __forceinline__ void load_ids(int (&id)[kIds], const int32_t* ids, int base, int end,
+                                         int lane) {
+    const int n = min(64 * kIds, end - base);
+    const auto rs = buffer_rsrc(reinterpret_cast<const float*>(ids) + base, 4 * n);
+#pragma unroll
+    for (int e = 0; e < kIds; ++e)
+        id[e] = __builtin_bit_cast(int, buffer_load1(rs, 4 * lane + 256 * e));
+    if (n < 64 * kIds) {
+#pragma unroll
+        for (int e = 0; e < kIds; ++e)
+            if (64 * e + lane >= n) id[e] = -1;
+    }
+}
 
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(BackwardArgs a) {
     __shared__ int hist[kSortWaves][kMaxBins];
@@ -81,29 +120,28 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(BackwardAr
     __shared__ int below[kSortWaves];
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if ((int)blockIdx.x >= a.groups) {
+        clear_table(a, blockIdx.x - a.groups, gridDim.x - a.groups);
+        return;
+    }
     const int lo = blockIdx.x * a.bins, bins = min(a.bins, a.vocab - lo);
     // the wave's part of the ids
-    const int per = ((a.count + kSortWaves - 1) / kSortWaves + 255) & ~255;
+    const int per = ((a.count + kSortWaves - 1) / kSortWaves + 63) & ~63;
     const int i0 = (int)min((int64_t)a.count, (int64_t)w * per), i1 = (int)min((int64_t)a.count, (int64_t)i0 + per);
     for (int i = threadIdx.x; i < kSortWaves * a.bins; i += kSortThreads)
         hist[i / a.bins][i % a.bins] = 0;
     __syncthreads();
     int less = 0;  // this lane's ids of lower tokens
-    for (int i = i0 + 4 * lane; i < i1; i += 256) {
-        int id[4];
-        if (i + 4 <= i1) {
-            const IdQuad v = *reinterpret_cast<const IdQuad*>(a.ids + i);
+    for (int base = i0; base < i1; base += 64 * kIds) {
+        int id[kIds];
+        load_ids(id, a.ids, base, i1, lane);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) id[e] = v.v[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) id[e] = i + e < i1 ? a.ids[i + e] : -1;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < kIds; ++e) {
             less += (uint32_t)id[e] < (uint32_t)lo;
             const uint32_t bin = (uint32_t)id[e] - (uint32_t)lo;
-            if (bin < (uint32_t)bins) atomicAdd(&hist[w][bin], 1);  // whole numbers: any order
+            // (whole numbers: the order does not matter)
+            if (__ballot(bin < (uint32_t)bins) != 0 && bin < (uint32_t)bins)
+                atomicAdd(&hist[w][bin], 1);
         }
     }
 #pragma unroll
@@ -139,53 +177,59 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(BackwardAr
         if (lo + t == a.vocab - 1) a.start[a.vocab] = at;
     }
     __syncthreads();
-    // the rows of absent tokens
-    if (a.beta != 1.0f) {
+    // the rows of absent tokens (beta 0: cleared by other workgroups)
+    if (a.beta != 1.0f && a.beta != 0.0f) {
         for (int bin = w; bin < bins; bin += kSortWaves) {
             if (totals[bin] != 0) continue;
             float* const row = a.dtable + (int64_t)(lo + bin) * a.dim;
             for (int d = 4 * lane; d < a.dim; d += 256) {
                 if (d + 4 <= a.dim) {
                     Quad* const to = reinterpret_cast<Quad*>(row + d);
-                    to->v = a.beta != 0.0f ? a.beta * to->v : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    to->v = a.beta * to->v;
                 } else {
-                    for (int e = d; e < a.dim; ++e) row[e] = a.beta != 0.0f ? a.beta * row[e] : 0.0f;
+                    for (int e = d; e < a.dim; ++e) row[e] = a.beta * row[e];
                 }
             }
         }
     }
     // place the positions: 64 ids at a time, in order. Only this wave uses its
-    // row of `hist` now; one lane writes what all read in the next turn.
+    // row of `hist` now. Up to 64 bins stay in registers, bin b's next place in
+    // lane b (a turn through LDS takes 250 cycles, and few bins mean that most
+    // steps hold some of them); past that one lane writes what all read in the
+    // next turn.
     volatile int* const places = hist[w];
-    for (int base = i0; base < i1; base += 256) {
-        int id[4];
+    const bool few = bins <= 64;
+    int place = lane < bins ? hist[w][lane] : 0;
+    for (int base = i0; base < i1; base += 64 * kIds) {
+        int id[kIds];
+        load_ids(id, a.ids, base, i1, lane);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = base + 64 * e + lane;
-            id[e] = i < i1 ? a.ids[i] : -1;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < kIds; ++e) {
             const uint32_t bin = (uint32_t)id[e] - (uint32_t)lo;
             uint64_t mine = __ballot(bin < (uint32_t)bins);
             while (mine) {
                 const uint32_t one = __builtin_amdgcn_readlane(bin, __builtin_ctzll(mine));
                 const uint64_t same = __ballot(bin == one);
-                const int first = places[one];
+                const int first = few ? __builtin_amdgcn_readlane(place, one) : places[one];
                 if (bin == one)
                     a.sorted[first + __popcll(same & ((1ull << lane) - 1))] = base + 64 * e + lane;
-                if (lane == 0) places[one] = first + __popcll(same);
+                if (few)
+                    place += lane == (int)one ? __popcll(same) : 0;
+                else if (lane == 0)
+                    places[one] = first + __popcll(same);
                 mine &= ~same;
             }
         }
     }
 }
 
-// One wave per tile of sorted positions and 256 columns.
+// One wave per tile of sorted positions and 256 columns, a row's columns one
+// after the other: their loads come to a page of memory together.
 __global__ __launch_bounds__(64) void embedding_sum_kernel(BackwardArgs a) {
-    const int lane = threadIdx.x, d = blockIdx.y * 256 + 4 * lane;
+    const int lane = threadIdx.x, tile = blockIdx.x / a.blocks;
+    const int d0 = (blockIdx.x - tile * a.blocks) * 256, d = d0 + 4 * lane;
     const int total = a.start[a.vocab];
-    const int64_t e0 = (int64_t)blockIdx.x * a.tile;
+    const int64_t e0 = (int64_t)tile * a.tile;
     if (e0 >= total) return;
     const int e1 = (int)min((int64_t)total, e0 + a.tile);
     const bool whole = d + 4 <= a.dim;
@@ -206,15 +250,11 @@ __global__ __launch_bounds__(64) void embedding_sum_kernel(BackwardArgs a) {
             f32x4 rows[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                rows[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                if (i0 + i < n) {
-                    const float* src =
-                        a.grad + (int64_t)__builtin_amdgcn_readlane(pos, i0 + i) * a.dim + d;
-                    if (whole)
-                        rows[i] = reinterpret_cast<const Quad*>(src)->v;
-                    else
-                        for (int k = 0; k < live; ++k) rows[i][k] = src[k];
-                }
+                // past the row, and past the chunk, a load gives zeros
+                const int64_t row = __builtin_amdgcn_readlane(pos, min(i0 + i, 63));
+                rows[i] = buffer_load4(buffer_rsrc(a.grad + row * a.dim + d0,
+                                                   i0 + i < n ? (int64_t)(a.dim - d0) * 4 : 0),
+                                       16 * lane);
             }
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
@@ -226,7 +266,7 @@ __global__ __launch_bounds__(64) void embedding_sum_kernel(BackwardArgs a) {
                            tail = __builtin_amdgcn_readlane(end, i0 + i) > e;
                 const bool inside = !head && !tail;
                 float* dst = inside ? a.dtable + (int64_t)t * a.dim + d
-                                    : a.part + ((int64_t)blockIdx.x * 2 + (head ? 0 : 1)) * a.dim + d;
+                                    : a.part + ((int64_t)tile * 2 + (head ? 0 : 1)) * a.dim + d;
                 f32x4 v = sum;
                 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 if (inside) v = v * a.scale;
@@ -243,36 +283,42 @@ __global__ __launch_bounds__(64) void embedding_sum_kernel(BackwardArgs a) {
     }
 }
 
-// One wave per tile and 256 columns: the run that begins in the tile and goes
-// on past it, if there is one.
-__global__ __launch_bounds__(64) void embedding_join_kernel(BackwardArgs a) {
+// One workgroup per tile and 256 columns: the run that begins in the tile and
+// goes on past it, if there is one. Its waves add a quarter of the run's parts
+// each, in order, and the quarters are added in order.
+__global__ __launch_bounds__(256) void embedding_join_kernel(BackwardArgs a) {
+    __shared__ f32x4 quarter[4][64];
     const int total = a.start[a.vocab];
-    const int64_t e0 = (int64_t)blockIdx.x * a.tile;
+    const int tile = blockIdx.x / a.blocks;
+    const int64_t e0 = (int64_t)tile * a.tile;
     const int64_t e1 = e0 + a.tile;
     if (e1 >= total) return;  // the last tile's runs end in it
     const int token = a.ids[a.sorted[e1 - 1]];
     const int begin = a.start[token], end = a.start[token + 1];
     if (begin < e0 || end <= e1) return;
-    const int d = blockIdx.y * 256 + 4 * threadIdx.x, live = max(0, min(4, a.dim - d));
-    if (live == 0) return;
-    const int last = (int)((end - 1) / a.tile);
-    float sum[4] = {};
-    const float* src = a.part + ((int64_t)blockIdx.x * 2 + 1) * a.dim + d;
-    for (int e = 0; e < live; ++e) sum[e] = src[e];
-    src = a.part + (int64_t)(blockIdx.x + 1) * 2 * a.dim + d;
-    const int n = last - (int)blockIdx.x;
-    for (int i = 0; i < n; i += kBatch) {
-        float rows[kBatch][4];
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int d0 = (blockIdx.x - tile * a.blocks) * 256, d = d0 + 4 * lane, live = max(0, min(4, a.dim - d));
+    // part 0 is the tile's own, part i the beginning of tile + i
+    const int n = (int)((end - 1) / a.tile) - tile + 1;
+    const int p0 = (int)((int64_t)n * w / 4), p1 = (int)((int64_t)n * (w + 1) / 4);
+    f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = p0; p < p1; p += kBatch) {
+        f32x4 rows[kBatch];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k)
+        for (int k = 0; k < kBatch; ++k) {
+            const float* src =
+                a.part + ((int64_t)(tile + p + k) * 2 + (p + k == 0)) * a.dim + d0;
+            rows[k] = buffer_load4(
+                buffer_rsrc(src, p + k < p1 ? (int64_t)(a.dim - d0) * 4 : 0), 16 * lane);
+        }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                rows[k][e] = i + k < n && e < live ? src[(int64_t)(i + k) * 2 * a.dim + e] : 0.0f;
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] += rows[k][e];
+        for (int k = 0; k < kBatch; ++k) sum = sum + rows[k];
     }
+    quarter[w][lane] = sum;
+    __syncthreads();
+    if (w != 0) return;
+    sum = (quarter[0][lane] + quarter[1][lane]) + (quarter[2][lane] + quarter[3][lane]);
     float* dst = a.dtable + (int64_t)token * a.dim + d;
     for (int e = 0; e < live; ++e)
         dst[e] = a.beta != 0.0f ? a.scale * sum[e] + a.beta * dst[e] : a.scale * sum[e];
@@ -290,9 +336,9 @@ BackwardPlan plan_backward(int64_t count, int64_t vocab, int64_t dim) {
     const int64_t cus = num_cus();
     p.bins = (int)std::min<int64_t>(kMaxBins, (vocab + cus - 1) / cus);
     p.groups = (vocab + p.bins - 1) / p.bins;
-    // about four waves to a compute unit, a column block each; tiles of at least 16
+    // about 16 waves to a compute unit, a column block each; tiles of at least 16
     const int64_t blocks = (dim + 255) / 256;
-    const int64_t even = count * blocks / (4 * cus);
+    const int64_t even = count * blocks / (16 * cus);
     p.tile = (int)std::max<int64_t>(16, std::min<int64_t>(256, (even + 15) / 16 * 16));
     p.tiles = (count + p.tile - 1) / p.tile;
     auto round4 = [](int64_t n) { return (size_t)((n + 3) / 4 * 4); };
@@ -304,9 +350,10 @@ BackwardPlan plan_backward(int64_t count, int64_t vocab, int64_t dim) {
 
 int check_shape(const char* what, int64_t count, int64_t vocab, int64_t dim) {
     NRS_ARG_CHECK(count >= 0 && count <= (1 << 30) && vocab >= 1 && vocab < INT32_MAX &&
-                      dim >= 1 && dim <= (1 << 20),
+                      dim >= 1 && dim <= (1 << 20) && count * dim <= (1ll << 39),
                   "%s: unsupported sizes (count %lld, vocab %lld, dim %lld): count is at most 2^30, "
-                  "vocab below 2^31 - 1, dim at most 2^20, vocab and dim at least 1",
+                  "vocab below 2^31 - 1, dim at most 2^20, count * dim at most 2^39, vocab and dim "
+                  "at least 1",
                   what, (long long)count, (long long)vocab, (long long)dim);
     return NRS_OK;
 }
@@ -361,17 +408,21 @@ int nrs_embedding_backward(float* dtable, const float* grad, const int32_t* ids,
     a.dim = (int)dim;
     a.bins = plan.bins;
     a.tile = plan.tile;
+    a.blocks = (int)((dim + 255) / 256);
+    a.groups = (int)plan.groups;
     a.scale = scale;
     a.beta = beta;
     a.sorted = reinterpret_cast<int32_t*>(scratch);
     a.start = a.sorted + plan.sorted;
     a.part = scratch + plan.sorted + plan.start;
-    hipLaunchKernelGGL(nrs::embedding_sort_kernel, dim3((unsigned)plan.groups),
+    const int64_t clear =
+        beta != 0.0f ? 0 : std::min<int64_t>((vocab * dim + 16383) / 16384, nrs::num_cus());
+    hipLaunchKernelGGL(nrs::embedding_sort_kernel, dim3((unsigned)(plan.groups + clear)),
                        dim3(nrs::kSortThreads), 0, nrs::stream(), a);
     if (count > 0) {
-        const dim3 grid((unsigned)plan.tiles, (unsigned)((dim + 255) / 256));
+        const dim3 grid((unsigned)(plan.tiles * a.blocks));
         hipLaunchKernelGGL(nrs::embedding_sum_kernel, grid, dim3(64), 0, nrs::stream(), a);
-        hipLaunchKernelGGL(nrs::embedding_join_kernel, grid, dim3(64), 0, nrs::stream(), a);
+        hipLaunchKernelGGL(nrs::embedding_join_kernel, grid, dim3(256), 0, nrs::stream(), a);
     }
     NRS_LAUNCH_CHECK("embedding backward");
     return NRS_OK;
