@@ -122,166 +122,315 @@ __device__ __forceinline__ float across_groups(float x) {
 }
 
 constexpr int kRowWaves = 4;
+constexpr int kMaxSharedBatch = 1024;  // batch items of a shared launch
 
 // Few rows: K and V stream from HBM straight into registers, as operands of
 // v_mfma_f32_16x16x4_f32 (16 rows at 157 TFLOP/s keep pace with 8 TB/s of f32
 // keys and values). Waves of a workgroup take turns at tiles of 16 keys, each
-// with its next tile on the way, and are joined at the end; workgroups share
-// the keys of an item when there are few of them.
+// with its next tile on the way, and are joined at the end.
+//
+// A unit is 16 rows of an item. With `groups` 0 a workgroup takes a unit. Else
+// the key tiles of all units lie one after the other and `groups` workgroups
+// take equal parts of that line, whatever the items' lengths: a unit that a
+// part begins or ends in leaves sums for cross_rows_join_kernel, in slot
+// (workgroup + unit), which no two share.
+template <int NJ>
+struct RowsWalk {
+    const CrossArgs& a;
+    float (&sums)[kRowWaves][4 * NJ][64];
+    float (&tops)[kRowWaves][16];
+    float (&totals)[kRowWaves][16];
+
+    // Tiles t0 .. t1 - 1 of unit `unit` (rows r0 .. of (b, kv)), L live keys:
+    // the whole of it (slot < 0) or a part.
+    __device__ __forceinline__ void run(int b, int kv, int r0, int L, int t0, int t1,
+                                        int64_t slot) const {
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+        const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int R = a.Sq * a.G;
+        f32x4 qf[NJ], acc[NJ], kf[NJ];
+        float vf[4][NJ];
+        auto load_keys = [&](int t) {
+            Rows<false>(a, a.k, b, kv, a.ld_kv, 16 * t, min(16, L - 16 * t))
+                .template along<NJ>(kf, c, g);
+        };
+        auto load_values = [&](int t) {
+            const Rows<false> vs(a, a.v, b, kv, a.ld_kv, 16 * t, min(16, L - 16 * t));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) vs.template across<NJ>(vf[r], 4 * g + r, c);
+        };
+        if (t0 + w < t1) {
+            load_keys(t0 + w);
+            load_values(t0 + w);
+        }
+        Rows<true>(a, a.q, b, kv, a.ld_q, r0, min(16, R - r0)).template along<NJ>(qf, c, g);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            qf[j] = qf[j] * a.scale2;
+            acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        float m = -INFINITY, l = 0.0f;
+        for (int t = t0 + w; t < t1; t += kRowWaves) {
+            f32x4 p = dot_rows<NJ>(kf, qf);
+            if (t + kRowWaves < t1) load_keys(t + kRowWaves);
+            float mt = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (16 * t + 4 * g + r >= L) p[r] = -INFINITY;
+                mt = fmaxf(mt, p[r]);
+            }
+            mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+            const float top = fmaxf(m, mt);
+            const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l *= alpha;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[j] = acc[j] * alpha;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[r] = 16 * t + 4 * g + r < L ? __builtin_amdgcn_exp2f(p[r] - m) : 0.0f;
+                l += p[r];
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[j] = mfma16(vf[r][j], p[r], acc[j]);
+            }
+            if (t + kRowWaves < t1) load_values(t + kRowWaves);
+        }
+        l = across_groups(l);
+        if (g == 0) {
+            tops[w][c] = m;
+            totals[w][c] = l;
+        }
+        __syncthreads();
+        float top = tops[0][c];
+#pragma unroll
+        for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, tops[i][c]);
+        // a wave without keys adds nothing; NaN must not be taken for that
+        const float f = m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) sums[w][r * NJ + j][lane] = acc[j][r] * f;
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRowWaves; ++i) {
+            const float li = totals[i][c];
+            total += tops[i][c] == -INFINITY && li == 0.0f
+                         ? 0.0f
+                         : li * __builtin_amdgcn_exp2f(tops[i][c] - top);
+        }
+        __syncthreads();
+        if (r0 + c < R) {
+            // wave w adds the waves' register w: NJ neighbouring columns of row c
+            static_assert(kRowWaves == 4, "a register of an accumulator to each wave");
+            const bool whole = slot < 0;
+            const float scale = !whole ? 1.0f : L > 0 ? 1.0f / total : 0.0f;
+            const int64_t at = slot * min(R, 16) + c;
+            float* dst = whole ? a.out + query_offset(a, b, kv, r0 + c, a.ld_out) : a.part + at * a.D;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                float v = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kRowWaves; ++i) v += sums[i][w * NJ + j][lane];
+                const int d = (4 * g + w) * NJ + j;
+                if (d < a.D) dst[d] = v * scale;
+            }
+            if (w == 0 && g == 0 && (!whole || a.stats)) {
+                float* st = whole ? row_stats(a, b, kv, r0 + c) : a.part_stats + 2 * at;
+                st[0] = whole && L == 0 ? 0.0f : top;
+                st[1] = total;
+            }
+        }
+        __syncthreads();  // before the shared arrays serve the next unit
+    }
+};
+
 template <int NJ>
 __global__ __launch_bounds__(64 * kRowWaves) void cross_rows_fwd_kernel(CrossArgs a) {
     __shared__ float sums[kRowWaves][4 * NJ][64];
     __shared__ float tops[kRowWaves][16], totals[kRowWaves][16];
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int R = a.Sq * a.G, row_tiles = (R + 15) / 16, items = a.B * a.KV;
-    int rest = blockIdx.x;
-    const int r0 = rest % row_tiles * 16;
-    rest /= row_tiles;
-    const int item = rest % items, split_no = rest / items;
-    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
-    const int all = (L + 15) / 16;
-    const int t0 = (int)((int64_t)all * split_no / a.splits),
-              t1 = (int)((int64_t)all * (split_no + 1) / a.splits);
-    f32x4 qf[NJ], acc[NJ], kf[NJ];
-    float vf[4][NJ];
-    auto load = [&](int t) {
-        const int n = min(16, L - 16 * t);
-        Rows<false>(a, a.k, b, kv, a.ld_kv, 16 * t, n).template along<NJ>(kf, c, g);
-        const Rows<false> vs(a, a.v, b, kv, a.ld_kv, 16 * t, n);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) vs.template across<NJ>(vf[r], 4 * g + r, c);
-    };
-    if (t0 + w < t1) load(t0 + w);
-    Rows<true>(a, a.q, b, kv, a.ld_q, r0, min(16, R - r0)).template along<NJ>(qf, c, g);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        qf[j] = qf[j] * a.scale2;
-        acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    __shared__ int wave_sum[kRowWaves], found[2];
+    const RowsWalk<NJ> walk{a, sums, tops, totals};
+    const int row_tiles = (a.Sq * a.G + 15) / 16, per_item = a.KV * row_tiles;
+    if (a.groups == 0) {
+        const int unit = blockIdx.x, b = unit / per_item, sub = unit - b * per_item;
+        const int L = live_keys(a, b);
+        walk.run(b, sub / row_tiles, sub % row_tiles * 16, L, 0, (L + 15) / 16, -1);
+        return;
     }
-    float m = -INFINITY, l = 0.0f;
-    for (int t = t0 + w; t < t1; t += kRowWaves) {
-        f32x4 p = dot_rows<NJ>(kf, qf);
-        float vt[4][NJ];
+    // where on the line each batch item begins: a scan of their lengths, which
+    // finds the item of this workgroup's first tile
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+    const int each = (a.B + 255) / 256;
+    int own = 0;
+    for (int i = 0; i < each; ++i)
+        if (t * each + i < a.B) own += (live_keys(a, t * each + i) + 15) / 16 * per_item;
+    int upto = own;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) vt[r][j] = vf[r][j];
-        if (t + kRowWaves < t1) load(t + kRowWaves);
-        float mt = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (16 * t + 4 * g + r >= L) p[r] = -INFINITY;
-            mt = fmaxf(mt, p[r]);
-        }
-        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-        const float top = fmaxf(m, mt);
-        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-        m = top;
-        l *= alpha;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[j] = acc[j] * alpha;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            p[r] = 16 * t + 4 * g + r < L ? __builtin_amdgcn_exp2f(p[r] - m) : 0.0f;
-            l += p[r];
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) acc[j] = mfma16(vt[r][j], p[r], acc[j]);
-        }
+    for (int d = 1; d < 64; d *= 2) {
+        const int v = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += v;
     }
-    l = across_groups(l);
-    if (g == 0) {
-        tops[w][c] = m;
-        totals[w][c] = l;
-    }
+    if (lane == 63) wave_sum[w] = upto;
     __syncthreads();
-    float top = tops[0][c];
-#pragma unroll
-    for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, tops[i][c]);
-    // a wave without keys adds nothing; NaN must not be taken for that
-    const float f = m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) sums[w][r * NJ + j][lane] = acc[j][r] * f;
-    float total = 0.0f;
-#pragma unroll
+    int begin = upto - own, total = 0;
     for (int i = 0; i < kRowWaves; ++i) {
-        const float li = totals[i][c];
-        total += tops[i][c] == -INFINITY && li == 0.0f
-                     ? 0.0f
-                     : li * __builtin_amdgcn_exp2f(tops[i][c] - top);
+        begin += i < w ? wave_sum[i] : 0;
+        total += wave_sum[i];
+    }
+    const int no = blockIdx.x;
+    const int p0 = (int)((int64_t)total * no / a.groups),
+              p1 = (int)((int64_t)total * (no + 1) / a.groups);
+    if (p0 >= p1) return;
+    for (int i = 0; i < each && t * each + i < a.B; ++i) {
+        const int n = (live_keys(a, t * each + i) + 15) / 16 * per_item;
+        if (begin <= p0 && p0 < begin + n) {
+            found[0] = t * each + i;
+            found[1] = begin;
+        }
+        begin += n;
     }
     __syncthreads();
-    if (r0 + c >= R) return;
-    // wave w adds the waves' register w: NJ neighbouring columns of row c
-    static_assert(kRowWaves == 4, "a register of an accumulator to each wave");
-    const bool whole = a.splits == 1;
-    const float scale = !whole ? 1.0f : L > 0 ? 1.0f / total : 0.0f;
-    const int64_t at = ((int64_t)split_no * items + item) * R + r0 + c;
-    float* dst = whole ? a.out + query_offset(a, b, kv, r0 + c, a.ld_out) : a.part + at * a.D;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        float v = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kRowWaves; ++i) v += sums[i][w * NJ + j][lane];
-        const int d = (4 * g + w) * NJ + j;
-        if (d < a.D) dst[d] = v * scale;
-    }
-    if (w == 0 && g == 0 && (!whole || a.stats)) {
-        float* st = whole ? row_stats(a, b, kv, r0 + c) : a.part_stats + 2 * at;
-        st[0] = whole && L == 0 ? 0.0f : top;
-        st[1] = total;
+    int b = found[0], base = found[1];
+    for (int p = p0; p < p1;) {
+        const int L = live_keys(a, b), tiles = (L + 15) / 16;
+        if (p >= base + tiles * per_item) {  // the next item (those without keys have no tiles)
+            base += tiles * per_item;
+            ++b;
+            continue;
+        }
+        const int sub = (p - base) / tiles, t0 = p - base - sub * tiles;
+        const int t1 = min(tiles, t0 + p1 - p), unit = b * per_item + sub;
+        if (t == 0) {
+            if (t0 == 0) a.shares[2 * unit] = no;
+            if (t1 == tiles) a.shares[2 * unit + 1] = no;
+        }
+        walk.run(b, sub / row_tiles, sub % row_tiles * 16, L, t0, t1,
+                 t0 == 0 && t1 == tiles ? -1 : (int64_t)no + unit);
+        p += t1 - t0;
     }
 }
 
-// Joins the splits of a row: out = sum O_s 2^(m_s - M) / sum l_s 2^(m_s - M).
-// PER_ROW threads share a row, 32 (four columns each, d_head <= 128) or 256,
-// whose eight groups of 32 take turns at the splits and add up in LDS.
-template <int PER_ROW>
-__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
-    __shared__ float sums[256][5];
-    const int R = a.Sq * a.G, items = a.B * a.KV;
-    const int x = threadIdx.x % 32, turn = PER_ROW == 256 ? threadIdx.x / 32 : 0;
-    const int64_t at = (int64_t)blockIdx.x * (256 / PER_ROW) + threadIdx.x / PER_ROW;
-    const int64_t rows = (int64_t)items * R;
-    if (PER_ROW != 256 && at >= rows) return;
-    float top = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_stats[2 * (s * rows + at)]);
-    float v[4] = {}, total = 0.0f;
-    const int live = max(0, min(4, a.D - 4 * x));
-    for (int s = turn; s < a.splits; s += PER_ROW / 32) {
-        const float m = a.part_stats[2 * (s * rows + at)], l = a.part_stats[2 * (s * rows + at) + 1];
-        if (m == -INFINITY && l == 0.0f) continue;  // no keys in this split
-        const float f = __builtin_amdgcn_exp2f(m - top);
-        total = fmaf(l, f, total);
-        const float* src = a.part + (s * rows + at) * a.D + 4 * x;
-        for (int e = 0; e < live; ++e) v[e] = fmaf(src[e], f, v[e]);
+struct __attribute__((packed, aligned(4))) Quad {  // 128 bits at any float
+    f32x4 v;
+};
+
+// The sums of `count` parts of a row: each has its columns at stats(s), where
+// the reference and the sum are, and at part(s). 32 threads share the columns,
+// four each (d_head <= 128); lane s of them looks up part s, and the parts are
+// asked for eight at a time.
+struct Joined {
+    float top = -INFINITY, total = 0.0f;
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+
+    // The weight of sums taken against m when the reference is `top`: a part
+    // without keys has none (NaN sums are not taken for that).
+    __device__ __forceinline__ static float weight(float m, float l, float top) {
+        return m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
     }
-    if constexpr (PER_ROW == 256) {
+
+    template <class S, class P>
+    __device__ __forceinline__ void add(int s0, int s1, int live, S stats, P part) {
+        const int x = threadIdx.x % 32;
+        for (int c0 = s0; c0 < s1; c0 += 32) {
+            float m = -INFINITY, l = 0.0f;
+            if (c0 + x < s1) {
+                const float* st = stats(c0 + x);
+                m = st[0];
+                l = st[1];
+            }
+            float most = m;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sums[threadIdx.x][e] = v[e];
-        sums[threadIdx.x][4] = total;
-        __syncthreads();
-        if (turn != 0) return;
-        for (int t = 1; t < 8; ++t) {
+            for (int i = 1; i < 32; i *= 2) most = fmaxf(most, __shfl_xor(most, i, 32));
+            most = fmaxf(most, top);
+            const float old = weight(top, total, most), f = weight(m, l, most);
+            float sum = l * f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += sums[32 * t + x][e];
-            total += sums[32 * t + x][4];
+            for (int i = 1; i < 32; i *= 2) sum += __shfl_xor(sum, i, 32);
+            total = total * old + sum;
+            top = most;
+            v = v * old;
+            for (int s = c0; s < min(c0 + 32, s1); s += 8) {
+                f32x4 x8[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x8[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (s + i >= s1) continue;
+                    const float* src = part(s + i) + 4 * x;
+                    if (live == 4)
+                        x8[i] = reinterpret_cast<const Quad*>(src)->v;
+                    else
+                        for (int e = 0; e < live; ++e) x8[i][e] = src[e];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v = v + x8[i] * __shfl(f, s + i - c0, 32);
+            }
         }
     }
-    const int item = (int)(at / R), r = (int)(at - (int64_t)item * R);
-    const int b = item / a.KV, kv = item - b * a.KV;
-    const bool any = live_keys(a, b) > 0;
-    const float scale = any ? 1.0f / total : 0.0f;
-    float* dst = a.out + query_offset(a, b, kv, r, a.ld_out) + 4 * x;
-    for (int e = 0; e < live; ++e) dst[e] = v[e] * scale;
-    if (a.stats && x == 0) {
-        float* st = row_stats(a, b, kv, r);
-        st[0] = any ? top : 0.0f;
-        st[1] = any ? total : 0.0f;
+
+    __device__ __forceinline__ void store(const CrossArgs& a, int b, int kv, int r, int live) const {
+        const int x = threadIdx.x % 32;
+        const bool any = live_keys(a, b) > 0;
+        const float scale = any ? 1.0f / total : 0.0f;
+        float* dst = a.out + query_offset(a, b, kv, r, a.ld_out) + 4 * x;
+        for (int e = 0; e < live; ++e) dst[e] = v[e] * scale;
+        if (a.stats && x == 0) {
+            float* st = row_stats(a, b, kv, r);
+            st[0] = any ? top : 0.0f;
+            st[1] = any ? total : 0.0f;
+        }
     }
+};
+
+// A workgroup to a row of cross_rows_fwd_kernel's units: eight groups of 32
+// threads take an eighth of the row's parts each and are added up in LDS.
+__global__ __launch_bounds__(256) void cross_rows_join_kernel(CrossArgs a) {
+    __shared__ f32x4 sums[8][32];
+    __shared__ float tops[8], totals[8];
+    const int x = threadIdx.x % 32, group = threadIdx.x / 32;
+    const int R = a.Sq * a.G, row_tiles = (R + 15) / 16, per = min(R, 16);
+    const int item = blockIdx.x / R, r = blockIdx.x - item * R;
+    const int b = item / a.KV, kv = item - b * a.KV, unit = item * row_tiles + r / 16;
+    const int live = max(0, min(4, a.D - 4 * x));
+    Joined sum;
+    if (live_keys(a, b) > 0) {
+        const int first = a.shares[2 * unit], n = a.shares[2 * unit + 1] - first + 1;
+        if (n == 1) return;  // one workgroup took all of the unit
+        const int64_t at = ((int64_t)first + unit) * per + r % 16;
+        sum.add(n * group / 8, n * (group + 1) / 8, live,
+                [&](int s) { return a.part_stats + 2 * (at + (int64_t)s * per); },
+                [&](int s) { return a.part + (at + (int64_t)s * per) * a.D; });
+    }
+    sums[group][x] = sum.v;
+    if (x == 0) {
+        tops[group] = sum.top;
+        totals[group] = sum.total;
+    }
+    __syncthreads();
+    if (group != 0) return;
+    for (int i = 1; i < 8; ++i) {
+        const float most = fmaxf(sum.top, tops[i]);
+        const float f = Joined::weight(sum.top, sum.total, most),
+                    g = Joined::weight(tops[i], totals[i], most);
+        sum.v = sum.v * f + sums[i][x] * g;
+        sum.total = sum.total * f + totals[i] * g;
+        sum.top = most;
+    }
+    sum.store(a, b, kv, r, live);
+}
+
+// Joins the splits of cross_tile_fwd_kernel: 32 threads to a row.
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
+    const int R = a.Sq * a.G, x = threadIdx.x % 32;
+    const int64_t rows = (int64_t)a.B * a.KV * R;
+    const int64_t at = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    if (at >= rows) return;
+    const int item = (int)(at / R), r = (int)(at - (int64_t)item * R), b = item / a.KV;
+    const int live = max(0, min(4, a.D - 4 * x));
+    Joined sum;
+    sum.add(0, a.splits, live, [&](int s) { return a.part_stats + 2 * (at * a.splits + s); },
+            [&](int s) { return a.part + (s * rows + at) * a.D; });
+    sum.store(a, b, item - b * a.KV, r, live);
 }
 
 // Adds the shares of a gradient in order: dst = f * sum + beta * dst, 32
@@ -359,9 +508,12 @@ int check_shape(const char* what, int64_t batch, int64_t heads, int64_t kv_heads
 }
 
 struct ForwardPlan {
-    bool tiles;  // the kernel of many rows
-    int splits;
-    int64_t blocks;  // workgroups, splits included
+    bool tiles;        // the kernel of many rows
+    int splits;        // tiles: workgroups that share an item's keys
+    int groups;        // few rows: workgroups that share all units, 0: one each
+    int64_t blocks;    // workgroups of the launch
+    size_t part, stats, shares;  // scratch, in 4-byte words
+    size_t bytes() const { return 4 * (part + stats + shares); }
 };
 
 // Rows of an item up to which the kernel of few rows takes the call.
@@ -370,14 +522,27 @@ constexpr int64_t kFewRows = 32;
 ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
                          int64_t seq_k, int64_t d_head) {
     const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads, cus = num_cus();
-    ForwardPlan p{R > kFewRows, 1, 0};
+    ForwardPlan p{R > kFewRows, 1, 0, 0, 0, 0, 0};
     if (items == 0 || R == 0) return p;
     if (!p.tiles) {
-        // 16 waves to a compute unit, at least a tile of 16 keys for each
-        const int64_t base = items * ((R + 15) / 16);
-        const int64_t most = std::max<int64_t>(1, seq_k / (16 * kRowWaves));
-        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({4 * cus / base, most, 256}));
-        p.blocks = base * p.splits;
+        const int64_t units = items * ((R + 15) / 16);
+        // Shared unless there are enough units to even out by themselves; at
+        // least two tiles of 16 keys to a wave. Workgroups to a compute unit
+        // by the bytes that each has on the way (a tile of K and V to a wave):
+        // 1, 2 and 4 of them take 47, 48 and 51 us at d_head 128 (2 x 16384
+        // keys, 8 key heads) and 38, 30 and 26 us, 3 26 us, at d_head 64 (32
+        // items of up to 1500 keys, 8 key heads).
+        const int64_t groups = std::min<int64_t>((d_head > 64 ? 1 : d_head > 32 ? 3 : 6) * cus,
+                                                 units * ((seq_k + 15) / 16) / (2 * kRowWaves));
+        p.blocks = units;
+        if (units < 4 * cus && batch <= kMaxSharedBatch && groups > 1) {
+            p.groups = (int)groups;
+            p.blocks = groups;
+            const int64_t slots = (groups + units) * std::min<int64_t>(R, 16);
+            p.part = (size_t)((slots * d_head + 3) / 4 * 4);
+            p.stats = (size_t)((2 * slots + 3) / 4 * 4);
+            p.shares = (size_t)(2 * units);
+        }
     } else {
         // one workgroup to a compute unit: the split with the least time, in
         // key tiles, of the fullest one; a workgroup's beginning and end cost
@@ -396,6 +561,10 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
             }
         }
         p.blocks = base * p.splits;
+        if (p.splits > 1) {
+            p.part = (size_t)((p.splits * items * R * d_head + 3) / 4 * 4);
+            p.stats = (size_t)(2 * p.splits * items * R);
+        }
     }
     return p;
 }
@@ -433,10 +602,6 @@ BackwardPlan plan_backward(int64_t batch, int64_t heads, int64_t kv_heads, int64
     return p;
 }
 
-size_t forward_scratch(const ForwardPlan& p, int64_t rows, int64_t d_head) {
-    return p.splits > 1 ? sizeof(float) * (size_t)p.splits * rows * (d_head + 2) : 0;
-}
-
 }  // namespace
 }  // namespace nrs
 
@@ -457,9 +622,7 @@ int nrs_cross_attention_workspace(size_t* bytes, int64_t batch, int64_t heads, i
         return rc;
     *bytes = backward
                  ? nrs::plan_backward(batch, heads, kv_heads, seq_q, seq_k, d_head).bytes()
-                 : nrs::forward_scratch(
-                       nrs::plan_forward(batch, heads, kv_heads, seq_q, seq_k, d_head),
-                       batch * heads * seq_q, d_head);
+                 : nrs::plan_forward(batch, heads, kv_heads, seq_q, seq_k, d_head).bytes();
     return NRS_OK;
 }
 
@@ -479,13 +642,13 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
     const auto plan = nrs::plan_forward(batch, heads, kv_heads, seq_q, seq_k, d_head);
     const int64_t rows = batch * heads * seq_q;
     float* scratch = nullptr;
-    if (int rc = nrs::call_scratch(&scratch, nrs::forward_scratch(plan, rows, d_head), work,
-                                   work_bytes, what))
-        return rc;
+    if (int rc = nrs::call_scratch(&scratch, plan.bytes(), work, work_bytes, what)) return rc;
     nrs::CrossArgs a{};
     a.splits = plan.splits;
+    a.groups = plan.groups;
     a.part = scratch;
-    a.part_stats = scratch ? scratch + plan.splits * rows * d_head : nullptr;
+    a.part_stats = scratch + plan.part;
+    a.shares = reinterpret_cast<int32_t*>(scratch + plan.part + plan.stats);
     a.q = q;
     a.k = k;
     a.v = v;
@@ -515,13 +678,12 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
         });
     }
     NRS_LAUNCH_CHECK(what);
-    if (a.splits > 1) {
-        // many splits: a workgroup to a row
-        const bool wide = a.splits > 8;
-        auto join = wide ? nrs::cross_join_kernel<256> : nrs::cross_join_kernel<32>;
-        hipLaunchKernelGGL(join, dim3((unsigned)(wide ? rows : (rows + 7) / 8)), dim3(256), 0,
+    if (a.groups > 0)
+        hipLaunchKernelGGL(nrs::cross_rows_join_kernel, dim3((unsigned)rows), dim3(256), 0,
                            nrs::stream(), a);
-    }
+    else if (a.splits > 1)
+        hipLaunchKernelGGL(nrs::cross_join_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0,
+                           nrs::stream(), a);
     NRS_LAUNCH_CHECK(what);
     return NRS_OK;
 }

@@ -22,9 +22,17 @@ struct CrossArgs {
     FastDiv by_group;     // division by G
     float scale, scale2;  // scale2 = scale * log2(e)
     float beta_q, beta_kv;
-    int splits;         // forward: workgroups that share an item's keys
-    float* part;        // splits > 1: [splits][items][R][D] sums, not yet divided
-    float* part_stats;  // and their [splits][items][R][2]
+    // forward of many rows: workgroups that share an item's keys. Past 1,
+    // `part` has [splits][items][R][D] sums, not yet divided, and part_stats
+    // their reference and sum, [items][R][splits][2]
+    int splits;
+    // forward of few rows: workgroups that share the launch's key tiles, or 0.
+    // Then `part` has [slots][min(R, 16)][D], part_stats [slots][min(R, 16)][2]
+    // and `shares` the first and the last workgroup of each unit
+    int groups;
+    float* part;
+    float* part_stats;
+    int32_t* shares;
     // backward
     float *neg_lse, *neg_delta;  // [items][R]: -log2 sum 2^u and -dout . out
     int q_splits, kv_splits;     // workgroups that share a dq (dk and dv) tile's walk

@@ -374,8 +374,9 @@ __global__ __launch_bounds__(64 * WAVES) void cross_tile_fwd_kernel(CrossArgs a)
         const int64_t at = ((int64_t)split_no * items + item) * R + row;
         store_own<C, FULL>(a.part + at * a.D, acc, 1.0f, 0.0f, a.D, h);
         if (h == 0) {
-            a.part_stats[2 * at] = t0 < t1 ? m : -INFINITY;
-            a.part_stats[2 * at + 1] = l;
+            float* st = a.part_stats + 2 * (((int64_t)item * R + row) * a.splits + split_no);
+            st[0] = t0 < t1 ? m : -INFINITY;
+            st[1] = l;
         }
         return;
     }
