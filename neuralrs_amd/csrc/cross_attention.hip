@@ -311,10 +311,6 @@ __global__ __launch_bounds__(64 * kRowWaves) void cross_rows_fwd_kernel(CrossArg
     }
 }
 
-struct __attribute__((packed, aligned(4))) Quad {  // 128 bits at any float
-    f32x4 v;
-};
-
 // The sums of `count` parts of a row: each has its columns at stats(s), where
 // the reference and the sum are, and at part(s). 32 threads share the columns,
 // four each (d_head <= 128); lane s of them looks up part s, and the parts are
@@ -433,32 +429,52 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
     sum.store(a, b, item - b * a.KV, r, live);
 }
 
-// Adds the shares of a gradient in order: dst = f * sum + beta * dst, 32
-// threads to a row of d_head. KEYS: rows are keys, dead ones without shares.
-template <bool KEYS>
+// Adds the shares of a gradient in order: dst = f * sum + beta * dst, D / 4
+// threads to a row. KEYS: rows are keys (dead ones have no shares), blockIdx.y
+// is 0 for dk and 1 for dv.
+template <int D, bool KEYS>
 __global__ __launch_bounds__(256) void cross_sum_kernel(CrossArgs a) {
-    const int n = KEYS ? a.Sk : a.Sq * a.G, x = threadIdx.x % 32;
-    const int64_t at = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    constexpr int LANES = D / 4;
+    const int n = KEYS ? a.Sk : a.Sq * a.G, x = threadIdx.x % LANES;
+    const int64_t at = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     const int64_t rows = (int64_t)a.B * a.KV * n;
     if (at >= rows) return;
     const int item = (int)(at / n), r = (int)(at - (int64_t)item * n);
     const int b = item / a.KV, kv = item - b * a.KV;
-    const bool live = !KEYS || r < live_keys(a, b);
-    const float beta = KEYS ? a.beta_kv : a.beta_q;
+    const bool live = !KEYS || r < live_keys(a, b), second = KEYS && blockIdx.y == 1;
+    const float beta = KEYS ? a.beta_kv : a.beta_q, f = second ? 1.0f : a.scale;
     if (!live && beta == 1.0f) return;
-    for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
-        const float* part = KEYS ? (which ? a.dv_part : a.dk_part) : a.dq_part;
-        float* dst = KEYS ? (which ? a.dv : a.dk) + key_offset(a, b, kv, r)
-                          : a.dq + query_offset(a, b, kv, r, a.ld_q);
-        const float f = which ? 1.0f : a.scale;
-        const int shares = KEYS ? a.kv_splits : a.q_splits;
-        for (int d = 4 * x; d < min(a.D, 4 * x + 4); ++d) {
+    const float* part = (KEYS ? (second ? a.dv_part : a.dk_part) : a.dq_part) + at * a.D + 4 * x;
+    float* dst = (KEYS ? (second ? a.dv : a.dk) + key_offset(a, b, kv, r)
+                       : a.dq + query_offset(a, b, kv, r, a.ld_q)) + 4 * x;
+    const int shares = live ? (KEYS ? a.kv_splits : a.q_splits) : 0;
+    if (4 * x + 4 <= a.D) {
+        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int s = 0; s < shares; ++s)
+            v = v + reinterpret_cast<const Quad*>(part + s * rows * a.D)->v;
+        v = v * f;
+        Quad* const to = reinterpret_cast<Quad*>(dst);
+        if (beta != 0.0f) v = v + beta * to->v;
+        to->v = v;
+    } else {
+        for (int e = 0; 4 * x + e < a.D; ++e) {
             float v = 0.0f;
-            if (live)
-                for (int s = 0; s < shares; ++s) v += part[(s * rows + at) * a.D + d];
-            dst[d] = beta != 0.0f ? v * f + beta * dst[d] : v * f;
+            for (int s = 0; s < shares; ++s) v += part[s * rows * a.D + e];
+            dst[e] = beta != 0.0f ? v * f + beta * dst[e] : v * f;
         }
     }
+}
+
+template <int D>
+void launch_sums(const CrossArgs& a, int64_t rows, int64_t keys, bool dq, bool dkv) {
+    constexpr int PER = 1024 / D;
+    if (dq)
+        hipLaunchKernelGGL((cross_sum_kernel<D, false>), dim3((unsigned)((rows + PER - 1) / PER)),
+                           dim3(256), 0, stream(), a);
+    if (dkv)
+        hipLaunchKernelGGL((cross_sum_kernel<D, true>), dim3((unsigned)((keys + PER - 1) / PER), 2),
+                           dim3(256), 0, stream(), a);
 }
 
 template <class F>
@@ -576,8 +592,10 @@ struct BackwardPlan {
     size_t bytes() const { return sizeof(float) * (prepared + q_part + 2 * kv_part); }
 };
 
-// A workgroup to a compute unit: a walk that is longer than a compute unit's
-// even part of all the work is shared out. A step of dq is three products a
+// A workgroup to a compute unit: a walk that is longer than half a compute
+// unit's even part of all the work is shared out, so that the last walks to end
+// leave less idle (2 x 777 rows of 4 heads, 4096 keys and fewer, d_head 128:
+// 1164 us in whole walks, 1080 in halves). A step of dq is three products a
 // tile, one of dk and dv four. Asked for both gradients or not, the plan is
 // that of both: each has the same bits by itself.
 BackwardPlan plan_backward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
@@ -591,7 +609,7 @@ BackwardPlan plan_backward(int64_t batch, int64_t heads, int64_t kv_heads, int64
     const int64_t q_len = (seq_k + tile - 1) / tile, kv_len = (R + tile - 1) / tile;
     const int64_t q_groups = items * ((R + own - 1) / own),
                   kv_groups = items * ((seq_k + own - 1) / own);
-    const int64_t even = std::max<int64_t>(8, (3 * q_groups * q_len + 4 * kv_groups * kv_len) / cus);
+    const int64_t even = std::max<int64_t>(8, (3 * q_groups * q_len + 4 * kv_groups * kv_len) / (2 * cus));
     auto shares = [&](int64_t cost, int64_t len) {
         return (int)std::max<int64_t>(1, std::min<int64_t>({(cost + even - 1) / even, len, 64}));
     };
@@ -747,12 +765,12 @@ int nrs_cross_attention_backward(float* dq, float* dk, float* dv, const float* d
         a.q_blocks = (int)((a.Sq * a.G + own - 1) / own * batch * kv_heads * plan.q_splits);
     if (!keys) a.dk = a.dv = nullptr;
     nrs::cross_tile_backward(a);
-    if (dq && plan.q_splits > 1)
-        hipLaunchKernelGGL(nrs::cross_sum_kernel<false>, dim3((unsigned)((plan.rows + 7) / 8)),
-                           dim3(256), 0, nrs::stream(), a);
-    if (a.dk && plan.kv_splits > 1)
-        hipLaunchKernelGGL(nrs::cross_sum_kernel<true>, dim3((unsigned)((plan.keys + 7) / 8)),
-                           dim3(256), 0, nrs::stream(), a);
+    const int width = nrs::cross_tile_width(a.D);
+    const bool sum_q = a.q_blocks > 0 && plan.q_splits > 1, sum_kv = a.dk && plan.kv_splits > 1;
+    auto sums = width == 32   ? nrs::launch_sums<32>
+                : width == 64 ? nrs::launch_sums<64>
+                              : nrs::launch_sums<128>;
+    sums(a, plan.rows, plan.keys, sum_q, sum_kv);
     NRS_LAUNCH_CHECK(what);
     return NRS_OK;
 }

@@ -44,10 +44,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-struct __attribute__((packed, aligned(4))) Quad {  // 128 bits at any float
-    f32x4 v;
-};
-
 // The three pieces of 8 floats: an operand of the matrix instructions each.
 __device__ __forceinline__ void split8(const float (&x)[8], u32x4 (&p)[3]) {
 #pragma unroll
@@ -391,18 +387,27 @@ __global__ __launch_bounds__(64 * WAVES) void cross_tile_fwd_kernel(CrossArgs a)
 
 // What the backward starts its products from: per row -log2 of its sum of
 // exponentials (-infinity where no key is live: no probability) and
-// -dout . out. 32 lanes to a row, four columns each.
+// -dout . out. D / 4 lanes to a row, four columns each.
+template <int D>
 __global__ __launch_bounds__(256) void cross_rows_prepare_kernel(CrossArgs a) {
-    const int R = a.Sq * a.G, x = threadIdx.x % 32;
-    const int64_t at = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    constexpr int LANES = D / 4;
+    const int R = a.Sq * a.G, x = threadIdx.x % LANES;
+    const int64_t at = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     if (at >= (int64_t)a.B * a.KV * R) return;
     const int item = (int)(at / R), r = (int)(at - (int64_t)item * R);
     const int b = item / a.KV, kv = item - b * a.KV;
-    const int64_t off = query_offset(a, b, kv, r, a.ld_out);
+    const int64_t off = query_offset(a, b, kv, r, a.ld_out) + 4 * x;
     float dot = 0.0f;
-    for (int d = 4 * x; d < min(a.D, 4 * x + 4); ++d) dot = fmaf(a.dout[off + d], a.o[off + d], dot);
+    if (4 * x + 4 <= a.D) {
+        const f32x4 g = reinterpret_cast<const Quad*>(a.dout + off)->v,
+                    o = reinterpret_cast<const Quad*>(a.o + off)->v;
 #pragma unroll
-    for (int i = 1; i < 32; i *= 2) dot += __shfl_xor(dot, i, 64);
+        for (int e = 0; e < 4; ++e) dot = fmaf(g[e], o[e], dot);
+    } else {
+        for (int e = 0; 4 * x + e < a.D; ++e) dot = fmaf(a.dout[off + e], a.o[off + e], dot);
+    }
+#pragma unroll
+    for (int i = 1; i < LANES; i *= 2) dot += __shfl_xor(dot, i, 64);
     if (x == 0) {
         const float* st = row_stats(a, b, kv, r);
         a.neg_lse[at] = live_keys(a, b) > 0 ? -(st[0] + __builtin_amdgcn_logf(st[1])) : -INFINITY;
@@ -644,8 +649,11 @@ void cross_tile_backward(const CrossArgs& a) {
     const int R = a.Sq * a.G, rows = cross_backward_rows(R, a.Sk, a.D);
     const int64_t items = (int64_t)a.B * a.KV;
     if (R > 0) {
-        const int64_t n = items * R;
-        hipLaunchKernelGGL(cross_rows_prepare_kernel, dim3((unsigned)((n + 7) / 8)), dim3(256), 0,
+        const int width = cross_tile_width(a.D), per = 1024 / width;
+        auto prepare = width == 32   ? cross_rows_prepare_kernel<32>
+                       : width == 64 ? cross_rows_prepare_kernel<64>
+                                     : cross_rows_prepare_kernel<128>;
+        hipLaunchKernelGGL(prepare, dim3((unsigned)((items * R + per - 1) / per)), dim3(256), 0,
                            stream(), a);
     }
     const unsigned grid =

@@ -13,6 +13,10 @@ of its probability (e = the score's error, twice: the row's sum has it too).
 import numpy as np
 
 U = 2.0 ** -24
+# What a weight (p or ds) may lose absolutely: an exponential under 2^-126, the
+# smallest normal float, may come out as zero, and so may the weight's product
+# or the pieces of it that are under that: 2^-126 each.
+TINY = 2 * 2.0 ** -126
 
 
 def gamma(n):
@@ -35,7 +39,7 @@ def forward(q, k, v, scale):
     # (u times the score) are in the 4 of the next line
     es = (gamma(q.shape[1]) + 4 * U) * (np.abs(q) @ np.abs(k).T * abs(scale)).max(axis=1, keepdims=True)
     ep = 2 * es + gamma(len(k)) + 8 * U  # relative error of p
-    bound = (ep + gamma(len(k))) * (p @ np.abs(v))
+    bound = (ep + gamma(len(k))) * (p @ np.abs(v)) + TINY * np.abs(v).sum(axis=0)
     return p @ v, np.concatenate([m * np.log2(np.e), total], axis=1), bound, p, ep
 
 
@@ -53,10 +57,12 @@ def backward(q, k, v, g, scale):
     e_dp = gamma(d) * (np.abs(g) @ np.abs(v).T)
     e_delta = (gamma(d) * (np.abs(g) * np.abs(out)) + np.abs(g) * out_bound).sum(axis=1, keepdims=True)
     e_ds = abs(scale) * p * ((ep + 4 * U) * np.abs(dp - delta) + e_dp + e_delta)
+    e_ds += TINY * (1 + abs(scale) * np.abs(dp - delta))
+    e_p = ep * p + TINY
     dq, dk, dv = ds @ k, ds.T @ q, p.T @ g
     bounds = [e_ds @ np.abs(k) + gamma(L) * (np.abs(ds) @ np.abs(k)),
               e_ds.T @ np.abs(q) + gamma(R) * (np.abs(ds).T @ np.abs(q)),
-              (ep * p).T @ np.abs(g) + gamma(R) * (p.T @ np.abs(g))]
+              e_p.T @ np.abs(g) + gamma(R) * (p.T @ np.abs(g))]
     return [dq, dk, dv], bounds
 
 

@@ -37,7 +37,7 @@ class Device:
 
 def compare(got, value, bound, what):
     """Within the bound (plus what a float of the value's size rounds)."""
-    tol = bound + 2.0 ** -24 * np.abs(value) + 1e-37
+    tol = bound + 2.0 ** -24 * np.abs(value) + 2.0 ** -126
     bad = ~(np.abs(got - value) <= tol)
     assert not bad.any(), (
         f"{what}: {bad.sum()} of {bad.size} off; worst {np.nanmax(np.abs(got - value) / tol):.3g} of "
@@ -136,6 +136,18 @@ def test_lopsided_lengths(hip, seq_q, seq_k):
 def test_large_scores(hip):
     """Scores in the hundreds: only the differences to the maximum count."""
     check(hip, Problem(1, 2, 2, 40, 90, 32, seed=3, magnitude=8.0))
+
+
+@pytest.mark.parametrize("seq_q", [1, 200])
+@pytest.mark.parametrize("step", [0.05, 2.0, -2.0])
+def test_scores_that_climb(hip, seq_q, step):
+    """Every key's score is above (or below) the one before: the running
+    maximum moves at each tile, or never after the first, to scores in the
+    thousands, whose powers of two no float holds."""
+    p = Problem(1, 2, 1, seq_q, 1000, 64, seed=11)
+    p.q[:] = np.abs(p.q) + np.float32(0.5)
+    p.k[:] = np.abs(p.k) * np.float32(0.01) + (np.arange(1000) * step / 30).astype(np.float32)[:, None]
+    check(hip, p)
 
 
 def test_zero_lengths(hip):
