@@ -252,6 +252,21 @@ std::vector<float> DeviceBuffer::to_host() const {
 void DeviceBuffer::zero() { pending_zero_ = true; }
 
 // -------------------------------------------------------------------- Node
+DeviceInts::DeviceInts(const std::vector<int32_t>& v) : len_(v.size()) {
+    void* p = nullptr;
+    check_raw(nrs_malloc(&p, v.size() * sizeof(int32_t)), "device ints: allocation failed");
+    ptr_ = static_cast<int32_t*>(p);
+    if (nrs_memcpy_htod(ptr_, v.data(), v.size() * sizeof(int32_t)) != NRS_OK) {
+        const std::string why = nrs_last_error();  // (the destructor will not run)
+        nrs_free(ptr_);
+        throw Panic("device ints: copy failed: " + why);
+    }
+}
+
+DeviceInts::~DeviceInts() { nrs_free(ptr_); }
+
+IntsRef device_ints(const std::vector<int32_t>& v) { return std::make_shared<DeviceInts>(v); }
+
 NodeRef Node::create(std::vector<float> data, std::vector<size_t> shape) {
     NodeRef n = std::make_shared<Node>();
     n->grad.assign(data.size(), 0.0f);
@@ -1167,6 +1182,141 @@ static NodeRef multihead(const MultiHeadAttention& mha, const NodeRef& flat, siz
         concat = merge_heads(att, rows, heads, dh, {rows, d});
     }
     return graph::matmul(concat, mha.w_o);
+}
+
+// The fused node of cross_attention and forward_cross: q and the output
+// [batch * seq_q, heads * d] rows, k and v [batch * seq_k, kv_heads * d], each
+// in any leading shape of that many elements.
+static NodeRef fused_cross_attention(const NodeRef& q, const NodeRef& k, const NodeRef& v,
+                                     const IntsRef& key_len, size_t batch, size_t heads,
+                                     size_t kv_heads, size_t seq_q, size_t seq_k, size_t d) {
+    GpuBuffers& qg = gpu_of(q, "cross attention: q not on GPU");
+    GpuBuffers& kg = gpu_of(k, "cross attention: k not on GPU");
+    GpuBuffers& vg = gpu_of(v, "cross attention: v not on GPU");
+    if (key_len && key_len->len() != batch)
+        throw Panic("cross attention: key_len must have one length per item");
+    const size_t ld_q = heads * d, ld_kv = kv_heads * d;
+    const float scale = 1.0f / std::sqrt(static_cast<float>(d));
+    const size_t q_len = batch * seq_q * ld_q, kv_len = batch * seq_k * ld_kv;
+    DeviceBuffer out(q_len, false);
+    auto stats = std::make_shared<DeviceBuffer>(batch * heads * seq_q * 2, false);
+    check(nrs_cross_attention_forward(out.ptr(), stats->ptr(), qg.data.ptr(), kg.data.ptr(),
+                                      vg.data.ptr(), key_len ? key_len->ptr() : nullptr, batch,
+                                      heads, kv_heads, seq_q, seq_k, d, ld_q, ld_kv, ld_q, scale,
+                                      nullptr, 0),
+          "cross attention: launch failed");
+    NodeRef node = make_output(q->shape, {q, k, v}, std::move(out));
+    Node* self = node.get();
+    node->backward_fn = [grad = node->gpu->grad, self, q, k, v, key_len, stats, q_len, kv_len,
+                         batch, heads, kv_heads, seq_q, seq_k, d, ld_q, ld_kv,
+                         scale](const std::vector<float>&) {
+        GpuBuffers& qg = gpu_of(q, "cross attention bwd: q not on GPU");
+        GpuBuffers& kg = gpu_of(k, "cross attention bwd: k not on GPU");
+        GpuBuffers& vg = gpu_of(v, "cross attention bwd: v not on GPU");
+        auto run = [&](float* dq, float* dk, float* dv, float beta_q, float beta_kv) {
+            check(nrs_cross_attention_backward(
+                      dq, dk, dv, grad->ptr(), self->gpu->data.ptr(), qg.data.ptr(),
+                      kg.data.ptr(), vg.data.ptr(), stats->ptr(),
+                      key_len ? key_len->ptr() : nullptr, batch, heads, kv_heads, seq_q, seq_k, d,
+                      ld_q, ld_kv, ld_q, scale, beta_q, beta_kv, nullptr, 0),
+                  "cross attention bwd: launch");
+        };
+        if (qg.grad != kg.grad && kg.grad != vg.grad && qg.grad != vg.grad) {
+            const float beta_kv = joint_beta({kg.grad.get(), vg.grad.get()});
+            float beta_q = 1.0f;
+            float* dq = qg.grad->acc_target(beta_q);
+            run(dq, kg.grad->write_target(), vg.grad->write_target(), beta_q, beta_kv);
+            return;
+        }
+        // q, k or v are one node: the gradients go to temporaries, then add up
+        DeviceBuffer tq(q_len, false), tk(kv_len, false), tv(kv_len, false);
+        run(tq.ptr(), tk.ptr(), tv.ptr(), 0.0f, 0.0f);
+        accumulate_into(*qg.grad, tq.ptr(), q_len);
+        accumulate_into(*kg.grad, tk.ptr(), kv_len);
+        accumulate_into(*vg.grad, tv.ptr(), kv_len);
+    };
+    return node;
+}
+
+NodeRef cross_attention(const NodeRef& q, const NodeRef& k, const NodeRef& v, size_t heads,
+                        size_t kv_heads, const IntsRef& key_len) {
+    if (q->shape.size() != 3 || k->shape.size() != 3)
+        throw Panic("cross attention: q and k must be [batch, seq, width]");
+    const size_t batch = q->shape[0], width = q->shape[2];
+    if (heads == 0 || kv_heads == 0 || width % heads != 0)
+        throw Panic("cross attention: width % heads != 0");
+    const size_t d = width / heads;
+    if (k->shape[0] != batch || k->shape[2] != kv_heads * d || v->shape != k->shape)
+        throw Panic("cross attention: shape mismatch");
+    return fused_cross_attention(q, k, v, key_len, batch, heads, kv_heads, q->shape[1],
+                                 k->shape[1], d);
+}
+
+NodeRef MultiHeadAttention::forward_cross(const NodeRef& x, const NodeRef& memory,
+                                          const IntsRef& key_len) const {
+    if (x->shape.size() != 3 || memory->shape.size() != 3)
+        throw Panic("multihead: x and memory must be [batch, seq, d_model]");
+    if (num_heads == 0 || d_model % num_heads != 0) throw Panic("multihead: d_model % heads != 0");
+    const size_t batch = x->shape[0], seq_q = x->shape[1], seq_k = memory->shape[1];
+    if (x->shape[2] != d_model || memory->shape[2] != d_model || memory->shape[0] != batch)
+        throw Panic("multihead: input width is not d_model");
+    const NodeRef q = graph::matmul(reshape_view(x, {batch * seq_q, d_model}), w_q);
+    const std::vector<NodeRef> kv =
+        matmul_shared_lhs(reshape_view(memory, {batch * seq_k, d_model}), {w_k, w_v});
+    const NodeRef heads = fused_cross_attention(q, kv[0], kv[1], key_len, batch, num_heads,
+                                                num_heads, seq_q, seq_k, d_model / num_heads);
+    return graph::reshape(graph::matmul(heads, w_o), {batch, seq_q, d_model});
+}
+
+NodeRef Embedding::forward(const IntsRef& ids, std::vector<size_t> shape) const {
+    GpuBuffers& tg = gpu_of(table, "embedding: table not on GPU");
+    if (table->shape.size() != 2) throw Panic("embedding: table must be [vocab, dim]");
+    const size_t vocab = table->shape[0], dim = table->shape[1], count = product(shape);
+    if (!ids || ids->len() != count) throw Panic("embedding: shape does not match the ids");
+    DeviceBuffer out(count * dim, false);
+    check(nrs_embedding_forward(out.ptr(), tg.data.ptr(), ids->ptr(), count, vocab, dim, scale),
+          "embedding: launch failed");
+    shape.push_back(dim);
+    NodeRef node = make_output(std::move(shape), {table}, std::move(out));
+    node->backward_fn = [grad = node->gpu->grad, ids, table = table, count, vocab, dim,
+                         scale = scale](const std::vector<float>&) {
+        float beta = 1.0f;
+        float* dtable = gpu_of(table, "embedding bwd: table not on GPU").grad->acc_target(beta);
+        check(nrs_embedding_backward(dtable, grad->ptr(), ids->ptr(), count, vocab, dim, scale,
+                                     beta, nullptr, 0),
+              "embedding bwd: launch");
+    };
+    return node;
+}
+
+NodeRef dropout(const NodeRef& x, float p, uint64_t seed, uint64_t call, const NodeRef& residual) {
+    GpuBuffers& xg = gpu_of(x, "dropout: input not on GPU");
+    const size_t n = product(x->shape);
+    if (residual && residual->shape != x->shape) throw Panic("dropout: residual shape mismatch");
+    const float* add =
+        residual ? gpu_of(residual, "dropout: residual not on GPU").data.ptr() : nullptr;
+    DeviceBuffer out(n, false);
+    check(nrs_dropout_forward(out.ptr(), xg.data.ptr(), add, n, p, seed, call, nullptr),
+          "dropout: launch failed");
+    std::vector<NodeRef> parents{x};
+    if (residual) parents.push_back(residual);
+    NodeRef node = make_output(x->shape, std::move(parents), std::move(out));
+    node->backward_fn = [grad = node->gpu->grad, x, residual, n, p, seed,
+                         call](const std::vector<float>&) {
+        float beta = 1.0f;
+        float* gx = gpu_of(x, "dropout bwd: input not on GPU").grad->acc_target(beta);
+        check(nrs_dropout_backward(gx, grad->ptr(), n, p, seed, call, nullptr, beta),
+              "dropout bwd: launch");
+        if (residual)
+            accumulate_into(*gpu_of(residual, "dropout bwd: residual not on GPU").grad,
+                            grad->ptr(), n);
+    };
+    return node;
+}
+
+NodeRef Dropout::forward(const NodeRef& x, const NodeRef& residual) {
+    if (training) return dropout(x, p, seed, calls++, residual);
+    return residual ? graph::add(residual, x) : x;
 }
 
 NodeRef SelfAttention::forward(const NodeRef& x) const {

@@ -12,6 +12,7 @@
 //          concat_cols, scaled_softmax}
 //                                        src/cuda/graph/*.rs
 //   nn::{conv2d, maxpool2d, Linear, attention, attention_batch, layernorm,
+//        cross_attention, Embedding, dropout, Dropout,
 //        SelfAttention, MultiHeadAttention, TransformerBlock}
 //                                        src/cuda/nn/*.rs
 // Rc<RefCell<Node>> becomes std::shared_ptr<Node>; a panic ("cuda matmul: lhs
@@ -26,6 +27,7 @@
 #pragma once
 
 #include <cstddef>
+#include <cstdint>
 #include <functional>
 #include <memory>
 #include <stdexcept>
@@ -110,6 +112,23 @@ private:
     mutable bool pending_zero_ = false;
     bool owned_ = true;
 };
+
+// Whole numbers on the device that no gradient flows to: token ids, lengths.
+class DeviceInts {
+public:
+    explicit DeviceInts(const std::vector<int32_t>& v);  // copies v
+    ~DeviceInts();
+    DeviceInts(const DeviceInts&) = delete;
+    DeviceInts& operator=(const DeviceInts&) = delete;
+    const int32_t* ptr() const { return ptr_; }
+    size_t len() const { return len_; }
+
+private:
+    int32_t* ptr_ = nullptr;
+    size_t len_ = 0;
+};
+using IntsRef = std::shared_ptr<const DeviceInts>;
+IntsRef device_ints(const std::vector<int32_t>& v);
 
 // src/autograd/node.rs:49-53: device data plus a shared, swappable gradient.
 struct GpuBuffers {
@@ -249,6 +268,43 @@ NodeRef attention_batch(const NodeRef& q, const NodeRef& k, const NodeRef& v);
 // with gamma/beta [features].
 NodeRef layernorm(const NodeRef& input, const NodeRef& gamma, const NodeRef& beta, float eps);
 
+// softmax(q . k^T / sqrt(d)) . v for every head over item b's first key_len[b]
+// keys (null: all): q [batch, seq_q, heads * d], k and v [batch, seq_k,
+// kv_heads * d], heads / kv_heads query heads to a key head, d at most 128. One
+// fused node.
+NodeRef cross_attention(const NodeRef& q, const NodeRef& k, const NodeRef& v, size_t heads,
+                        size_t kv_heads, const IntsRef& key_len = nullptr);
+
+// The reference's embedding layer (src/cuda/nn/embedding): resident table
+// [vocab, dim]; the rows of `ids`, times scale (sqrt(dim) in a Transformer). An
+// id outside the table, -1 for padding, gives zeros and no gradient.
+struct Embedding {
+    NodeRef table;
+    float scale = 1.0f;
+    // ids of any shape -> [shape..., dim]
+    NodeRef forward(const IntsRef& ids, std::vector<size_t> shape) const;
+    NodeRef forward(const std::vector<int32_t>& ids, std::vector<size_t> shape) const {
+        return forward(device_ints(ids), std::move(shape));
+    }
+};
+
+// x / (1 - p) where kept, else 0, plus residual unless null. The mask is a
+// function of p, seed and call (nrs_dropout_forward) and is made again by the
+// backward. x unchanged (or the sum alone) with p 0.
+NodeRef dropout(const NodeRef& x, float p, uint64_t seed, uint64_t call,
+                const NodeRef& residual = nullptr);
+// The reference's dropout layer (src/cuda/nn/dropout): another mask at every
+// call while training, nothing otherwise. Layers of one model take seeds of
+// their own.
+struct Dropout {
+    float p;
+    uint64_t seed;
+    bool training = true;
+    uint64_t calls = 0;
+    Dropout(float p, uint64_t seed) : p(p), seed(seed) {}
+    NodeRef forward(const NodeRef& x, const NodeRef& residual = nullptr);
+};
+
 // src/cuda/nn/self_attention.rs:10-37: single-head self-attention over
 // resident projections w_q, w_k, w_v [d_model, d_k]: x [seq, d_model] ->
 // attention(x w_q, x w_k, x w_v) [seq, d_k] (the three projections of one
@@ -283,6 +339,12 @@ struct MultiHeadAttention {
           d_model(d), num_heads(heads) {}
     NodeRef forward(const NodeRef& x) const;        // [seq, d_model]
     NodeRef forward_batch(const NodeRef& x) const;  // [batch, seq, d_model]
+    // A decoder's attention to an encoder's states of another length, which
+    // the reference has no counterpart for: queries from x [batch, seq_q,
+    // d_model], keys and values from memory [batch, seq_k, d_model], of which
+    // item b's first key_len[b] are live (null: all). Heads of at most 128.
+    NodeRef forward_cross(const NodeRef& x, const NodeRef& memory,
+                          const IntsRef& key_len = nullptr) const;
 };
 
 // src/cuda/nn/transformer_block.rs:9-45: post-norm block, x + MHA(x) -> norm1
