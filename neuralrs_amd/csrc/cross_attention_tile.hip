@@ -28,9 +28,10 @@
 // The forward's softmax is online in base 2, against a reference m that
 // follows the running maximum only when that passes it by 2^8: sums of
 // probabilities up to 256 lose nothing in f32, and most tiles need no
-// rescaling of the accumulators. The products start from -m (in the backward
-// from -log2 of the row's sum, and from -dout . out), so neither needs a
-// subtraction.
+// rescaling of the accumulators. The products start from -m, so the exponent
+// needs no subtraction. (The backward subtracts: -log2 of a row's sum is larger
+// than the scores that matter, and every rounding on the way would be of its
+// size. dout . out is small, and dout . v starts from its negative.)
 #include <algorithm>
 
 #include "cross_attention.hpp"
@@ -192,6 +193,12 @@ __device__ __forceinline__ void own_pieces(u32x4 (&own)[C::NS][3], const CrossAr
     }
 }
 
+// The operand of step s of the rows of block kb of a tile.
+template <class C>
+__device__ __forceinline__ u32x4 met_piece(const u32x4* set, int kb, int s, int p, int c, int h) {
+    return set[p * C::PLANE + unit_at<C>(kb * 32 + c, 2 * s + h)];
+}
+
 // start + met . own^T of block kb of a tile.
 template <class C>
 __device__ __forceinline__ f32x16 products(const u32x4* set, const u32x4 (&own)[C::NS][3], int kb,
@@ -199,11 +206,35 @@ __device__ __forceinline__ f32x16 products(const u32x4* set, const u32x4 (&own)[
 #pragma unroll
     for (int s = 0; s < C::NS; ++s) {
         u32x4 met[3];
-        const int unit = unit_at<C>(kb * 32 + c, 2 * s + h);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) met[p] = set[p * C::PLANE + unit];
+        for (int p = 0; p < 3; ++p) met[p] = met_piece<C>(set, kb, s, p, c, h);
         start = mfma_split(met, own[s], start);
     }
+    return start;
+}
+
+// The same with fewer roundings: the five small products of all steps, then
+// the large ones. An instruction rounds its sum twice, and the small ones'
+// sum is 2^-7 of the whole, so that is rounded 2 NS times in place of 12 NS.
+template <class C>
+__device__ __forceinline__ f32x16 close_products(const u32x4* set, const u32x4 (&own)[C::NS][3],
+                                                 int kb, f32x16 start, int c, int h) {
+#pragma unroll
+    for (int s = 0; s < C::NS; ++s) {
+        u32x4 met[3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) met[p] = met_piece<C>(set, kb, s, p, c, h);
+        start = mfma32(met[2], own[s][0], start);
+        start = mfma32(met[1], own[s][1], start);
+        start = mfma32(met[0], own[s][2], start);
+        start = mfma32(met[1], own[s][0], start);
+        start = mfma32(met[0], own[s][1], start);
+    }
+    // (read again: the registers cannot hold the first pieces until now)
+    asm volatile("" : "+v"(c));
+#pragma unroll
+    for (int s = 0; s < C::NS; ++s)
+        start = mfma32(met_piece<C>(set, kb, s, 0, c, h), own[s][0], start);
     return start;
 }
 
@@ -458,8 +489,8 @@ __device__ __forceinline__ void dq_walk(const CrossArgs& a, u32x4* lds, int bloc
             const int n = L - t * C::KT;
 #pragma unroll
             for (int kb = 0; kb < C::NB; ++kb) {
-                f32x16 s = products<C>(kl, qf, kb, all16(nl), c, h);
-                const f32x16 dp = products<C>(kl + C::SET, gf, kb, all16(nd), c, h);
+                f32x16 s = close_products<C>(kl, qf, kb, all16(0.0f), c, h);
+                const f32x16 dp = close_products<C>(kl + C::SET, gf, kb, all16(nd), c, h);
                 if (n < C::KT) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
@@ -470,7 +501,7 @@ __device__ __forceinline__ void dq_walk(const CrossArgs& a, u32x4* lds, int bloc
                     float x[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        x[i] = __builtin_amdgcn_exp2f(s[8 * u + i]) * dp[8 * u + i];
+                        x[i] = __builtin_amdgcn_exp2f(s[8 * u + i] + nl) * dp[8 * u + i];
                     u32x4 p[3];
                     split8(x, p);
                     add_transposed<C>(acc, kl, kb, u, p, lane);
@@ -548,17 +579,19 @@ __device__ __forceinline__ void dkv_walk(const CrossArgs& a, u32x4* lds, float* 
         if (wave_live) {
 #pragma unroll
             for (int rb = 0; rb < C::NB; ++rb) {
-                f32x16 s, dp;  // start at -lse and -delta of the 16 rows
+                // the 16 rows' -lse and -delta; the latter is where dp starts
                 const float* const st = starts + buf * 2 * C::KT + rb * 32 + 4 * h;
+                f32x16 dp;
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[i + e] = st[2 * i + e];
-                        dp[i + e] = st[C::KT + 2 * i + e];
-                    }
-                s = products<C>(ql, kf, rb, s, c, h);
-                dp = products<C>(ql + C::SET, vf, rb, dp, c, h);
+                    for (int e = 0; e < 4; ++e) dp[i + e] = st[C::KT + 2 * i + e];
+                f32x16 s = close_products<C>(ql, kf, rb, all16(0.0f), c, h);
+                dp = close_products<C>(ql + C::SET, vf, rb, dp, c, h);
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i + e] += st[2 * i + e];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     float x[8], y[8];
