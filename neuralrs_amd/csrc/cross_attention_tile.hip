@@ -490,7 +490,7 @@ __device__ __forceinline__ void dq_walk(const CrossArgs& a, u32x4* lds, int bloc
 #pragma unroll
             for (int kb = 0; kb < C::NB; ++kb) {
                 f32x16 s = close_products<C>(kl, qf, kb, all16(0.0f), c, h);
-                const f32x16 dp = close_products<C>(kl + C::SET, gf, kb, all16(nd), c, h);
+                const f32x16 dp = products<C>(kl + C::SET, gf, kb, all16(nd), c, h);
                 if (n < C::KT) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
@@ -587,7 +587,7 @@ __device__ __forceinline__ void dkv_walk(const CrossArgs& a, u32x4* lds, float* 
 #pragma unroll
                     for (int e = 0; e < 4; ++e) dp[i + e] = st[C::KT + 2 * i + e];
                 f32x16 s = close_products<C>(ql, kf, rb, all16(0.0f), c, h);
-                dp = close_products<C>(ql + C::SET, vf, rb, dp, c, h);
+                dp = products<C>(ql + C::SET, vf, rb, dp, c, h);
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
 #pragma unroll
