@@ -542,8 +542,8 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
     if (items == 0 || R == 0) return p;
     if (!p.tiles) {
         const int64_t units = items * ((R + 15) / 16);
-        // Shared unless there are enough units to even out by themselves; at
-        // least two tiles of 16 keys to a wave. Workgroups to a compute unit
+        // Shared unless there are enough units by themselves; at least two
+        // tiles of 16 keys to a wave. Workgroups to a compute unit
         // by the bytes that each has on the way (a tile of K and V to a wave):
         // 1, 2 and 4 of them take 47, 48 and 51 us at d_head 128 (2 x 16384
         // keys, 8 key heads) and 38, 30 and 26 us, 3 26 us, at d_head 64 (32
@@ -551,7 +551,7 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
         const int64_t groups = std::min<int64_t>((d_head > 64 ? 1 : d_head > 32 ? 3 : 6) * cus,
                                                  units * ((seq_k + 15) / 16) / (2 * kRowWaves));
         p.blocks = units;
-        if (units < 4 * cus && batch <= kMaxSharedBatch && groups > 1) {
+        if (groups > units && batch <= kMaxSharedBatch) {
             p.groups = (int)groups;
             p.blocks = groups;
             const int64_t slots = (groups + units) * std::min<int64_t>(R, 16);
@@ -563,9 +563,9 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
         // one workgroup to a compute unit: the split with the least time, in
         // key tiles, of the fullest one; a workgroup's beginning and end cost
         // two tiles, a join four
-        const int rows = cross_forward_rows((int)R, (int)d_head);
+        const int rows = cross_forward_rows((int)R);
         const int64_t base = items * ((R + rows - 1) / rows);
-        const int64_t keys = cross_tile_keys((int)d_head), tiles = (seq_k + keys - 1) / keys;
+        const int64_t keys = cross_tile_keys((int)d_head, rows / 32), tiles = (seq_k + keys - 1) / keys;
         int64_t best = INT64_MAX;
         p.splits = 1;
         for (int s = 1; s <= 16 && s <= std::max<int64_t>(1, tiles / 2); ++s) {
@@ -604,8 +604,7 @@ BackwardPlan plan_backward(int64_t batch, int64_t heads, int64_t kv_heads, int64
     BackwardPlan p{1, 1, items * R, items * seq_k, 0, 0, 0};
     p.prepared = (size_t)((2 * p.rows + 3) / 4 * 4);  // needed without keys, too
     if (p.rows == 0 || p.keys == 0) return p;
-    const int64_t tile = cross_tile_keys((int)d_head),
-                  own = cross_backward_rows((int)R, (int)seq_k, (int)d_head);
+    const int64_t tile = cross_tile_keys((int)d_head, 4), own = kCrossBackwardRows;
     const int64_t q_len = (seq_k + tile - 1) / tile, kv_len = (R + tile - 1) / tile;
     const int64_t q_groups = items * ((R + own - 1) / own),
                   kv_groups = items * ((seq_k + own - 1) / own);
@@ -760,7 +759,7 @@ int nrs_cross_attention_backward(float* dq, float* dk, float* dv, const float* d
     a.dq_part = scratch + plan.prepared;
     a.dk_part = a.dq_part + plan.q_part;
     a.dv_part = a.dk_part + plan.kv_part;
-    const int own = nrs::cross_backward_rows(a.Sq * a.G, a.Sk, a.D);
+    const int own = nrs::kCrossBackwardRows;
     if (dq && rows)
         a.q_blocks = (int)((a.Sq * a.G + own - 1) / own * batch * kv_heads * plan.q_splits);
     if (!keys) a.dk = a.dv = nullptr;

@@ -63,13 +63,19 @@ __device__ __forceinline__ float* row_stats(const CrossArgs& a, int b, int kv, i
     return a.stats + (((int64_t)b * a.H + kv * a.G + (r - s * a.G)) * a.Sq + s) * 2;
 }
 
-// The kernels of cross_attention_tile.hip. Rows of a workgroup of the forward
-// (backward) and rows of K or of the queries it takes at a time, by which the
-// calls are planned.
+// The kernels of cross_attention_tile.hip, and the sizes by which calls are
+// planned. A workgroup of the forward owns 32 rows to a wave: 8 waves past 128
+// rows, 4 up to that. The backward has 4 waves, and two workgroups to a compute
+// unit up to d_head 64: the same time as one of 8 waves at 4 x 1000 x 1500
+// (16 heads of 64: 513 us, 527), and fewer idle waves where an item has few
+// rows or keys.
+constexpr int kCrossBackwardRows = 128;
+constexpr int cross_forward_rows(int R) { return R > 128 ? 256 : 128; }
 constexpr int cross_tile_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
-constexpr int cross_tile_keys(int D) { return 4096 / cross_tile_width(D); }
-int cross_forward_rows(int R, int D);
-int cross_backward_rows(int R, int Sk, int D);
+// Keys (or rows) that a workgroup of that many waves takes at a time.
+constexpr int cross_tile_keys(int D, int waves) {
+    return (waves == 8 || D > 64 ? 4096 : 2048) / cross_tile_width(D);
+}
 void cross_tile_forward(const CrossArgs& a);
 void cross_tile_backward(const CrossArgs& a);
 

@@ -84,10 +84,13 @@ __device__ __forceinline__ f32x16 all16(float x) {
     return v;
 }
 
+// One wave to a SIMD when a wide head's operands fill its registers.
+constexpr int waves_per_simd(int D, int waves) { return D > 64 && waves == 4 ? 1 : 2; }
+
 template <int D_, int WAVES_>
 struct TileCfg {
     static constexpr int D = D_, WAVES = WAVES_, NT = 64 * WAVES;
-    static constexpr int KT = 4096 / D;       // rows of a tile
+    static constexpr int KT = cross_tile_keys(D, WAVES);  // rows of a tile
     static constexpr int Q = D / 8;           // units of a row
     static constexpr int PLANE = KT * Q;      // units of a plane
     static constexpr int U = PLANE / NT;      // units a thread stages
@@ -301,7 +304,7 @@ __device__ __forceinline__ void share(int count, int no, int shares, int& from, 
 }
 
 template <int D, int WAVES, bool FULL>
-__global__ __launch_bounds__(64 * WAVES) void cross_tile_fwd_kernel(CrossArgs a) {
+__global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void cross_tile_fwd_kernel(CrossArgs a) {
     using C = TileCfg<D, WAVES>;
     __shared__ u32x4 lds[2][2 * C::SET];
     const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
@@ -634,8 +637,9 @@ __device__ __forceinline__ void dkv_walk(const CrossArgs& a, u32x4* lds, float* 
 
 // One launch for both: they need nothing of each other, and the workgroups of
 // one fill the compute units that the other leaves idle.
-template <int D, int WAVES, bool FULL>
-__global__ __launch_bounds__(64 * WAVES) void cross_tile_bwd_kernel(CrossArgs a) {
+template <int D, bool FULL>
+__global__ __launch_bounds__(256, waves_per_simd(D, 4)) void cross_tile_bwd_kernel(CrossArgs a) {
+    constexpr int WAVES = 4;
     using C = TileCfg<D, WAVES>;
     __shared__ u32x4 lds[4 * C::SET];
     __shared__ float starts[4 * C::KT];
@@ -647,7 +651,7 @@ __global__ __launch_bounds__(64 * WAVES) void cross_tile_bwd_kernel(CrossArgs a)
 
 template <int D>
 void launch_forward(const CrossArgs& a) {
-    const int R = a.Sq * a.G, rows = cross_forward_rows(R, D);
+    const int R = a.Sq * a.G, rows = cross_forward_rows(R);
     const unsigned grid = (unsigned)(((R + rows - 1) / rows) * (int64_t)a.B * a.KV * a.splits);
     const bool full = a.D == D;
     auto kernel = rows == 256
@@ -656,18 +660,22 @@ void launch_forward(const CrossArgs& a) {
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(2 * rows), 0, stream(), a);
 }
 
-template <int D, int WAVES>
-void launch_backward(const CrossArgs& a, unsigned grid) {
-    auto kernel = a.D == D ? cross_tile_bwd_kernel<D, WAVES, true> : cross_tile_bwd_kernel<D, WAVES, false>;
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * WAVES), 0, stream(), a);
+template <int D>
+void launch_backward(const CrossArgs& a) {
+    const int64_t items = (int64_t)a.B * a.KV, rows = items * a.Sq * a.G;
+    if (rows > 0) {
+        constexpr int PER = 1024 / D;
+        hipLaunchKernelGGL(cross_rows_prepare_kernel<D>, dim3((unsigned)((rows + PER - 1) / PER)),
+                           dim3(256), 0, stream(), a);
+    }
+    const int64_t kv_blocks =
+        a.dk ? (a.Sk + kCrossBackwardRows - 1) / kCrossBackwardRows * items * a.kv_splits : 0;
+    if (a.q_blocks + kv_blocks == 0) return;
+    auto kernel = a.D == D ? cross_tile_bwd_kernel<D, true> : cross_tile_bwd_kernel<D, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.q_blocks + kv_blocks)), dim3(256), 0, stream(), a);
 }
 
 }  // namespace
-
-int cross_forward_rows(int R, int) { return R > 128 ? 256 : 128; }
-
-// Wide heads' operands fill the registers of one wave to a SIMD.
-int cross_backward_rows(int R, int Sk, int D) { return D <= 64 && std::max(R, Sk) > 128 ? 256 : 128; }
 
 void cross_tile_forward(const CrossArgs& a) {
     if (a.D <= 32)
@@ -679,25 +687,12 @@ void cross_tile_forward(const CrossArgs& a) {
 }
 
 void cross_tile_backward(const CrossArgs& a) {
-    const int R = a.Sq * a.G, rows = cross_backward_rows(R, a.Sk, a.D);
-    const int64_t items = (int64_t)a.B * a.KV;
-    if (R > 0) {
-        const int width = cross_tile_width(a.D), per = 1024 / width;
-        auto prepare = width == 32   ? cross_rows_prepare_kernel<32>
-                       : width == 64 ? cross_rows_prepare_kernel<64>
-                                     : cross_rows_prepare_kernel<128>;
-        hipLaunchKernelGGL(prepare, dim3((unsigned)((items * R + per - 1) / per)), dim3(256), 0,
-                           stream(), a);
-    }
-    const unsigned grid =
-        (unsigned)(a.q_blocks + (a.dk ? (a.Sk + rows - 1) / rows * items * a.kv_splits : 0));
-    if (grid == 0) return;
     if (a.D <= 32)
-        rows == 256 ? launch_backward<32, 8>(a, grid) : launch_backward<32, 4>(a, grid);
+        launch_backward<32>(a);
     else if (a.D <= 64)
-        rows == 256 ? launch_backward<64, 8>(a, grid) : launch_backward<64, 4>(a, grid);
+        launch_backward<64>(a);
     else
-        launch_backward<128, 4>(a, grid);
+        launch_backward<128>(a);
 }
 
 }  // namespace nrs
