@@ -525,6 +525,7 @@ int check_shape(const char* what, int64_t batch, int64_t heads, int64_t kv_heads
 
 struct ForwardPlan {
     bool tiles;        // the kernel of many rows
+    int rows;          // tiles: rows of a workgroup
     int splits;        // tiles: workgroups that share an item's keys
     int groups;        // few rows: workgroups that share all units, 0: one each
     int64_t blocks;    // workgroups of the launch
@@ -538,7 +539,7 @@ constexpr int64_t kFewRows = 32;
 ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
                          int64_t seq_k, int64_t d_head) {
     const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads, cus = num_cus();
-    ForwardPlan p{R > kFewRows, 1, 0, 0, 0, 0, 0};
+    ForwardPlan p{R > kFewRows, 128, 1, 0, 0, 0, 0, 0};
     if (items == 0 || R == 0) return p;
     if (!p.tiles) {
         const int64_t units = items * ((R + 15) / 16);
@@ -563,9 +564,16 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
         // one workgroup to a compute unit: the split with the least time, in
         // key tiles, of the fullest one; a workgroup's beginning and end cost
         // two tiles, a join four
-        const int rows = cross_forward_rows((int)R);
-        const int64_t base = items * ((R + rows - 1) / rows);
-        const int64_t keys = cross_tile_keys((int)d_head, rows / 32), tiles = (seq_k + keys - 1) / keys;
+        // 256 rows to a workgroup when the call has eight steps of such a one
+        // for every compute unit, else 128: 7 x 266 x 425, 8 heads of 128
+        // (6 steps), 65 us with 256 and 53 with 128; 4 x 512 x 1500, 16 heads of
+        // 64 (12), 86 and 101
+        const int width = cross_tile_width((int)d_head);
+        const int64_t steps = items * ((R + 255) / 256) * ((seq_k * width + 4095) / 4096);
+        p.rows = R > 128 && steps >= 8 * cus ? 256 : 128;
+        const int64_t base = items * ((R + p.rows - 1) / p.rows);
+        const int64_t keys = cross_tile_keys((int)d_head, p.rows / 32),
+                      tiles = (seq_k + keys - 1) / keys;
         int64_t best = INT64_MAX;
         p.splits = 1;
         for (int s = 1; s <= 16 && s <= std::max<int64_t>(1, tiles / 2); ++s) {
@@ -608,7 +616,7 @@ BackwardPlan plan_backward(int64_t batch, int64_t heads, int64_t kv_heads, int64
     const int64_t q_len = (seq_k + tile - 1) / tile, kv_len = (R + tile - 1) / tile;
     const int64_t q_groups = items * ((R + own - 1) / own),
                   kv_groups = items * ((seq_k + own - 1) / own);
-    const int64_t even = std::max<int64_t>(8, (3 * q_groups * q_len + 4 * kv_groups * kv_len) / (2 * cus));
+    const int64_t even = std::max<int64_t>(16, (3 * q_groups * q_len + 4 * kv_groups * kv_len) / (2 * cus));
     auto shares = [&](int64_t cost, int64_t len) {
         return (int)std::max<int64_t>(1, std::min<int64_t>({(cost + even - 1) / even, len, 64}));
     };
@@ -661,6 +669,7 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
     float* scratch = nullptr;
     if (int rc = nrs::call_scratch(&scratch, plan.bytes(), work, work_bytes, what)) return rc;
     nrs::CrossArgs a{};
+    a.rows = plan.rows;
     a.splits = plan.splits;
     a.groups = plan.groups;
     a.part = scratch;

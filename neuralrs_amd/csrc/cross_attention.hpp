@@ -25,7 +25,7 @@ struct CrossArgs {
     // forward of many rows: workgroups that share an item's keys. Past 1,
     // `part` has [splits][items][R][D] sums, not yet divided, and part_stats
     // their reference and sum, [items][R][splits][2]
-    int splits;
+    int rows, splits;  // rows: of a workgroup
     // forward of few rows: workgroups that share the launch's key tiles, or 0.
     // Then `part` has [slots][min(R, 16)][D], part_stats [slots][min(R, 16)][2]
     // and `shares` the first and the last workgroup of each unit
@@ -64,13 +64,11 @@ __device__ __forceinline__ float* row_stats(const CrossArgs& a, int b, int kv, i
 }
 
 // The kernels of cross_attention_tile.hip, and the sizes by which calls are
-// planned. A workgroup of the forward owns 32 rows to a wave: 8 waves past 128
-// rows, 4 up to that. The backward has 4 waves, and two workgroups to a compute
-// unit up to d_head 64: the same time as one of 8 waves at 4 x 1000 x 1500
-// (16 heads of 64: 513 us, 527), and fewer idle waves where an item has few
-// rows or keys.
+// planned. A workgroup of the forward owns 256 rows (8 waves) or 128 (4), one of
+// the backward 128 rows or keys, two workgroups to a compute unit up to d_head
+// 64: the time of one of 8 waves at 4 x 1000 x 1500 (16 heads of 64: 534 us,
+// 553), and fewer idle waves where an item has few rows or keys.
 constexpr int kCrossBackwardRows = 128;
-constexpr int cross_forward_rows(int R) { return R > 128 ? 256 : 128; }
 constexpr int cross_tile_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 // Keys (or rows) that a workgroup of that many waves takes at a time.
 constexpr int cross_tile_keys(int D, int waves) {

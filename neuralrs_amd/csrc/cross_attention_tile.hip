@@ -651,7 +651,7 @@ __global__ __launch_bounds__(256, waves_per_simd(D, 4)) void cross_tile_bwd_kern
 
 template <int D>
 void launch_forward(const CrossArgs& a) {
-    const int R = a.Sq * a.G, rows = cross_forward_rows(R);
+    const int R = a.Sq * a.G, rows = a.rows;
     const unsigned grid = (unsigned)(((R + rows - 1) / rows) * (int64_t)a.B * a.KV * a.splits);
     const bool full = a.D == D;
     auto kernel = rows == 256
