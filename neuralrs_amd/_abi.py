@@ -261,6 +261,15 @@ def bmm_backward(layout, dA, dB, G, A, B, batch, m, k, n, beta=0.0):
          batch, m, k, n, beta)
 
 
+def _launch(fn, *args):
+    """An entry point's call with arguments that are pointers and numbers already:
+    `call` looks at each of them (dropout of 8192 floats, both directions, takes
+    9.9 us through it, 9.2 like this)."""
+    rc = fn(*args)
+    if rc != 0:
+        check(rc, fn.__name__)
+
+
 def _work(buf):
     """The (work, work_bytes) arguments of an optional scratch buffer."""
     if buf is None:
@@ -280,9 +289,9 @@ def cross_attention_forward(out, stats, q, k, v, key_len, batch, heads, kv_heads
                             d_head, ld_q, ld_kv, ld_out, scale, work=None):
     """out = softmax(scale * q . k^T) . v of every head over each item's first
     key_len keys (None: all); stats may be None when no backward follows."""
-    call("nrs_cross_attention_forward", _ptr(out), _ptr(stats), _ptr(q), _ptr(k), _ptr(v),
-         _ptr(key_len), batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv, ld_out, scale,
-         *_work(work))
+    _launch(load().nrs_cross_attention_forward, _ptr(out), _ptr(stats), _ptr(q), _ptr(k), _ptr(v),
+            _ptr(key_len), batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv, ld_out,
+            scale, *_work(work))
 
 
 def cross_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, key_len, batch, heads,
@@ -290,14 +299,16 @@ def cross_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, key_len, bat
                              beta_q=0.0, beta_kv=0.0, work=None):
     """dq, dk and dv (+ beta * old) from the forward's out and stats; dq, or dk
     and dv, may be None."""
-    call("nrs_cross_attention_backward", _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dout), _ptr(out),
-         _ptr(q), _ptr(k), _ptr(v), _ptr(stats), _ptr(key_len), batch, heads, kv_heads, seq_q,
-         seq_k, d_head, ld_q, ld_kv, ld_out, scale, beta_q, beta_kv, *_work(work))
+    _launch(load().nrs_cross_attention_backward, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dout),
+            _ptr(out), _ptr(q), _ptr(k), _ptr(v), _ptr(stats), _ptr(key_len), batch, heads,
+            kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv, ld_out, scale, beta_q, beta_kv,
+            *_work(work))
 
 
 def embedding_forward(out, table, ids, count, vocab, dim, scale=1.0):
     """out[i] = scale * table[ids[i]] (int32 ids; zeros outside the table)."""
-    call("nrs_embedding_forward", _ptr(out), _ptr(table), _ptr(ids), count, vocab, dim, scale)
+    _launch(load().nrs_embedding_forward, _ptr(out), _ptr(table), _ptr(ids), count, vocab, dim,
+            scale)
 
 
 def embedding_workspace(count, vocab, dim):
@@ -309,19 +320,21 @@ def embedding_workspace(count, vocab, dim):
 
 def embedding_backward(dtable, grad, ids, count, vocab, dim, scale=1.0, beta=0.0, work=None):
     """dtable[t] = beta * dtable[t] + scale * sum of grad[i] over ids[i] = t."""
-    call("nrs_embedding_backward", _ptr(dtable), _ptr(grad), _ptr(ids), count, vocab, dim, scale,
-         beta, *_work(work))
+    _launch(load().nrs_embedding_backward, _ptr(dtable), _ptr(grad), _ptr(ids), count, vocab, dim,
+            scale, beta, *_work(work))
 
 
 def dropout_forward(out, x, residual, n, p, seed, number, step=None):
     """out = x / (1 - p) where kept, else 0 (+ residual unless None); `number`
     is the call's, step an optional device uint64 added to it."""
-    call("nrs_dropout_forward", _ptr(out), _ptr(x), _ptr(residual), n, p, seed, number, _ptr(step))
+    _launch(load().nrs_dropout_forward, _ptr(out), _ptr(x), _ptr(residual), n, p, seed, number,
+            _ptr(step))
 
 
 def dropout_backward(gin, grad, n, p, seed, number, step=None, beta=0.0):
     """gin = grad / (1 - p) where kept, else 0 (+ beta * gin)."""
-    call("nrs_dropout_backward", _ptr(gin), _ptr(grad), n, p, seed, number, _ptr(step), beta)
+    _launch(load().nrs_dropout_backward, _ptr(gin), _ptr(grad), n, p, seed, number,
+            _ptr(step), beta)
 
 
 def sync():
