@@ -87,15 +87,21 @@ struct BackwardArgs {
     int32_t* sorted;  // [count] positions by token, then by position
     int32_t* start;   // [vocab + 1] where each token's begin
     float* part;      // [tiles][2][dim] sums of runs from before, and into after, a tile
+    int32_t* crossing;  // [tiles][2] the run that begins in a tile and goes on past
+                        // it: its token (-1: none) and its last tile
 };
 
 // Zeros over workgroup `no` of `shares`' part of the table.
 __device__ __forceinline__ void clear_table(const BackwardArgs& a, int no, int shares) {
     const int64_t n = (int64_t)a.vocab * a.dim, quads = n / 4;
     Quad* const to = reinterpret_cast<Quad*>(a.dtable);
-    for (int64_t i = (int64_t)no * kSortThreads + threadIdx.x; i < quads;
-         i += (int64_t)shares * kSortThreads)
-        to[i].v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int64_t step = (int64_t)shares * kSortThreads;
+    int64_t i = (int64_t)no * kSortThreads + threadIdx.x;
+    for (; i + 3 * step < quads; i += 4 * step)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            __builtin_nontemporal_store(f32x4{0.0f, 0.0f, 0.0f, 0.0f}, &to[i + k * step].v);
+    for (; i < quads; i += step) to[i].v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     if (no == 0 && threadIdx.x < n - 4 * quads) a.dtable[4 * quads + threadIdx.x] = 0.0f;
 }
 
@@ -230,7 +236,10 @@ __global__ __launch_bounds__(64) void embedding_sum_kernel(BackwardArgs a) {
     const int d0 = (blockIdx.x - tile * a.blocks) * 256, d = d0 + 4 * lane;
     const int total = a.start[a.vocab];
     const int64_t e0 = (int64_t)tile * a.tile;
-    if (e0 >= total) return;
+    if (e0 >= total) {
+        if (d == 0) a.crossing[2 * tile] = -1;
+        return;
+    }
     const int e1 = (int)min((int64_t)total, e0 + a.tile);
     const bool whole = d + 4 <= a.dim;
     const int live = max(0, min(4, a.dim - d));
@@ -265,6 +274,11 @@ __global__ __launch_bounds__(64) void embedding_sum_kernel(BackwardArgs a) {
                 const bool head = __builtin_amdgcn_readlane(begin, i0 + i) < e0,
                            tail = __builtin_amdgcn_readlane(end, i0 + i) > e;
                 const bool inside = !head && !tail;
+                if (e == e1 && d == 0) {
+                    a.crossing[2 * tile] = tail && !head ? t : -1;
+                    a.crossing[2 * tile + 1] =
+                        (__builtin_amdgcn_readlane(end, i0 + i) - 1) / a.tile;
+                }
                 float* dst = inside ? a.dtable + (int64_t)t * a.dim + d
                                     : a.part + ((int64_t)tile * 2 + (head ? 0 : 1)) * a.dim + d;
                 f32x4 v = sum;
@@ -288,19 +302,13 @@ __global__ __launch_bounds__(64) void embedding_sum_kernel(BackwardArgs a) {
 // each, in order, and the quarters are added in order.
 __global__ __launch_bounds__(256) void embedding_join_kernel(BackwardArgs a) {
     __shared__ f32x4 quarter[4][64];
-    const int total = a.start[a.vocab];
-    const int tile = blockIdx.x / a.blocks;
-    const int64_t e0 = (int64_t)tile * a.tile;
-    const int64_t e1 = e0 + a.tile;
-    if (e1 >= total) return;  // the last tile's runs end in it
-    const int token = a.ids[a.sorted[e1 - 1]];
-    const int begin = a.start[token], end = a.start[token + 1];
-    if (begin < e0 || end <= e1) return;
+    const int tile = blockIdx.x / a.blocks, token = a.crossing[2 * tile];
+    if (token < 0) return;
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int d0 = (blockIdx.x - tile * a.blocks) * 256, d = d0 + 4 * lane, live = max(0, min(4, a.dim - d));
     // part 0 is the tile's own, part i the beginning of tile + i
-    const int n = (int)((end - 1) / a.tile) - tile + 1;
+    const int n = a.crossing[2 * tile + 1] - tile + 1;
     const int p0 = (int)((int64_t)n * w / 4), p1 = (int)((int64_t)n * (w + 1) / 4);
     f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int p = p0; p < p1; p += kBatch) {
@@ -327,8 +335,8 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(BackwardArgs a) {
 struct BackwardPlan {
     int bins, tile;
     int64_t groups, tiles;
-    size_t sorted, start, part;  // scratch, in 4-byte words
-    size_t bytes() const { return 4 * (sorted + start + part); }
+    size_t sorted, start, part, crossing;  // scratch, in 4-byte words
+    size_t bytes() const { return 4 * (sorted + start + part + crossing); }
 };
 
 BackwardPlan plan_backward(int64_t count, int64_t vocab, int64_t dim) {
@@ -345,6 +353,7 @@ BackwardPlan plan_backward(int64_t count, int64_t vocab, int64_t dim) {
     p.sorted = round4(count);
     p.start = round4(vocab + 1);
     p.part = round4(p.tiles * 2 * dim);
+    p.crossing = (size_t)(2 * p.tiles);
     return p;
 }
 
@@ -415,6 +424,7 @@ int nrs_embedding_backward(float* dtable, const float* grad, const int32_t* ids,
     a.sorted = reinterpret_cast<int32_t*>(scratch);
     a.start = a.sorted + plan.sorted;
     a.part = scratch + plan.sorted + plan.start;
+    a.crossing = reinterpret_cast<int32_t*>(a.part + plan.part);
     const int64_t clear =
         beta != 0.0f ? 0 : std::min<int64_t>((vocab * dim + 16383) / 16384, nrs::num_cus());
     hipLaunchKernelGGL(nrs::embedding_sort_kernel, dim3((unsigned)(plan.groups + clear)),
