@@ -502,10 +502,11 @@ const char* refusal(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_
         return "a row stride is shorter than its heads";
     if (ld_q > kMaxLd || ld_kv > kMaxLd || ld_out > kMaxLd) return "a row stride is past 2^20";
     if (seq_q > kMaxLen || seq_k > kMaxLen) return "a length is past 2^26";
-    // a launch has fewer than 2^32 threads, 256 for 16 rows or keys at most
+    // A launch has fewer than 2^32 threads, 256 for 16 rows or keys at most. Each
+    // factor is below 2^47: divided, not multiplied.
     const int64_t rows = (seq_q * (heads / kv_heads) + 15) / 16, keys = (seq_k + 15) / 16;
-    if (batch > kMaxGroups ||
-        batch * kv_heads * std::max<int64_t>({rows, keys, 1}) > kMaxGroups)
+    if (std::max<int64_t>({rows, keys, 1}) > kMaxGroups / kv_heads ||
+        batch > kMaxGroups / kv_heads / std::max<int64_t>({rows, keys, 1}))
         return "more than 2^26 rows or keys (in groups of 16 of an item)";
     return nullptr;
 }
@@ -642,8 +643,7 @@ int nrs_cross_attention_workspace(size_t* bytes, int64_t batch, int64_t heads, i
                                   int64_t seq_q, int64_t seq_k, int64_t d_head, int backward) {
     NRS_ARG_CHECK(bytes, "cross attention workspace: null pointer");
     if (int rc = nrs::check_shape("cross attention workspace", batch, heads, kv_heads, seq_q,
-                                  seq_k, d_head, heads * d_head, kv_heads * d_head,
-                                  heads * d_head))
+                                  seq_k, d_head, nrs::kMaxLd, nrs::kMaxLd, nrs::kMaxLd))
         return rc;
     *bytes = backward
                  ? nrs::plan_backward(batch, heads, kv_heads, seq_q, seq_k, d_head).bytes()

@@ -28,6 +28,11 @@ BAD = [
     (dict(batch=2 ** 20, seq_q=2 ** 20), "2\\^26"), (dict(batch=2 ** 12, seq_k=2 ** 16), "2\\^26"),
     (dict(seq_q=2 ** 26, heads=2 ** 14, kv_heads=1, ld_q=2 ** 19, ld_out=2 ** 19), "2\\^26"),
     (dict(heads=2 ** 62, kv_heads=1), "stride"),
+    # products of the sizes that 64 bits do not hold
+    (dict(batch=2 ** 22, heads=2 ** 15, kv_heads=2 ** 15, seq_q=2 ** 26, seq_k=2 ** 26, ld_q=2 ** 20,
+          ld_kv=2 ** 20, ld_out=2 ** 20), "2\\^26"),
+    (dict(batch=2 ** 62, heads=1, kv_heads=1), "2\\^26"),
+    (dict(batch=2 ** 22, heads=2 ** 15, kv_heads=1, seq_q=2 ** 26, ld_q=2 ** 20, ld_out=2 ** 20), "2\\^26"),
 ]
 
 
@@ -126,6 +131,14 @@ def test_workspace_of_a_backward_without_keys_or_rows():
     assert _abi.cross_attention_workspace(2, 4, 2, 0, 5, 32, backward=True) == 0
     assert _abi.cross_attention_workspace(2, 4, 2, 0, 5, 32) == 0
     assert _abi.cross_attention_workspace(0, 4, 2, 3, 5, 32) == 0
+
+
+@pytest.mark.parametrize("sizes", [(2, 4, 3, 3, 5, 32), (2, 2 ** 62, 1, 3, 5, 128), (2, 4, 2, 3, 5, 0),
+                                   (-1, 4, 2, 3, 5, 32), (2 ** 40, 4, 2, 3, 5, 32)])
+def test_workspace_refuses_what_the_calls_refuse(sizes):
+    for backward in (False, True):
+        with pytest.raises(_abi.NrsError):
+            _abi.cross_attention_workspace(*sizes, backward=backward)
 
 
 def test_workspace_queries():
