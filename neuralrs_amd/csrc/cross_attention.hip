@@ -311,10 +311,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void cross_rows_fwd_kernel(CrossArg
     }
 }
 
-// The sums of `count` parts of a row: each has its columns at stats(s), where
-// the reference and the sum are, and at part(s). 32 threads share the columns,
-// four each (d_head <= 128); lane s of them looks up part s, and the parts are
-// asked for eight at a time.
+// The sums of a row's parts: the reference and the sum of part s at stats(s),
+// its columns at part(s). LANES threads share the columns, four each; lane s of
+// them looks up part s, and the parts are asked for eight at a time.
+template <int LANES>
 struct Joined {
     float top = -INFINITY, total = 0.0f;
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -327,8 +327,8 @@ struct Joined {
 
     template <class S, class P>
     __device__ __forceinline__ void add(int s0, int s1, int live, S stats, P part) {
-        const int x = threadIdx.x % 32;
-        for (int c0 = s0; c0 < s1; c0 += 32) {
+        const int x = threadIdx.x % LANES;
+        for (int c0 = s0; c0 < s1; c0 += LANES) {
             float m = -INFINITY, l = 0.0f;
             if (c0 + x < s1) {
                 const float* st = stats(c0 + x);
@@ -337,16 +337,16 @@ struct Joined {
             }
             float most = m;
 #pragma unroll
-            for (int i = 1; i < 32; i *= 2) most = fmaxf(most, __shfl_xor(most, i, 32));
+            for (int i = 1; i < LANES; i *= 2) most = fmaxf(most, __shfl_xor(most, i, LANES));
             most = fmaxf(most, top);
             const float old = weight(top, total, most), f = weight(m, l, most);
             float sum = l * f;
 #pragma unroll
-            for (int i = 1; i < 32; i *= 2) sum += __shfl_xor(sum, i, 32);
+            for (int i = 1; i < LANES; i *= 2) sum += __shfl_xor(sum, i, LANES);
             total = total * old + sum;
             top = most;
             v = v * old;
-            for (int s = c0; s < min(c0 + 32, s1); s += 8) {
+            for (int s = c0; s < min(c0 + LANES, s1); s += 8) {
                 f32x4 x8[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -359,17 +359,20 @@ struct Joined {
                         for (int e = 0; e < live; ++e) x8[i][e] = src[e];
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v = v + x8[i] * __shfl(f, s + i - c0, 32);
+                for (int i = 0; i < 8; ++i) v = v + x8[i] * __shfl(f, s + i - c0, LANES);
             }
         }
     }
 
     __device__ __forceinline__ void store(const CrossArgs& a, int b, int kv, int r, int live) const {
-        const int x = threadIdx.x % 32;
+        const int x = threadIdx.x % LANES;
         const bool any = live_keys(a, b) > 0;
         const float scale = any ? 1.0f / total : 0.0f;
         float* dst = a.out + query_offset(a, b, kv, r, a.ld_out) + 4 * x;
-        for (int e = 0; e < live; ++e) dst[e] = v[e] * scale;
+        if (live == 4)
+            reinterpret_cast<Quad*>(dst)->v = v * scale;
+        else
+            for (int e = 0; e < live; ++e) dst[e] = v[e] * scale;
         if (a.stats && x == 0) {
             float* st = row_stats(a, b, kv, r);
             st[0] = any ? top : 0.0f;
@@ -388,7 +391,7 @@ __global__ __launch_bounds__(256) void cross_rows_join_kernel(CrossArgs a) {
     const int item = blockIdx.x / R, r = blockIdx.x - item * R;
     const int b = item / a.KV, kv = item - b * a.KV, unit = item * row_tiles + r / 16;
     const int live = max(0, min(4, a.D - 4 * x));
-    Joined sum;
+    Joined<32> sum;
     if (live_keys(a, b) > 0) {
         const int first = a.shares[2 * unit], n = a.shares[2 * unit + 1] - first + 1;
         if (n == 1) return;  // one workgroup took all of the unit
@@ -406,8 +409,8 @@ __global__ __launch_bounds__(256) void cross_rows_join_kernel(CrossArgs a) {
     if (group != 0) return;
     for (int i = 1; i < 8; ++i) {
         const float most = fmaxf(sum.top, tops[i]);
-        const float f = Joined::weight(sum.top, sum.total, most),
-                    g = Joined::weight(tops[i], totals[i], most);
+        const float f = Joined<32>::weight(sum.top, sum.total, most),
+                    g = Joined<32>::weight(tops[i], totals[i], most);
         sum.v = sum.v * f + sums[i][x] * g;
         sum.total = sum.total * f + totals[i] * g;
         sum.top = most;
@@ -415,15 +418,17 @@ __global__ __launch_bounds__(256) void cross_rows_join_kernel(CrossArgs a) {
     sum.store(a, b, kv, r, live);
 }
 
-// Joins the splits of cross_tile_fwd_kernel: 32 threads to a row.
+// Joins the splits of cross_tile_fwd_kernel: D / 4 threads to a row.
+template <int D>
 __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
-    const int R = a.Sq * a.G, x = threadIdx.x % 32;
+    constexpr int LANES = D / 4;
+    const int R = a.Sq * a.G, x = threadIdx.x % LANES;
     const int64_t rows = (int64_t)a.B * a.KV * R;
-    const int64_t at = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
+    const int64_t at = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
     if (at >= rows) return;
     const int item = (int)(at / R), r = (int)(at - (int64_t)item * R), b = item / a.KV;
     const int live = max(0, min(4, a.D - 4 * x));
-    Joined sum;
+    Joined<LANES> sum;
     sum.add(0, a.splits, live, [&](int s) { return a.part_stats + 2 * (at * a.splits + s); },
             [&](int s) { return a.part + (s * rows + at) * a.D; });
     sum.store(a, b, item - b * a.KV, r, live);
@@ -704,12 +709,17 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
         });
     }
     NRS_LAUNCH_CHECK(what);
-    if (a.groups > 0)
+    if (a.groups > 0) {
         hipLaunchKernelGGL(nrs::cross_rows_join_kernel, dim3((unsigned)rows), dim3(256), 0,
                            nrs::stream(), a);
-    else if (a.splits > 1)
-        hipLaunchKernelGGL(nrs::cross_join_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0,
+    } else if (a.splits > 1) {
+        const int width = nrs::cross_tile_width(a.D), per = 1024 / width;
+        auto join = width == 32   ? nrs::cross_join_kernel<32>
+                    : width == 64 ? nrs::cross_join_kernel<64>
+                                  : nrs::cross_join_kernel<128>;
+        hipLaunchKernelGGL(join, dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0,
                            nrs::stream(), a);
+    }
     NRS_LAUNCH_CHECK(what);
     return NRS_OK;
 }
