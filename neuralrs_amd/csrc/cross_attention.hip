@@ -122,18 +122,11 @@ __device__ __forceinline__ float across_groups(float x) {
 }
 
 constexpr int kRowWaves = 4;
-constexpr int kMaxSharedBatch = 1024;  // batch items of a shared launch
 
 // Few rows: K and V stream from HBM straight into registers, as operands of
 // v_mfma_f32_16x16x4_f32 (16 rows at 157 TFLOP/s keep pace with 8 TB/s of f32
 // keys and values). Waves of a workgroup take turns at tiles of 16 keys, each
 // with its next tile on the way, and are joined at the end.
-//
-// A unit is 16 rows of an item. With `groups` 0 a workgroup takes a unit. Else
-// the key tiles of all units lie one after the other and `groups` workgroups
-// take equal parts of that line, whatever the items' lengths: a unit that a
-// part begins or ends in leaves sums for cross_rows_join_kernel, in slot
-// (workgroup + unit), which no two share.
 template <int NJ>
 struct RowsWalk {
     const CrossArgs& a;
@@ -225,7 +218,7 @@ struct RowsWalk {
             static_assert(kRowWaves == 4, "a register of an accumulator to each wave");
             const bool whole = slot < 0;
             const float scale = !whole ? 1.0f : L > 0 ? 1.0f / total : 0.0f;
-            const int64_t at = slot * min(R, 16) + c;
+            const int64_t at = slot * a.unit_rows + c;
             float* dst = whole ? a.out + query_offset(a, b, kv, r0 + c, a.ld_out) : a.part + at * a.D;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
@@ -249,7 +242,7 @@ template <int NJ>
 __global__ __launch_bounds__(64 * kRowWaves) void cross_rows_fwd_kernel(CrossArgs a) {
     __shared__ float sums[kRowWaves][4 * NJ][64];
     __shared__ float tops[kRowWaves][16], totals[kRowWaves][16];
-    __shared__ int wave_sum[kRowWaves], found[2];
+    __shared__ int scan[kRowWaves], found[2];
     const RowsWalk<NJ> walk{a, sums, tops, totals};
     const int row_tiles = (a.Sq * a.G + 15) / 16, per_item = a.KV * row_tiles;
     if (a.groups == 0) {
@@ -258,57 +251,11 @@ __global__ __launch_bounds__(64 * kRowWaves) void cross_rows_fwd_kernel(CrossArg
         walk.run(b, sub / row_tiles, sub % row_tiles * 16, L, 0, (L + 15) / 16, -1);
         return;
     }
-    // where on the line each batch item begins: a scan of their lengths, which
-    // finds the item of this workgroup's first tile
-    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-    const int each = (a.B + 255) / 256;
-    int own = 0;
-    for (int i = 0; i < each; ++i)
-        if (t * each + i < a.B) own += (live_keys(a, t * each + i) + 15) / 16 * per_item;
-    int upto = own;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int v = __shfl_up(upto, d, 64);
-        if (lane >= d) upto += v;
-    }
-    if (lane == 63) wave_sum[w] = upto;
-    __syncthreads();
-    int begin = upto - own, total = 0;
-    for (int i = 0; i < kRowWaves; ++i) {
-        begin += i < w ? wave_sum[i] : 0;
-        total += wave_sum[i];
-    }
-    const int no = blockIdx.x;
-    const int p0 = (int)((int64_t)total * no / a.groups),
-              p1 = (int)((int64_t)total * (no + 1) / a.groups);
-    if (p0 >= p1) return;
-    for (int i = 0; i < each && t * each + i < a.B; ++i) {
-        const int n = (live_keys(a, t * each + i) + 15) / 16 * per_item;
-        if (begin <= p0 && p0 < begin + n) {
-            found[0] = t * each + i;
-            found[1] = begin;
-        }
-        begin += n;
-    }
-    __syncthreads();
-    int b = found[0], base = found[1];
-    for (int p = p0; p < p1;) {
-        const int L = live_keys(a, b), tiles = (L + 15) / 16;
-        if (p >= base + tiles * per_item) {  // the next item (those without keys have no tiles)
-            base += tiles * per_item;
-            ++b;
-            continue;
-        }
-        const int sub = (p - base) / tiles, t0 = p - base - sub * tiles;
-        const int t1 = min(tiles, t0 + p1 - p), unit = b * per_item + sub;
-        if (t == 0) {
-            if (t0 == 0) a.shares[2 * unit] = no;
-            if (t1 == tiles) a.shares[2 * unit + 1] = no;
-        }
-        walk.run(b, sub / row_tiles, sub % row_tiles * 16, L, t0, t1,
-                 t0 == 0 && t1 == tiles ? -1 : (int64_t)no + unit);
-        p += t1 - t0;
-    }
+    LinePart<64 * kRowWaves> part;
+    if (!part.begin(a, per_item, 16, scan, found)) return;
+    while (part.next(a))
+        walk.run(part.b, part.sub / row_tiles, part.sub % row_tiles * 16, part.L, part.t0, part.t1,
+                 part.slot());
 }
 
 // The sums of a row's parts: the reference and the sum of part s at stats(s),
@@ -381,25 +328,31 @@ struct Joined {
     }
 };
 
-// A workgroup to a row of cross_rows_fwd_kernel's units: eight groups of 32
-// threads take an eighth of the row's parts each and are added up in LDS.
+// The parts of row r of an item: their number (0: no live keys) and where the
+// first one is, in rows of `part`; the others follow unit_rows apart.
+__device__ __forceinline__ int row_parts(const CrossArgs& a, int item, int b, int r, int64_t& at) {
+    if (live_keys(a, b) == 0) return 0;
+    const int units = (a.Sq * a.G + a.unit_rows - 1) / a.unit_rows;
+    const int unit = item * units + r / a.unit_rows, first = a.shares[2 * unit];
+    at = ((int64_t)first + unit) * a.unit_rows + r % a.unit_rows;
+    return a.shares[2 * unit + 1] - first + 1;
+}
+
+// Joins the parts of cross_rows_fwd_kernel, a workgroup to a row: eight groups of
+// 32 threads take an eighth of them each and are added up in LDS.
 __global__ __launch_bounds__(256) void cross_rows_join_kernel(CrossArgs a) {
     __shared__ f32x4 sums[8][32];
     __shared__ float tops[8], totals[8];
-    const int x = threadIdx.x % 32, group = threadIdx.x / 32;
-    const int R = a.Sq * a.G, row_tiles = (R + 15) / 16, per = min(R, 16);
-    const int item = blockIdx.x / R, r = blockIdx.x - item * R;
-    const int b = item / a.KV, kv = item - b * a.KV, unit = item * row_tiles + r / 16;
+    const int x = threadIdx.x % 32, group = threadIdx.x / 32, R = a.Sq * a.G;
+    const int item = blockIdx.x / R, r = blockIdx.x - item * R, b = item / a.KV;
     const int live = max(0, min(4, a.D - 4 * x));
+    int64_t at = 0;
+    const int n = row_parts(a, item, b, r, at);
+    if (n == 1) return;  // one workgroup took all of the unit
     Joined<32> sum;
-    if (live_keys(a, b) > 0) {
-        const int first = a.shares[2 * unit], n = a.shares[2 * unit + 1] - first + 1;
-        if (n == 1) return;  // one workgroup took all of the unit
-        const int64_t at = ((int64_t)first + unit) * per + r % 16;
-        sum.add(n * group / 8, n * (group + 1) / 8, live,
-                [&](int s) { return a.part_stats + 2 * (at + (int64_t)s * per); },
-                [&](int s) { return a.part + (at + (int64_t)s * per) * a.D; });
-    }
+    sum.add(n * group / 8, n * (group + 1) / 8, live,
+            [&](int s) { return a.part_stats + 2 * (at + (int64_t)s * a.unit_rows); },
+            [&](int s) { return a.part + (at + (int64_t)s * a.unit_rows) * a.D; });
     sums[group][x] = sum.v;
     if (x == 0) {
         tops[group] = sum.top;
@@ -415,22 +368,24 @@ __global__ __launch_bounds__(256) void cross_rows_join_kernel(CrossArgs a) {
         sum.total = sum.total * f + totals[i] * g;
         sum.top = most;
     }
-    sum.store(a, b, kv, r, live);
+    sum.store(a, b, item - b * a.KV, r, live);
 }
 
-// Joins the splits of cross_tile_fwd_kernel: D / 4 threads to a row.
+// Joins the parts of cross_tile_fwd_kernel, which are few: D / 4 threads to a row.
 template <int D>
 __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
     constexpr int LANES = D / 4;
     const int R = a.Sq * a.G, x = threadIdx.x % LANES;
-    const int64_t rows = (int64_t)a.B * a.KV * R;
-    const int64_t at = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-    if (at >= rows) return;
-    const int item = (int)(at / R), r = (int)(at - (int64_t)item * R), b = item / a.KV;
+    const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    if (row >= (int64_t)a.B * a.KV * R) return;
+    const int item = (int)(row / R), r = (int)(row - (int64_t)item * R), b = item / a.KV;
     const int live = max(0, min(4, a.D - 4 * x));
+    int64_t at = 0;
+    const int n = row_parts(a, item, b, r, at);
+    if (n == 1) return;
     Joined<LANES> sum;
-    sum.add(0, a.splits, live, [&](int s) { return a.part_stats + 2 * (at * a.splits + s); },
-            [&](int s) { return a.part + (s * rows + at) * a.D; });
+    sum.add(0, n, live, [&](int s) { return a.part_stats + 2 * (at + (int64_t)s * a.unit_rows); },
+            [&](int s) { return a.part + (at + (int64_t)s * a.unit_rows) * a.D; });
     sum.store(a, b, item - b * a.KV, r, live);
 }
 
@@ -530,11 +485,10 @@ int check_shape(const char* what, int64_t batch, int64_t heads, int64_t kv_heads
 }
 
 struct ForwardPlan {
-    bool tiles;        // the kernel of many rows
-    int rows;          // tiles: rows of a workgroup
-    int splits;        // tiles: workgroups that share an item's keys
-    int groups;        // few rows: workgroups that share all units, 0: one each
-    int64_t blocks;    // workgroups of the launch
+    bool tiles;      // the kernel of many rows
+    int unit_rows;   // of a unit (the scratch of a call with fewer holds no more)
+    int groups;      // workgroups that share all units, 0: one each
+    int64_t blocks;  // workgroups of the launch
     size_t part, stats, shares;  // scratch, in 4-byte words
     size_t bytes() const { return 4 * (part + stats + shares); }
 };
@@ -542,59 +496,52 @@ struct ForwardPlan {
 // Rows of an item up to which the kernel of few rows takes the call.
 constexpr int64_t kFewRows = 32;
 
+// The scratch does not depend on key_len being there; the kernels read it.
 ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
                          int64_t seq_k, int64_t d_head) {
     const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads, cus = num_cus();
-    ForwardPlan p{R > kFewRows, 128, 1, 0, 0, 0, 0, 0};
+    ForwardPlan p{R > kFewRows, 16, 0, 0, 0, 0, 0};
     if (items == 0 || R == 0) return p;
+    int64_t units, groups;
+    bool share;
     if (!p.tiles) {
-        const int64_t units = items * ((R + 15) / 16);
+        units = items * ((R + 15) / 16);
         // Shared unless there are enough units by themselves; at least two
         // tiles of 16 keys to a wave. Workgroups to a compute unit
         // by the bytes that each has on the way (a tile of K and V to a wave):
         // 1, 2 and 4 of them take 47, 48 and 51 us at d_head 128 (2 x 16384
         // keys, 8 key heads) and 38, 30 and 26 us, 3 26 us, at d_head 64 (32
         // items of up to 1500 keys, 8 key heads).
-        const int64_t groups = std::min<int64_t>((d_head > 64 ? 1 : d_head > 32 ? 3 : 6) * cus,
-                                                 units * ((seq_k + 15) / 16) / (2 * kRowWaves));
-        p.blocks = units;
-        if (groups > units && batch <= kMaxSharedBatch) {
-            p.groups = (int)groups;
-            p.blocks = groups;
-            const int64_t slots = (groups + units) * std::min<int64_t>(R, 16);
-            p.part = (size_t)((slots * d_head + 3) / 4 * 4);
-            p.stats = (size_t)((2 * slots + 3) / 4 * 4);
-            p.shares = (size_t)(2 * units);
-        }
+        groups = std::min<int64_t>((d_head > 64 ? 1 : d_head > 32 ? 3 : 6) * cus,
+                                   units * ((seq_k + 15) / 16) / (2 * kRowWaves));
+        share = groups > units;
+        p.unit_rows = (int)std::min<int64_t>(R, 16);
     } else {
-        // one workgroup to a compute unit: the split with the least time, in
-        // key tiles, of the fullest one; a workgroup's beginning and end cost
-        // two tiles, a join four
         // 256 rows to a workgroup when the call has eight steps of such a one
         // for every compute unit, else 128: 7 x 266 x 425, 8 heads of 128
         // (6 steps), 65 us with 256 and 53 with 128; 4 x 512 x 1500, 16 heads of
         // 64 (12), 86 and 101
         const int width = cross_tile_width((int)d_head);
         const int64_t steps = items * ((R + 255) / 256) * ((seq_k * width + 4095) / 4096);
-        p.rows = R > 128 && steps >= 8 * cus ? 256 : 128;
-        const int64_t base = items * ((R + p.rows - 1) / p.rows);
-        const int64_t keys = cross_tile_keys((int)d_head, p.rows / 32),
+        p.unit_rows = R > 128 && steps >= 8 * cus ? 256 : 128;
+        units = items * ((R + p.unit_rows - 1) / p.unit_rows);
+        const int64_t keys = cross_tile_keys((int)d_head, p.unit_rows / 32),
                       tiles = (seq_k + keys - 1) / keys;
-        int64_t best = INT64_MAX;
-        p.splits = 1;
-        for (int s = 1; s <= 16 && s <= std::max<int64_t>(1, tiles / 2); ++s) {
-            const int64_t turns = (base * s + cus - 1) / cus;
-            const int64_t cost = turns * ((tiles + s - 1) / s + 2) + (s > 1 ? 4 : 0);
-            if (cost < best) {
-                best = cost;
-                p.splits = s;
-            }
-        }
-        p.blocks = base * p.splits;
-        if (p.splits > 1) {
-            p.part = (size_t)((p.splits * items * R * d_head + 3) / 4 * 4);
-            p.stats = (size_t)(2 * p.splits * items * R);
-        }
+        // Workgroups at once, and the time of the fullest one in key tiles: a
+        // piece's beginning and end cost two tiles, a join four.
+        const int64_t at_once = p.unit_rows == 128 && d_head <= 64 ? 2 * cus : cus;
+        groups = std::min<int64_t>(at_once, units * tiles / 2);
+        share = groups > 1 && (units + at_once - 1) / at_once * (tiles + 2) >
+                                  (units * tiles + groups - 1) / groups + 8;
+    }
+    p.blocks = units;
+    if (share && batch <= kMaxSharedBatch) {
+        p.groups = (int)groups;
+        p.blocks = groups;
+        const int64_t slots = (groups + units) * p.unit_rows;
+        p.part = (size_t)((slots * d_head + 3) / 4 * 4);
+        p.stats = (size_t)((2 * slots + 3) / 4 * 4);
+        p.shares = (size_t)(2 * units);
     }
     return p;
 }
@@ -674,8 +621,7 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
     float* scratch = nullptr;
     if (int rc = nrs::call_scratch(&scratch, plan.bytes(), work, work_bytes, what)) return rc;
     nrs::CrossArgs a{};
-    a.rows = plan.rows;
-    a.splits = plan.splits;
+    a.unit_rows = plan.unit_rows;
     a.groups = plan.groups;
     a.part = scratch;
     a.part_stats = scratch + plan.part;
@@ -700,7 +646,7 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
     a.scale = scale;
     a.scale2 = scale * 1.4426950408889634f;
     if (plan.tiles) {
-        nrs::cross_tile_forward(a);
+        nrs::cross_tile_forward(a, (unsigned)plan.blocks);
     } else {
         nrs::for_width(a.D, [&](auto nj) {
             hipLaunchKernelGGL(nrs::cross_rows_fwd_kernel<decltype(nj)::value>,
@@ -709,10 +655,10 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
         });
     }
     NRS_LAUNCH_CHECK(what);
-    if (a.groups > 0) {
+    if (a.groups > 0 && !plan.tiles) {
         hipLaunchKernelGGL(nrs::cross_rows_join_kernel, dim3((unsigned)rows), dim3(256), 0,
                            nrs::stream(), a);
-    } else if (a.splits > 1) {
+    } else if (a.groups > 0) {
         const int width = nrs::cross_tile_width(a.D), per = 1024 / width;
         auto join = width == 32   ? nrs::cross_join_kernel<32>
                     : width == 64 ? nrs::cross_join_kernel<64>

@@ -22,14 +22,16 @@ struct CrossArgs {
     FastDiv by_group;     // division by G
     float scale, scale2;  // scale2 = scale * log2(e)
     float beta_q, beta_kv;
-    // forward of many rows: workgroups that share an item's keys. Past 1,
-    // `part` has [splits][items][R][D] sums, not yet divided, and part_stats
-    // their reference and sum, [items][R][splits][2]
-    int rows, splits;  // rows: of a workgroup
-    // forward of few rows: workgroups that share the launch's key tiles, or 0.
-    // Then `part` has [slots][min(R, 16)][D], part_stats [slots][min(R, 16)][2]
-    // and `shares` the first and the last workgroup of each unit
-    int groups;
+    // The forward. A unit is `unit_rows` rows of an item (16, or a workgroup's of
+    // the kernel of many rows), the last one of an item maybe fewer. With
+    // `groups` 0 a workgroup takes a unit; else the key tiles of all units lie
+    // one after the other, and `groups` workgroups take equal parts of that
+    // line, whatever the items' lengths. A unit that a part begins or ends in
+    // leaves sums, not yet divided, in slot (workgroup + unit) of `part`
+    // [slots][unit_rows][D], which no two of them share, with their reference
+    // and sum in part_stats [slots][unit_rows][2]; `shares` has the first and the
+    // last workgroup of each unit.
+    int unit_rows, groups;
     float* part;
     float* part_stats;
     int32_t* shares;
@@ -63,6 +65,84 @@ __device__ __forceinline__ float* row_stats(const CrossArgs& a, int b, int kv, i
     return a.stats + (((int64_t)b * a.H + kv * a.G + (r - s * a.G)) * a.Sq + s) * 2;
 }
 
+constexpr int kMaxSharedBatch = 1024;  // batch items of a shared launch
+
+// A workgroup's part of the line of key tiles: an unbroken run of (unit, tiles)
+// pieces. `per_item` units to a batch item, tiles of `keys` keys.
+template <int NT>
+struct LinePart {
+    int b, base, p, end, per_item, keys;
+    // of the piece at hand:
+    int sub, L, t0, t1, tiles;
+
+    // False if the part is empty. All NT threads call it; `scan` and `found` are
+    // shared memory. A scan of the items' lengths finds where each begins on
+    // the line, and the item of the part's first tile.
+    __device__ __forceinline__ bool begin(const CrossArgs& a, int per_item_, int keys_,
+                                          int (&scan)[NT / 64], int (&found)[2]) {
+        per_item = per_item_;
+        keys = keys_;
+        const int t = threadIdx.x, lane = t & 63, w = t >> 6, each = (a.B + NT - 1) / NT;
+        int own = 0;
+        for (int i = 0; i < each; ++i)
+            if (t * each + i < a.B) own += (live_keys(a, t * each + i) + keys - 1) / keys * per_item;
+        int upto = own;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int v = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += v;
+        }
+        if (lane == 63) scan[w] = upto;
+        __syncthreads();
+        int at = upto - own, total = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) {
+            at += i < w ? scan[i] : 0;
+            total += scan[i];
+        }
+        p = (int)((int64_t)total * blockIdx.x / a.groups);
+        end = (int)((int64_t)total * (blockIdx.x + 1) / a.groups);
+        if (p >= end) return false;
+        for (int i = 0; i < each && t * each + i < a.B; ++i) {
+            const int n = (live_keys(a, t * each + i) + keys - 1) / keys * per_item;
+            if (at <= p && p < at + n) {
+                found[0] = t * each + i;
+                found[1] = at;
+            }
+            at += n;
+        }
+        __syncthreads();
+        b = found[0];
+        base = found[1];
+        return true;
+    }
+    // The next piece, if any: tiles t0 .. t1 - 1 of unit b * per_item + sub.
+    __device__ __forceinline__ bool next(const CrossArgs& a) {
+        if (p >= end) return false;
+        for (;;) {  // (items without keys have no tiles)
+            L = live_keys(a, b);
+            tiles = (L + keys - 1) / keys;
+            if (p < base + tiles * per_item) break;
+            base += tiles * per_item;
+            ++b;
+        }
+        sub = (p - base) / tiles;
+        t0 = p - base - sub * tiles;
+        t1 = min(tiles, t0 + end - p);
+        p += t1 - t0;
+        const int unit = b * per_item + sub;
+        if (threadIdx.x == 0) {
+            if (t0 == 0) a.shares[2 * unit] = blockIdx.x;
+            if (t1 == tiles) a.shares[2 * unit + 1] = blockIdx.x;
+        }
+        return true;
+    }
+    // Where the piece's sums go: -1 if it is all of its unit.
+    __device__ __forceinline__ int64_t slot() const {
+        return t0 == 0 && t1 == tiles ? -1 : (int64_t)blockIdx.x + b * per_item + sub;
+    }
+};
+
 // The kernels of cross_attention_tile.hip, and the sizes by which calls are
 // planned. A workgroup of the forward owns 256 rows (8 waves) or 128 (4), one of
 // the backward 128 rows or keys, two workgroups to a compute unit up to d_head
@@ -74,7 +154,7 @@ constexpr int cross_tile_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128
 constexpr int cross_tile_keys(int D, int waves) {
     return (waves == 8 || D > 64 ? 4096 : 2048) / cross_tile_width(D);
 }
-void cross_tile_forward(const CrossArgs& a);
+void cross_tile_forward(const CrossArgs& a, unsigned blocks);
 void cross_tile_backward(const CrossArgs& a);
 
 }  // namespace nrs

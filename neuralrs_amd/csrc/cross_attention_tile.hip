@@ -303,24 +303,18 @@ __device__ __forceinline__ void share(int count, int no, int shares, int& from, 
     to = (int)((int64_t)count * (no + 1) / shares);
 }
 
+// Key tiles t0 .. t1 - 1 of the rows of row tile `tile` of (b, kv), L live keys:
+// all of them (slot < 0) or a part.
 template <int D, int WAVES, bool FULL>
-__global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void cross_tile_fwd_kernel(CrossArgs a) {
+__device__ __forceinline__ void forward_walk(const CrossArgs& a,
+                                             u32x4 (&lds)[2][2 * TileCfg<D, WAVES>::SET], int b,
+                                             int kv, int tile, int L, int t0, int t1,
+                                             int64_t slot) {
     using C = TileCfg<D, WAVES>;
-    __shared__ u32x4 lds[2][2 * C::SET];
     const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int R = a.Sq * a.G, tiles = (R + 32 * WAVES - 1) / (32 * WAVES);
-    const int items = a.B * a.KV;
-    int rest = blockIdx.x;
-    const int tile = rest % tiles;
-    rest /= tiles;
-    const int item = rest % items, split_no = rest / items;
-    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
-    const int row = (tile * WAVES + w) * 32 + c;
+    const int R = a.Sq * a.G, row = (tile * WAVES + w) * 32 + c;
     const bool wave_live = (tile * WAVES + w) * 32 < R, live = row < R;
-    int t0, t1;  // this split's key tiles of the item's
-    share((L + C::KT - 1) / C::KT, split_no, a.splits, t0, t1);
-
     Stage<C, FULL> k, v;
     auto load = [&](int t) {
         const int n = min(C::KT, L - t * C::KT);
@@ -400,22 +394,37 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void cross_ti
     }
     l += __shfl_xor(l, 32, 64);
     if (!live) return;
-    if (a.splits > 1) {
-        const int64_t at = ((int64_t)split_no * items + item) * R + row;
-        store_own<C, FULL>(a.part + at * a.D, acc, 1.0f, 0.0f, a.D, h);
-        if (h == 0) {
-            float* st = a.part_stats + 2 * (((int64_t)item * R + row) * a.splits + split_no);
-            st[0] = t0 < t1 ? m : -INFINITY;
-            st[1] = l;
-        }
-        return;
-    }
-    store_own<C, FULL>(a.out + query_offset(a, b, kv, row, a.ld_out), acc,
-                       L > 0 ? 1.0f / l : 0.0f, 0.0f, a.D, h);
-    if (a.stats && h == 0) {
-        float* st = row_stats(a, b, kv, row);
+    const bool whole = slot < 0;
+    const int64_t at = slot * a.unit_rows + w * 32 + c;
+    store_own<C, FULL>(whole ? a.out + query_offset(a, b, kv, row, a.ld_out) : a.part + at * a.D,
+                       acc, !whole ? 1.0f : L > 0 ? 1.0f / l : 0.0f, 0.0f, a.D, h);
+    if (h == 0 && (!whole || a.stats)) {
+        float* st = whole ? row_stats(a, b, kv, row) : a.part_stats + 2 * at;
         st[0] = m;
         st[1] = l;
+    }
+}
+
+template <int D, int WAVES, bool FULL>
+__global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void cross_tile_fwd_kernel(
+    CrossArgs a) {
+    using C = TileCfg<D, WAVES>;
+    __shared__ u32x4 lds[2][2 * C::SET];
+    __shared__ int scan[WAVES], found[2];
+    const int tiles = (a.Sq * a.G + 32 * WAVES - 1) / (32 * WAVES), per_item = a.KV * tiles;
+    if (a.groups == 0) {
+        const int unit = blockIdx.x, b = unit / per_item, sub = unit - b * per_item;
+        const int L = live_keys(a, b);
+        forward_walk<D, WAVES, FULL>(a, lds, b, sub / tiles, sub % tiles, L, 0,
+                                     (L + C::KT - 1) / C::KT, -1);
+        return;
+    }
+    LinePart<64 * WAVES> part;
+    if (!part.begin(a, per_item, C::KT, scan, found)) return;
+    while (part.next(a)) {
+        forward_walk<D, WAVES, FULL>(a, lds, part.b, part.sub / tiles, part.sub % tiles, part.L,
+                                     part.t0, part.t1, part.slot());
+        __syncthreads();  // before the next piece's tiles take the place of this one's
     }
 }
 
@@ -650,14 +659,12 @@ __global__ __launch_bounds__(256, waves_per_simd(D, 4)) void cross_tile_bwd_kern
 }
 
 template <int D>
-void launch_forward(const CrossArgs& a) {
-    const int R = a.Sq * a.G, rows = a.rows;
-    const unsigned grid = (unsigned)(((R + rows - 1) / rows) * (int64_t)a.B * a.KV * a.splits);
+void launch_forward(const CrossArgs& a, unsigned blocks) {
     const bool full = a.D == D;
-    auto kernel = rows == 256
+    auto kernel = a.unit_rows == 256
                       ? (full ? cross_tile_fwd_kernel<D, 8, true> : cross_tile_fwd_kernel<D, 8, false>)
                       : (full ? cross_tile_fwd_kernel<D, 4, true> : cross_tile_fwd_kernel<D, 4, false>);
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(2 * rows), 0, stream(), a);
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(2 * a.unit_rows), 0, stream(), a);
 }
 
 template <int D>
@@ -677,13 +684,13 @@ void launch_backward(const CrossArgs& a) {
 
 }  // namespace
 
-void cross_tile_forward(const CrossArgs& a) {
+void cross_tile_forward(const CrossArgs& a, unsigned blocks) {
     if (a.D <= 32)
-        launch_forward<32>(a);
+        launch_forward<32>(a, blocks);
     else if (a.D <= 64)
-        launch_forward<64>(a);
+        launch_forward<64>(a, blocks);
     else
-        launch_forward<128>(a);
+        launch_forward<128>(a, blocks);
 }
 
 void cross_tile_backward(const CrossArgs& a) {
