@@ -103,19 +103,6 @@ __device__ __forceinline__ void add_rows(f32x4 (&acc)[NJ], const R& x, f32x4 w, 
     }
 }
 
-// Stores acc (as add_rows leaves it) times `f` into a row of d_head floats.
-template <int NJ>
-__device__ __forceinline__ void store_row(float* dst, const f32x4 (&acc)[NJ], float f, float beta,
-                                          int D, int g) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int d = (4 * g + r) * NJ + j;
-            if (d < D) dst[d] = beta != 0.0f ? acc[j][r] * f + beta * dst[d] : acc[j][r] * f;
-        }
-}
-
 __device__ __forceinline__ float across_groups(float x) {
     x += __shfl_xor(x, 16, 64);
     return x + __shfl_xor(x, 32, 64);
@@ -389,6 +376,93 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
     sum.store(a, b, item - b * a.KV, r, live);
 }
 
+// The backward where one side is short (up to kFewRows rows of an item, or
+// keys): 32 rows of a wave of the kernel of many would be mostly idle. As in
+// cross_rows_fwd_kernel, 16 rows (KEYS: keys) are a workgroup's own, and the
+// other side streams from memory into operands of the f32 matrix instructions,
+// in tiles of 16 that the waves take in turns; the waves are joined in LDS.
+// Rows own: S^T = K . Q^T, dQ = scale K^T dS. Keys own: S = Q . K^T, dV = dO^T P,
+// dK = scale Q^T dS.
+template <int NJ, bool KEYS>
+__global__ __launch_bounds__(64 * kRowWaves) void cross_narrow_bwd_kernel(CrossArgs a) {
+    __shared__ float sums[kRowWaves][4 * NJ][64];
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Sq * a.G, own_n = KEYS ? a.Sk : R, own_tiles = (own_n + 15) / 16;
+    const int items = a.B * a.KV, unit = blockIdx.x % (items * own_tiles);
+    const int no = blockIdx.x / (items * own_tiles), shares = KEYS ? a.kv_splits : a.q_splits;
+    const int item = unit / own_tiles, o0 = (unit - item * own_tiles) * 16;
+    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
+    // live ones of the workgroup's own, and all that it may meet
+    const int n = min(16, (KEYS ? L : R) - o0), met = KEYS ? (n > 0 ? R : 0) : L;
+    const int all = (met + 15) / 16, t0 = (int)((int64_t)all * no / shares),
+              t1 = (int)((int64_t)all * (no + 1) / shares);
+    f32x4 xf[NJ], yf[NJ], acc[NJ], acc_v[NJ];  // own: Q and dO, or K and V
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+        xf[j] = yf[j] = acc[j] = acc_v[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (n > 0) {
+        Rows<!KEYS>(a, KEYS ? a.k : a.q, b, kv, KEYS ? a.ld_kv : a.ld_q, o0, n)
+            .template along<NJ>(xf, c, g);
+        Rows<!KEYS>(a, KEYS ? a.v : a.dout, b, kv, KEYS ? a.ld_kv : a.ld_out, o0, n)
+            .template along<NJ>(yf, c, g);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) xf[j] = xf[j] * a.scale2;
+    }
+    const float* const lse = a.neg_lse + (int64_t)item * R;
+    const float* const delta = a.neg_delta + (int64_t)item * R;
+    const float own_lse = !KEYS && c < n ? lse[o0 + c] : -INFINITY;
+    const float own_delta = !KEYS && c < n ? delta[o0 + c] : 0.0f;
+    for (int t = t0 + w; t < t1; t += kRowWaves) {
+        const int m0 = 16 * t, nm = min(16, met - m0);
+        const Rows<KEYS> xs(a, KEYS ? a.q : a.k, b, kv, KEYS ? a.ld_q : a.ld_kv, m0, nm),
+            ys(a, KEYS ? a.dout : a.v, b, kv, KEYS ? a.ld_out : a.ld_kv, m0, nm);
+        f32x4 mx[NJ], my[NJ];
+        xs.template along<NJ>(mx, c, g);
+        ys.template along<NJ>(my, c, g);
+        f32x4 p = dot_rows<NJ>(mx, xf), dp = dot_rows<NJ>(my, yf);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool live = 4 * g + r < nm && c < n;
+            const float nl = !KEYS ? own_lse : live ? lse[m0 + 4 * g + r] : -INFINITY;
+            const float nd = !KEYS ? own_delta : live ? delta[m0 + 4 * g + r] : 0.0f;
+            p[r] = live ? __builtin_amdgcn_exp2f(p[r] + nl) : 0.0f;
+            dp[r] = live ? p[r] * (dp[r] + nd) : 0.0f;
+        }
+        if (KEYS) add_rows<NJ>(acc_v, ys, p, c, g);
+        add_rows<NJ>(acc, xs, dp, c, g);
+    }
+    for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) sums[w][r * NJ + j][lane] = which ? acc_v[j][r] : acc[j][r];
+        __syncthreads();
+        const int o = o0 + c;
+        // (shares of dead keys are not looked at, and a beta of 1 leaves them)
+        const bool left = KEYS && c >= n && (shares > 1 || a.beta_kv == 1.0f);
+        if (o < own_n && !left) {
+            float* const dst =
+                shares > 1 ? (!KEYS ? a.dq_part : which ? a.dv_part : a.dk_part) +
+                                 (((int64_t)no * items + item) * own_n + o) * a.D
+                : !KEYS    ? a.dq + query_offset(a, b, kv, o, a.ld_q)
+                           : (which ? a.dv : a.dk) + key_offset(a, b, kv, o);
+            const float f = shares > 1 || which ? 1.0f : a.scale;
+            const float beta = shares > 1 ? 0.0f : KEYS ? a.beta_kv : a.beta_q;
+            // wave w adds the waves' register w: NJ neighbouring columns of o
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                float v = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kRowWaves; ++i) v += sums[i][w * NJ + j][lane];
+                const int d = (4 * g + w) * NJ + j;
+                if (d < a.D) dst[d] = beta != 0.0f ? v * f + beta * dst[d] : v * f;
+            }
+        }
+    }
+}
+
 // Adds the shares of a gradient in order: dst = f * sum + beta * dst, D / 4
 // threads to a row. KEYS: rows are keys (dead ones have no shares), blockIdx.y
 // is 0 for dk and 1 for dv.
@@ -549,6 +623,7 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
 struct BackwardPlan {
     int q_splits, kv_splits;
     int64_t rows, keys;  // of all items
+    bool few_rows, few_keys;  // dq, or dk and dv, by the narrow kernel
     size_t prepared, q_part, kv_part;  // floats of each kind of scratch
     size_t bytes() const { return sizeof(float) * (prepared + q_part + 2 * kv_part); }
 };
@@ -562,7 +637,7 @@ struct BackwardPlan {
 BackwardPlan plan_backward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
                            int64_t seq_k, int64_t d_head) {
     const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads, cus = num_cus();
-    BackwardPlan p{1, 1, items * R, items * seq_k, 0, 0, 0};
+    BackwardPlan p{1, 1, items * R, items * seq_k, false, false, 0, 0, 0};
     p.prepared = (size_t)((2 * p.rows + 3) / 4 * 4);  // needed without keys, too
     if (p.rows == 0 || p.keys == 0) return p;
     const int64_t tile = cross_tile_keys((int)d_head, 4), own = kCrossBackwardRows;
@@ -575,6 +650,17 @@ BackwardPlan plan_backward(int64_t batch, int64_t heads, int64_t kv_heads, int64
     };
     p.q_splits = shares(3 * q_len, q_len);
     p.kv_splits = shares(4 * kv_len, kv_len);
+    // the narrow kernels: three workgroups to a compute unit, two tiles of 16 to
+    // a wave at least
+    auto narrow = [&](int64_t own_rows, int64_t met) {
+        const int64_t units = items * ((own_rows + 15) / 16);
+        return (int)std::max<int64_t>(1, std::min<int64_t>({3 * cus / units,
+                                                            (met + 15) / 16 / (2 * kRowWaves), 64}));
+    };
+    p.few_rows = R <= kFewRows;
+    p.few_keys = seq_k <= kFewRows;
+    if (p.few_rows) p.q_splits = narrow(R, seq_k);
+    if (p.few_keys) p.kv_splits = narrow(seq_k, R);
     if (p.q_splits > 1) p.q_part = (size_t)((p.q_splits * p.rows * d_head + 3) / 4 * 4);
     if (p.kv_splits > 1) p.kv_part = (size_t)((p.kv_splits * p.keys * d_head + 3) / 4 * 4);
     return p;
@@ -724,13 +810,23 @@ int nrs_cross_attention_backward(float* dq, float* dk, float* dv, const float* d
     a.dq_part = scratch + plan.prepared;
     a.dk_part = a.dq_part + plan.q_part;
     a.dv_part = a.dk_part + plan.kv_part;
-    const int own = nrs::kCrossBackwardRows;
-    if (dq && rows)
-        a.q_blocks = (int)((a.Sq * a.G + own - 1) / own * batch * kv_heads * plan.q_splits);
+    if (!rows) a.dq = nullptr;
     if (!keys) a.dk = a.dv = nullptr;
-    nrs::cross_tile_backward(a);
+    nrs::cross_tile_backward(a, plan.few_rows, plan.few_keys);
+    nrs::for_width(a.D, [&](auto nj) {
+        constexpr int NJ = decltype(nj)::value;
+        const int64_t items = batch * kv_heads;
+        if (a.dq && plan.few_rows)
+            hipLaunchKernelGGL((nrs::cross_narrow_bwd_kernel<NJ, false>),
+                               dim3((unsigned)(items * ((a.Sq * a.G + 15) / 16) * plan.q_splits)),
+                               dim3(64 * nrs::kRowWaves), 0, nrs::stream(), a);
+        if (a.dk && plan.few_keys)
+            hipLaunchKernelGGL((nrs::cross_narrow_bwd_kernel<NJ, true>),
+                               dim3((unsigned)(items * ((a.Sk + 15) / 16) * plan.kv_splits)),
+                               dim3(64 * nrs::kRowWaves), 0, nrs::stream(), a);
+    });
     const int width = nrs::cross_tile_width(a.D);
-    const bool sum_q = a.q_blocks > 0 && plan.q_splits > 1, sum_kv = a.dk && plan.kv_splits > 1;
+    const bool sum_q = a.dq && plan.q_splits > 1, sum_kv = a.dk && plan.kv_splits > 1;
     auto sums = width == 32   ? nrs::launch_sums<32>
                 : width == 64 ? nrs::launch_sums<64>
                               : nrs::launch_sums<128>;

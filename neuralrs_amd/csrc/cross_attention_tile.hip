@@ -668,15 +668,16 @@ void launch_forward(const CrossArgs& a, unsigned blocks) {
 }
 
 template <int D>
-void launch_backward(const CrossArgs& a) {
-    const int64_t items = (int64_t)a.B * a.KV, rows = items * a.Sq * a.G;
+void launch_backward(CrossArgs a, bool few_rows, bool few_keys) {
+    const int R = a.Sq * a.G, own = kCrossBackwardRows;
+    const int64_t items = (int64_t)a.B * a.KV, rows = items * R;
     if (rows > 0) {
         constexpr int PER = 1024 / D;
         hipLaunchKernelGGL(cross_rows_prepare_kernel<D>, dim3((unsigned)((rows + PER - 1) / PER)),
                            dim3(256), 0, stream(), a);
     }
-    const int64_t kv_blocks =
-        a.dk ? (a.Sk + kCrossBackwardRows - 1) / kCrossBackwardRows * items * a.kv_splits : 0;
+    a.q_blocks = a.dq && !few_rows ? (int)((R + own - 1) / own * items * a.q_splits) : 0;
+    const int64_t kv_blocks = a.dk && !few_keys ? (a.Sk + own - 1) / own * items * a.kv_splits : 0;
     if (a.q_blocks + kv_blocks == 0) return;
     auto kernel = a.D == D ? cross_tile_bwd_kernel<D, true> : cross_tile_bwd_kernel<D, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(a.q_blocks + kv_blocks)), dim3(256), 0, stream(), a);
@@ -693,13 +694,13 @@ void cross_tile_forward(const CrossArgs& a, unsigned blocks) {
         launch_forward<128>(a, blocks);
 }
 
-void cross_tile_backward(const CrossArgs& a) {
+void cross_tile_backward(const CrossArgs& a, bool few_rows, bool few_keys) {
     if (a.D <= 32)
-        launch_backward<32>(a);
+        launch_backward<32>(a, few_rows, few_keys);
     else if (a.D <= 64)
-        launch_backward<64>(a);
+        launch_backward<64>(a, few_rows, few_keys);
     else
-        launch_backward<128>(a);
+        launch_backward<128>(a, few_rows, few_keys);
 }
 
 }  // namespace nrs
