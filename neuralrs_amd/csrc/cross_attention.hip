@@ -90,19 +90,6 @@ __device__ __forceinline__ f32x4 dot_rows(const f32x4 (&x)[NJ], const f32x4 (&y)
     return acc;
 }
 
-// acc[j][d'][n] += sum over the tile's 16 rows of x[row][d] w[row][n]: w as
-// dot_rows leaves it, lane (c, g) of acc[j] gets d = (4g + r) * NJ + j of n = c.
-template <int NJ, class R>
-__device__ __forceinline__ void add_rows(f32x4 (&acc)[NJ], const R& x, f32x4 w, int c, int g) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        float f[NJ];
-        x.template across<NJ>(f, 4 * g + r, c);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[j] = mfma16(f[j], w[r], acc[j]);
-    }
-}
-
 __device__ __forceinline__ float across_groups(float x) {
     x += __shfl_xor(x, 16, 64);
     return x + __shfl_xor(x, 32, 64);
@@ -376,91 +363,221 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
     sum.store(a, b, item - b * a.KV, r, live);
 }
 
-// The backward where one side is short (up to kFewRows rows of an item, or
-// keys): 32 rows of a wave of the kernel of many would be mostly idle. As in
-// cross_rows_fwd_kernel, 16 rows (KEYS: keys) are a workgroup's own, and the
-// other side streams from memory into operands of the f32 matrix instructions,
-// in tiles of 16 that the waves take in turns; the waves are joined in LDS.
-// Rows own: S^T = K . Q^T, dQ = scale K^T dS. Keys own: S = Q . K^T, dV = dO^T P,
-// dK = scale Q^T dS.
-template <int NJ, bool KEYS>
-__global__ __launch_bounds__(64 * kRowWaves) void cross_narrow_bwd_kernel(CrossArgs a) {
-    __shared__ float sums[kRowWaves][4 * NJ][64];
+// The backward where one side is short (up to 16 T rows of an item, or KEYS:
+// keys). The short side is the workgroup's own, X and Y (Q and dO, or K and V) in
+// LDS; the long side streams from memory once, in tiles of 16 that the waves take
+// in turns, as operands of the f32 matrix instructions. Of a tile
+//   S = X Xm^T, dP = Y Ym^T, P = 2^(S - lse), dS = P (dP - delta),
+// lane (c, g) with rows 4g + r of X and row c of the tile. Products over the short
+// side finish the tile's gradients (dK = scale dS^T Q and dV = P^T dO, or
+// dQ = scale dS K); those over the tile, with P and dS turned about in LDS, add to
+// the short side's own (dQ, or dK and dV), which the waves and the workgroups that
+// share an item join at the end.
+template <int NJ, int T, bool KEYS>
+__global__ __launch_bounds__(64 * kRowWaves) void cross_short_bwd_kernel(CrossArgs a) {
+    constexpr int W = 16 * NJ + 4, OWN = 2 * 16 * T * W, SUMS = kRowWaves * 4 * NJ * 64;
+    __shared__ f32x4 shared[(OWN > SUMS ? OWN : SUMS) / 4];
+    __shared__ f32x4 turned[kRowWaves][KEYS ? 2 : 1][16][5];
+    __shared__ f32x4 starts[2][4 * T];  // !KEYS: -lse and -delta of the own rows
+    float(&own)[2][16 * T][W] = *reinterpret_cast<float(*)[2][16 * T][W]>(shared);
+    float(&sums)[kRowWaves][4 * NJ][64] = *reinterpret_cast<float(*)[kRowWaves][4 * NJ][64]>(shared);
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int R = a.Sq * a.G, own_n = KEYS ? a.Sk : R, own_tiles = (own_n + 15) / 16;
-    const int items = a.B * a.KV, unit = blockIdx.x % (items * own_tiles);
-    const int no = blockIdx.x / (items * own_tiles), shares = KEYS ? a.kv_splits : a.q_splits;
-    const int item = unit / own_tiles, o0 = (unit - item * own_tiles) * 16;
+    const int R = a.Sq * a.G, items = a.B * a.KV, item = blockIdx.x % items;
+    const int no = blockIdx.x / items, shares = KEYS ? a.kv_splits : a.q_splits;
     const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
-    // live ones of the workgroup's own, and all that it may meet
-    const int n = min(16, (KEYS ? L : R) - o0), met = KEYS ? (n > 0 ? R : 0) : L;
-    const int all = (met + 15) / 16, t0 = (int)((int64_t)all * no / shares),
-              t1 = (int)((int64_t)all * (no + 1) / shares);
-    f32x4 xf[NJ], yf[NJ], acc[NJ], acc_v[NJ];  // own: Q and dO, or K and V
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-        xf[j] = yf[j] = acc[j] = acc_v[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (n > 0) {
-        Rows<!KEYS>(a, KEYS ? a.k : a.q, b, kv, KEYS ? a.ld_kv : a.ld_q, o0, n)
-            .template along<NJ>(xf, c, g);
-        Rows<!KEYS>(a, KEYS ? a.v : a.dout, b, kv, KEYS ? a.ld_kv : a.ld_out, o0, n)
-            .template along<NJ>(yf, c, g);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) xf[j] = xf[j] * a.scale2;
-    }
+    const bool finish = KEYS ? a.dq != nullptr : a.dk != nullptr;  // the tiles' gradients
+    const bool add = KEYS ? a.dk != nullptr : a.dq != nullptr;     // the short side's
+    // live rows of the short side and of the long one, and those to be written
+    const int own_n = KEYS ? a.Sk : R, n = KEYS ? L : R;
+    const int met = KEYS ? (L > 0 ? R : 0) : L, all = KEYS ? R : a.Sk;
     const float* const lse = a.neg_lse + (int64_t)item * R;
     const float* const delta = a.neg_delta + (int64_t)item * R;
-    const float own_lse = !KEYS && c < n ? lse[o0 + c] : -INFINITY;
-    const float own_delta = !KEYS && c < n ? delta[o0 + c] : 0.0f;
-    for (int t = t0 + w; t < t1; t += kRowWaves) {
-        const int m0 = 16 * t, nm = min(16, met - m0);
-        const Rows<KEYS> xs(a, KEYS ? a.q : a.k, b, kv, KEYS ? a.ld_q : a.ld_kv, m0, nm),
-            ys(a, KEYS ? a.dout : a.v, b, kv, KEYS ? a.ld_out : a.ld_kv, m0, nm);
-        f32x4 mx[NJ], my[NJ];
-        xs.template along<NJ>(mx, c, g);
-        ys.template along<NJ>(my, c, g);
-        f32x4 p = dot_rows<NJ>(mx, xf), dp = dot_rows<NJ>(my, yf);
+    for (int i = threadIdx.x; i < 2 * 16 * T * 4 * NJ; i += 64 * kRowWaves) {
+        const int which = i / (16 * T * 4 * NJ), at = i % (16 * T * 4 * NJ), row = at / (4 * NJ),
+                  d = at % (4 * NJ) * 4;
+        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (row < n) {
+            const float* const src =
+                KEYS ? (which ? a.v : a.k) + key_offset(a, b, kv, row)
+                     : (which ? a.dout + query_offset(a, b, kv, row, a.ld_out)
+                              : a.q + query_offset(a, b, kv, row, a.ld_q));
+            if (d + 4 <= a.D)
+                v = reinterpret_cast<const Quad*>(src + d)->v;
+            else
+                for (int e = 0; d + e < a.D; ++e) v[e] = src[d + e];
+        }
+        *reinterpret_cast<f32x4*>(&own[which][row][d]) = v;
+    }
+    if (!KEYS && threadIdx.x < 16 * T) {
+        const bool live = (int)threadIdx.x < n;
+        reinterpret_cast<float*>(starts[0])[threadIdx.x] = live ? lse[threadIdx.x] : -INFINITY;
+        reinterpret_cast<float*>(starts[1])[threadIdx.x] = live ? delta[threadIdx.x] : 0.0f;
+    }
+    __syncthreads();
+    f32x4 acc[T][NJ], acc_y[KEYS ? T : 1][NJ];
+#pragma unroll
+    for (int ot = 0; ot < T; ++ot)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            acc[ot][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (KEYS) acc_y[ot][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    // weight[r] of the own rows 4g + r times their columns c NJ ..
+    auto add_own = [&](f32x4(&to)[NJ], int which, int ot, f32x4 weight) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const bool live = 4 * g + r < nm && c < n;
-            const float nl = !KEYS ? own_lse : live ? lse[m0 + 4 * g + r] : -INFINITY;
-            const float nd = !KEYS ? own_delta : live ? delta[m0 + 4 * g + r] : 0.0f;
-            p[r] = live ? __builtin_amdgcn_exp2f(p[r] + nl) : 0.0f;
-            dp[r] = live ? p[r] * (dp[r] + nd) : 0.0f;
+            const float* const src = &own[which][16 * ot + 4 * g + r][c * NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) to[j] = mfma16(src[j], weight[r], to[j]);
         }
-        if (KEYS) add_rows<NJ>(acc_v, ys, p, c, g);
-        add_rows<NJ>(acc, xs, dp, c, g);
-    }
-    for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
-        __syncthreads();
+    };
+    auto add_met = [&](f32x4(&to)[NJ], const float (&x)[4][NJ], f32x4 weight) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) sums[w][r * NJ + j][lane] = which ? acc_v[j][r] : acc[j][r];
-        __syncthreads();
-        const int o = o0 + c;
-        // (shares of dead keys are not looked at, and a beta of 1 leaves them)
-        const bool left = KEYS && c >= n && (shares > 1 || a.beta_kv == 1.0f);
-        if (o < own_n && !left) {
-            float* const dst =
-                shares > 1 ? (!KEYS ? a.dq_part : which ? a.dv_part : a.dk_part) +
-                                 (((int64_t)no * items + item) * own_n + o) * a.D
-                : !KEYS    ? a.dq + query_offset(a, b, kv, o, a.ld_q)
-                           : (which ? a.dv : a.dk) + key_offset(a, b, kv, o);
-            const float f = shares > 1 || which ? 1.0f : a.scale;
-            const float beta = shares > 1 ? 0.0f : KEYS ? a.beta_kv : a.beta_q;
-            // wave w adds the waves' register w: NJ neighbouring columns of o
+            for (int j = 0; j < NJ; ++j) to[j] = mfma16(x[r][j], weight[r], to[j]);
+    };
+    // w[4g + r][c] -> w[c][4g + r]
+    auto turn = [&](f32x4 x, int which) {
+        f32x4(&at)[16][5] = turned[w][which];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        at[c][g] = x;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        f32x4 y;
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                float v = 0.0f;
+        for (int r = 0; r < 4; ++r) y[r] = reinterpret_cast<const float*>(at[4 * g + r])[c];
+        return y;
+    };
+    // The gradient of the tile's row c: 4 NJ neighbouring columns to a lane.
+    auto store = [&](float* dst, const f32x4(&x)[NJ], float f, float beta) {
 #pragma unroll
-                for (int i = 0; i < kRowWaves; ++i) v += sums[i][w * NJ + j][lane];
-                const int d = (4 * g + w) * NJ + j;
-                if (d < a.D) dst[d] = beta != 0.0f ? v * f + beta * dst[d] : v * f;
+        for (int e = 0; e < 4 * NJ; e += 4) {
+            const int d = 4 * NJ * g + e;
+            f32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = x[(e + i) % NJ][(e + i) / NJ] * f;
+            if (d + 4 <= a.D) {
+                Quad* const to = reinterpret_cast<Quad*>(dst + d);
+                if (beta != 0.0f) v = v + beta * to->v;
+                to->v = v;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    if (d + i < a.D) dst[d + i] = beta != 0.0f ? v[i] + beta * dst[d + i] : v[i];
+            }
+        }
+    };
+    const int tiles = (all + 15) / 16, t1 = (int)((int64_t)tiles * (no + 1) / shares);
+    for (int t = (int)((int64_t)tiles * no / shares) + w; t < t1; t += kRowWaves) {
+        const int m0 = 16 * t, nm = min(16, met - m0);
+        f32x4 dx[NJ], dy[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) dx[j] = dy[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (nm > 0) {
+            const Rows<KEYS> xs(a, KEYS ? a.q : a.k, b, kv, KEYS ? a.ld_q : a.ld_kv, m0, nm),
+                ys(a, KEYS ? a.dout : a.v, b, kv, KEYS ? a.ld_out : a.ld_kv, m0, nm);
+            f32x4 mx[NJ], my[NJ];
+            float cx[4][NJ], cy[4][NJ];
+            xs.template along<NJ>(mx, c, g);
+            ys.template along<NJ>(my, c, g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (add) xs.template across<NJ>(cx[r], 4 * g + r, c);
+                if (KEYS && add) ys.template across<NJ>(cy[r], 4 * g + r, c);
+            }
+            const float met_lse = KEYS && c < nm ? lse[m0 + c] : -INFINITY;
+            const float met_delta = KEYS && c < nm ? delta[m0 + c] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) mx[j] = mx[j] * a.scale2;
+#pragma unroll
+            for (int ot = 0; ot < T; ++ot) {
+                if (16 * ot >= n) break;
+                f32x4 p = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, ds = p;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int at = 16 * j + 4 * g;
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(&own[0][16 * ot + c][at]),
+                                y = *reinterpret_cast<const f32x4*>(&own[1][16 * ot + c][at]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        p = mfma16(x[e], mx[j][e], p);
+                        ds = mfma16(y[e], my[j][e], ds);
+                    }
+                }
+                const f32x4 nl = starts[0][4 * ot + g], nd = starts[1][4 * ot + g];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool live = c < nm && 16 * ot + 4 * g + r < n;
+                    p[r] = live ? __builtin_amdgcn_exp2f(p[r] + (KEYS ? met_lse : nl[r])) : 0.0f;
+                    ds[r] = live ? p[r] * (ds[r] + (KEYS ? met_delta : nd[r])) : 0.0f;
+                }
+                if (finish) {
+                    add_own(dx, 0, ot, ds);
+                    if (!KEYS) add_own(dy, 1, ot, p);
+                }
+                if (add) {
+                    add_met(acc[ot], cx, turn(ds, 0));
+                    if constexpr (KEYS) add_met(acc_y[ot], cy, turn(p, 1));
+                }
+            }
+        }
+        if (finish && m0 + c < all) {
+            if (KEYS) {
+                store(a.dq + query_offset(a, b, kv, m0 + c, a.ld_q), dx, a.scale, a.beta_q);
+            } else if (c < nm || a.beta_kv != 1.0f) {  // else a dead key's, left as it is
+                const int64_t at = key_offset(a, b, kv, m0 + c);
+                store(a.dk + at, dx, a.scale, a.beta_kv);
+                store(a.dv + at, dy, 1.0f, a.beta_kv);
             }
         }
     }
+    if (!add) return;
+#pragma unroll
+    for (int ot = 0; ot < T; ++ot) {
+        if (16 * ot >= own_n) break;
+#pragma unroll
+        for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                    sums[w][r * NJ + j][lane] = which ? acc_y[KEYS ? ot : 0][j][r] : acc[ot][j][r];
+            __syncthreads();
+            const int o = 16 * ot + c;
+            // (shares of dead keys are not looked at, and a beta of 1 leaves them)
+            const bool left = KEYS && o >= n && (shares > 1 || a.beta_kv == 1.0f);
+            if (o < own_n && !left) {
+                float* const dst =
+                    shares > 1 ? (!KEYS ? a.dq_part : which ? a.dv_part : a.dk_part) +
+                                     (((int64_t)no * items + item) * own_n + o) * a.D
+                    : !KEYS    ? a.dq + query_offset(a, b, kv, o, a.ld_q)
+                               : (which ? a.dv : a.dk) + key_offset(a, b, kv, o);
+                const float f = shares > 1 || which ? 1.0f : a.scale;
+                const float beta = shares > 1 ? 0.0f : KEYS ? a.beta_kv : a.beta_q;
+                // wave w adds the waves' register w: NJ neighbouring columns of o
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    float v = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kRowWaves; ++i) v += sums[i][w * NJ + j][lane];
+                    const int d = (4 * g + w) * NJ + j;
+                    if (d < a.D) dst[d] = beta != 0.0f ? v * f + beta * dst[d] : v * f;
+                }
+            }
+        }
+    }
+}
+
+template <int NJ, bool KEYS>
+void launch_short(const CrossArgs& a) {
+    const int n = KEYS ? a.Sk : a.Sq * a.G;
+    auto kernel = n <= 16   ? cross_short_bwd_kernel<NJ, 1, KEYS>
+                  : n <= 32 ? cross_short_bwd_kernel<NJ, 2, KEYS>
+                            : cross_short_bwd_kernel<NJ, 4, KEYS>;
+    const unsigned blocks = (unsigned)(a.B * a.KV * (KEYS ? a.kv_splits : a.q_splits));
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kRowWaves), 0, stream(), a);
 }
 
 // Adds the shares of a gradient in order: dst = f * sum + beta * dst, D / 4
@@ -620,10 +737,14 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
     return p;
 }
 
+// Rows or keys of an item up to which the backward's kernel of a short side takes
+// the call.
+constexpr int64_t kShort = 64;
+
 struct BackwardPlan {
     int q_splits, kv_splits;
     int64_t rows, keys;  // of all items
-    bool few_rows, few_keys;  // dq, or dk and dv, by the narrow kernel
+    bool short_rows, short_keys;  // the kernel of a short side
     size_t prepared, q_part, kv_part;  // floats of each kind of scratch
     size_t bytes() const { return sizeof(float) * (prepared + q_part + 2 * kv_part); }
 };
@@ -650,17 +771,16 @@ BackwardPlan plan_backward(int64_t batch, int64_t heads, int64_t kv_heads, int64
     };
     p.q_splits = shares(3 * q_len, q_len);
     p.kv_splits = shares(4 * kv_len, kv_len);
-    // the narrow kernels: three workgroups to a compute unit, two tiles of 16 to
-    // a wave at least
-    auto narrow = [&](int64_t own_rows, int64_t met) {
-        const int64_t units = items * ((own_rows + 15) / 16);
-        return (int)std::max<int64_t>(1, std::min<int64_t>({3 * cus / units,
-                                                            (met + 15) / 16 / (2 * kRowWaves), 64}));
-    };
-    p.few_rows = R <= kFewRows;
-    p.few_keys = seq_k <= kFewRows;
-    if (p.few_rows) p.q_splits = narrow(R, seq_k);
-    if (p.few_keys) p.kv_splits = narrow(seq_k, R);
+    p.short_rows = R <= kShort;
+    p.short_keys = !p.short_rows && seq_k <= kShort;
+    if (p.short_rows || p.short_keys) {
+        // three workgroups to a compute unit, two tiles of 16 to a wave at least
+        const int64_t tiles = ((p.short_rows ? seq_k : R) + 15) / 16;
+        const int splits = (int)std::max<int64_t>(
+            1, std::min<int64_t>({3 * cus / items, tiles / (2 * kRowWaves), 64}));
+        p.q_splits = p.short_rows ? splits : 1;
+        p.kv_splits = p.short_keys ? splits : 1;
+    }
     if (p.q_splits > 1) p.q_part = (size_t)((p.q_splits * p.rows * d_head + 3) / 4 * 4);
     if (p.kv_splits > 1) p.kv_part = (size_t)((p.kv_splits * p.keys * d_head + 3) / 4 * 4);
     return p;
@@ -812,19 +932,14 @@ int nrs_cross_attention_backward(float* dq, float* dk, float* dv, const float* d
     a.dv_part = a.dk_part + plan.kv_part;
     if (!rows) a.dq = nullptr;
     if (!keys) a.dk = a.dv = nullptr;
-    nrs::cross_tile_backward(a, plan.few_rows, plan.few_keys);
-    nrs::for_width(a.D, [&](auto nj) {
-        constexpr int NJ = decltype(nj)::value;
-        const int64_t items = batch * kv_heads;
-        if (a.dq && plan.few_rows)
-            hipLaunchKernelGGL((nrs::cross_narrow_bwd_kernel<NJ, false>),
-                               dim3((unsigned)(items * ((a.Sq * a.G + 15) / 16) * plan.q_splits)),
-                               dim3(64 * nrs::kRowWaves), 0, nrs::stream(), a);
-        if (a.dk && plan.few_keys)
-            hipLaunchKernelGGL((nrs::cross_narrow_bwd_kernel<NJ, true>),
-                               dim3((unsigned)(items * ((a.Sk + 15) / 16) * plan.kv_splits)),
-                               dim3(64 * nrs::kRowWaves), 0, nrs::stream(), a);
-    });
+    const bool is_short = plan.short_rows || plan.short_keys;
+    nrs::cross_tile_backward(a, is_short);
+    if (is_short && (a.dq || a.dk)) {
+        nrs::for_width(a.D, [&](auto nj) {
+            constexpr int NJ = decltype(nj)::value;
+            (plan.short_rows ? nrs::launch_short<NJ, false> : nrs::launch_short<NJ, true>)(a);
+        });
+    }
     const int width = nrs::cross_tile_width(a.D);
     const bool sum_q = a.dq && plan.q_splits > 1, sum_kv = a.dk && plan.kv_splits > 1;
     auto sums = width == 32   ? nrs::launch_sums<32>

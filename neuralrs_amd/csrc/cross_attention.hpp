@@ -155,8 +155,8 @@ constexpr int cross_tile_keys(int D, int waves) {
     return (waves == 8 || D > 64 ? 4096 : 2048) / cross_tile_width(D);
 }
 void cross_tile_forward(const CrossArgs& a, unsigned blocks);
-// The rows' statistics, then dq and dk, dv where they are asked for and not
-// few_rows or few_keys.
-void cross_tile_backward(const CrossArgs& a, bool few_rows, bool few_keys);
+// The rows' statistics, then (unless only they are wanted) what is asked for of
+// dq and dk, dv.
+void cross_tile_backward(const CrossArgs& a, bool only_rows);
 
 }  // namespace nrs

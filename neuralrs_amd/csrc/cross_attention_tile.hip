@@ -668,7 +668,7 @@ void launch_forward(const CrossArgs& a, unsigned blocks) {
 }
 
 template <int D>
-void launch_backward(CrossArgs a, bool few_rows, bool few_keys) {
+void launch_backward(CrossArgs a, bool only_rows) {
     const int R = a.Sq * a.G, own = kCrossBackwardRows;
     const int64_t items = (int64_t)a.B * a.KV, rows = items * R;
     if (rows > 0) {
@@ -676,8 +676,9 @@ void launch_backward(CrossArgs a, bool few_rows, bool few_keys) {
         hipLaunchKernelGGL(cross_rows_prepare_kernel<D>, dim3((unsigned)((rows + PER - 1) / PER)),
                            dim3(256), 0, stream(), a);
     }
-    a.q_blocks = a.dq && !few_rows ? (int)((R + own - 1) / own * items * a.q_splits) : 0;
-    const int64_t kv_blocks = a.dk && !few_keys ? (a.Sk + own - 1) / own * items * a.kv_splits : 0;
+    if (only_rows) return;
+    a.q_blocks = a.dq ? (int)((R + own - 1) / own * items * a.q_splits) : 0;
+    const int64_t kv_blocks = a.dk ? (a.Sk + own - 1) / own * items * a.kv_splits : 0;
     if (a.q_blocks + kv_blocks == 0) return;
     auto kernel = a.D == D ? cross_tile_bwd_kernel<D, true> : cross_tile_bwd_kernel<D, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(a.q_blocks + kv_blocks)), dim3(256), 0, stream(), a);
@@ -694,13 +695,13 @@ void cross_tile_forward(const CrossArgs& a, unsigned blocks) {
         launch_forward<128>(a, blocks);
 }
 
-void cross_tile_backward(const CrossArgs& a, bool few_rows, bool few_keys) {
+void cross_tile_backward(const CrossArgs& a, bool only_rows) {
     if (a.D <= 32)
-        launch_backward<32>(a, few_rows, few_keys);
+        launch_backward<32>(a, only_rows);
     else if (a.D <= 64)
-        launch_backward<64>(a, few_rows, few_keys);
+        launch_backward<64>(a, only_rows);
     else
-        launch_backward<128>(a, few_rows, few_keys);
+        launch_backward<128>(a, only_rows);
 }
 
 }  // namespace nrs
