@@ -575,7 +575,7 @@ void launch_short(const CrossArgs& a) {
     const int n = KEYS ? a.Sk : a.Sq * a.G;
     auto kernel = n <= 16   ? cross_short_bwd_kernel<NJ, 1, KEYS>
                   : n <= 32 ? cross_short_bwd_kernel<NJ, 2, KEYS>
-                            : cross_short_bwd_kernel<NJ, 4, KEYS>;
+                            : cross_short_bwd_kernel<NJ, 3, KEYS>;
     const unsigned blocks = (unsigned)(a.B * a.KV * (KEYS ? a.kv_splits : a.q_splits));
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kRowWaves), 0, stream(), a);
 }
@@ -738,8 +738,10 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
 }
 
 // Rows or keys of an item up to which the backward's kernel of a short side takes
-// the call.
-constexpr int64_t kShort = 64;
+// the call, against the kernel of many: 35 rows, 5256 keys (256 items of 128)
+// 1140 us and 2255; 33 keys, 4067 rows (32 items of 98) 177 and 283; but 64 keys,
+// 1000 rows (64 items of 64) 81 and 55, 64 rows, 1500 keys 88 and 62.
+constexpr int64_t kShort = 48;
 
 struct BackwardPlan {
     int q_splits, kv_splits;
