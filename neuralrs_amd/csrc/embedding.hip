@@ -16,6 +16,13 @@
 //     tile's beginning or end goes to scratch.
 //  3. join: adds the parts of every run that crosses tiles, in order.
 // No floating-point atomics: the order of a sum depends on the ids alone.
+// Memory bounds the large calls, round trips and launches the small ones:
+//                                       lookup    sort    sum   join (us)
+//   4096 ids of 32000 tokens, 256 wide       4.0    11.1    6.5    3.0
+//   49999 of 50021, 1000 wide               60      49     73      6.4
+//   65536 of 259, 512 wide                  24      26     23     10
+// The lookup moves 6.7 TB/s in the second and the sum 5.5 (the 200 MB of the
+// table's gradient are cleared beside the sort, in its 49 us).
 #include <algorithm>
 
 #include "buffer_ops.hpp"
