@@ -374,7 +374,7 @@ int nrs_cross_attention_backward(float *dq, float *dk, float *dv, const float *d
  * scale of the table's rows folded in): out[i] = scale * table[ids[i]], out
  * [count, dim], table [vocab, dim], ids int32 [count]. An id outside
  * [0, vocab), -1 for padding say, gives a zero row. count is at most 2^30,
- * vocab below 2^31 - 1, dim at most 2^20, count * dim at most 2^39.                                                */
+ * vocab below 2^31 - 1, dim at most 2^20, count * dim at most 2^39.          */
 int nrs_embedding_forward(float *out, const float *table, const int32_t *ids, int64_t count,
                           int64_t vocab, int64_t dim, float scale);
 /* Its gradient: dtable[t] = beta * dtable[t] + scale * sum of grad[i] over the

@@ -200,6 +200,23 @@ def test_parts_and_optional_outputs_have_the_same_bits(hip):
         assert np.array_equal(v.to_host(), full[2].to_host())
 
 
+@pytest.mark.parametrize("shape,lens", [((2, 4, 2, 11, 2500, 64), [2500, 700]),
+                                        ((2, 4, 2, 900, 40, 64), [40, 17]),
+                                        ((1, 2, 2, 1, 130, 128), None), ((2, 2, 1, 60, 5, 16), [5, 0])])
+def test_gradients_of_short_sides_alone_have_the_same_bits(hip, shape, lens):
+    p = Problem(*shape, lens=lens, seed=12)
+    dev = Device(hip, p)
+    dev.forward()
+    shapes = [p.q.shape, p.k.shape, p.v.shape]
+    full, q, k, v = ([hip.DeviceBuffer.from_host(np.full(s, MARK)) for s in shapes]
+                     for _ in range(4))
+    dev.backward(*full)
+    dev.backward(q[0], None, None)
+    dev.backward(None, k[1], v[2])
+    for i, got in enumerate((q[0], k[1], v[2])):
+        assert np.array_equal(got.to_host(), full[i].to_host())
+
+
 def test_an_item_does_not_depend_on_its_batch(hip):
     """NaN in one item's live keys stays in that item."""
     p = Problem(3, 2, 2, 40, 70, 32, lens=[70, 60, 50], seed=6)
