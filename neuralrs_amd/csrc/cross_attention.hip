@@ -731,7 +731,7 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
                       tiles = (seq_k + keys - 1) / keys;
         // Workgroups at once, and the time of the fullest one in key tiles: a
         // piece's beginning and end cost two tiles, a join four.
-        const int64_t at_once = p.unit_rows == 128 && d_head <= 64 ? 2 * cus : cus;
+        const int64_t at_once = p.unit_rows == 128 && d_head <= 96 ? 2 * cus : cus;
         groups = std::min<int64_t>(at_once, units * tiles / 2);
         share = groups > 1 && (units + at_once - 1) / at_once * (tiles + 2) >
                                   (units * tiles + groups - 1) / groups + 8;
@@ -878,7 +878,7 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
         hipLaunchKernelGGL(nrs::cross_rows_join_kernel, dim3((unsigned)rows), dim3(256), 0,
                            nrs::stream(), a);
     } else if (a.groups > 0) {
-        const int width = nrs::cross_tile_width(a.D), per = 1024 / width;
+        const int width = nrs::cross_row_width(a.D), per = 1024 / width;
         auto join = width == 32   ? nrs::cross_join_kernel<32>
                     : width == 64 ? nrs::cross_join_kernel<64>
                                   : nrs::cross_join_kernel<128>;
@@ -953,7 +953,7 @@ int nrs_cross_attention_backward(float* dq, float* dk, float* dv, const float* d
             (plan.short_rows ? nrs::launch_short<NJ, false> : nrs::launch_short<NJ, true>)(a);
         });
     }
-    const int width = nrs::cross_tile_width(a.D);
+    const int width = nrs::cross_row_width(a.D);
     const bool sum_q = a.dq && plan.q_splits > 1, sum_kv = a.dk && plan.kv_splits > 1;
     auto sums = width == 32   ? nrs::launch_sums<32>
                 : width == 64 ? nrs::launch_sums<64>

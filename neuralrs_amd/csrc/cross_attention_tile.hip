@@ -96,7 +96,7 @@ __device__ __forceinline__ f32x16 all16(float x) {
 }
 
 // One wave to a SIMD when a wide head's operands fill its registers.
-constexpr int waves_per_simd(int D, int waves) { return D > 64 && waves == 4 ? 1 : 2; }
+constexpr int waves_per_simd(int D, int waves) { return D > 96 && waves == 4 ? 1 : 2; }
 
 template <int D_, int WAVES_>
 struct TileCfg {
@@ -104,10 +104,12 @@ struct TileCfg {
     static constexpr int KT = cross_tile_keys(D, WAVES);  // rows of a tile
     static constexpr int Q = D / 8;           // units of a row
     static constexpr int PLANE = KT * Q;      // units of a plane
-    static constexpr int U = PLANE / NT;      // units a thread stages
+    static constexpr int U = (PLANE + NT - 1) / NT;  // units a thread stages at most
     static constexpr int SET = 3 * PLANE;     // units of a tensor's tile
     static constexpr int NS = D / 16, NJ = D / 32, NB = KT / 32;
-    static_assert(U * NT == PLANE && KT % 32 == 0 && D % 32 == 0, "units");
+    static_assert(KT % 32 == 0 && D % 32 == 0, "blocks of 32");
+    // Whether unit i is one of the tile (the last ones of a thread may not be).
+    __device__ static constexpr bool has(int i) { return U * NT == PLANE || i < PLANE; }
 };
 
 // Unit q of row r in a plane: the 32 rows of a block are contiguous for the
@@ -157,7 +159,7 @@ struct Stage {
             for (int s = 0; s < 2; ++s) {
                 const int d = 4 * q + s * (C::D / 2);
                 x[u][s] = buffer_load4(
-                    rs, row < n && (FULL || d < a.D) ? (off + d) * 4 : kOutOfRange);
+                    rs, C::has(i) && row < n && (FULL || d < a.D) ? (off + d) * 4 : kOutOfRange);
             }
         }
     }
@@ -176,7 +178,8 @@ struct Stage {
             u32x4 p[3];
             split8(f, p);
 #pragma unroll
-            for (int n = 0; n < 3; ++n) lds[n * C::PLANE + unit_at<C>(row, q)] = p[n];
+            for (int n = 0; n < 3; ++n)
+                if (C::has(i)) lds[n * C::PLANE + unit_at<C>(row, q)] = p[n];
         }
     }
 };
@@ -658,7 +661,7 @@ __device__ __forceinline__ void dkv_walk(const CrossArgs& a, u32x4* lds, float* 
 // One launch for both: they need nothing of each other, and the workgroups of
 // one fill the compute units that the other leaves idle.
 template <int D, bool FULL>
-__global__ __launch_bounds__(256, waves_per_simd(D, 4)) void cross_tile_bwd_kernel(CrossArgs a) {
+__global__ __launch_bounds__(256, D > 64 ? 1 : 2) void cross_tile_bwd_kernel(CrossArgs a) {
     constexpr int WAVES = 4;
     using C = TileCfg<D, WAVES>;
     __shared__ u32x4 lds[4 * C::SET];
@@ -683,8 +686,8 @@ void launch_backward(CrossArgs a, bool only_rows) {
     const int R = a.Sq * a.G, own = kCrossBackwardRows;
     const int64_t items = (int64_t)a.B * a.KV, rows = items * R;
     if (rows > 0) {
-        constexpr int PER = 1024 / D;
-        hipLaunchKernelGGL(cross_rows_prepare_kernel<D>, dim3((unsigned)((rows + PER - 1) / PER)),
+        constexpr int WIDE = cross_row_width(D), PER = 1024 / WIDE;
+        hipLaunchKernelGGL(cross_rows_prepare_kernel<WIDE>, dim3((unsigned)((rows + PER - 1) / PER)),
                            dim3(256), 0, stream(), a);
     }
     if (only_rows) return;
@@ -702,6 +705,8 @@ void cross_tile_forward(const CrossArgs& a, unsigned blocks) {
         launch_forward<32>(a, blocks);
     else if (a.D <= 64)
         launch_forward<64>(a, blocks);
+    else if (a.D <= 96)
+        launch_forward<96>(a, blocks);
     else
         launch_forward<128>(a, blocks);
 }
@@ -711,6 +716,8 @@ void cross_tile_backward(const CrossArgs& a, bool only_rows) {
         launch_backward<32>(a, only_rows);
     else if (a.D <= 64)
         launch_backward<64>(a, only_rows);
+    else if (a.D <= 96)
+        launch_backward<96>(a, only_rows);
     else
         launch_backward<128>(a, only_rows);
 }

@@ -93,6 +93,7 @@ SHAPES = [
     (1, 7, 1, 9, 100, 24, [99]),
     (2, 6, 3, 33, 129, 40, [-5, 1000]),
     (1, 2, 1, 70, 257, 80, None),
+    (2, 4, 2, 90, 300, 72, [300, 201]),
     (2, 2, 1, 13, 96, 96, [96, 95]),
     (1, 3, 3, 20, 40, 127, None),
     (1, 2, 2, 10, 50, 3, [49]),
@@ -131,6 +132,12 @@ def test_single_tokens(hip, batch, heads, kv, seq_k, d, lens):
 @pytest.mark.parametrize("seq_q,seq_k", [(2, 5000), (40, 9), (3000, 5), (1, 3000)])
 def test_lopsided_lengths(hip, seq_q, seq_k):
     check(hip, Problem(1, 2, 1, seq_q, seq_k, 64, seed=seq_q))
+
+
+@pytest.mark.parametrize("d,heads", [(20, 86), (64, 43), (80, 29), (128, 22)])
+def test_much_work(hip, d, heads):
+    """Enough for every compute unit to take 256 rows at a time."""
+    check(hip, Problem(2, heads, heads, 130, 1500, d, lens=[1500, 1211], seed=d))
 
 
 @pytest.mark.parametrize("batch,heads,kv,seq_q,seq_k,d,lens", [
