@@ -4,7 +4,7 @@
 //   dtable[t] = scale * sum over ids[i] = t of grad[i] + beta * dtable[t]
 //                                              outside the table, no gradient)
 //
-// The gradient takes three launches:
+// The gradient of more than 256 positions takes three launches:
 //  1. sort: every workgroup owns a range of tokens, looks through all ids twice
 //     (they stay in the caches) and places its own tokens' positions, in order,
 //     behind those of lower tokens: a counting sort without a pass between
@@ -83,6 +83,7 @@ constexpr int kSortWaves = 16, kSortThreads = 64 * kSortWaves;
 constexpr int kMaxBins = 1024;  // tokens of a sorting workgroup
 constexpr int kIds = 16;        // ids a lane has in flight
 constexpr int kBatch = 8;       // rows a wave has in flight
+constexpr int kFew = 256;       // positions up to which one launch does it
 
 struct BackwardArgs {
     float* dtable;
@@ -339,6 +340,112 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(BackwardArgs a) {
         dst[e] = a.beta != 0.0f ? a.scale * sum[e] + a.beta * dst[e] : a.scale * sum[e];
 }
 
+// The gradient of few positions in one launch: a workgroup owns a range of
+// tokens and 256 columns of them, finds its own among the ids (one to a thread),
+// sorts them in LDS, clears its rows (beta 0) and adds. Its waves share a run, or
+// take a run each where there are several short ones. The three launches for the
+// same: 16 ids of 15 tokens, 704 wide, 4.3 us and 11.1; 256 of 32000, 256 wide, 9.2
+// and 16.3 (half of them one token: 12.5 and 16.7). Past 256 positions, in groups
+// of 1024 threads, it was 1.7 times as fast or 2 times as slow.
+__global__ __launch_bounds__(kFew) void embedding_few_kernel(BackwardArgs a) {
+    constexpr int WAVES = kFew / 64;
+    __shared__ int token[kFew], position[kFew], runs[kFew], sums[2][WAVES];
+    __shared__ f32x4 part[2][WAVES][64];
+    const int t = threadIdx.x, lane = t & 63;
+    const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int range = blockIdx.x / a.blocks, d0 = (blockIdx.x - range * a.blocks) * 256;
+    const int lo = range * a.bins, bins = min(a.bins, a.vocab - lo);
+    const int cols = min(256, a.dim - d0);
+    const int id = t < a.count ? a.ids[t] : -1;
+    const bool mine = id >= lo && id - lo < bins;
+    if (a.beta == 0.0f) {
+        int lanes = 1;
+        while (4 * lanes < cols) lanes *= 2;
+        const int c = 4 * (t & (lanes - 1));
+        for (int row = t / lanes; row < bins; row += kFew / lanes) {
+            float* const to = a.dtable + (int64_t)(lo + row) * a.dim + d0 + c;
+            if (c + 4 <= cols)
+                reinterpret_cast<Quad*>(to)->v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            else
+                for (int e = 0; c + e < cols; ++e) to[e] = 0.0f;
+        }
+    }
+    // the range's own positions, in order
+    const uint64_t before = (1ull << lane) - 1;
+    auto place = [&](bool one, int (&counts)[WAVES], int& n) {
+        const uint64_t all = __ballot(one);
+        if (lane == 0) counts[w] = __popcll(all);
+        __syncthreads();
+        int at = __popcll(all & before);
+        n = 0;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            at += i < w ? counts[i] : 0;
+            n += counts[i];
+        }
+        return at;
+    };
+    int n, n_runs;
+    const int at = place(mine, sums[0], n);
+    if (n == 0) return;
+    if (mine) runs[at] = id;  // (the tokens, until they are sorted)
+    __syncthreads();
+    if (mine) {
+        int rank = at;
+        if (bins > 1) {
+            rank = 0;
+            for (int j = 0; j < n; ++j) rank += runs[j] < id || (runs[j] == id && j < at);
+        }
+        token[rank] = id;
+        position[rank] = t;
+    }
+    __syncthreads();
+    const bool begins = t < n && (t == 0 || token[t] != token[t - 1]);
+    const int run = place(begins, sums[1], n_runs);
+    if (begins) runs[run] = t;
+    __syncthreads();
+    // entries p0 .. p1 - 1, in order
+    auto add = [&](int p0, int p1) {
+        f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int p = p0; p < p1; p += kBatch) {
+            f32x4 rows[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int64_t row = __builtin_amdgcn_readfirstlane(position[min(p + k, p1 - 1)]);
+                rows[k] = buffer_load4(
+                    buffer_rsrc(a.grad + row * a.dim + d0, p + k < p1 ? (int64_t)cols * 4 : 0),
+                    16 * lane);
+            }
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) sum = sum + rows[k];
+        }
+        return sum;
+    };
+    auto store = [&](int one, f32x4 sum) {
+        float* const dst = a.dtable + (int64_t)one * a.dim + d0 + 4 * lane;
+        const int live = min(4, cols - 4 * lane);
+        for (int e = 0; e < live; ++e)
+            dst[e] = a.beta != 0.0f ? a.scale * sum[e] + a.beta * dst[e] : a.scale * sum[e];
+    };
+    const bool together = n_runs < WAVES || n > 4 * n_runs;
+    for (int i = together ? 0 : w; i < n_runs; i += together ? 1 : WAVES) {
+        const int p0 = runs[i], p1 = i + 1 < n_runs ? runs[i + 1] : n;
+        const int one = __builtin_amdgcn_readfirstlane(token[p0]);
+        if (!together) {
+            store(one, add(p0, p1));
+            continue;
+        }
+        part[i & 1][w][lane] = add(p0 + (p1 - p0) * w / WAVES, p0 + (p1 - p0) * (w + 1) / WAVES);
+        __syncthreads();
+        if (w == 0) {
+            f32x4 sum = part[i & 1][0][lane];
+#pragma unroll
+            for (int k = 1; k < WAVES; ++k) sum = sum + part[i & 1][k][lane];
+            store(one, sum);
+        }
+    }
+}
+
 struct BackwardPlan {
     int bins, tile;
     int64_t groups, tiles;
@@ -428,6 +535,16 @@ int nrs_embedding_backward(float* dtable, const float* grad, const int32_t* ids,
     a.groups = (int)plan.groups;
     a.scale = scale;
     a.beta = beta;
+    // (a wide table, or one whose absent rows change, too, has the three launches)
+    if (count <= nrs::kFew && a.blocks <= 16 && (beta == 0.0f || beta == 1.0f)) {
+        const int64_t ranges = std::min<int64_t>(vocab, 4 * (int64_t)nrs::num_cus() / a.blocks);
+        a.bins = (int)((vocab + ranges - 1) / ranges);
+        const int64_t used = (vocab + a.bins - 1) / a.bins;
+        hipLaunchKernelGGL(nrs::embedding_few_kernel, dim3((unsigned)(used * a.blocks)),
+                           dim3(nrs::kFew), 0, nrs::stream(), a);
+        NRS_LAUNCH_CHECK("embedding backward");
+        return NRS_OK;
+    }
     a.sorted = reinterpret_cast<int32_t*>(scratch);
     a.start = a.sorted + plan.sorted;
     a.part = scratch + plan.sorted + plan.start;

@@ -46,6 +46,8 @@ CASES = [
     (3000, 70000, 64, "uniform"), (2000, 50021, 1000, "zipf"), (300, 40, 5, "outside"),
     (20000, 259, 128, "zipf"), (9000, 100, 30, "one"), (70001, 33000, 9, "zipf"),
     (513, 513, 2048, "zipf"), (63, 4000, 1027, "uniform"), (100000, 17, 3, "uniform"),
+    (256, 1, 4096, "one"), (256, 1500, 70, "zipf"), (250, 20, 4100, "zipf"), (256, 3000, 1025, "uniform"),
+    (200, 3000, 5, "one"), (255, 9, 130, "outside"), (130, 5000, 2, "zipf"),
 ]
 
 
