@@ -672,6 +672,309 @@ __global__ __launch_bounds__(256, D > 64 ? 1 : 2) void cross_tile_bwd_kernel(Cro
         dkv_walk<D, WAVES, FULL>(a, lds, starts, blockIdx.x - a.q_blocks);
 }
 
+// ---- own blocks of 16
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <class C, bool FULL>
+__device__ __forceinline__ void own16(u32x4 (&own)[C::D / 32][3], const CrossArgs& a,
+                                      const float* src, bool live, int g, float f) {
+#pragma unroll
+    for (int s = 0; s < C::D / 32; ++s) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int d = 4 * (4 * s + g) + e * (C::D / 2);
+            f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (live) {
+                if (FULL || d + 4 <= a.D) {
+                    v = reinterpret_cast<const Quad*>(src + d)->v;
+                } else {
+                    for (int i = 0; i < 4; ++i)
+                        if (d + i < a.D) v[i] = src[d + i];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[4 * e + i] = v[i] * f;
+        }
+        split8(x, own[s]);
+    }
+}
+
+template <class C>
+__device__ __forceinline__ u32x4 piece16(const u32x4* set, int row, int s, int p, int c, int g) {
+    return set[p * C::PLANE + unit_at<C>(row + c, 4 * s + g)];
+}
+
+template <class C, bool CLOSE>
+__device__ __forceinline__ void products16(f32x4 (&out)[2], const u32x4* set,
+                                           const u32x4 (&own)[C::D / 32][3], int kb, int c, int g) {
+#pragma unroll
+    for (int s = 0; s < C::D / 32; ++s) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            u32x4 met[3];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) met[p] = piece16<C>(set, kb * 32 + 16 * half, s, p, c, g);
+            f32x4& o = out[half];
+            o = mfma16(met[2], own[s][0], o);
+            o = mfma16(met[1], own[s][1], o);
+            o = mfma16(met[0], own[s][2], o);
+            o = mfma16(met[1], own[s][0], o);
+            o = mfma16(met[0], own[s][1], o);
+            if (!CLOSE) o = mfma16(met[0], own[s][0], o);
+        }
+    }
+    if (CLOSE) {
+        asm volatile("" : "+v"(c));
+#pragma unroll
+        for (int s = 0; s < C::D / 32; ++s)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                out[half] = mfma16(piece16<C>(set, kb * 32 + 16 * half, s, 0, c, g), own[s][0], out[half]);
+    }
+}
+
+template <class C>
+__device__ __forceinline__ void add16(f32x4 (&acc)[C::D / 16], const u32x4* set, int kb,
+                                      const u32x4 (&w)[3], int lane) {
+    const int x = lane & 3, e = (lane >> 2) & 3, g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < C::D / 16; ++j) {
+        u32x4 met[3];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int unit = unit_at<C>(kb * 32 + 16 * half + 4 * g + e,
+                                        4 * (j >> 1) + (j & 1) + 2 * (x >> 1));
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                const u32x2 v = read_transposed(
+                    reinterpret_cast<const u32x2*>(set + p * C::PLANE + unit) + (x & 1));
+                met[p][2 * half] = v[0];
+                met[p][2 * half + 1] = v[1];
+            }
+        }
+        f32x4& o = acc[j];
+        o = mfma16(met[2], w[0], o);
+        o = mfma16(met[1], w[1], o);
+        o = mfma16(met[0], w[2], o);
+        o = mfma16(met[1], w[0], o);
+        o = mfma16(met[0], w[1], o);
+        o = mfma16(met[0], w[0], o);
+    }
+}
+
+template <class C, bool FULL>
+__device__ __forceinline__ void store16(float* dst, const f32x4 (&acc)[C::D / 16], float f,
+                                        float beta, int D, int g) {
+#pragma unroll
+    for (int j = 0; j < C::D / 16; ++j) {
+        const int d = 4 * (4 * (j >> 1) + (j & 1) + 2 * (g >> 1)) + (g & 1) * (C::D / 2);
+        f32x4 v = acc[j] * f;
+        if (FULL || d + 4 <= D) {
+            Quad* const to = reinterpret_cast<Quad*>(dst + d);
+            if (beta != 0.0f) v = v + beta * to->v;
+            to->v = v;
+        } else {
+            for (int e = 0; e < 4; ++e)
+                if (d + e < D) dst[d + e] = beta != 0.0f ? v[e] + beta * dst[d + e] : v[e];
+        }
+    }
+}
+
+template <int D, bool FULL>
+__device__ __forceinline__ void dq_walk16(const CrossArgs& a, u32x4* lds, int block) {
+    using C = TileCfg<D, 8>;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Sq * a.G, tiles = (R + 127) / 128, items = a.B * a.KV;
+    const int tile = block % tiles, item = block / tiles % items, no = block / tiles / items;
+    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
+    const int row = (tile * 8 + w) * 16 + c;
+    const bool wave_live = (tile * 8 + w) * 16 < R, live = row < R;
+    int t0, t1;
+    share((L + C::KT - 1) / C::KT, no, a.q_splits, t0, t1);
+    Stage<C, FULL> k, v;
+    auto load = [&](int t) {
+        const int n = min(C::KT, L - t * C::KT);
+        k.template load<false>(a, a.k, a.ld_kv, b, kv, t * C::KT, n);
+        v.template load<false>(a, a.v, a.ld_kv, b, kv, t * C::KT, n);
+    };
+    if (t0 < t1) load(t0);
+    u32x4 qf[D / 32][3], gf[D / 32][3];
+    own16<C, FULL>(qf, a, a.q + (live ? query_offset(a, b, kv, row, a.ld_q) : 0), live, g, a.scale2);
+    own16<C, FULL>(gf, a, a.dout + (live ? query_offset(a, b, kv, row, a.ld_out) : 0), live, g, 1.0f);
+    const float nl = live ? a.neg_lse[(int64_t)item * R + row] : -INFINITY;
+    const float nd = live ? a.neg_delta[(int64_t)item * R + row] : 0.0f;
+    f32x4 acc[D / 16];
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (t0 < t1) {
+        k.store(a, lds);
+        v.store(a, lds + C::SET);
+        if (t0 + 1 < t1) load(t0 + 1);
+        __syncthreads();
+    }
+    for (int t = t0; t < t1; ++t) {
+        u32x4* const kl = lds + ((t - t0) & 1) * 2 * C::SET;
+        if (wave_live) {
+            const int n = L - t * C::KT;
+#pragma unroll
+            for (int kb = 0; kb < C::NB; ++kb) {
+                f32x4 s[2], dp[2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    s[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    dp[half] = f32x4{nd, nd, nd, nd};
+                }
+                products16<C, true>(s, kl, qf, kb, c, g);
+                products16<C, false>(dp, kl + C::SET, gf, kb, c, g);
+                if (n < C::KT) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (kb * 32 + 16 * (i / 4) + 4 * g + i % 4 >= n) s[i / 4][i % 4] = -INFINITY;
+                }
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[i] = __builtin_amdgcn_exp2f(s[i / 4][i % 4] + nl) * dp[i / 4][i % 4];
+                u32x4 p[3];
+                split8(x, p);
+                add16<C>(acc, kl, kb, p, lane);
+            }
+        }
+        if (t + 1 < t1) {
+            u32x4* const other = lds + ((t + 1 - t0) & 1) * 2 * C::SET;
+            k.store(a, other);
+            v.store(a, other + C::SET);
+            if (t + 2 < t1) load(t + 2);
+            __syncthreads();
+        }
+    }
+    if (!live) return;
+    if (a.q_splits > 1)
+        store16<C, FULL>(a.dq_part + (((int64_t)no * items + item) * R + row) * a.D, acc, 1.0f, 0.0f,
+                         a.D, g);
+    else
+        store16<C, FULL>(a.dq + query_offset(a, b, kv, row, a.ld_q), acc, a.scale, a.beta_q, a.D, g);
+}
+
+template <int D, bool FULL>
+__device__ __forceinline__ void dkv_walk16(const CrossArgs& a, u32x4* lds, f32x4* starts, int block) {
+    using C = TileCfg<D, 8>;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Sq * a.G, tiles = (a.Sk + 127) / 128, items = a.B * a.KV;
+    const int tile = block % tiles, item = block / tiles % items, no = block / tiles / items;
+    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
+    const int key = (tile * 8 + w) * 16 + c;
+    const bool wave_live = (tile * 8 + w) * 16 < L, live = key < L;
+    int t0, t1;
+    share((R + C::KT - 1) / C::KT, no, a.kv_splits, t0, t1);
+    if (tile * 128 >= L) t1 = t0;  // no live key here
+    Stage<C, FULL> q, go;
+    float start[2];  // of threads below KT: -lse and -delta of a row of the tile
+    auto load = [&](int t) {
+        const int r0 = t * C::KT, n = min(C::KT, R - r0);
+        q.template load<true>(a, a.q, a.ld_q, b, kv, r0, n);
+        go.template load<true>(a, a.dout, a.ld_out, b, kv, r0, n);
+        start[0] = -INFINITY;
+        start[1] = 0.0f;
+        if ((int)threadIdx.x < n) {
+            start[0] = a.neg_lse[(int64_t)item * R + r0 + threadIdx.x];
+            start[1] = a.neg_delta[(int64_t)item * R + r0 + threadIdx.x];
+        }
+    };
+    auto store = [&](int buf) {
+        q.store(a, lds + buf * 2 * C::SET);
+        go.store(a, lds + buf * 2 * C::SET + C::SET);
+        if ((int)threadIdx.x < C::KT) {
+            float* const to = reinterpret_cast<float*>(starts) + buf * 2 * C::KT;
+            to[threadIdx.x] = start[0];
+            to[C::KT + threadIdx.x] = start[1];
+        }
+    };
+    if (t0 < t1) load(t0);
+    u32x4 kf[D / 32][3], vf[D / 32][3];
+    own16<C, FULL>(kf, a, a.k + (live ? key_offset(a, b, kv, key) : 0), live, g, a.scale2);
+    own16<C, FULL>(vf, a, a.v + (live ? key_offset(a, b, kv, key) : 0), live, g, 1.0f);
+    f32x4 acc_k[D / 16], acc_v[D / 16];
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) acc_k[j] = acc_v[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (t0 < t1) {
+        store(0);
+        if (t0 + 1 < t1) load(t0 + 1);
+        __syncthreads();
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        u32x4* const ql = lds + buf * 2 * C::SET;
+        if (wave_live) {
+#pragma unroll
+            for (int rb = 0; rb < C::NB; ++rb) {
+                const f32x4* const st = starts + (buf * 2 * C::KT + rb * 32) / 4 + g;
+                f32x4 s[2], dp[2];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    s[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    dp[half] = st[C::KT / 4 + 4 * half];
+                }
+                products16<C, true>(s, ql, kf, rb, c, g);
+                products16<C, false>(dp, ql + C::SET, vf, rb, c, g);
+                float x[8], y[8];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const f32x4 nl = st[4 * half];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        x[4 * half + r] = __builtin_amdgcn_exp2f(s[half][r] + nl[r]);
+                        y[4 * half + r] = x[4 * half + r] * dp[half][r];
+                    }
+                }
+                u32x4 p[3];
+                split8(x, p);
+                add16<C>(acc_v, ql + C::SET, rb, p, lane);
+                split8(y, p);
+                add16<C>(acc_k, ql, rb, p, lane);
+            }
+        }
+        if (t + 1 < t1) {
+            store(buf ^ 1);
+            if (t + 2 < t1) load(t + 2);
+            __syncthreads();
+        }
+    }
+    if (key >= a.Sk) return;
+    if (a.kv_splits > 1) {
+        if (!live) return;  // the sum takes dead keys as zeros
+        const int64_t at = (((int64_t)no * items + item) * a.Sk + key) * a.D;
+        store16<C, FULL>(a.dk_part + at, acc_k, 1.0f, 0.0f, a.D, g);
+        store16<C, FULL>(a.dv_part + at, acc_v, 1.0f, 0.0f, a.D, g);
+        return;
+    }
+    if (!live) {
+        if (a.beta_kv == 1.0f) return;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) acc_k[j] = acc_v[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const int64_t at = key_offset(a, b, kv, key);
+    store16<C, FULL>(a.dk + at, acc_k, a.scale, a.beta_kv, a.D, g);
+    store16<C, FULL>(a.dv + at, acc_v, 1.0f, a.beta_kv, a.D, g);
+}
+
+template <int D, bool FULL>
+__global__ __launch_bounds__(512, 2) void cross_tile_bwd16_kernel(CrossArgs a) {
+    using C = TileCfg<D, 8>;
+    __shared__ u32x4 lds[4 * C::SET];
+    __shared__ f32x4 starts[C::KT];
+    if ((int)blockIdx.x < a.q_blocks)
+        dq_walk16<D, FULL>(a, lds, blockIdx.x);
+    else
+        dkv_walk16<D, FULL>(a, lds, starts, blockIdx.x - a.q_blocks);
+}
+
 template <int D>
 void launch_forward(const CrossArgs& a, unsigned blocks) {
     const bool full = a.D == D;
@@ -694,6 +997,11 @@ void launch_backward(CrossArgs a, bool only_rows) {
     a.q_blocks = a.dq ? (int)((R + own - 1) / own * items * a.q_splits) : 0;
     const int64_t kv_blocks = a.dk ? (a.Sk + own - 1) / own * items * a.kv_splits : 0;
     if (a.q_blocks + kv_blocks == 0) return;
+    if constexpr (D > 64) {
+        auto kernel = a.D == D ? cross_tile_bwd16_kernel<D, true> : cross_tile_bwd16_kernel<D, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(a.q_blocks + kv_blocks)), dim3(512), 0, stream(), a);
+        return;
+    }
     auto kernel = a.D == D ? cross_tile_bwd_kernel<D, true> : cross_tile_bwd_kernel<D, false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(a.q_blocks + kv_blocks)), dim3(256), 0, stream(), a);
 }
