@@ -763,27 +763,28 @@ struct BackwardPlan {
 };
 
 // A workgroup to a compute unit: a walk that is longer than half a compute
-// unit's even part of all the work is shared out, so that the last walks to end
-// leave less idle (2 x 777 rows of 4 heads, 4096 keys and fewer, d_head 128:
-// 1164 us in whole walks, 1080 in halves). A step of dq is three products a
-// tile, one of dk and dv four. Asked for both gradients or not, the plan is
-// that of both: each has the same bits by itself.
+// unit's even part of all the work is shared out, one of dq, which begin last,
+// than a quarter, so that the last walks to end leave less idle (2 x 777 rows of
+// 16 heads, 4096 keys and fewer, 4 key heads of 128: 1042 us with both by halves,
+// 1000 like this; whole walks took 8% longer than halves). A step of dq is three
+// products a tile, one of dk and dv four. Asked for both gradients or not, the plan
+// is that of both: each has the same bits by itself.
 BackwardPlan plan_backward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
                            int64_t seq_k, int64_t d_head) {
     const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads, cus = num_cus();
     BackwardPlan p{1, 1, items * R, items * seq_k, false, false, 0, 0, 0};
     p.prepared = (size_t)((2 * p.rows + 3) / 4 * 4);  // needed without keys, too
     if (p.rows == 0 || p.keys == 0) return p;
-    const int64_t tile = cross_tile_keys((int)d_head, 4), own = kCrossBackwardRows;
+    const int64_t tile = cross_tile_keys((int)d_head, d_head > 32 ? 8 : 4), own = kCrossBackwardRows;
     const int64_t q_len = (seq_k + tile - 1) / tile, kv_len = (R + tile - 1) / tile;
     const int64_t q_groups = items * ((R + own - 1) / own),
                   kv_groups = items * ((seq_k + own - 1) / own);
     const int64_t even = std::max<int64_t>(16, (3 * q_groups * q_len + 4 * kv_groups * kv_len) / (2 * cus));
-    auto shares = [&](int64_t cost, int64_t len) {
-        return (int)std::max<int64_t>(1, std::min<int64_t>({(cost + even - 1) / even, len, 64}));
+    auto shares = [](int64_t cost, int64_t len, int64_t part) {
+        return (int)std::max<int64_t>(1, std::min<int64_t>({(cost + part - 1) / part, len, 64}));
     };
-    p.q_splits = shares(3 * q_len, q_len);
-    p.kv_splits = shares(4 * kv_len, kv_len);
+    p.q_splits = shares(3 * q_len, q_len, std::max<int64_t>(16, even / 2));
+    p.kv_splits = shares(4 * kv_len, kv_len, even);
     p.short_rows = R <= kShort;
     p.short_keys = !p.short_rows && seq_k <= kShort;
     if (p.short_rows || p.short_keys) {

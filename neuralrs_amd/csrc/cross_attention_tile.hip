@@ -661,7 +661,7 @@ __device__ __forceinline__ void dkv_walk(const CrossArgs& a, u32x4* lds, float* 
 // One launch for both: they need nothing of each other, and the workgroups of
 // one fill the compute units that the other leaves idle.
 template <int D, bool FULL>
-__global__ __launch_bounds__(256, D > 64 ? 1 : 2) void cross_tile_bwd_kernel(CrossArgs a) {
+__global__ __launch_bounds__(256, 2) void cross_tile_bwd_kernel(CrossArgs a) {
     constexpr int WAVES = 4;
     using C = TileCfg<D, WAVES>;
     __shared__ u32x4 lds[4 * C::SET];
@@ -672,12 +672,22 @@ __global__ __launch_bounds__(256, D > 64 ? 1 : 2) void cross_tile_bwd_kernel(Cro
         dkv_walk<D, WAVES, FULL>(a, lds, starts, blockIdx.x - a.q_blocks);
 }
 
-// ---- own blocks of 16
+// The backward of heads past 32 columns, 16 rows or keys to a wave on
+// v_mfma_f32_16x16x32_bf16 (rate and operands of the same size): a wave reads as
+// much from LDS for half as many, but its operands and accumulators leave room for
+// two waves on a SIMD, which hide each other's exponentials and splits. With 32 to a
+// wave: 4 x 1000 x 1500, 16 heads of 64, 563 us and here 552; 4 x 512 x 1500 of 96,
+// 539 and 440; 2 x 777 x 4096, 16 heads of 128 on 4, 1419 and 1162; but 32 x 128 x
+// 200, 8 heads of 32, 33 and 39. A wave computes met . own^T in two blocks of 16:
+// lane (c, g) = (lane % 16, lane / 16) gets its own c with the met 16 half + 4 g + r,
+// which lie as the operand of the product over the 32 met rows: place 8 g + 4 half + r.
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// The lane's operands of its own row at `src` (zeros unless live), times f: unit
+// 4 s + g of it is step s.
 template <class C, bool FULL>
 __device__ __forceinline__ void own16(u32x4 (&own)[C::D / 32][3], const CrossArgs& a,
                                       const float* src, bool live, int g, float f) {
@@ -703,11 +713,14 @@ __device__ __forceinline__ void own16(u32x4 (&own)[C::D / 32][3], const CrossArg
     }
 }
 
+// The operand of step s of 16 rows of a tile.
 template <class C>
 __device__ __forceinline__ u32x4 piece16(const u32x4* set, int row, int s, int p, int c, int g) {
     return set[p * C::PLANE + unit_at<C>(row + c, 4 * s + g)];
 }
 
+// out += met . own^T of block kb of a tile; CLOSE: the large products last, as in
+// close_products.
 template <class C, bool CLOSE>
 __device__ __forceinline__ void products16(f32x4 (&out)[2], const u32x4* set,
                                            const u32x4 (&own)[C::D / 32][3], int kb, int c, int g) {
@@ -728,7 +741,7 @@ __device__ __forceinline__ void products16(f32x4 (&out)[2], const u32x4* set,
         }
     }
     if (CLOSE) {
-        asm volatile("" : "+v"(c));
+        asm volatile("" : "+v"(c));  // read again, as there
 #pragma unroll
         for (int s = 0; s < C::D / 32; ++s)
 #pragma unroll
@@ -737,6 +750,9 @@ __device__ __forceinline__ void products16(f32x4 (&out)[2], const u32x4* set,
     }
 }
 
+// acc[j] += met^T . w over the 32 met rows of block kb, w split. Of the 16 places m of
+// output block j, 4 x + y is d = 4 unit + (x % 2) D/2 + y, unit = 4 (j / 2) + j % 2 +
+// 2 (x / 2): each x a half of one unit, as a transposing read takes them.
 template <class C>
 __device__ __forceinline__ void add16(f32x4 (&acc)[C::D / 16], const u32x4* set, int kb,
                                       const u32x4 (&w)[3], int lane) {
@@ -766,6 +782,7 @@ __device__ __forceinline__ void add16(f32x4 (&acc)[C::D / 16], const u32x4* set,
     }
 }
 
+// Stores a lane's acc * f (+ beta * old) into its own row of d_head floats.
 template <class C, bool FULL>
 __device__ __forceinline__ void store16(float* dst, const f32x4 (&acc)[C::D / 16], float f,
                                         float beta, int D, int g) {
@@ -784,6 +801,7 @@ __device__ __forceinline__ void store16(float* dst, const f32x4 (&acc)[C::D / 16
     }
 }
 
+// dq_walk with 16 rows to a wave.
 template <int D, bool FULL>
 __device__ __forceinline__ void dq_walk16(const CrossArgs& a, u32x4* lds, int block) {
     using C = TileCfg<D, 8>;
@@ -861,6 +879,7 @@ __device__ __forceinline__ void dq_walk16(const CrossArgs& a, u32x4* lds, int bl
         store16<C, FULL>(a.dq + query_offset(a, b, kv, row, a.ld_q), acc, a.scale, a.beta_q, a.D, g);
 }
 
+// dkv_walk with 16 keys to a wave.
 template <int D, bool FULL>
 __device__ __forceinline__ void dkv_walk16(const CrossArgs& a, u32x4* lds, f32x4* starts, int block) {
     using C = TileCfg<D, 8>;
@@ -969,10 +988,11 @@ __global__ __launch_bounds__(512, 2) void cross_tile_bwd16_kernel(CrossArgs a) {
     using C = TileCfg<D, 8>;
     __shared__ u32x4 lds[4 * C::SET];
     __shared__ f32x4 starts[C::KT];
-    if ((int)blockIdx.x < a.q_blocks)
-        dq_walk16<D, FULL>(a, lds, blockIdx.x);
+    const int kv_blocks = gridDim.x - a.q_blocks;  // (the longer walks begin first)
+    if ((int)blockIdx.x >= kv_blocks)
+        dq_walk16<D, FULL>(a, lds, blockIdx.x - kv_blocks);
     else
-        dkv_walk16<D, FULL>(a, lds, starts, blockIdx.x - a.q_blocks);
+        dkv_walk16<D, FULL>(a, lds, starts, blockIdx.x);
 }
 
 template <int D>
@@ -997,13 +1017,15 @@ void launch_backward(CrossArgs a, bool only_rows) {
     a.q_blocks = a.dq ? (int)((R + own - 1) / own * items * a.q_splits) : 0;
     const int64_t kv_blocks = a.dk ? (a.Sk + own - 1) / own * items * a.kv_splits : 0;
     if (a.q_blocks + kv_blocks == 0) return;
-    if constexpr (D > 64) {
-        auto kernel = a.D == D ? cross_tile_bwd16_kernel<D, true> : cross_tile_bwd16_kernel<D, false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(a.q_blocks + kv_blocks)), dim3(512), 0, stream(), a);
-        return;
+    if constexpr (D > 32) {
+        auto kernel =
+            a.D == D ? cross_tile_bwd16_kernel<D, true> : cross_tile_bwd16_kernel<D, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(a.q_blocks + kv_blocks)), dim3(512), 0, stream(),
+                           a);
+    } else {
+        auto kernel = a.D == D ? cross_tile_bwd_kernel<D, true> : cross_tile_bwd_kernel<D, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(a.q_blocks + kv_blocks)), dim3(256), 0, stream(), a);
     }
-    auto kernel = a.D == D ? cross_tile_bwd_kernel<D, true> : cross_tile_bwd_kernel<D, false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.q_blocks + kv_blocks)), dim3(256), 0, stream(), a);
 }
 
 }  // namespace
