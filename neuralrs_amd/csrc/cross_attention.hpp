@@ -145,9 +145,7 @@ struct LinePart {
 
 // The kernels of cross_attention_tile.hip, and the sizes by which calls are
 // planned. A workgroup of the forward owns 256 rows (8 waves) or 128 (4), one of
-// the backward 128 rows or keys, two workgroups to a compute unit up to d_head
-// 64: the time of one of 8 waves at 4 x 1000 x 1500 (16 heads of 64: 534 us,
-// 553), and fewer idle waves where an item has few rows or keys.
+// the backward 128 rows or keys: 32 to a wave up to d_head 32, else 16.
 constexpr int kCrossBackwardRows = 128;
 // Columns of a tile: a multiple of 32, and 96 for those in between (2 x 1037 rows,
 // 2506 keys, 2 heads of 96: backward 153 us, in tiles of 128 columns 229).

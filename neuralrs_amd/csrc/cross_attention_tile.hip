@@ -38,11 +38,12 @@
 // them about 5 an instruction, of which two waves to a SIMD hide a part.
 //   rows x keys, heads of d          forward          backward
 //   32 x 128 x 200, 8 of 32           12.8 us            27 us
-//   4 x 1000 x 1500, 16 of 64          134 (183 TFLOP/s) 542 (113; 159 with the
+//   4 x 1000 x 1500, 16 of 64          134 (183 TFLOP/s) 543 (113; 158 with the
 //                                                        two products it repeats)
-//   2 x 777 x 4096, 16 of 128, 4 key   264 (155)        1260 (81; 114)
-// The backward at 128 has one wave to a SIMD and some 100 of its registers in
-// scratch memory.
+//   2 x 777 x 4096, 16 of 128, 4 key   259 (158)         990 (103; 145)
+// In the last one's backward the matrix instructions run 38% of the time, the rest of
+// the vector work 33, and compute units are idle for some of the rest, as walks end
+// at different times.
 #include <algorithm>
 
 #include "cross_attention.hpp"
