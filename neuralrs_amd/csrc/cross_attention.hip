@@ -734,7 +734,7 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
         const int64_t at_once = p.unit_rows == 128 && d_head <= 96 ? 2 * cus : cus;
         groups = std::min<int64_t>(at_once, units * tiles / 2);
         share = groups > 1 && (units + at_once - 1) / at_once * (tiles + 2) >
-                                  (units * tiles + groups - 1) / groups + 8;
+                                  (units * (tiles + 2) + groups - 1) / groups + 8;
     }
     p.blocks = units;
     if (share && batch <= kMaxSharedBatch) {
