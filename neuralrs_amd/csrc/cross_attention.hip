@@ -368,6 +368,125 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
     sum.store(a, b, item - b * a.KV, r, live);
 }
 
+// A short side in LDS: 16 T rows of two tensors, zeros past `n` and past d_head.
+// from(which, row) is where a row begins.
+template <int NJ, int T, class F>
+__device__ __forceinline__ void fill_short(float (&own)[2][16 * T][16 * NJ + 4], int n, int D,
+                                           F from) {
+    for (int i = threadIdx.x; i < 2 * 16 * T * 4 * NJ; i += 64 * kRowWaves) {
+        const int which = i / (16 * T * 4 * NJ), at = i % (16 * T * 4 * NJ), row = at / (4 * NJ),
+                  d = at % (4 * NJ) * 4;
+        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (row < n) {
+            const float* const src = from(which, row);
+            if (d + 4 <= D)
+                v = reinterpret_cast<const Quad*>(src + d)->v;
+            else
+                for (int e = 0; d + e < D; ++e) v[e] = src[d + e];
+        }
+        *reinterpret_cast<f32x4*>(&own[which][row][d]) = v;
+    }
+}
+
+// Adds, over the own rows 4g + r at `rows`, weight[r] (own row, tile's row c) times
+// the row: lane (c, g) of to[j] gets column c NJ + j of the tile's rows 4g + r.
+template <int NJ>
+__device__ __forceinline__ void add_short(f32x4 (&to)[NJ], const float (*rows)[16 * NJ + 4],
+                                          f32x4 weight, int c, int g) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float* const src = &rows[4 * g + r][c * NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) to[j] = mfma16(weight[r], src[j], to[j]);
+    }
+}
+
+// Row 4g + r of a tile, as add_short leaves it, NJ neighbouring columns to a lane:
+// 16 lanes store a row one after the other.
+template <int NJ>
+__device__ __forceinline__ void store_short(float* dst, const f32x4 (&x)[NJ], int r, float f,
+                                            float beta, int D, int c) {
+#pragma unroll
+    for (int j = 0; j < NJ; j += 4) {
+        const int d = c * NJ + j;
+        if (NJ % 4 == 0 && d + 4 <= D) {
+            f32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = x[(j + i) % NJ][r] * f;
+            Quad* const to = reinterpret_cast<Quad*>(dst + d);
+            if (beta != 0.0f) v = v + beta * to->v;
+            to->v = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < (NJ < 4 ? NJ : 4); ++i) {
+                const float v = x[(j + i) % NJ][r] * f;
+                if (d + i < D) dst[d + i] = beta != 0.0f ? v + beta * dst[d + i] : v;
+            }
+        }
+    }
+}
+
+// The forward of many rows over up to 16 keys: K and V stay in LDS, and the rows
+// stream in tiles of 16 that the waves take in turns, read once and written once.
+// 8 x 1951 rows of 56 heads, 10 keys, 8 key heads of 96: 156 us, 4.3 TB/s (the
+// kernel of many keys 253); 50 x 102 rows of 112 heads, 6 keys, 16 key heads of 40:
+// 58 us and 105. With more keys, up to 48, it was faster (57 and 73 us) or slower
+// (20 and 17) by the sizes.
+template <int NJ>
+__global__ __launch_bounds__(64 * kRowWaves) void cross_short_fwd_kernel(CrossArgs a) {
+    __shared__ f32x4 shared[2 * 16 * (16 * NJ + 4) / 4];
+    float(&own)[2][16][16 * NJ + 4] = *reinterpret_cast<float(*)[2][16][16 * NJ + 4]>(shared);
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Sq * a.G, items = a.B * a.KV, item = blockIdx.x % items;
+    const int no = blockIdx.x / items, shares = gridDim.x / items;
+    const int b = item / a.KV, kv = item - b * a.KV, L = live_keys(a, b);
+    fill_short<NJ, 1>(own, L, a.D, [&](int which, int row) {
+        return (which ? a.v : a.k) + key_offset(a, b, kv, row);
+    });
+    __syncthreads();
+    const int tiles = (R + 15) / 16, t1 = (int)((int64_t)tiles * (no + 1) / shares);
+    for (int t = (int)((int64_t)tiles * no / shares) + w; t < t1; t += kRowWaves) {
+        const int r0 = 16 * t, n = min(16, R - r0);
+        f32x4 q[NJ], p = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, sum[NJ];
+        Rows<true>(a, a.q, b, kv, a.ld_q, r0, n).template along<NJ>(q, c, g);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            q[j] = q[j] * a.scale2;
+            sum[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            const f32x4 x = *reinterpret_cast<const f32x4*>(&own[0][c][16 * j + 4 * g]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p = mfma16(x[e], q[j][e], p);
+        }
+        float top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (4 * g + r < L) top = fmaxf(top, p[r]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            p[r] = 4 * g + r < L ? __builtin_amdgcn_exp2f(p[r] - top) : 0.0f;
+            total += p[r];
+        }
+        add_short<NJ>(sum, own[1], p, c, g);
+        total = across_groups(total);
+        const float f = L > 0 ? 1.0f / total : 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float own_f = __shfl(f, 4 * g + r, 64);
+            if (4 * g + r < n)
+                store_short<NJ>(a.out + query_offset(a, b, kv, r0 + 4 * g + r, a.ld_out), sum, r,
+                                own_f, 0.0f, a.D, c);
+        }
+        if (a.stats && g == 0 && c < n) {
+            float* const st = row_stats(a, b, kv, r0 + c);
+            st[0] = L > 0 ? top : 0.0f;
+            st[1] = total;
+        }
+    }
+}
+
 // The backward where one side is short (up to 16 T rows of an item, or KEYS:
 // keys). The short side is the workgroup's own, X and Y (Q and dO, or K and V) in
 // LDS; the long side streams from memory once, in tiles of 16 that the waves take
@@ -378,12 +497,12 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
 // dQ = scale dS K); those over the tile, with P and dS turned about in LDS, add to
 // the short side's own (dQ, or dK and dV), which the waves and the workgroups that
 // share an item join at the end.
-// 16 x 5 rows of 112 heads, 5256 keys (16 key heads of 128): 1140 us, of which the
+// 16 x 5 rows of 112 heads, 5256 keys (16 key heads of 128): 1119 us, of which the
 // matrix instructions are some 525 and the 2.8 GB some 560, with a wave to a SIMD;
-// 5 x 2 rows, 9000 keys, 4 heads of 128: 127 us, 2.9 TB/s. Three workgroups to a
+// 5 x 2 rows, 9000 keys, 4 heads of 128: 109 us, 3.4 TB/s. Three workgroups to a
 // compute unit: six took 1262 us in the first and 148 in the second. The next tile
 // asked for a tile ahead took 1242 and 121, and 284 in place of 230 at 19 x 4 rows,
-// 12867 keys, 3 key heads of 40.
+// 12867 keys, 3 key heads of 40 (178 now that rows are stored by neighbouring lanes).
 template <int NJ, int T, bool KEYS>
 __global__ __launch_bounds__(64 * kRowWaves) void cross_short_bwd_kernel(CrossArgs a) {
     constexpr int W = 16 * NJ + 4, OWN = 2 * 16 * T * W, SUMS = kRowWaves * 4 * NJ * 64;
@@ -404,22 +523,11 @@ __global__ __launch_bounds__(64 * kRowWaves) void cross_short_bwd_kernel(CrossAr
     const int met = KEYS ? (L > 0 ? R : 0) : L, all = KEYS ? R : a.Sk;
     const float* const lse = a.neg_lse + (int64_t)item * R;
     const float* const delta = a.neg_delta + (int64_t)item * R;
-    for (int i = threadIdx.x; i < 2 * 16 * T * 4 * NJ; i += 64 * kRowWaves) {
-        const int which = i / (16 * T * 4 * NJ), at = i % (16 * T * 4 * NJ), row = at / (4 * NJ),
-                  d = at % (4 * NJ) * 4;
-        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (row < n) {
-            const float* const src =
-                KEYS ? (which ? a.v : a.k) + key_offset(a, b, kv, row)
-                     : (which ? a.dout + query_offset(a, b, kv, row, a.ld_out)
-                              : a.q + query_offset(a, b, kv, row, a.ld_q));
-            if (d + 4 <= a.D)
-                v = reinterpret_cast<const Quad*>(src + d)->v;
-            else
-                for (int e = 0; d + e < a.D; ++e) v[e] = src[d + e];
-        }
-        *reinterpret_cast<f32x4*>(&own[which][row][d]) = v;
-    }
+    fill_short<NJ, T>(own, n, a.D, [&](int which, int row) {
+        if (KEYS) return (which ? a.v : a.k) + key_offset(a, b, kv, row);
+        return which ? a.dout + query_offset(a, b, kv, row, a.ld_out)
+                     : a.q + query_offset(a, b, kv, row, a.ld_q);
+    });
     if (!KEYS && threadIdx.x < 16 * T) {
         const bool live = (int)threadIdx.x < n;
         reinterpret_cast<float*>(starts[0])[threadIdx.x] = live ? lse[threadIdx.x] : -INFINITY;
@@ -434,15 +542,6 @@ __global__ __launch_bounds__(64 * kRowWaves) void cross_short_bwd_kernel(CrossAr
             acc[ot][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             if (KEYS) acc_y[ot][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-    // weight[r] of the own rows 4g + r times their columns c NJ ..
-    auto add_own = [&](f32x4(&to)[NJ], int which, int ot, f32x4 weight) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float* const src = &own[which][16 * ot + 4 * g + r][c * NJ];
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) to[j] = mfma16(src[j], weight[r], to[j]);
-        }
-    };
     auto add_met = [&](f32x4(&to)[NJ], const float (&x)[4][NJ], f32x4 weight) {
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -459,25 +558,6 @@ __global__ __launch_bounds__(64 * kRowWaves) void cross_short_bwd_kernel(CrossAr
 #pragma unroll
         for (int r = 0; r < 4; ++r) y[r] = reinterpret_cast<const float*>(at[4 * g + r])[c];
         return y;
-    };
-    // The gradient of the tile's row c: 4 NJ neighbouring columns to a lane.
-    auto store = [&](float* dst, const f32x4(&x)[NJ], float f, float beta) {
-#pragma unroll
-        for (int e = 0; e < 4 * NJ; e += 4) {
-            const int d = 4 * NJ * g + e;
-            f32x4 v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = x[(e + i) % NJ][(e + i) / NJ] * f;
-            if (d + 4 <= a.D) {
-                Quad* const to = reinterpret_cast<Quad*>(dst + d);
-                if (beta != 0.0f) v = v + beta * to->v;
-                to->v = v;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 3; ++i)
-                    if (d + i < a.D) dst[d + i] = beta != 0.0f ? v[i] + beta * dst[d + i] : v[i];
-            }
-        }
     };
     const int tiles = (all + 15) / 16, t1 = (int)((int64_t)tiles * (no + 1) / shares);
     for (int t = (int)((int64_t)tiles * no / shares) + w; t < t1; t += kRowWaves) {
@@ -524,8 +604,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void cross_short_bwd_kernel(CrossAr
                     ds[r] = live ? p[r] * (ds[r] + (KEYS ? met_delta : nd[r])) : 0.0f;
                 }
                 if (finish) {
-                    add_own(dx, 0, ot, ds);
-                    if (!KEYS) add_own(dy, 1, ot, p);
+                    add_short<NJ>(dx, &own[0][16 * ot], ds, c, g);
+                    if (!KEYS) add_short<NJ>(dy, &own[1][16 * ot], p, c, g);
                 }
                 if (add) {
                     add_met(acc[ot], cx, turn(ds, 0));
@@ -533,13 +613,19 @@ __global__ __launch_bounds__(64 * kRowWaves) void cross_short_bwd_kernel(CrossAr
                 }
             }
         }
-        if (finish && m0 + c < all) {
-            if (KEYS) {
-                store(a.dq + query_offset(a, b, kv, m0 + c, a.ld_q), dx, a.scale, a.beta_q);
-            } else if (c < nm || a.beta_kv != 1.0f) {  // else a dead key's, left as it is
-                const int64_t at = key_offset(a, b, kv, m0 + c);
-                store(a.dk + at, dx, a.scale, a.beta_kv);
-                store(a.dv + at, dy, 1.0f, a.beta_kv);
+        if (finish) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int m = 4 * g + r;
+                if (m0 + m >= all) continue;
+                if (KEYS) {
+                    store_short<NJ>(a.dq + query_offset(a, b, kv, m0 + m, a.ld_q), dx, r, a.scale,
+                                    a.beta_q, a.D, c);
+                } else if (m < nm || a.beta_kv != 1.0f) {  // else a dead key's, left as it is
+                    const int64_t at = key_offset(a, b, kv, m0 + m);
+                    store_short<NJ>(a.dk + at, dx, r, a.scale, a.beta_kv, a.D, c);
+                    store_short<NJ>(a.dv + at, dy, r, 1.0f, a.beta_kv, a.D, c);
+                }
             }
         }
     }
@@ -688,6 +774,7 @@ int check_shape(const char* what, int64_t batch, int64_t heads, int64_t kv_heads
 
 struct ForwardPlan {
     bool tiles;      // the kernel of many rows
+    bool few_keys;   // the kernel of many rows over up to 16 keys
     int unit_rows;   // of a unit (the scratch of a call with fewer holds no more)
     int groups;      // workgroups that share all units, 0: one each
     int64_t blocks;  // workgroups of the launch
@@ -702,8 +789,14 @@ constexpr int64_t kFewRows = 32;
 ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
                          int64_t seq_k, int64_t d_head) {
     const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads, cus = num_cus();
-    ForwardPlan p{R > kFewRows, 16, 0, 0, 0, 0, 0};
+    ForwardPlan p{R > kFewRows && seq_k > 16, R > kFewRows && seq_k <= 16, 16, 0, 0, 0, 0, 0};
     if (items == 0 || R == 0) return p;
+    if (p.few_keys) {
+        // four workgroups to a compute unit, a tile of 16 rows to a wave at least
+        p.blocks = items * std::max<int64_t>(
+            1, std::min<int64_t>(4 * cus / items, (R + 15) / 16 / kRowWaves));
+        return p;
+    }
     int64_t units, groups;
     bool share;
     if (!p.tiles) {
@@ -865,7 +958,13 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
     a.by_group = nrs::make_fastdiv((uint32_t)a.G);
     a.scale = scale;
     a.scale2 = scale * 1.4426950408889634f;
-    if (plan.tiles) {
+    if (plan.few_keys) {
+        nrs::for_width(a.D, [&](auto nj) {
+            hipLaunchKernelGGL(nrs::cross_short_fwd_kernel<decltype(nj)::value>,
+                               dim3((unsigned)plan.blocks), dim3(64 * nrs::kRowWaves), 0,
+                               nrs::stream(), a);
+        });
+    } else if (plan.tiles) {
         nrs::cross_tile_forward(a, (unsigned)plan.blocks);
     } else {
         nrs::for_width(a.D, [&](auto nj) {

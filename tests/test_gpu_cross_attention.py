@@ -145,7 +145,7 @@ def test_much_work(hip, d, heads):
     (2, 6, 2, 5, 3000, 98, [3000, 1501]), (1, 32, 1, 1, 2047, 128, None),
     (40, 8, 8, 3, 140, 16, list(range(0, 160, 4))), (2, 3, 1, 10, 31, 17, [31, 16]),
     (1, 2, 2, 4000, 1, 80, None), (2, 4, 1, 13, 1500, 128, [1490, 0]), (2, 1, 1, 500, 48, 128, [33, 48]),
-    (1, 2, 2, 48, 3000, 32, None), (3, 2, 1, 2500, 47, 16, [0, 47, 5]), (2, 1, 1, 49, 90, 8, [90, 6]), (2, 1, 1, 90, 49, 8, [49, 6]),
+    (1, 2, 2, 48, 3000, 32, None), (3, 4, 2, 130, 16, 100, [16, 1, 0]), (2, 4, 4, 37, 17, 33, [17, 4]), (3, 2, 1, 2500, 47, 16, [0, 47, 5]), (2, 1, 1, 49, 90, 8, [90, 6]), (2, 1, 1, 90, 49, 8, [49, 6]),
 ])
 @pytest.mark.parametrize("beta", [0.0, 1.0])
 def test_short_sides(hip, batch, heads, kv, seq_q, seq_k, d, lens, beta):
