@@ -797,10 +797,11 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
             1, std::min<int64_t>(4 * cus / items, (R + 15) / 16 / kRowWaves));
         return p;
     }
-    int64_t units, groups;
+    int64_t units, groups, tiles;
     bool share;
     if (!p.tiles) {
         units = items * ((R + 15) / 16);
+        tiles = (seq_k + 15) / 16;
         // Shared unless there are enough units by themselves; at least two
         // tiles of 16 keys to a wave. Workgroups to a compute unit
         // by the bytes that each has on the way (a tile of K and V to a wave):
@@ -808,7 +809,7 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
         // keys, 8 key heads) and 38, 30 and 26 us, 3 26 us, at d_head 64 (32
         // items of up to 1500 keys, 8 key heads).
         groups = std::min<int64_t>((d_head > 64 ? 1 : d_head > 32 ? 3 : 6) * cus,
-                                   units * ((seq_k + 15) / 16) / (2 * kRowWaves));
+                                   units * tiles / (2 * kRowWaves));
         share = groups > units;
         p.unit_rows = (int)std::min<int64_t>(R, 16);
     } else {
@@ -820,8 +821,8 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
         const int64_t steps = items * ((R + 255) / 256) * ((seq_k * width + 4095) / 4096);
         p.unit_rows = R > 128 && steps >= 8 * cus ? 256 : 128;
         units = items * ((R + p.unit_rows - 1) / p.unit_rows);
-        const int64_t keys = cross_tile_keys((int)d_head, p.unit_rows / 32),
-                      tiles = (seq_k + keys - 1) / keys;
+        const int64_t keys = cross_tile_keys((int)d_head, p.unit_rows / 32);
+        tiles = (seq_k + keys - 1) / keys;
         // Workgroups at once, and the time of the fullest one in key tiles: a
         // piece's beginning and end cost two tiles, a join four.
         const int64_t at_once = p.unit_rows == 128 && d_head <= 96 ? 2 * cus : cus;
@@ -830,7 +831,8 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
                                   (units * (tiles + 2) + groups - 1) / groups + 8;
     }
     p.blocks = units;
-    if (share && batch <= kMaxSharedBatch) {
+    // (places on the line are 32-bit numbers)
+    if (share && batch <= kMaxSharedBatch && units * tiles <= INT32_MAX) {
         p.groups = (int)groups;
         p.blocks = groups;
         const int64_t slots = (groups + units) * p.unit_rows;

@@ -133,6 +133,13 @@ def test_workspace_of_a_backward_without_keys_or_rows():
     assert _abi.cross_attention_workspace(0, 4, 2, 3, 5, 32) == 0
 
 
+def test_a_line_of_key_tiles_past_32_bits_is_not_shared():
+    """2049 units of 256 rows with 2^20 tiles of keys each: their places on one
+    line would pass 2^31. (257 units of 2^14 tiles are shared, with scratch.)"""
+    assert _abi.cross_attention_workspace(1, 1, 1, 256 * 257, 2 ** 20, 64) > 0
+    assert _abi.cross_attention_workspace(1, 1, 1, 256 * 2049, 2 ** 26, 64) == 0
+
+
 @pytest.mark.parametrize("sizes", [(2, 4, 3, 3, 5, 32), (2, 2 ** 62, 1, 3, 5, 128), (2, 4, 2, 3, 5, 0),
                                    (-1, 4, 2, 3, 5, 32), (2 ** 40, 4, 2, 3, 5, 32)])
 def test_workspace_refuses_what_the_calls_refuse(sizes):
