@@ -231,7 +231,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void cross_rows_fwd_kernel(CrossArg
     if (!part.begin(a, per_item, 16, scan, found)) return;
     while (part.next(a))
         walk.run(part.b, part.sub / row_tiles, part.sub % row_tiles * 16, part.L, part.t0, part.t1,
-                 part.slot());
+                 part.slot(a));
 }
 
 // The sums of a row's parts: the reference and the sum of part s at stats(s),
@@ -304,15 +304,24 @@ struct Joined {
     }
 };
 
-// The parts of row r of an item: their number (0: no live keys) and where the
-// first one is, in rows of `part`; the others follow unit_rows apart.
-__device__ __forceinline__ int row_parts(const CrossArgs& a, int item, int b, int r, int64_t& at) {
-    if (live_keys(a, b) == 0) return 0;
-    const int units = (a.Sq * a.G + a.unit_rows - 1) / a.unit_rows;
-    const int unit = item * units + r / a.unit_rows, first = a.shares[2 * unit];
-    at = ((int64_t)first + unit) * a.unit_rows + r % a.unit_rows;
-    return a.shares[2 * unit + 1] - first + 1;
-}
+// The parts of row r of an item: their number (0: no live keys) and where in rows
+// of `part` each one is.
+struct RowParts {
+    int n = 0, unit_rows, begun = 0, line = 0;  // the rows of part 0, and of one before part 1
+    __device__ __forceinline__ RowParts(const CrossArgs& a, int item, int b, int r)
+        : unit_rows(a.unit_rows) {
+        if (live_keys(a, b) == 0) return;
+        const int units = (a.Sq * a.G + unit_rows - 1) / unit_rows, in_item = r / unit_rows;
+        const int unit = item * units + in_item, first = a.shares[2 * unit];
+        n = a.shares[2 * unit + 1] - first + 1;
+        const int in_unit = r - in_item * unit_rows;
+        begun = begun_slot(a, unit, first) * unit_rows + in_unit;
+        line = first * unit_rows + in_unit;
+    }
+    __device__ __forceinline__ int64_t at(int s) const {
+        return s == 0 ? begun : line + s * unit_rows;
+    }
+};
 
 // Joins the parts of cross_rows_fwd_kernel, a workgroup to a row: eight groups of
 // 32 threads take an eighth of them each and are added up in LDS: 4.8 us for 64
@@ -323,13 +332,12 @@ __global__ __launch_bounds__(256) void cross_rows_join_kernel(CrossArgs a) {
     const int x = threadIdx.x % 32, group = threadIdx.x / 32, R = a.Sq * a.G;
     const int item = blockIdx.x / R, r = blockIdx.x - item * R, b = item / a.KV;
     const int live = max(0, min(4, a.D - 4 * x));
-    int64_t at = 0;
-    const int n = row_parts(a, item, b, r, at);
-    if (n == 1) return;  // one workgroup took all of the unit
+    const RowParts parts(a, item, b, r);
+    if (parts.n == 1) return;  // one workgroup took all of the unit
     Joined<32> sum;
-    sum.add(n * group / 8, n * (group + 1) / 8, live,
-            [&](int s) { return a.part_stats + 2 * (at + (int64_t)s * a.unit_rows); },
-            [&](int s) { return a.part + (at + (int64_t)s * a.unit_rows) * a.D; });
+    sum.add(parts.n * group / 8, parts.n * (group + 1) / 8, live,
+            [&](int s) { return a.part_stats + 2 * parts.at(s); },
+            [&](int s) { return a.part + parts.at(s) * a.D; });
     sums[group][x] = sum.v;
     if (x == 0) {
         tops[group] = sum.top;
@@ -359,12 +367,11 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
     if (row >= (int64_t)a.B * a.KV * R) return;
     const int item = (int)(row / R), r = (int)(row - (int64_t)item * R), b = item / a.KV;
     const int live = max(0, min(4, a.D - 4 * x));
-    int64_t at = 0;
-    const int n = row_parts(a, item, b, r, at);
-    if (n == 1) return;
+    const RowParts parts(a, item, b, r);
+    if (parts.n == 1) return;
     Joined<LANES> sum;
-    sum.add(0, n, live, [&](int s) { return a.part_stats + 2 * (at + (int64_t)s * a.unit_rows); },
-            [&](int s) { return a.part + (at + (int64_t)s * a.unit_rows) * a.D; });
+    sum.add(0, parts.n, live, [&](int s) { return a.part_stats + 2 * parts.at(s); },
+            [&](int s) { return a.part + parts.at(s) * a.D; });
     sum.store(a, b, item - b * a.KV, r, live);
 }
 
@@ -777,6 +784,7 @@ struct ForwardPlan {
     bool few_keys;   // the kernel of many rows over up to 16 keys
     int unit_rows;   // of a unit (the scratch of a call with fewer holds no more)
     int groups;      // workgroups that share all units, 0: one each
+    bool few_units;  // fewer than those workgroups
     int64_t blocks;  // workgroups of the launch
     size_t part, stats, shares;  // scratch, in 4-byte words
     size_t bytes() const { return 4 * (part + stats + shares); }
@@ -789,7 +797,7 @@ constexpr int64_t kFewRows = 32;
 ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
                          int64_t seq_k, int64_t d_head) {
     const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads, cus = num_cus();
-    ForwardPlan p{R > kFewRows && seq_k > 16, R > kFewRows && seq_k <= 16, 16, 0, 0, 0, 0, 0};
+    ForwardPlan p{R > kFewRows && seq_k > 16, R > kFewRows && seq_k <= 16, 16, 0, false, 0, 0, 0, 0};
     if (items == 0 || R == 0) return p;
     if (p.few_keys) {
         // four workgroups to a compute unit, a tile of 16 rows to a wave at least
@@ -834,8 +842,9 @@ ForwardPlan plan_forward(int64_t batch, int64_t heads, int64_t kv_heads, int64_t
     // (places on the line are 32-bit numbers)
     if (share && batch <= kMaxSharedBatch && units * tiles <= INT32_MAX) {
         p.groups = (int)groups;
+        p.few_units = units < groups;
         p.blocks = groups;
-        const int64_t slots = (groups + units) * p.unit_rows;
+        const int64_t slots = (groups + std::min(groups, units)) * p.unit_rows;
         p.part = (size_t)((slots * d_head + 3) / 4 * 4);
         p.stats = (size_t)((2 * slots + 3) / 4 * 4);
         p.shares = (size_t)(2 * units);
@@ -938,6 +947,7 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
     nrs::CrossArgs a{};
     a.unit_rows = plan.unit_rows;
     a.groups = plan.groups;
+    a.few_units = plan.few_units;
     a.part = scratch;
     a.part_stats = scratch + plan.part;
     a.shares = reinterpret_cast<int32_t*>(scratch + plan.part + plan.stats);

@@ -27,11 +27,14 @@ struct CrossArgs {
     // `groups` 0 a workgroup takes a unit; else the key tiles of all units lie
     // one after the other, and `groups` workgroups take equal parts of that
     // line, whatever the items' lengths. A unit that a part begins or ends in
-    // leaves sums, not yet divided, in slot (workgroup + unit) of `part`
-    // [slots][unit_rows][D], which no two of them share, with their reference
-    // and sum in part_stats [slots][unit_rows][2]; `shares` has the first and the
-    // last workgroup of each unit.
+    // leaves sums, not yet divided, in a slot of `part` [slots][unit_rows][D],
+    // with their reference and sum in part_stats [slots][unit_rows][2]; `shares`
+    // has the first and the last workgroup of each unit. A workgroup goes on with
+    // an earlier one's unit once at most, in slot `workgroup`, and leaves a unit
+    // that it began to a later one once at most, in slot groups + workgroup, or
+    // groups + unit where there are fewer units.
     int unit_rows, groups;
+    bool few_units;  // fewer than workgroups
     float* part;
     float* part_stats;
     int32_t* shares;
@@ -63,6 +66,11 @@ __device__ __forceinline__ int64_t key_offset(const CrossArgs& a, int b, int kv,
 __device__ __forceinline__ float* row_stats(const CrossArgs& a, int b, int kv, int r) {
     const int s = (int)fast_div((uint32_t)r, a.by_group);
     return a.stats + (((int64_t)b * a.H + kv * a.G + (r - s * a.G)) * a.Sq + s) * 2;
+}
+
+// The slot of the sums of a unit that workgroup `first` began and left.
+__device__ __forceinline__ int begun_slot(const CrossArgs& a, int unit, int first) {
+    return a.groups + (a.few_units ? unit : first);
 }
 
 constexpr int kMaxSharedBatch = 1024;  // batch items of a shared launch
@@ -138,8 +146,9 @@ struct LinePart {
         return true;
     }
     // Where the piece's sums go: -1 if it is all of its unit.
-    __device__ __forceinline__ int64_t slot() const {
-        return t0 == 0 && t1 == tiles ? -1 : (int64_t)blockIdx.x + b * per_item + sub;
+    __device__ __forceinline__ int64_t slot(const CrossArgs& a) const {
+        if (t0 > 0) return blockIdx.x;
+        return t1 == tiles ? -1 : begun_slot(a, b * per_item + sub, blockIdx.x);
     }
 };
 

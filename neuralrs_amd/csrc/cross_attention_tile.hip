@@ -438,7 +438,7 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void cross_ti
     if (!part.begin(a, per_item, C::KT, scan, found)) return;
     while (part.next(a)) {
         forward_walk<D, WAVES, FULL>(a, lds, part.b, part.sub / tiles, part.sub % tiles, part.L,
-                                     part.t0, part.t1, part.slot());
+                                     part.t0, part.t1, part.slot(a));
         __syncthreads();  // before the next piece's tiles take the place of this one's
     }
 }

@@ -152,3 +152,16 @@ def test_workspace_queries():
     assert _abi.cross_attention_workspace(2, 4, 2, 3, 5, 32) >= 0
     assert _abi.cross_attention_workspace(2, 4, 2, 3, 5, 32, backward=True) >= 0
     assert _abi.embedding_workspace(100, 50, 8) >= 0
+
+
+@pytest.mark.parametrize("sizes", [(16, 32, 8, 4100, 2000, 128), (2, 33, 33, 9000, 700, 64),
+                                   (3, 40, 40, 5000, 1000, 96), (2, 40, 40, 9000, 3001, 20)])
+def test_scratch_of_a_shared_forward_does_not_grow_with_its_rows(sizes):
+    """A workgroup leaves the sums of two units at most, the one that its part
+    begins in and the one that it ends in: of 256 rows with a workgroup to each
+    of 256 compute units, or of 128 with two. A unit has its first and last
+    workgroup on record."""
+    batch, heads, _, seq_q, _, d = sizes
+    units = batch * heads * seq_q // 128 + batch * heads
+    need = _abi.cross_attention_workspace(*sizes)
+    assert 0 < need <= 2 * 256 * 256 * (d + 2) * 4 + 8 * units
