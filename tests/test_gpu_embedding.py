@@ -144,3 +144,27 @@ def test_own_scratch(hip):
         hip.embedding_backward(b, grad, d_ids, count, vocab, dim, work=work)
         assert np.array_equal(a.to_host(), b.to_host())
         assert np.all(work.to_host()[(need + 3) // 4:] == 7)
+
+
+# Long runs of one token, over many tiles and several blocks of columns, beside
+# the cases above.
+LONG = [(30000, 1, 515, "one"), (20011, 3, 600, "uniform"), (300000, 5, 300, "uniform"),
+        (65536, 259, 512, "zipf"), (12345, 7, 257, "zipf"), (1100, 2, 1024, "uniform")]
+
+
+@pytest.mark.parametrize("count,vocab,dim,how", CASES + LONG)
+@pytest.mark.parametrize("beta", [0.0, 1.0, 0.5])
+def test_integer_gradients_are_exact(hip, count, vocab, dim, how, beta):
+    """Integers of up to 8, at most 300000 of them to a sum, whose partial sums
+    all lie below 2^24: no order rounds, and a row that is lost or taken twice
+    shows. The scale is a power of two and the old values are even."""
+    rng = np.random.default_rng(count + dim)
+    ids = make_ids(rng, count, vocab, how)
+    grad = rng.integers(-8, 9, (count, dim)).astype(np.float32)
+    old = 2 * rng.integers(-50, 51, (vocab, dim)).astype(np.float32)
+    print(f"embedding, integers, {count} of {vocab} x {dim} {how} beta {beta}", flush=True)
+    value, _, _ = reference(ids, grad, vocab, 2.0)
+    dtable = hip.DeviceBuffer.from_host(old if beta else np.full_like(old, np.nan))
+    hip.embedding_backward(dtable, hip.DeviceBuffer.from_host(grad),
+                           hip.DeviceBuffer.from_host(ids, np.int32), count, vocab, dim, 2.0, beta)
+    assert np.array_equal(dtable.to_host((vocab, dim)), (value + beta * old).astype(np.float32))
