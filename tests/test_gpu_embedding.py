@@ -168,3 +168,46 @@ def test_integer_gradients_are_exact(hip, count, vocab, dim, how, beta):
     hip.embedding_backward(dtable, hip.DeviceBuffer.from_host(grad),
                            hip.DeviceBuffer.from_host(ids, np.int32), count, vocab, dim, 2.0, beta)
     assert np.array_equal(dtable.to_host((vocab, dim)), (value + beta * old).astype(np.float32))
+
+
+@pytest.mark.parametrize("count,dim,constant", [(1 << 24, 1, True), (1 << 22, 5, True), (3 << 20, 4, False)])
+def test_error_of_a_long_run_is_that_of_a_tile(hip, count, dim, constant):
+    """Tiles of at most 256 positions are added one after another: 255 half steps
+    of the sum of magnitudes at most, and a few for what comes after, however many
+    tiles a token's run has. Equal gradients round all in one direction."""
+    rng = np.random.default_rng(dim)
+    grad = np.full((count, dim), 1.1, np.float32)
+    if not constant:
+        grad = rng.uniform(0.5, 1.5, (count, dim)).astype(np.float32)
+    ids = np.full(count, 1, np.int32)
+    print(f"embedding, {count} positions of one token x {dim}", flush=True)
+    dtable = hip.DeviceBuffer(3 * dim)
+    hip.embedding_backward(dtable, hip.DeviceBuffer.from_host(grad),
+                           hip.DeviceBuffer.from_host(ids, np.int32), count, 3, dim, 1.0)
+    got = dtable.to_host((3, dim))
+    want = grad.astype(np.float64).sum(axis=0)
+    assert np.all(got[[0, 2]] == 0)
+    error = np.abs(got[1] - want) / want
+    assert np.all(error <= (255 + 8) * U), error.max() / U
+
+
+@pytest.mark.parametrize("count", [200, 40000])
+def test_gradients_that_are_not_finite(hip, count):
+    """An infinity stays one, in its own column of its own token; two of different
+    sign, or a NaN, give NaN."""
+    rng = np.random.default_rng(5)
+    dim, vocab = 260, 3
+    ids = np.full(count, 2, np.int32)
+    ids[::7] = 0
+    grad = rng.standard_normal((count, dim)).astype(np.float32)
+    grad[count // 2 // 7 * 7 + 1, 3] = np.inf
+    grad[[1, count - count % 7 - 3], 8] = np.inf, -np.inf
+    grad[count // 3 // 7 * 7 + 2, 259] = np.nan
+    print(f"embedding, infinities, {count}", flush=True)
+    dtable = hip.DeviceBuffer(vocab * dim)
+    hip.embedding_backward(dtable, hip.DeviceBuffer.from_host(grad),
+                           hip.DeviceBuffer.from_host(ids, np.int32), count, vocab, dim, 1.0)
+    got = dtable.to_host((vocab, dim))
+    assert got[2, 3] == np.inf and np.isnan(got[2, [8, 259]]).all()
+    got[2, [3, 8, 259]] = 0
+    assert np.isfinite(got).all()
