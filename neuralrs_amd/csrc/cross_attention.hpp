@@ -9,6 +9,7 @@
 #pragma once
 
 #include "buffer_ops.hpp"
+#include "cross_attention_plan.hpp"
 #include "fastdiv.hpp"
 
 namespace nrs {
@@ -72,8 +73,6 @@ __device__ __forceinline__ float* row_stats(const CrossArgs& a, int b, int kv, i
 __device__ __forceinline__ int begun_slot(const CrossArgs& a, int unit, int first) {
     return a.groups + (a.few_units ? unit : first);
 }
-
-constexpr int kMaxSharedBatch = 1024;  // batch items of a shared launch
 
 // A workgroup's part of the line of key tiles: an unbroken run of (unit, tiles)
 // pieces. `per_item` units to a batch item, tiles of `keys` keys.
@@ -152,19 +151,7 @@ struct LinePart {
     }
 };
 
-// The kernels of cross_attention_tile.hip, and the sizes by which calls are
-// planned. A workgroup of the forward owns 256 rows (8 waves) or 128 (4), one of
-// the backward 128 rows or keys: 32 to a wave up to d_head 32, else 16.
-constexpr int kCrossBackwardRows = 128;
-// Columns of a tile: a multiple of 32, and 96 for those in between (2 x 1037 rows,
-// 2506 keys, 2 heads of 96: backward 153 us, in tiles of 128 columns 229).
-constexpr int cross_tile_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
-// A quarter as many threads share a row in the kernels that go by rows.
-constexpr int cross_row_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
-// Keys (or rows) that a workgroup of that many waves takes at a time.
-constexpr int cross_tile_keys(int D, int waves) {
-    return (waves == 8 || D > 64 ? 4096 : 2048) / cross_tile_width(D) / 32 * 32;
-}
+// The kernels of cross_attention_tile.hip.
 void cross_tile_forward(const CrossArgs& a, unsigned blocks);
 // The rows' statistics, then (unless only they are wanted) what is asked for of
 // dq and dk, dv.

@@ -1,0 +1,122 @@
+"""Cross attention on every kernel that its planner can choose (cross_plan.py lists the
+calls, test_cross_plan.py holds them to their kernels), against the algebra of
+attention_ref.py in 64 bits on the device, with its bounds."""
+import math
+
+import pytest
+import torch
+
+import cross_plan
+from attention_ref import TINY, U, gamma
+
+pytestmark = pytest.mark.gpu
+
+MARK = -12345.0
+
+
+def mm(a, b):
+    return torch.mm(a.contiguous(), b.contiguous())
+
+
+def reference(q, k, v, g, scale):
+    """(value, bound) of out, the log2 of the rows' sums, dq, dk and dv: as
+    attention_ref.forward and backward, one item and key head."""
+    n, d, rows = len(k), q.shape[1], len(q)
+    if n == 0:
+        zero = [torch.zeros_like(x) for x in (q, q, k, v)]
+        none = torch.zeros(rows, dtype=torch.float64, device=q.device)
+        return [(x, x) for x in [zero[0], none] + zero[1:]]
+    s = mm(q, k.t()) * scale
+    m = s.amax(dim=1, keepdim=True)
+    p = torch.exp(s - m)
+    total = p.sum(dim=1, keepdim=True)
+    p = p / total
+    es = (gamma(d) + 4 * U) * (mm(q.abs(), k.abs().t()) * scale).amax(dim=1, keepdim=True)
+    ep = 2 * es + gamma(n) + 8 * U
+    out = mm(p, v)
+    out_bound = (ep + gamma(n)) * mm(p, v.abs()) + TINY * v.abs().sum(dim=0)
+    lse = m / math.log(2.0) + torch.log2(total)
+    lse_bound = 1.45 * ep + 4 * U * m.abs() / math.log(2.0)
+    dp = mm(g, v.t())
+    delta = (g * out).sum(dim=1, keepdim=True)
+    ds = p * (dp - delta) * scale
+    e_delta = (gamma(d) * g.abs() * out.abs() + g.abs() * out_bound).sum(dim=1, keepdim=True)
+    e_ds = scale * p * ((ep + 4 * U) * (dp - delta).abs() + gamma(d) * mm(g.abs(), v.abs().t()) + e_delta)
+    e_ds = e_ds + TINY * (1 + scale * (dp - delta).abs())
+    e_p = ep * p + TINY
+    return [(out, out_bound), (lse[:, 0], lse_bound[:, 0]),
+            (mm(ds, k), mm(e_ds + gamma(n) * ds.abs(), k.abs())),
+            (mm(ds.t(), q), mm((e_ds + gamma(rows) * ds.abs()).t(), q.abs())),
+            (mm(p.t(), g), mm((e_p + gamma(rows) * p).t(), g.abs()))]
+
+
+def within(got, value, bound, what):
+    tol = bound + 2.0 ** -24 * value.abs() + 2.0 ** -126
+    error = (got.double() - value).abs()
+    assert (error <= tol).all(), f"{what}: worst {(error / tol).nan_to_num(math.inf).max().item():.3g} of its bound"
+
+
+@pytest.mark.parametrize("number", range(len(cross_plan.SHAPES)),
+                         ids=lambda i: "x".join(map(str, cross_plan.SHAPES[i])))
+def test_every_kernel(hip, number):
+    """Every second call has padded rows and K and V in one tensor; where there are
+    several items their lengths differ and one is empty. The gradients are written,
+    added to the old ones, or added to half of them."""
+    batch, heads, kv, seq_q, seq_k, d = shape = cross_plan.SHAPES[number]
+    print(f"cross attention {shape}", flush=True)
+    packed, beta = number % 2 == 1, (0.0, 1.0, 0.5)[number % 3]
+    gen = torch.Generator(device="cuda").manual_seed(number)
+    new = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    hd, kd, group = heads * d, kv * d, heads // kv
+    ld_q, ld_out, ld_kv = hd + 3 * packed, hd + 5 * packed, kd * (1 + packed) + packed
+    lens = [seq_k] * batch
+    if batch > 1:
+        lens = [max(1, seq_k - i * seq_k // (2 * batch)) for i in range(batch)]
+        lens[batch // 2] = 0
+    key_len = torch.tensor(lens, dtype=torch.int32, device="cuda") if batch > 1 else None
+    q, dout, old_q = new(batch * seq_q, ld_q), new(batch * seq_q, ld_out), new(batch * seq_q, ld_q)
+    kb, old_k = new(batch * seq_k, ld_kv), new(batch * seq_k, ld_kv)
+    vb, old_v = (kb, old_k) if packed else (new(batch * seq_k, ld_kv), new(batch * seq_k, ld_kv))
+    for b, n in enumerate(lens):  # never looked at
+        kb[b * seq_k + n:(b + 1) * seq_k] = math.nan
+        vb[b * seq_k + n:(b + 1) * seq_k] = math.nan
+    at = kd if packed else 0
+    k, v = kb[:, :kd], vb[:, at:at + kd]
+    dq, dkb = old_q.clone(), old_k.clone()
+    dvb = dkb if packed else old_v.clone()
+    dk, dv = dkb[:, :kd], dvb[:, at:at + kd]
+    if beta == 0.0:  # the old gradients are never read
+        dq[:, :hd] = math.nan
+        dk.fill_(math.nan)
+        dv.fill_(math.nan)
+    out = torch.full((batch * seq_q, ld_out), MARK, device="cuda")
+    stats = torch.full((batch, heads, seq_q, 2), MARK, device="cuda")
+    scale = torch.tensor(1 / math.sqrt(d)).item()
+    args = (*shape, ld_q, ld_kv, ld_out, scale)
+    hip.cross_attention_forward(out, stats, q, k, v, key_len, *args)
+    hip.cross_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, key_len, *args, beta, beta)
+    torch.cuda.synchronize()
+    assert (out[:, hd:] == MARK).all()
+    assert torch.equal(dq[:, hd:], old_q[:, hd:]) and torch.equal(dkb[:, at + kd:], old_k[:, at + kd:])
+    for b, n in enumerate(lens):
+        rows, keys = slice(b * seq_q, (b + 1) * seq_q), slice(b * seq_k, (b + 1) * seq_k)
+        for j in range(kv):
+            qc, kc = slice(j * group * d, (j + 1) * group * d), slice(j * d, (j + 1) * d)
+            as_rows = lambda x: x[rows, qc].double().reshape(seq_q * group, d)
+            live = lambda x: x[keys, kc][:n].double()
+            ref = reference(as_rows(q), live(k), live(v), as_rows(dout), scale)
+            what = f"item {b}, key head {j}: "
+            within(as_rows(out), *ref[0], what + "out")
+            st = stats[b, j * group:(j + 1) * group].double().transpose(0, 1).reshape(-1, 2)
+            if n:
+                within(st[:, 0] + torch.log2(st[:, 1]), *ref[1], what + "log of the sum")
+            else:
+                assert (st == 0).all()
+            was = beta * as_rows(old_q)
+            within(as_rows(dq), ref[2][0] + was, ref[2][1] + 2 * U * (ref[2][0].abs() + was.abs()), what + "dq")
+            for got, old, (value, bound), name in ((dk, old_k[:, :kd], ref[3], "dk"),
+                                                   (dv, old_v[:, at:at + kd], ref[4], "dv")):
+                was = beta * live(old)
+                within(live(got), value + was, bound + 2 * U * (value.abs() + was.abs()), what + name)
+                dead = beta * old[keys, kc][n:]  # (exact: a half of a float, or all of it)
+                assert torch.equal(got[keys, kc][n:], dead), what + name + " of dead keys"
