@@ -382,7 +382,10 @@ int nrs_embedding_forward(float *out, const float *table, const int32_t *ids, in
  * into the rows of absent tokens; beta 1 leaves them as they are, unread). Ids
  * outside the table add nothing. Added by sorted tokens, without atomics: the
  * same ids give the same order of every sum. work as in
- * nrs_cross_attention_forward.                                               */
+ * nrs_cross_attention_forward: what nrs_embedding_workspace says goes by the
+ * sizes alone, and a captured call, or one that brings a buffer, is held to it.
+ * (Up to 256 positions, of at most 4096 columns, with beta 0 or 1, take one
+ * launch and no scratch.)                                                    */
 int nrs_embedding_workspace(size_t *bytes, int64_t count, int64_t vocab, int64_t dim);
 int nrs_embedding_backward(float *dtable, const float *grad, const int32_t *ids, int64_t count,
                            int64_t vocab, int64_t dim, float scale, float beta, void *work,

@@ -537,8 +537,12 @@ int nrs_embedding_backward(float* dtable, const float* grad, const int32_t* ids,
     NRS_REQUIRE_INIT();
     if (int rc = nrs::check_device("embedding backward")) return rc;
     const auto plan = nrs::plan_backward(count, vocab, dim);
+    const int64_t blocks = (dim + 255) / 256;
+    // (a wide table, or one whose absent rows change, too, has the three launches)
+    const bool few = count <= nrs::kFew && blocks <= 16 && (beta == 0.0f || beta == 1.0f);
     float* scratch = nullptr;
-    if (int rc = nrs::call_scratch(&scratch, plan.bytes(), work, work_bytes, "embedding backward"))
+    if (int rc = nrs::call_scratch(&scratch, plan.bytes(), work, work_bytes, "embedding backward",
+                                   !few))
         return rc;
     nrs::BackwardArgs a{};
     a.dtable = dtable;
@@ -549,12 +553,11 @@ int nrs_embedding_backward(float* dtable, const float* grad, const int32_t* ids,
     a.dim = (int)dim;
     a.bins = plan.bins;
     a.tile = plan.tile;
-    a.blocks = (int)((dim + 255) / 256);
+    a.blocks = (int)blocks;
     a.groups = (int)plan.groups;
     a.scale = scale;
     a.beta = beta;
-    // (a wide table, or one whose absent rows change, too, has the three launches)
-    if (count <= nrs::kFew && a.blocks <= 16 && (beta == 0.0f || beta == 1.0f)) {
+    if (few) {
         const int64_t ranges = std::min<int64_t>(vocab, 4 * (int64_t)nrs::num_cus() / a.blocks);
         a.bins = (int)((vocab + ranges - 1) / ranges);
         const int64_t used = (vocab + a.bins - 1) / a.bins;

@@ -43,8 +43,10 @@ float* noalloc_scratch();
 // else the library's slot 7. A captured call has to bring its own: the
 // library's scratch moves when a later call needs more, which would leave the
 // graph with an address that is no longer allocated. `need` 0 gives a null
-// pointer.
-int call_scratch(float** p, size_t need, void* work, size_t work_bytes, const char* what);
+// pointer, and so does `used` false where the caller brings none: a call that is
+// held to what calls of its sizes need, but writes to no scratch.
+int call_scratch(float** p, size_t need, void* work, size_t work_bytes, const char* what,
+                 bool used = true);
 
 // Refuses a call made while another device than the library's is current: its
 // launches would go there.

@@ -154,7 +154,8 @@ float* workspace(size_t bytes, int slot) {
     return g.ws[slot];
 }
 
-int call_scratch(float** p, size_t need, void* work, size_t work_bytes, const char* what) {
+int call_scratch(float** p, size_t need, void* work, size_t work_bytes, const char* what,
+                 bool used) {
     *p = nullptr;
     NRS_ARG_CHECK(work || work_bytes == 0, "%s: work is null but work_bytes is %zu", what,
                   work_bytes);
@@ -172,6 +173,7 @@ int call_scratch(float** p, size_t need, void* work, size_t work_bytes, const ch
         NRS_ARG_CHECK(status == hipStreamCaptureStatusNone,
                       "%s: a captured call needs its own work buffer of %zu bytes", what, need);
     }
+    if (!used) return NRS_OK;
     *p = workspace(need, 7);
     return *p ? NRS_OK : NRS_ERR_ALLOC;
 }

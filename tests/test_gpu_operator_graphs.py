@@ -204,3 +204,24 @@ def test_keys_past_32_bits(hip, seq_q):
         assert torch.all((got - value).abs() <= bound + 2.0 ** -24 * value.abs() + 2.0 ** -126)
     # (and the rows behind the 32nd bit hold more than rounding can)
     assert value[-5:].abs().max() > 100 * bound[-5:].max()
+
+
+def test_an_embedding_gradient_of_few_positions_takes_no_scratch(hip):
+    """The one launch of up to 256 positions writes to none: without a work buffer
+    the library's own scratch does not grow (by a place for each of 2^28 tokens)."""
+    count, vocab = 200, 1 << 28
+    hip.call("nrs_shutdown")  # gives the scratch of earlier calls back
+    table = torch.zeros(vocab, device="cuda")
+    grad = torch.ones(count, device="cuda")
+    ids = torch.arange(count, device="cuda", dtype=torch.int32) * (vocab // count)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    print(f"embedding, {count} of {vocab}", flush=True)
+    for beta in (0.0, 1.0):
+        hip.embedding_backward(table, grad, ids, count, vocab, 1, 1.0, beta)
+    hip.sync()
+    taken = before - torch.cuda.mem_get_info()[0]
+    assert taken < 1 << 28
+    assert torch.count_nonzero(table) == count and torch.all(table[ids.long()] == 2.0)
+    del table
+    torch.cuda.empty_cache()
