@@ -335,8 +335,14 @@ int nrs_attention_backward(float *dq, float *dk, float *dv, const float *dout, c
  * d_head is 1 to 128; strides are at most 2^20 floats; tensors may be longer
  * than 4 GiB. nrs_cross_attention_supported says whether a shape is taken;
  * one that is not is refused with NRS_ERR_ARG. Values of live keys and their
- * queries must be finite and below 2^127 in magnitude: a row that meets
- * another gets NaN or infinities, other rows are untouched by it.
+ * queries must be finite and below 2^127 in magnitude, and so must scale *
+ * log2(e) * q, u and, as the sums over the keys are divided last, 256 * seq_k
+ * times the largest of v: a row that meets another gets NaN or infinities, other
+ * rows are untouched by it.
+ *   With many rows floats are multiplied as sums of three bf16 pieces, as good
+ * as f32 for magnitudes from 2^-110 on. Below, an operand of a product (q, k, v,
+ * dout, the probabilities or dS) may be off by up to 2^-125: gradients that are
+ * all that small want a larger loss scale.
  *   work: NULL, or work_bytes of the caller's device memory (16-byte aligned)
  * in place of the library's scratch, at least what
  * nrs_cross_attention_workspace says for the call. A call under stream capture
@@ -360,7 +366,7 @@ int nrs_cross_attention_forward(float *out, float *stats, const float *q, const 
  * are with 1. beta 0 never reads the old values. dq (strides of q), or dk and
  * dv together (strides of k), may be NULL: not computed. dout has the strides
  * of out. No output may overlap another or an input. Sums are taken in an
- * order that depends on the sizes alone.                                     */
+ * order that depends on the sizes and lengths alone.                         */
 int nrs_cross_attention_backward(float *dq, float *dk, float *dv, const float *dout,
                                  const float *out, const float *q, const float *k, const float *v,
                                  const float *stats, const int32_t *key_len, int64_t batch,

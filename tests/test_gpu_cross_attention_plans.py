@@ -18,9 +18,10 @@ def mm(a, b):
     return torch.mm(a.contiguous(), b.contiguous())
 
 
-def reference(q, k, v, g, scale):
+def reference(q, k, v, g, scale, lost=0.0):
     """(value, bound) of out, the log2 of the rows' sums, dq, dk and dv: as
-    attention_ref.forward and backward, one item and key head."""
+    attention_ref.forward and backward, one item and key head. Every operand of a
+    product, and every term of a sum, may be off by `lost` besides."""
     n, d, rows = len(k), q.shape[1], len(q)
     if n == 0:
         zero = [torch.zeros_like(x) for x in (q, q, k, v)]
@@ -31,23 +32,26 @@ def reference(q, k, v, g, scale):
     p = torch.exp(s - m)
     total = p.sum(dim=1, keepdim=True)
     p = p / total
+    size = lambda x: x.abs().sum(dim=1, keepdim=True)
     es = (gamma(d) + 4 * U) * (mm(q.abs(), k.abs().t()) * scale).amax(dim=1, keepdim=True)
+    es = es + lost * scale * (size(q) + size(k).max() + d)
     ep = 2 * es + gamma(n) + 8 * U
     out = mm(p, v)
-    out_bound = (ep + gamma(n)) * mm(p, v.abs()) + TINY * v.abs().sum(dim=0)
+    out_bound = (ep + gamma(n)) * mm(p, v.abs()) + (TINY + lost) * v.abs().sum(dim=0) + lost * (n + 1)
     lse = m / math.log(2.0) + torch.log2(total)
     lse_bound = 1.45 * ep + 4 * U * m.abs() / math.log(2.0)
     dp = mm(g, v.t())
     delta = (g * out).sum(dim=1, keepdim=True)
     ds = p * (dp - delta) * scale
     e_delta = (gamma(d) * g.abs() * out.abs() + g.abs() * out_bound).sum(dim=1, keepdim=True)
-    e_ds = scale * p * ((ep + 4 * U) * (dp - delta).abs() + gamma(d) * mm(g.abs(), v.abs().t()) + e_delta)
-    e_ds = e_ds + TINY * (1 + scale * (dp - delta).abs())
-    e_p = ep * p + TINY
+    e_dp = gamma(d) * mm(g.abs(), v.abs().t()) + lost * (size(g) + size(v).t() + d)
+    e_ds = scale * p * ((ep + 4 * U) * (dp - delta).abs() + e_dp + e_delta)
+    e_ds = e_ds + (TINY + lost) * (1 + scale) * (1 + (dp - delta).abs())
+    e_p = ep * p + TINY + lost
     return [(out, out_bound), (lse[:, 0], lse_bound[:, 0]),
-            (mm(ds, k), mm(e_ds + gamma(n) * ds.abs(), k.abs())),
-            (mm(ds.t(), q), mm((e_ds + gamma(rows) * ds.abs()).t(), q.abs())),
-            (mm(p.t(), g), mm((e_p + gamma(rows) * p).t(), g.abs()))]
+            (mm(ds, k), mm(e_ds + gamma(n) * ds.abs(), k.abs()) + lost * (size(ds) + n)),
+            (mm(ds.t(), q), mm((e_ds + gamma(rows) * ds.abs()).t(), q.abs()) + lost * (size(ds.t()) + rows)),
+            (mm(p.t(), g), mm((e_p + gamma(rows) * p).t(), g.abs()) + lost * (size(p.t()) + rows))]
 
 
 def within(got, value, bound, what):
@@ -120,3 +124,35 @@ def test_every_kernel(hip, number):
                 within(live(got), value + was, bound + 2 * U * (value.abs() + was.abs()), what + name)
                 dead = beta * old[keys, kc][n:]  # (exact: a half of a float, or all of it)
                 assert torch.equal(got[keys, kc][n:], dead), what + name + " of dead keys"
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 2, 20, 90, 64), (1, 2, 2, 90, 30, 32), (1, 2, 2, 70, 90, 32),
+                                   (1, 2, 2, 200, 150, 64), (1, 2, 2, 70, 90, 128)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("small", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("power", [-90, -115, -130])
+def test_small_magnitudes(hip, shape, small, power):
+    """An operand of a product may be off by 2^-125, whichever kernel takes the
+    call: with it, the bounds hold where a tensor, and what is made of it, is near
+    the smallest floats or among the subnormal ones."""
+    batch, heads, kv, seq_q, seq_k, d = shape
+    print(f"cross attention {shape}, {small} about 2^{power}", flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(power + 1000)
+    t = {n: torch.randn(rows, heads * d, generator=gen, device="cuda")
+         for n, rows in (("q", seq_q), ("k", seq_k), ("v", seq_k), ("dout", seq_q))}
+    t[small] = (t[small].double() * 2.0 ** power).float()
+    out, stats = torch.empty_like(t["q"]), torch.empty(heads * seq_q * 2, device="cuda")
+    dq, dk, dv = (torch.empty_like(t[n]) for n in ("q", "k", "v"))
+    scale = torch.tensor(1 / math.sqrt(d)).item()
+    args = (*shape, heads * d, heads * d, heads * d, scale)
+    hip.cross_attention_forward(out, stats, t["q"], t["k"], t["v"], None, *args)
+    hip.cross_attention_backward(dq, dk, dv, t["dout"], out, t["q"], t["k"], t["v"], stats, None, *args)
+    for j in range(heads):
+        c = slice(j * d, (j + 1) * d)
+        ref = reference(*(t[n][:, c].double() for n in ("q", "k", "v", "dout")), scale, 2.0 ** -125)
+        for got, (value, bound), name in zip((out, dq, dk, dv), ref[:1] + ref[2:], ("out", "dq", "dk", "dv")):
+            within(got[:, c], value, bound, f"head {j}: {name}")
+        if power == -90:  # (far above the smallest floats that adds next to nothing)
+            plain = reference(*(t[n][:, c].double() for n in ("q", "k", "v", "dout")), scale)
+            for (_, bound), (_, without) in zip(ref, plain):
+                assert (bound - without).max() < 1e-3 * without.max()
