@@ -397,8 +397,8 @@ int nrs_embedding_backward(float *dtable, const float *grad, const int32_t *ids,
                            int64_t vocab, int64_t dim, float scale, float beta, void *work,
                            size_t work_bytes);
 /* Dropout (the reference's src/cuda/nn/dropout layer) whose mask is never
- * stored: out = (kept ? x / (1 - p) : 0) (+ residual), rounded after the
- * quotient and after the sum. Element i is kept when word i % 4 of the
+ * stored: out = (kept ? x * f : 0) (+ residual) with f = 1 / (1 - p) rounded to
+ * f32, rounded after the product and after the sum. Element i is kept when word i % 4 of the
  * Philox4x32-10 block of counter (i / 4 in its low 64 bits, call + *step in
  * its high ones) under the key `seed` is at least round(p * 2^32): the mask
  * depends on i, p, seed and call + *step alone. A program counts `call` up
@@ -408,8 +408,8 @@ int nrs_embedding_backward(float *dtable, const float *grad, const int32_t *ids,
  * may be infinite or NaN. out may be x or residual. residual may be NULL.    */
 int nrs_dropout_forward(float *out, const float *x, const float *residual, int64_t n, float p,
                         uint64_t seed, uint64_t call, const uint64_t *step);
-/* Its backward with the same p, seed, call and step: gin = (kept ? grad /
- * (1 - p) : 0) + beta * gin. (The residual's gradient is grad itself.)       */
+/* Its backward with the same p, seed, call and step: gin = (kept ? grad * f : 0)
+ * + beta * gin. (The residual's gradient is grad itself.)                    */
 int nrs_dropout_backward(float *gin, const float *grad, int64_t n, float p, uint64_t seed,
                          uint64_t call, const uint64_t *step, float beta);
 

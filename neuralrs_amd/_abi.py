@@ -325,14 +325,14 @@ def embedding_backward(dtable, grad, ids, count, vocab, dim, scale=1.0, beta=0.0
 
 
 def dropout_forward(out, x, residual, n, p, seed, number, step=None):
-    """out = x / (1 - p) where kept, else 0 (+ residual unless None); `number`
-    is the call's, step an optional device uint64 added to it."""
+    """out = x * f32(1 / (1 - p)) where kept, else 0 (+ residual unless None);
+    `number` is the call's, step an optional device uint64 added to it."""
     _launch(load().nrs_dropout_forward, _ptr(out), _ptr(x), _ptr(residual), n, p, seed, number,
             _ptr(step))
 
 
 def dropout_backward(gin, grad, n, p, seed, number, step=None, beta=0.0):
-    """gin = grad / (1 - p) where kept, else 0 (+ beta * gin)."""
+    """gin = grad * f32(1 / (1 - p)) where kept, else 0 (+ beta * gin)."""
     _launch(load().nrs_dropout_backward, _ptr(gin), _ptr(grad), n, p, seed, number,
             _ptr(step), beta)
 

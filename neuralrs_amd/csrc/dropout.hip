@@ -47,8 +47,9 @@ __device__ __forceinline__ u32x4 philox(uint64_t block, uint64_t call, uint64_t 
     return u32x4{c0, c1, c2, c3};
 }
 
-// x / (1 - p) is rounded by itself before anything is added, so that dropout
-// with a residual has the bits of dropout followed by nrs_vadd. A dropped
+// x times the rounded 1 / (1 - p) (a product, where a quotient would take ten
+// instructions) is rounded by itself before anything is added, so that dropout with
+// a residual has the bits of dropout followed by nrs_vadd. A dropped
 // element is a zero whatever x holds there.
 __device__ __forceinline__ float drop(float x, uint32_t word, const DropoutArgs& a) {
 #pragma clang fp contract(off)

@@ -288,7 +288,7 @@ struct Embedding {
     }
 };
 
-// x / (1 - p) where kept, else 0, plus residual unless null. The mask is a
+// x * f32(1 / (1 - p)) where kept, else 0, plus residual unless null. The mask is a
 // function of p, seed and call (nrs_dropout_forward) and is made again by the
 // backward. x unchanged (or the sum alone) with p 0.
 NodeRef dropout(const NodeRef& x, float p, uint64_t seed, uint64_t call,
