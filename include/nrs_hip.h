@@ -404,8 +404,11 @@ int nrs_embedding_backward(float *dtable, const float *grad, const int32_t *ids,
  * depends on i, p, seed and call + *step alone. A program counts `call` up
  * for every dropout that it applies. step (device, or NULL: 0) is read when
  * the launch runs: a captured graph's masks change between replays when its
- * program changes *step. p is in [0, 1]; p = 1 drops everything. A dropped x
- * may be infinite or NaN. out may be x or residual. residual may be NULL.    */
+ * program changes *step. Since step and call are added, it has to move on by as
+ * many call numbers as the graph uses under one seed (or each of its dropouts has
+ * a seed of its own): a graph of calls 0, 1 and 2 whose step moves by 1 has call
+ * 1's mask again as the next replay's call 0. p is in [0, 1]; p = 1 drops
+ * everything. A dropped x may be infinite or NaN. out may be x or residual. residual may be NULL.    */
 int nrs_dropout_forward(float *out, const float *x, const float *residual, int64_t n, float p,
                         uint64_t seed, uint64_t call, const uint64_t *step);
 /* Its backward with the same p, seed, call and step: gin = (kept ? grad * f : 0)

@@ -326,7 +326,8 @@ def embedding_backward(dtable, grad, ids, count, vocab, dim, scale=1.0, beta=0.0
 
 def dropout_forward(out, x, residual, n, p, seed, number, step=None):
     """out = x * f32(1 / (1 - p)) where kept, else 0 (+ residual unless None);
-    `number` is the call's, step an optional device uint64 added to it."""
+    `number` is the call's, step an optional device uint64 added to it: it has to
+    move on by as many numbers as are used under one seed between its changes."""
     _launch(load().nrs_dropout_forward, _ptr(out), _ptr(x), _ptr(residual), n, p, seed, number,
             _ptr(step))
 

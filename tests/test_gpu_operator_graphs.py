@@ -225,3 +225,38 @@ def test_an_embedding_gradient_of_few_positions_takes_no_scratch(hip):
     assert torch.count_nonzero(table) == count and torch.all(table[ids.long()] == 2.0)
     del table
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("advance,again", [(3, False), (1, True)])
+def test_masks_of_replays_with_several_dropouts(hip, side, advance, again):
+    """Three dropouts of calls 0, 1 and 2 under one seed: no mask of a replay comes
+    again in another when the program adds at least 3 to *step, and the next
+    dropout's mask is this one's when it adds 1."""
+    n = 4096
+    print(f"dropouts, step + {advance}", flush=True)
+    with torch.cuda.stream(side):
+        x, step = torch.ones(n, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+        outs = [torch.empty(n, device="cuda") for _ in range(3)]
+
+        def run():
+            for call, out in enumerate(outs):
+                hip.dropout_forward(out, x, None, n, 0.5, 9, call, step)
+
+        run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run()
+        masks = []
+        for i in range(4):
+            step.fill_(advance * i)
+            graph.replay()
+            masks += [out.clone() for out in outs]
+            torch.cuda.synchronize()
+            run()
+            for out, mask in zip(outs, masks[-3:]):
+                assert torch.equal(out, mask)
+    same = [(i, j) for i in range(len(masks)) for j in range(i) if torch.equal(masks[i], masks[j])]
+    assert bool(same) == again
+    if again:  # call 0 of the next replay is call 1 of this one
+        assert (3, 1) in same
