@@ -107,9 +107,12 @@ struct LinePart {
             at += i < w ? scan[i] : 0;
             total += scan[i];
         }
-        p = (int)((int64_t)total * blockIdx.x / a.groups);
-        end = (int)((int64_t)total * (blockIdx.x + 1) / a.groups);
-        if (p >= end) return false;
+        // a tile to a workgroup at least: those that share a unit, which the join
+        // takes from the first to the last, have none without a part between them
+        const int parts = min(a.groups, total);
+        if ((int)blockIdx.x >= parts) return false;
+        p = (int)((int64_t)total * blockIdx.x / parts);
+        end = (int)((int64_t)total * (blockIdx.x + 1) / parts);
         for (int i = 0; i < each && t * each + i < a.B; ++i) {
             const int n = (live_keys(a, t * each + i) + keys - 1) / keys * per_item;
             if (at <= p && p < at + n) {

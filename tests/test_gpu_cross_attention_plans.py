@@ -33,8 +33,8 @@ def reference(q, k, v, g, scale, lost=0.0):
     total = p.sum(dim=1, keepdim=True)
     p = p / total
     size = lambda x: x.abs().sum(dim=1, keepdim=True)
-    es = (gamma(d) + 4 * U) * (mm(q.abs(), k.abs().t()) * scale).amax(dim=1, keepdim=True)
-    es = es + lost * scale * (size(q) + size(k).max() + d)
+    es = (gamma(d) + 4 * U) * (mm(q.abs(), k.abs().t()) * abs(scale)).amax(dim=1, keepdim=True)
+    es = es + lost * abs(scale) * (size(q) + size(k).max() + d)
     ep = 2 * es + gamma(n) + 8 * U
     out = mm(p, v)
     out_bound = (ep + gamma(n)) * mm(p, v.abs()) + (TINY + lost) * v.abs().sum(dim=0) + lost * (n + 1)
@@ -45,8 +45,8 @@ def reference(q, k, v, g, scale, lost=0.0):
     ds = p * (dp - delta) * scale
     e_delta = (gamma(d) * g.abs() * out.abs() + g.abs() * out_bound).sum(dim=1, keepdim=True)
     e_dp = gamma(d) * mm(g.abs(), v.abs().t()) + lost * (size(g) + size(v).t() + d)
-    e_ds = scale * p * ((ep + 4 * U) * (dp - delta).abs() + e_dp + e_delta)
-    e_ds = e_ds + (TINY + lost) * (1 + scale) * (1 + (dp - delta).abs())
+    e_ds = abs(scale) * p * ((ep + 4 * U) * (dp - delta).abs() + e_dp + e_delta)
+    e_ds = e_ds + (TINY + lost) * (1 + abs(scale)) * (1 + (dp - delta).abs())
     e_p = ep * p + TINY + lost
     return [(out, out_bound), (lse[:, 0], lse_bound[:, 0]),
             (mm(ds, k), mm(e_ds + gamma(n) * ds.abs(), k.abs()) + lost * (size(ds) + n)),
@@ -60,24 +60,24 @@ def within(got, value, bound, what):
     assert (error <= tol).all(), f"{what}: worst {(error / tol).nan_to_num(math.inf).max().item():.3g} of its bound"
 
 
-@pytest.mark.parametrize("number", range(len(cross_plan.SHAPES)),
-                         ids=lambda i: "x".join(map(str, cross_plan.SHAPES[i])))
-def test_every_kernel(hip, number):
-    """Every second call has padded rows and K and V in one tensor; where there are
-    several items their lengths differ and one is empty. The gradients are written,
-    added to the old ones, or added to half of them."""
-    batch, heads, kv, seq_q, seq_k, d = shape = cross_plan.SHAPES[number]
+def check(hip, shape, number, lens=None, scale=None):
+    """One call and its backward. Every second has padded rows and K and V in one
+    tensor; where there are several items their lengths differ and one is empty,
+    unless given. The gradients are written, added to the old ones, or added to half
+    of them. The scratch holds NaN: nothing is read that the call did not write."""
+    batch, heads, kv, seq_q, seq_k, d = shape
     print(f"cross attention {shape}", flush=True)
     packed, beta = number % 2 == 1, (0.0, 1.0, 0.5)[number % 3]
     gen = torch.Generator(device="cuda").manual_seed(number)
     new = lambda *s: torch.randn(*s, generator=gen, device="cuda")
     hd, kd, group = heads * d, kv * d, heads // kv
     ld_q, ld_out, ld_kv = hd + 3 * packed, hd + 5 * packed, kd * (1 + packed) + packed
-    lens = [seq_k] * batch
-    if batch > 1:
+    given = lens is not None
+    if not given:
         lens = [max(1, seq_k - i * seq_k // (2 * batch)) for i in range(batch)]
-        lens[batch // 2] = 0
-    key_len = torch.tensor(lens, dtype=torch.int32, device="cuda") if batch > 1 else None
+        if batch > 1:
+            lens[batch // 2] = 0
+    key_len = torch.tensor(lens, dtype=torch.int32, device="cuda") if given or batch > 1 else None
     q, dout, old_q = new(batch * seq_q, ld_q), new(batch * seq_q, ld_out), new(batch * seq_q, ld_q)
     kb, old_k = new(batch * seq_k, ld_kv), new(batch * seq_k, ld_kv)
     vb, old_v = (kb, old_k) if packed else (new(batch * seq_k, ld_kv), new(batch * seq_k, ld_kv))
@@ -95,10 +95,12 @@ def test_every_kernel(hip, number):
         dv.fill_(math.nan)
     out = torch.full((batch * seq_q, ld_out), MARK, device="cuda")
     stats = torch.full((batch, heads, seq_q, 2), MARK, device="cuda")
-    scale = torch.tensor(1 / math.sqrt(d)).item()
+    scale = torch.tensor(1 / math.sqrt(d) if scale is None else scale).item()
     args = (*shape, ld_q, ld_kv, ld_out, scale)
-    hip.cross_attention_forward(out, stats, q, k, v, key_len, *args)
-    hip.cross_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, key_len, *args, beta, beta)
+    work = [torch.full((hip.cross_attention_workspace(*shape, backward=b) // 4 + 1,), math.nan, device="cuda")
+            for b in (False, True)]
+    hip.cross_attention_forward(out, stats, q, k, v, key_len, *args, work[0])
+    hip.cross_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, key_len, *args, beta, beta, work[1])
     torch.cuda.synchronize()
     assert (out[:, hd:] == MARK).all()
     assert torch.equal(dq[:, hd:], old_q[:, hd:]) and torch.equal(dkb[:, at + kd:], old_k[:, at + kd:])
@@ -124,6 +126,39 @@ def test_every_kernel(hip, number):
                 within(live(got), value + was, bound + 2 * U * (value.abs() + was.abs()), what + name)
                 dead = beta * old[keys, kc][n:]  # (exact: a half of a float, or all of it)
                 assert torch.equal(got[keys, kc][n:], dead), what + name + " of dead keys"
+
+
+@pytest.mark.parametrize("number", range(len(cross_plan.SHAPES)),
+                         ids=lambda i: "x".join(map(str, cross_plan.SHAPES[i])))
+def test_every_kernel(hip, number):
+    check(hip, cross_plan.SHAPES[number], number)
+
+
+# More items than a workgroup has threads, which look for its part of the line of
+# key tiles, up to the 1024 of a shared launch and past them; empty items about the
+# parts' ends, or nothing but empty ones.
+@pytest.mark.parametrize("shape,live", [
+    ((300, 2, 1, 1, 200, 32), lambda i: 200 - i % 150), ((1000, 1, 1, 1, 250, 16), lambda i: 250 if i % 3 else 0),
+    ((1024, 1, 1, 3, 130, 24), lambda i: 130 if i in (0, 511, 1023) else 0),
+    ((1025, 1, 1, 1, 60, 40), lambda i: i % 61), ((700, 1, 1, 2, 100, 64), lambda i: 100 if i == 699 else 0),
+    ((520, 1, 1, 60, 3000, 32), lambda i: 3000 - i % 7 * 429),
+    ((513, 1, 1, 250, 2000, 24), lambda i: 2000 if i % 5 else 0), ((600, 1, 1, 33, 300, 16), lambda i: 300 * (i % 2)),
+    ((4, 8, 8, 1, 3000, 64), lambda i: 0), ((2, 8, 8, 700, 900, 64), lambda i: 0),
+    ((3, 8, 2, 500, 700, 128), lambda i: 700 if i == 1 else 0)],
+    ids=lambda x: "x".join(map(str, x)) if isinstance(x, tuple) else "")
+def test_many_items_and_empty_ones(hip, shape, live):
+    check(hip, shape, 2, lens=[live(i) for i in range(shape[0])])
+
+
+@pytest.mark.parametrize("shape", [
+    (32, 8, 8, 1, 1500, 64), (2, 32, 8, 1, 16384, 128), (9, 4, 2, 8, 3000, 32), (8, 4, 4, 60, 4000, 64),
+    (4, 16, 16, 512, 1500, 64), (3, 2, 1, 300, 9000, 128), (5, 6, 2, 400, 5000, 24), (2, 8, 8, 300, 7000, 96),
+    (3, 2, 2, 1000, 40000, 16)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("most", [40, 200])
+def test_short_lengths_in_a_long_cache(hip, shape, most):
+    """Fewer key tiles are live than there are workgroups to share those of a full
+    call."""
+    check(hip, shape, 0, lens=[1 + (i + 1) * 7919 % most for i in range(shape[0])])
 
 
 @pytest.mark.parametrize("shape", [(1, 2, 2, 20, 90, 64), (1, 2, 2, 90, 30, 32), (1, 2, 2, 70, 90, 32),
