@@ -161,6 +161,15 @@ def test_short_lengths_in_a_long_cache(hip, shape, most):
     check(hip, shape, 0, lens=[1 + (i + 1) * 7919 % most for i in range(shape[0])])
 
 
+@pytest.mark.parametrize("shape", [(2, 4, 2, 3, 90, 32), (2, 4, 2, 90, 150, 64), (1, 2, 2, 150, 9, 40),
+                                   (1, 3, 1, 70, 200, 128)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("scale", [0.0, -0.25, 1.0])
+def test_any_scale(hip, shape, scale):
+    """Zero gives every live key the same weight, a negative one the most to the
+    least product."""
+    check(hip, shape, 0, scale=scale)
+
+
 @pytest.mark.parametrize("shape", [(1, 2, 2, 20, 90, 64), (1, 2, 2, 90, 30, 32), (1, 2, 2, 70, 90, 32),
                                    (1, 2, 2, 200, 150, 64), (1, 2, 2, 70, 90, 128)],
                          ids=lambda s: "x".join(map(str, s)))

@@ -149,7 +149,10 @@ def test_own_scratch(hip):
 # Long runs of one token, over many tiles and several blocks of columns, beside
 # the cases above.
 LONG = [(30000, 1, 515, "one"), (20011, 3, 600, "uniform"), (300000, 5, 300, "uniform"),
-        (65536, 259, 512, "zipf"), (12345, 7, 257, "zipf"), (1100, 2, 1024, "uniform")]
+        (65536, 259, 512, "zipf"), (12345, 7, 257, "zipf"), (1100, 2, 1024, "uniform"),
+        # more tokens than 1024 for each of 256 workgroups, and very wide rows
+        (5000, 300007, 8, "zipf"), (70000, 2000003, 3, "uniform"), (300, 4, 20000, "uniform"),
+        (2, 3, 100001, "one")]
 
 
 @pytest.mark.parametrize("count,vocab,dim,how", CASES + LONG)
