@@ -60,7 +60,7 @@ def within(got, value, bound, what):
     assert (error <= tol).all(), f"{what}: worst {(error / tol).nan_to_num(math.inf).max().item():.3g} of its bound"
 
 
-def check(hip, shape, number, lens=None, scale=None):
+def check(hip, shape, number, lens=None, scale=None, ld=None):
     """One call and its backward. Every second has padded rows and K and V in one
     tensor; where there are several items their lengths differ and one is empty,
     unless given. The gradients are written, added to the old ones, or added to half
@@ -72,6 +72,8 @@ def check(hip, shape, number, lens=None, scale=None):
     new = lambda *s: torch.randn(*s, generator=gen, device="cuda")
     hd, kd, group = heads * d, kv * d, heads // kv
     ld_q, ld_out, ld_kv = hd + 3 * packed, hd + 5 * packed, kd * (1 + packed) + packed
+    if ld:
+        ld_q = ld_out = ld_kv = ld
     given = lens is not None
     if not given:
         lens = [max(1, seq_k - i * seq_k // (2 * batch)) for i in range(batch)]
@@ -168,6 +170,61 @@ def test_any_scale(hip, shape, scale):
     """Zero gives every live key the same weight, a negative one the most to the
     least product."""
     check(hip, shape, 0, scale=scale)
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 1, 200, 300, 64), (2, 4, 4, 1, 500, 128), (1, 2, 2, 150, 10, 24),
+                                   (1, 3, 3, 20, 200, 96)], ids=lambda s: "x".join(map(str, s)))
+def test_the_longest_strides(hip, shape):
+    check(hip, shape, 0, ld=1 << 20)
+
+
+@pytest.mark.parametrize("shape", [(1, 32768, 1, 2, 40, 32), (2, 8192, 2, 1, 20, 128), (1, 16384, 1, 1, 700, 64),
+                                   (1, 1500, 1500, 1, 3, 8), (1, 600, 600, 50, 60, 16)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_many_heads(hip, shape):
+    """Up to 32768, and as many to a key head: rows of up to 2^20 floats."""
+    check(hip, shape, 0)
+
+
+@pytest.mark.parametrize("seq_k,d", [(10, 64), (60, 64), (60, 24), (40, 100)])
+def test_rows_past_32_bits(hip, seq_k, d):
+    """Queries, outputs and their gradients whose offsets pass 2^31 floats. Sums of n
+    rows get six times the deviation of n roundings without a common sign, 6 sqrt(n)
+    half steps, as n half steps would be an eighth of them."""
+    n, ld = (1 << 21) + 37, 1056
+    print(f"{n} rows of stride {ld}, {seq_k} keys of {d}", flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(seq_k + d)
+    new = lambda rows: torch.randn(rows, d, generator=gen, device="cuda")
+    wide = [torch.empty(n, ld, device="cuda") for _ in range(4)]
+    q, dout, out, dq = (x[:, :d] for x in wide)
+    q.copy_(new(n))
+    dout.copy_(new(n))
+    dout[-5:] *= 1e5  # the last rows' share of the keys' gradients shows
+    k, v = new(seq_k), new(seq_k)
+    dk, dv, stats = torch.empty_like(k), torch.empty_like(v), torch.empty(2 * n, device="cuda")
+    scale = torch.tensor(1 / math.sqrt(d)).item()
+    args = (1, 1, 1, n, seq_k, d, ld, d, ld, scale)
+    hip.cross_attention_forward(out, stats, q, k, v, None, *args)
+    hip.cross_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, None, *args)
+    torch.cuda.synchronize()
+    total, size, parts = [0.0, 0.0], [0.0, 0.0], 16
+    for i in range(parts):
+        rows = slice(n * i // parts, n * (i + 1) // parts)
+        ref = reference(q[rows].double(), k.double(), v.double(), dout[rows].double(), scale)
+        within(out[rows], *ref[0], "out")
+        within(dq[rows], *ref[2], "dq")
+        s = torch.softmax(mm(q[rows].double(), k.double().t()) * scale, dim=1)
+        ds = s * (mm(dout[rows].double(), v.double().t()) - (dout[rows] * ref[0][0]).sum(1, keepdim=True)) * scale
+        for at, (x, y) in enumerate(((ds, q), (s, dout))):
+            total[at] = total[at] + mm(x.t(), y[rows].double())
+            size[at] = size[at] + mm(x.abs().t(), y[rows].double().abs())
+    for got, value, most in zip((dk, dv), total, size):
+        # (each row's own error, gamma(...) in reference's bound, has no common sign either)
+        assert ((got.double() - value).abs() <= (6 * math.sqrt(n) + 100) * U * most).all()
+    last = mm(s[-5:].t(), y[-5:].double()).abs().max()
+    assert last > 100 * ((6 * math.sqrt(n) + 100) * U * size[1]).min()
+    del wide, q, dout, out, dq
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("shape", [(1, 2, 2, 20, 90, 64), (1, 2, 2, 90, 30, 32), (1, 2, 2, 70, 90, 32),

@@ -152,7 +152,10 @@ LONG = [(30000, 1, 515, "one"), (20011, 3, 600, "uniform"), (300000, 5, 300, "un
         (65536, 259, 512, "zipf"), (12345, 7, 257, "zipf"), (1100, 2, 1024, "uniform"),
         # more tokens than 1024 for each of 256 workgroups, and very wide rows
         (5000, 300007, 8, "zipf"), (70000, 2000003, 3, "uniform"), (300, 4, 20000, "uniform"),
-        (2, 3, 100001, "one")]
+        (2, 3, 100001, "one"),
+        # a workgroup's tokens just fit, and do not fit, a wave's registers and the LDS
+        (16385, 16384, 20, "zipf"), (16384, 16640, 20, "zipf"), (3001, 262144, 5, "uniform"),
+        (3001, 262145, 5, "zipf"), (256, 16385, 9, "zipf"), (257, 2, 1030, "uniform")]
 
 
 @pytest.mark.parametrize("count,vocab,dim,how", CASES + LONG)
@@ -160,7 +163,8 @@ LONG = [(30000, 1, 515, "one"), (20011, 3, 600, "uniform"), (300000, 5, 300, "un
 def test_integer_gradients_are_exact(hip, count, vocab, dim, how, beta):
     """Integers of up to 8, at most 300000 of them to a sum, whose partial sums
     all lie below 2^24: no order rounds, and a row that is lost or taken twice
-    shows. The scale is a power of two and the old values are even."""
+    shows. The scale is a power of two and the old values are even. The scratch holds
+    NaN: nothing is read that the call did not write."""
     rng = np.random.default_rng(count + dim)
     ids = make_ids(rng, count, vocab, how)
     grad = rng.integers(-8, 9, (count, dim)).astype(np.float32)
@@ -168,8 +172,9 @@ def test_integer_gradients_are_exact(hip, count, vocab, dim, how, beta):
     print(f"embedding, integers, {count} of {vocab} x {dim} {how} beta {beta}", flush=True)
     value, _, _ = reference(ids, grad, vocab, 2.0)
     dtable = hip.DeviceBuffer.from_host(old if beta else np.full_like(old, np.nan))
+    work = hip.DeviceBuffer.from_host(np.full(hip.embedding_workspace(count, vocab, dim) // 4, np.nan))
     hip.embedding_backward(dtable, hip.DeviceBuffer.from_host(grad),
-                           hip.DeviceBuffer.from_host(ids, np.int32), count, vocab, dim, 2.0, beta)
+                           hip.DeviceBuffer.from_host(ids, np.int32), count, vocab, dim, 2.0, beta, work)
     assert np.array_equal(dtable.to_host((vocab, dim)), (value + beta * old).astype(np.float32))
 
 
