@@ -152,6 +152,50 @@ def test_many_items_and_empty_ones(hip, shape, live):
     check(hip, shape, 2, lens=[live(i) for i in range(shape[0])])
 
 
+@pytest.mark.parametrize("shape", [(3, 4, 2, 9, 700, 64), (3, 4, 2, 90, 300, 40), (3, 4, 2, 300, 400, 128),
+                                   (3, 4, 2, 100, 9, 24), (2, 2, 2, 130, 40, 16), (2, 4, 2, 1, 90, 100)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("where", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_what_is_not_finite_stays_where_it_is(hip, shape, where, value):
+    """A query row's NaN or infinity changes its own row and what its key head
+    gathers, a key's all of its item's key head; nothing else changes a bit."""
+    batch, heads, kv, seq_q, seq_k, d = shape
+    print(f"cross attention {shape}, {value} in {where}", flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    hd, kd, group = heads * d, kv * d, heads // kv
+    t = {n: torch.randn(*size, generator=gen, device="cuda")
+         for n, size in (("q", (batch, seq_q, hd)), ("k", (batch, seq_k, kd)), ("v", (batch, seq_k, kd)),
+                         ("dout", (batch, seq_q, hd)))}
+    lens = torch.tensor([seq_k, seq_k - seq_k // 3, seq_k][:batch], dtype=torch.int32, device="cuda")
+    args = (*shape, hd, kd, hd, 0.25)
+
+    def run():
+        out, stats = torch.empty_like(t["q"]), torch.empty(batch * heads * seq_q * 2, device="cuda")
+        dq, dk, dv = (torch.empty_like(t[n]) for n in ("q", "k", "v"))
+        hip.cross_attention_forward(out, stats, t["q"], t["k"], t["v"], lens, *args)
+        hip.cross_attention_backward(dq, dk, dv, t["dout"], out, t["q"], t["k"], t["v"], stats, lens, *args)
+        return [x.reshape(batch, -1, n, d) for x, n in ((out, heads), (dq, heads), (dk, kv), (dv, kv))]
+
+    want = run()
+    head = heads - 1 if where in ("q", "dout") else kv - 1
+    row = (seq_q if where in ("q", "dout") else lens[1].item()) // 2
+    t[where][1, row, head * d + d // 2] = value
+    got = run()
+    key_head = head // group if where in ("q", "dout") else head
+    for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
+        same = a == b
+        if name in ("dk", "dv"):
+            same[1, :, key_head] = True
+        elif where in ("q", "dout"):
+            same[1, row, head] = True
+        else:
+            same[1, :, key_head * group:(key_head + 1) * group] = True
+        assert same.all(), (name, torch.argwhere(~same)[:3].tolist())
+    if where != "dout":
+        assert not torch.isfinite(got[0][1, row if where == "q" else 0, head if where == "q" else key_head * group]).all()
+
+
 @pytest.mark.parametrize("shape", [
     (32, 8, 8, 1, 1500, 64), (2, 32, 8, 1, 16384, 128), (9, 4, 2, 8, 3000, 32), (8, 4, 4, 60, 4000, 64),
     (4, 16, 16, 512, 1500, 64), (3, 2, 1, 300, 9000, 128), (5, 6, 2, 400, 5000, 24), (2, 8, 8, 300, 7000, 96),
