@@ -347,7 +347,7 @@ int nrs_attention_backward(float *dq, float *dk, float *dv, const float *dout, c
  * in place of the library's scratch, at least what
  * nrs_cross_attention_workspace says for the call. A call under stream capture
  * that needs scratch has to pass it, its own for every graph that may run at
- * the same time as another.                                                  */
+ * the same time as another. No output may overlap another or an input.       */
 int nrs_cross_attention_supported(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
                                   int64_t seq_k, int64_t d_head, int64_t ld_q, int64_t ld_kv,
                                   int64_t ld_out);
@@ -391,7 +391,9 @@ int nrs_embedding_forward(float *out, const float *table, const int32_t *ids, in
  * nrs_cross_attention_forward: what nrs_embedding_workspace says goes by the
  * sizes alone, and a captured call, or one that brings a buffer, is held to it.
  * (Up to 256 positions, of at most 4096 columns, with beta 0 or 1, take one
- * launch and no scratch.)                                                    */
+ * launch and no scratch.) Every 1024 tokens of the table, or 1/256 of them where
+ * there are fewer than 262144, have a workgroup that looks through all ids
+ * twice: the time grows with count times that number.                       */
 int nrs_embedding_workspace(size_t *bytes, int64_t count, int64_t vocab, int64_t dim);
 int nrs_embedding_backward(float *dtable, const float *grad, const int32_t *ids, int64_t count,
                            int64_t vocab, int64_t dim, float scale, float beta, void *work,

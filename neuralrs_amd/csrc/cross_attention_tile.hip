@@ -37,13 +37,15 @@
 // 32 cycles each, and the exponentials, splits and transposing reads between
 // them about 5 an instruction, of which two waves to a SIMD hide a part.
 //   rows x keys, heads of d          forward          backward
-//   32 x 128 x 200, 8 of 32           12.8 us            27 us
-//   4 x 1000 x 1500, 16 of 64          134 (183 TFLOP/s) 543 (113; 158 with the
+//   32 x 128 x 200, 8 of 32           12.7 us            27 us
+//   4 x 1000 x 1500, 16 of 64          124 (198 TFLOP/s) 430 (143; 200 with the
 //                                                        two products it repeats)
-//   2 x 777 x 4096, 16 of 128, 4 key   259 (158)         990 (103; 145)
-// In the last one's backward the matrix instructions run 38% of the time, the rest of
-// the vector work 33, and compute units are idle for some of the rest, as walks end
-// at different times.
+//   2 x 777 x 4096, 16 of 128, 4 key   233 (176)         869 (118; 165)
+// (medians late in two hundred passes on the same inputs: after a pause the first dozen
+// take 15 to 40% longer, as the clocks settle). In the last two backwards, of the time that a compute unit has work, matrix
+// instructions run 53% and 49%, vector instructions issue 46% and 35%, and LDS is busy
+// 45% and 42%; in the last, compute units have none for a fifth of the launch, as walks
+// end at different times.
 #include <algorithm>
 
 #include "cross_attention.hpp"

@@ -251,7 +251,7 @@ std::vector<float> DeviceBuffer::to_host() const {
 
 void DeviceBuffer::zero() { pending_zero_ = true; }
 
-// -------------------------------------------------------------------- Node
+// -------------------------------------------------------------- DeviceInts
 DeviceInts::DeviceInts(const std::vector<int32_t>& v) : len_(v.size()) {
     void* p = nullptr;
     check_raw(nrs_malloc(&p, v.size() * sizeof(int32_t)), "device ints: allocation failed");
@@ -267,6 +267,7 @@ DeviceInts::~DeviceInts() { nrs_free(ptr_); }
 
 IntsRef device_ints(const std::vector<int32_t>& v) { return std::make_shared<DeviceInts>(v); }
 
+// -------------------------------------------------------------------- Node
 NodeRef Node::create(std::vector<float> data, std::vector<size_t> shape) {
     NodeRef n = std::make_shared<Node>();
     n->grad.assign(data.size(), 0.0f);

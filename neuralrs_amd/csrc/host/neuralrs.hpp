@@ -271,7 +271,9 @@ NodeRef layernorm(const NodeRef& input, const NodeRef& gamma, const NodeRef& bet
 // softmax(q . k^T / sqrt(d)) . v for every head over item b's first key_len[b]
 // keys (null: all): q [batch, seq_q, heads * d], k and v [batch, seq_k,
 // kv_heads * d], heads / kv_heads query heads to a key head, d at most 128. One
-// fused node.
+// fused node. It always keeps the softmax statistics (two floats a row and head) that
+// its backward reads. A loop that decodes token after token projects its memory
+// once and calls this with those nodes.
 NodeRef cross_attention(const NodeRef& q, const NodeRef& k, const NodeRef& v, size_t heads,
                         size_t kv_heads, const IntsRef& key_len = nullptr);
 
@@ -342,7 +344,8 @@ struct MultiHeadAttention {
     // A decoder's attention to an encoder's states of another length, which
     // the reference has no counterpart for: queries from x [batch, seq_q,
     // d_model], keys and values from memory [batch, seq_k, d_model], of which
-    // item b's first key_len[b] are live (null: all). Heads of at most 128.
+    // item b's first key_len[b] are live (null: all). Heads of at most 128. Projects
+    // the memory anew, to keys and values of their own, at every call.
     NodeRef forward_cross(const NodeRef& x, const NodeRef& memory,
                           const IntsRef& key_len = nullptr) const;
 };
