@@ -271,6 +271,61 @@ def test_rows_past_32_bits(hip, seq_k, d):
     torch.cuda.empty_cache()
 
 
+def test_the_most_rows(hip):
+    """2^26 rows of one key: each takes its value, and the key gathers them all."""
+    n = 1 << 26
+    print(f"{n} rows", flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(n, 1, generator=gen, device="cuda")
+    dout = torch.empty(n, 1, device="cuda").random_(-3, 4, generator=gen)
+    k, v = torch.ones(1, 1, device="cuda"), torch.full((1, 1), 2.0, device="cuda")
+    out, dq, stats = torch.empty_like(q), torch.empty_like(q), torch.empty(2 * n, device="cuda")
+    dk, dv = torch.empty_like(k), torch.empty_like(v)
+    args = (1, 1, 1, n, 1, 1, 1, 1, 1, 1.0)
+    hip.cross_attention_forward(out, stats, q, k, v, None, *args)
+    hip.cross_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, None, *args)
+    assert torch.all(out == 2.0) and torch.all(dq == 0.0) and dk.item() == 0.0
+    # (whole numbers of at most 3 x 2^20 in a share's sum, and few shares)
+    assert dv.item() == dout.double().sum().item()
+
+
+@pytest.mark.parametrize("d", [1, 4])
+def test_the_most_keys(hip, d):
+    """2^26 keys of one row. A sum of n terms without a common sign of its roundings
+    is off by 6 sqrt(n) half steps of the sum of magnitudes at most."""
+    n = 1 << 26
+    print(f"{n} keys of {d}", flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    q, dout = (torch.randn(1, d, generator=gen, device="cuda") for _ in range(2))
+    k, v = (torch.randn(n, d, generator=gen, device="cuda") for _ in range(2))
+    v[-3:] = 1e6  # the last keys' part shows
+    out, dq, stats = torch.empty_like(q), torch.empty_like(q), torch.empty(2, device="cuda")
+    dk, dv = torch.empty_like(k), torch.empty_like(v)
+    args = (1, 1, 1, 1, n, d, d, d, d, 1.0)
+    hip.cross_attention_forward(out, stats, q, k, v, None, *args)
+    hip.cross_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, None, *args)
+    # (sums by elements: the library's products refuse as many rows)
+    along = lambda x, row: (x.double() * row.double()).sum(dim=1)
+    down = lambda weight, x: (weight[:, None] * x.double()).sum(dim=0)
+    p = torch.softmax(along(k, q), dim=0)
+    some = 6 * math.sqrt(n) * U
+    want, size = down(p, v), down(p, v.abs())
+    ep = 2 * (gamma(d) + 4 * U) * along(k.abs(), q.abs()).max().item() + some + 8 * U
+    assert ((out[0] - want).abs() <= (ep + some) * size).all()
+    assert (down(p[-3:], v[-3:]).abs() > 3 * (ep + some) * size).all()
+    assert ((dv - p[:, None] * dout.double()).abs() <= (ep + 4 * U) * p[:, None] * dout.double().abs() + TINY).all()
+    del dv
+    dp = along(v, dout)
+    ds = p * (dp - (p * dp).sum())
+    # dp - dout . out: d products' roundings, and those of out, whose bound is above
+    e_ds = (ep + 4 * U) * ds.abs() + p * (gamma(d) * along(v.abs(), dout.abs())
+                                          + ((ep + some + gamma(d)) * size * dout[0].double().abs()).sum())
+    assert ((dk - ds[:, None] * q.double()).abs() <= (e_ds + 2 * U * ds.abs())[:, None] * q.double().abs() + TINY).all()
+    assert ((dq[0] - down(ds, k)).abs() <= down(e_ds + some * ds.abs(), k.abs())).all()
+    del k, v, dk, p, dp, ds, e_ds
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("shape", [(1, 2, 2, 20, 90, 64), (1, 2, 2, 90, 30, 32), (1, 2, 2, 70, 90, 32),
                                    (1, 2, 2, 200, 150, 64), (1, 2, 2, 70, 90, 128)],
                          ids=lambda s: "x".join(map(str, s)))

@@ -42,6 +42,30 @@ def test_embedding(hip, count):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("count,vocab,dim", [(5, (1 << 31) - 2, 1), (300, (1 << 31) - 2, 1),
+                                             (400, 3, 1 << 20), (100, 2, 1 << 20)])
+def test_the_largest_table_and_the_widest_rows(hip, count, vocab, dim):
+    print(f"embedding {count} of {vocab} x {dim}", flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(count)
+    ids = torch.randint(0, vocab, (count,), generator=gen, device="cuda", dtype=torch.int32)
+    ids[-2:] = vocab - 1
+    ids[0] = -1
+    grad, table = integers(gen, count, dim), torch.full((vocab, dim), 3.0, device="cuda")
+    out, dtable = torch.empty_like(grad), torch.empty_like(table)
+    hip.embedding_forward(out, table, ids, count, vocab, dim, 0.5)
+    assert torch.all(out[1:] == 1.5) and torch.all(out[0] == 0.0)
+    live = ids >= 0
+    for beta in (0.0, 0.5):
+        dtable.fill_(2.0)
+        hip.embedding_backward(dtable, grad, ids, count, vocab, dim, 1.0, beta)
+        want = torch.full_like(table, 2.0 * beta).index_add_(0, ids[live].long(), grad[live])
+        assert torch.equal(dtable, want)
+        del want
+    del out, dtable, table, grad
+    torch.cuda.empty_cache()
+    hip.call("nrs_shutdown")  # (gives the scratch back)
+
+
 def test_dropout_backward(hip):
     """The backward's mask is the forward's past 2^31 elements, and adds to what is
     there."""
