@@ -9,6 +9,12 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// 128 bits at any float: rows need not be 16-byte aligned, gfx950 loads and stores
+// them from any dword.
+struct __attribute__((packed, aligned(4))) Quad {
+    f32x4 v;
+};
+
 // Raw buffer resource over `bytes` bytes at `base` (gfx9 descriptor format).
 // A buffer load whose byte offset is >= bytes returns zero in hardware, so a
 // gathered operand needs neither a branch nor a select for its padding: out

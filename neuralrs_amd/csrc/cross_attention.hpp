@@ -46,10 +46,6 @@ struct CrossArgs {
     int q_blocks;                // workgroups of the dq part of the launch
 };
 
-struct __attribute__((packed, aligned(4))) Quad {  // 128 bits at any float
-    f32x4 v;
-};
-
 __device__ __forceinline__ int live_keys(const CrossArgs& a, int b) {
     return a.key_len ? max(0, min(a.key_len[b], a.Sk)) : a.Sk;
 }

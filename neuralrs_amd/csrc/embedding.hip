@@ -31,11 +31,6 @@
 namespace nrs {
 namespace {
 
-// Rows need not be 16-byte aligned: gfx950 loads 128 bits from any dword.
-struct __attribute__((packed, aligned(4))) Quad {
-    f32x4 v;
-};
-
 constexpr int kThreads = 256;
 constexpr int kRows = 4;  // rows a thread of the lookup has in flight
 
