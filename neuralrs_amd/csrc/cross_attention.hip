@@ -100,8 +100,8 @@ __device__ __forceinline__ float across_groups(float x) {
 // v_mfma_f32_16x16x4_f32 (16 rows at 157 TFLOP/s keep pace with 8 TB/s of f32
 // keys and values). Waves of a workgroup take turns at tiles of 16 keys, each
 // with its next tile on the way, and are joined at the end. 2 x 16384 keys, 8 key
-// heads of 128, 4 rows each: 46 us, 5.8 TB/s; 32 items of up to 1500 keys, 8 heads
-// of 64, a row each: 27 us, 4.3 TB/s, where a wave sees five tiles.
+// heads of 128, 4 rows each: 45 us, 5.9 TB/s; 32 items of up to 1500 keys, 8 heads
+// of 64, a row each: 26 us, 4.4 TB/s, where a wave sees five tiles.
 template <int NJ>
 struct RowsWalk {
     const CrossArgs& a;
