@@ -375,6 +375,84 @@ int nrs_cross_attention_backward(float *dq, float *dk, float *dv, const float *d
                                  float scale, float beta_q, float beta_kv, void *work,
                                  size_t work_bytes);
 
+/* -------------------------------------------------------- masked attention */
+/* Self-attention of a decoder over its own keys, or a cache of them: the
+ * reference's attention (src/cuda/nn/attention.rs:23-32) has no mask, so no
+ * counterpart there. Layouts, sizes, grouped key heads, strides, stats and scratch
+ * are those of nrs_cross_attention_forward. For query s of item b, which stands at
+ * position i = q_start[b] + s among the item's keys, and head h:
+ *   u_t = scale * q . k_t                    (cap 0), else cap * tanh(scale * q . k_t / cap)
+ *   u_t -= slopes[h] * |i - t|               (where slopes are given)
+ *   out = sum over the keys t that it sees of softmax(u)_t v_t, zeros if none.
+ * It sees key t when t < key_len[b], key_begin[b, s] <= t < key_end[b, s] and, if
+ * causal, t <= i or t < prefix_len[b]; a mask that is not given hides nothing. So
+ * key_begin, the first token of each token's document, keeps packed documents apart;
+ * with key_end it says any range. Every range is cut to 0 .. seq_k - 1.
+ *   Values of keys that a row does not see, infinite and NaN ones among them, do not
+ * change its results or gradients; keys that no row of an item sees get a zero gradient
+ * (written as zeros with beta_kv 0, left as they are with 1). A row that sees a key with
+ * a NaN, an infinity or a magnitude of 2^127 or more in it has no defined result (NaN as
+ * a rule), nor have the gradients of the keys that such a row sees.                 */
+typedef struct nrs_attention_mask {
+    int causal;                /* 0 or 1                                             */
+    const int32_t *q_start;    /* device [batch]; NULL: seq_k - seq_q, the last keys */
+    const int32_t *key_len;    /* device [batch]; NULL: seq_k                        */
+    const int32_t *prefix_len; /* device [batch]; NULL: 0 (needs causal)             */
+    const int32_t *key_begin;  /* device [batch * seq_q]; NULL: 0                    */
+    const int32_t *key_end;    /* device [batch * seq_q]; NULL: seq_k                */
+    const float *slopes;       /* device [heads], finite and 0 or more; NULL: 0      */
+    float cap;                 /* of the scores; 0: none                             */
+} nrs_attention_mask;
+int nrs_masked_attention_supported(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
+                                   int64_t seq_k, int64_t d_head, int64_t ld_q, int64_t ld_kv,
+                                   int64_t ld_out);
+int nrs_masked_attention_workspace(size_t *bytes, int64_t batch, int64_t heads, int64_t kv_heads,
+                                   int64_t seq_q, int64_t seq_k, int64_t d_head, int backward);
+/* mask is a host structure that the call reads, NULL: every key is seen.        */
+int nrs_masked_attention_forward(float *out, float *stats, const float *q, const float *k,
+                                 const float *v, const nrs_attention_mask *mask, int64_t batch,
+                                 int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_k,
+                                 int64_t d_head, int64_t ld_q, int64_t ld_kv, int64_t ld_out,
+                                 float scale, void *work, size_t work_bytes);
+/* Its backward, from the forward's out and stats and the same mask, as
+ * nrs_cross_attention_backward: with P the weights,
+ *   dS = P * (dout . v^T - dout . out) * (1 - tanh^2 where capped) * scale,
+ *   dq = beta_q * dq + dS . k,  dk = beta_kv * dk + dS^T . q,
+ *   dv = beta_kv * dv + P^T . dout.
+ * The slopes are constants: they get no gradient.                            */
+int nrs_masked_attention_backward(float *dq, float *dk, float *dv, const float *dout,
+                                  const float *out, const float *q, const float *k, const float *v,
+                                  const float *stats, const nrs_attention_mask *mask,
+                                  int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
+                                  int64_t seq_k, int64_t d_head, int64_t ld_q, int64_t ld_kv,
+                                  int64_t ld_out, float scale, float beta_q, float beta_kv,
+                                  void *work, size_t work_bytes);
+
+/* -------------------------------------------------------- rotary positions */
+/* Turns pairs of columns of every head by angles that grow with a token's position
+ * (of one axis, or several: time, height and width of a patch of video). No counterpart
+ * in the reference. x [rows, ld_x], out [rows, ld_out], head h in columns [h*d_head,
+ * (h+1)*d_head); for pair j < pairs, with angle = positions[axis[j] * rows + row] *
+ * freq[j] (taken in 64 bits):
+ *   (a, b) -> (a cos - b sin, b cos + a sin)
+ * (a, b) are columns j and pairs + j of the head, or 2j and 2j + 1 if interleaved.
+ * The other columns, and pairs whose axis is outside [0, axes), are copied. positions
+ * [axes, rows] (any sign), freq [pairs], axis [pairs] (NULL: all 0) are on the device.
+ * The queries and keys of one projection are turned together as heads side by side.
+ * out may be x, with the same stride; else they must not overlap. Strides are at most
+ * 2^20 floats, rows 2^30, and rows * heads * ceil(d_head / 8) about 2^31.            */
+int nrs_rotary_forward(float *out, const float *x, const int32_t *positions, const float *freq,
+                       const int32_t *axis, int64_t rows, int64_t heads, int64_t d_head,
+                       int64_t pairs, int64_t axes, int64_t ld_x, int64_t ld_out,
+                       int interleaved);
+/* Its backward: the same columns of grad turned by the negative angles, gin =
+ * that + beta * gin. gin may be grad when beta is 0. Positions and frequencies get no
+ * gradient.                                                                    */
+int nrs_rotary_backward(float *gin, const float *grad, const int32_t *positions, const float *freq,
+                        const int32_t *axis, int64_t rows, int64_t heads, int64_t d_head,
+                        int64_t pairs, int64_t axes, int64_t ld_gin, int64_t ld_grad,
+                        int interleaved, float beta);
+
 /* -------------------------------------------------- embedding and dropout */
 /* Token embedding (the reference's src/cuda/nn/embedding layer, with the
  * scale of the table's rows folded in): out[i] = scale * table[ids[i]], out
@@ -417,6 +495,34 @@ int nrs_dropout_forward(float *out, const float *x, const float *residual, int64
  * + beta * gin. (The residual's gradient is grad itself.)                    */
 int nrs_dropout_backward(float *gin, const float *grad, int64_t n, float p, uint64_t seed,
                          uint64_t call, const uint64_t *step, float beta);
+
+/* ------------------------------------------------------------ distillation */
+/* The loss of a student's logits against the k largest logits of a teacher, mixed
+ * with cross-entropy against a label (no counterpart in the reference, whose
+ * cross-entropy takes one-hot rows, src/cuda/loss/cross_entropy.rs:18-58). Row i, with
+ * p = softmax(top[i] / T) over its teacher tokens, q = softmax(logits[i] / T) and r =
+ * softmax(logits[i]) over the vocabulary, T = temperature:
+ *   row_loss[i] = (1 - hard) * T^2 * sum_j p_j (log p_j - log q[top_ids[i][j]])
+ *                 + hard * -log r[labels[i]]
+ * logits [rows, ld], vocab columns of each; top and top_ids [rows, k] (k at most 1024),
+ * labels [rows] (may be NULL when hard is 0). A teacher token whose id is outside
+ * [0, vocab), -1 say, is left out, and a token named twice has the sum of both weights.
+ * A row without teacher tokens, or with teacher logits of minus infinity alone, has the
+ * second part alone; one whose label is outside [0, vocab), the first alone. Logits may be minus
+ * infinity, but not all of a row.                                               */
+int nrs_distill_forward(float *row_loss, const float *logits, const float *top,
+                        const int32_t *top_ids, const int32_t *labels, int64_t rows, int64_t vocab,
+                        int64_t k, int64_t ld, float temperature, float hard);
+/* Its gradient, written (not accumulated) into grad [rows, ld]:
+ *   row_grad[i] * d row_loss[i] / d logits[i],
+ * row_grad (device) NULL: 1 / rows, the gradient of the mean, as in
+ * nrs_cross_entropy_backward. Also gives the loss where row_loss is not NULL: a
+ * training step needs this call alone. grad may be logits, else they must not overlap.
+ * Columns past vocab are left as they are.                                       */
+int nrs_distill_backward(float *grad, float *row_loss, const float *row_grad, const float *logits,
+                         const float *top, const int32_t *top_ids, const int32_t *labels,
+                         int64_t rows, int64_t vocab, int64_t k, int64_t ld, float temperature,
+                         float hard);
 
 /* ---------------------------------------------------------------- conv2d */
 /* The five primitive launches of src/cuda/nn/conv.rs:161-236, same index

@@ -33,6 +33,13 @@ class GemmDesc(ctypes.Structure):
                 ("bias", _P), ("epilogue", ctypes.c_int)]
 
 
+class AttentionMask(ctypes.Structure):
+    """nrs_attention_mask (include/nrs_hip.h). Made by attention_mask, which keeps
+    the arrays that it points to."""
+    _fields_ = [("causal", ctypes.c_int), ("q_start", _P), ("key_len", _P), ("prefix_len", _P),
+                ("key_begin", _P), ("key_end", _P), ("slopes", _P), ("cap", _F)]
+
+
 # name -> argtypes (all return int status unless listed in _RET)
 SIGNATURES = {
     "nrs_init": [ctypes.c_int],
@@ -68,11 +75,19 @@ SIGNATURES = {
     "nrs_cross_attention_workspace": [ctypes.POINTER(_S)] + [_I] * 6 + [ctypes.c_int],
     "nrs_cross_attention_forward": [_P] * 6 + [_I] * 9 + [_F, _P, _S],
     "nrs_cross_attention_backward": [_P] * 10 + [_I] * 9 + [_F, _F, _F, _P, _S],
+    "nrs_masked_attention_supported": [_I] * 9,
+    "nrs_masked_attention_workspace": [ctypes.POINTER(_S)] + [_I] * 6 + [ctypes.c_int],
+    "nrs_masked_attention_forward": [_P] * 6 + [_I] * 9 + [_F, _P, _S],
+    "nrs_masked_attention_backward": [_P] * 10 + [_I] * 9 + [_F, _F, _F, _P, _S],
+    "nrs_rotary_forward": [_P] * 5 + [_I] * 7 + [ctypes.c_int],
+    "nrs_rotary_backward": [_P] * 5 + [_I] * 7 + [ctypes.c_int, _F],
     "nrs_embedding_forward": [_P, _P, _P, _I, _I, _I, _F],
     "nrs_embedding_workspace": [ctypes.POINTER(_S), _I, _I, _I],
     "nrs_embedding_backward": [_P, _P, _P, _I, _I, _I, _F, _F, _P, _S],
     "nrs_dropout_forward": [_P, _P, _P, _I, _F, _U, _U, _P],
     "nrs_dropout_backward": [_P, _P, _I, _F, _U, _U, _P, _F],
+    "nrs_distill_forward": [_P] * 5 + [_I] * 4 + [_F, _F],
+    "nrs_distill_backward": [_P] * 7 + [_I] * 4 + [_F, _F],
     "nrs_im2col": [_P, _P] + [_I] * 8,
     "nrs_col2out": [_P, _P, _P, _I, _I, _I, _I],
     "nrs_out2mm": [_P, _P, _I, _I, _I, _I],
@@ -303,6 +318,76 @@ def cross_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, key_len, bat
             _ptr(out), _ptr(q), _ptr(k), _ptr(v), _ptr(stats), _ptr(key_len), batch, heads,
             kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv, ld_out, scale, beta_q, beta_kv,
             *_work(work))
+
+
+def attention_mask(causal=False, q_start=None, key_len=None, prefix_len=None, key_begin=None,
+                   key_end=None, slopes=None, cap=0.0):
+    """What masked attention hides and adds: device arrays (int32; slopes f32) or None."""
+    arrays = (q_start, key_len, prefix_len, key_begin, key_end, slopes)
+    m = AttentionMask(int(causal), *[_ptr(x) for x in arrays], cap)
+    m.arrays = arrays
+    return m
+
+
+def _mask(m):
+    return None if m is None else ctypes.addressof(m)
+
+
+def masked_attention_workspace(batch, heads, kv_heads, seq_q, seq_k, d_head, backward=False):
+    """Bytes of scratch that a masked attention call of these sizes needs."""
+    n = ctypes.c_size_t()
+    call("nrs_masked_attention_workspace", ctypes.byref(n), batch, heads, kv_heads, seq_q, seq_k,
+         d_head, int(backward))
+    return n.value
+
+
+def masked_attention_forward(out, stats, q, k, v, mask, batch, heads, kv_heads, seq_q, seq_k,
+                             d_head, ld_q, ld_kv, ld_out, scale, work=None):
+    """out = softmax of the keys that `mask` (an attention_mask, or None) lets each
+    query see, times v; stats may be None when no backward follows."""
+    _launch(load().nrs_masked_attention_forward, _ptr(out), _ptr(stats), _ptr(q), _ptr(k), _ptr(v),
+            _mask(mask), batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv, ld_out, scale,
+            *_work(work))
+
+
+def masked_attention_backward(dq, dk, dv, dout, out, q, k, v, stats, mask, batch, heads, kv_heads,
+                              seq_q, seq_k, d_head, ld_q, ld_kv, ld_out, scale, beta_q=0.0,
+                              beta_kv=0.0, work=None):
+    """dq, dk and dv (+ beta * old) from the forward's out and stats and its mask; dq,
+    or dk and dv, may be None."""
+    _launch(load().nrs_masked_attention_backward, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dout),
+            _ptr(out), _ptr(q), _ptr(k), _ptr(v), _ptr(stats), _mask(mask), batch, heads, kv_heads,
+            seq_q, seq_k, d_head, ld_q, ld_kv, ld_out, scale, beta_q, beta_kv, *_work(work))
+
+
+def rotary_forward(out, x, positions, freq, axis, rows, heads, d_head, pairs, axes, ld_x, ld_out,
+                   interleaved=False):
+    """Pair j of every head turned by positions[axis[j]][row] * freq[j] (axis None: 0)."""
+    _launch(load().nrs_rotary_forward, _ptr(out), _ptr(x), _ptr(positions), _ptr(freq), _ptr(axis),
+            rows, heads, d_head, pairs, axes, ld_x, ld_out, int(interleaved))
+
+
+def rotary_backward(gin, grad, positions, freq, axis, rows, heads, d_head, pairs, axes, ld_gin,
+                    ld_grad, interleaved=False, beta=0.0):
+    """gin = grad turned back (+ beta * gin)."""
+    _launch(load().nrs_rotary_backward, _ptr(gin), _ptr(grad), _ptr(positions), _ptr(freq),
+            _ptr(axis), rows, heads, d_head, pairs, axes, ld_gin, ld_grad, int(interleaved), beta)
+
+
+def distill_forward(row_loss, logits, top, top_ids, labels, rows, vocab, k, ld, temperature=1.0,
+                    hard=0.0):
+    """Each row's loss against a teacher's k largest logits, mixed with that against
+    its label by `hard` (labels may be None when it is 0)."""
+    _launch(load().nrs_distill_forward, _ptr(row_loss), _ptr(logits), _ptr(top), _ptr(top_ids),
+            _ptr(labels), rows, vocab, k, ld, temperature, hard)
+
+
+def distill_backward(grad, row_loss, row_grad, logits, top, top_ids, labels, rows, vocab, k, ld,
+                     temperature=1.0, hard=0.0):
+    """grad = row_grad (None: 1 / rows) * d row_loss / d logits, and the loss unless
+    row_loss is None. grad may be logits."""
+    _launch(load().nrs_distill_backward, _ptr(grad), _ptr(row_loss), _ptr(row_grad), _ptr(logits),
+            _ptr(top), _ptr(top_ids), _ptr(labels), rows, vocab, k, ld, temperature, hard)
 
 
 def embedding_forward(out, table, ids, count, vocab, dim, scale=1.0):

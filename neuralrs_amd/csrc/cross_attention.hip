@@ -765,8 +765,10 @@ const char* refusal(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_
     return nullptr;
 }
 
-int check_shape(const char* what, int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
-                int64_t seq_k, int64_t d_head, int64_t ld_q, int64_t ld_kv, int64_t ld_out) {
+}  // namespace
+
+int cross_check_shape(const char* what, int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
+                      int64_t seq_k, int64_t d_head, int64_t ld_q, int64_t ld_kv, int64_t ld_out) {
     const char* why =
         refusal(batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv, ld_out);
     NRS_ARG_CHECK(!why,
@@ -778,7 +780,6 @@ int check_shape(const char* what, int64_t batch, int64_t heads, int64_t kv_heads
     return NRS_OK;
 }
 
-}  // namespace
 }  // namespace nrs
 
 extern "C" {
@@ -792,7 +793,7 @@ int nrs_cross_attention_supported(int64_t batch, int64_t heads, int64_t kv_heads
 int nrs_cross_attention_workspace(size_t* bytes, int64_t batch, int64_t heads, int64_t kv_heads,
                                   int64_t seq_q, int64_t seq_k, int64_t d_head, int backward) {
     NRS_ARG_CHECK(bytes, "cross attention workspace: null pointer");
-    if (int rc = nrs::check_shape("cross attention workspace", batch, heads, kv_heads, seq_q,
+    if (int rc = nrs::cross_check_shape("cross attention workspace", batch, heads, kv_heads, seq_q,
                                   seq_k, d_head, nrs::kMaxLd, nrs::kMaxLd, nrs::kMaxLd))
         return rc;
     const int cus = nrs::num_cus();
@@ -809,7 +810,7 @@ int nrs_cross_attention_forward(float* out, float* stats, const float* q, const 
                                 int64_t d_head, int64_t ld_q, int64_t ld_kv, int64_t ld_out,
                                 float scale, void* work, size_t work_bytes) {
     const char* what = "cross attention forward";
-    if (int rc = nrs::check_shape(what, batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv,
+    if (int rc = nrs::cross_check_shape(what, batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv,
                                   ld_out))
         return rc;
     if (batch == 0 || seq_q == 0) return NRS_OK;
@@ -886,7 +887,7 @@ int nrs_cross_attention_backward(float* dq, float* dk, float* dv, const float* d
                                  float scale, float beta_q, float beta_kv, void* work,
                                  size_t work_bytes) {
     const char* what = "cross attention backward";
-    if (int rc = nrs::check_shape(what, batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv,
+    if (int rc = nrs::cross_check_shape(what, batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv,
                                   ld_out))
         return rc;
     NRS_ARG_CHECK((dk == nullptr) == (dv == nullptr), "%s: dk and dv go together", what);

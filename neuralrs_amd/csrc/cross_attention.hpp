@@ -150,6 +150,10 @@ struct LinePart {
     }
 };
 
+// NRS_ERR_ARG, with the reason, for sizes that are not taken.
+int cross_check_shape(const char* what, int64_t batch, int64_t heads, int64_t kv_heads,
+                      int64_t seq_q, int64_t seq_k, int64_t d_head, int64_t ld_q, int64_t ld_kv,
+                      int64_t ld_out);
 // The kernels of cross_attention_tile.hip.
 void cross_tile_forward(const CrossArgs& a, unsigned blocks);
 // The rows' statistics, then (unless only they are wanted) what is asked for of
