@@ -1,5 +1,6 @@
 // Attention whose rows see ranges of keys, with capped scores and a bias by
 // distance, forward and backward, all f32.
+#include "attention_rows.hpp"
 #include "masked_attention.hpp"
 
 #include <cmath>
@@ -7,162 +8,278 @@
 namespace nrs {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-// A row's score of a key from their product, in base 2; `inner` is the cap's
-// derivative.
-struct Scores {
-    float scale, cap, slope;
-    int64_t at, near;
-
-    __device__ __forceinline__ Scores(const MaskedArgs& a, const RowRange& r, int head)
-        : scale(a.scale), cap(a.cap), slope(a.slopes ? a.slopes[head] : 0.0f), at(r.at),
-          near(nearest(r)) {}
-    __device__ __forceinline__ float of(float dot, int key, float& inner) const {
-        float u = dot * scale;
-        inner = 1.0f;
-        if (cap > 0.0f) {
-            const float t = tanhf(u / cap);
-            inner = 1.0f - t * t;
-            u = cap * t;
-        }
-        const int64_t far = at < key ? key - at : at - key;
-        return (u - slope * (float)(far - near)) * kLog2e;
-    }
-};
-
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i, 64);
-    return x;
-}
-
-// Columns lane and lane + 64 of a row of d_head floats.
-__device__ __forceinline__ void row2(float (&x)[2], const float* p, int lane, int D) {
-    x[0] = lane < D ? p[lane] : 0.0f;
-    x[1] = lane + 64 < D ? p[lane + 64] : 0.0f;
-}
-
-// A wave to a row.
-__global__ __launch_bounds__(256) void masked_fwd_kernel(MaskedArgs a) {
-    const int lane = threadIdx.x & 63, R = a.Sq * a.G;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (int64_t)a.B * a.KV * R) return;
-    const int item = (int)(row / R), r = (int)(row - (int64_t)item * R);
+// Few rows (tokens being decoded): K and V stream from memory once, straight into
+// registers, as operands of v_mfma_f32_16x16x4_f32. A unit is 16 rows of an item, a
+// workgroup has a part of its keys, and its waves take turns at tiles of 16 keys, each
+// with its next tile on the way.
+template <int NJ, int MODE>
+__global__ __launch_bounds__(64 * kRowWaves) void masked_rows_fwd_kernel(MaskedArgs a) {
+    static_assert(kRowWaves == 4, "a register of an accumulator to each wave");
+    __shared__ float sums[kRowWaves][4 * NJ][64];
+    __shared__ float tops[kRowWaves][16], totals[kRowWaves][16];
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int R = a.Sq * a.G, row_tiles = (R + 15) / 16;
+    const int unit = blockIdx.x % a.units, no = blockIdx.x / a.units;
+    const int item = unit / row_tiles, r0 = unit % row_tiles * 16;
     const int b = item / a.KV, kv = item - b * a.KV;
-    const RowRange range = row_range(a, b, r / a.G);
-    const Scores scores(a, range, kv * a.G + r % a.G);
-    float q[2], acc[2] = {0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-    row2(q, a.q + query_offset(a, b, kv, r, a.ld_q), lane, a.D);
-    for (int t = range.lo; t < range.hi; ++t) {
-        float k[2], v[2], inner;
-        const int64_t at = key_offset(a, b, kv, t);
-        row2(k, a.k + at, lane, a.D);
-        row2(v, a.v + at, lane, a.D);
-        const float u = scores.of(wave_sum(q[0] * k[0] + q[1] * k[1]), t, inner);
-        const float top = fmaxf(m, u);
-        const float old = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-        const float p = __builtin_amdgcn_exp2f(u - top);
+    const bool live = r0 + c < R;
+    const int s_row = live ? (r0 + c) / a.G : 0;
+    RowRange range = row_range(a, b, s_row);
+    if (!live) range.lo = range.hi = range.at = 0;
+    int least = live && range.hi > 0 ? range.lo : INT32_MAX, most = range.hi;
+    int from = !live ? 0 : range.hi > 0 ? range.lo : INT32_MAX, to = live ? range.hi : INT32_MAX;
+#pragma unroll
+    for (int i = 1; i < 16; i *= 2) {
+        least = min(least, __shfl_xor(least, i, 64));
+        most = max(most, __shfl_xor(most, i, 64));
+        from = max(from, __shfl_xor(from, i, 64));
+        to = min(to, __shfl_xor(to, i, 64));
+    }
+    least = __builtin_amdgcn_readfirstlane(least);
+    most = __builtin_amdgcn_readfirstlane(most);
+    const int first = most > 0 ? least / 16 : 0, last = (most + 15) / 16;
+    const int used = max(1, (last - first + a.part_tiles - 1) / a.part_tiles);
+    if (no >= used) return;
+    if (a.parts > 1 && no == 0 && threadIdx.x == 0) a.counts[unit] = used;
+    const int t0 = first + no * a.part_tiles, t1 = min(last, t0 + a.part_tiles);
+    f32x4 qf[NJ], acc[NJ], kf[NJ];
+    float vf[4][NJ];
+    auto load_keys = [&](int t) {
+        Rows<false>(a, a.k, b, kv, a.ld_kv, 16 * t, min(16, most - 16 * t))
+            .template along<NJ>(kf, c, g);
+    };
+    auto load_values = [&](int t) {
+        const Rows<false> vs(a, a.v, b, kv, a.ld_kv, 16 * t, min(16, most - 16 * t));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) vs.template across<NJ>(vf[r], 4 * g + r, c);
+    };
+    if (t0 + w < t1) {
+        load_keys(t0 + w);
+        load_values(t0 + w);
+    }
+    const float slope2 =
+        MODE != kPlain && a.slopes && live ? a.slopes[kv * a.G + r0 + c - s_row * a.G] * kLog2e : 0.0f;
+    Rows<true>(a, a.q, b, kv, a.ld_q, r0, min(16, R - r0)).template along<NJ>(qf, c, g);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        qf[j] = qf[j] * a.scale_own;
+        acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float m = -INFINITY, l = 0.0f;
+    for (int t = t0 + w; t < t1; t += kRowWaves) {
+        f32x4 p = dot_rows<NJ>(kf, qf);
+        if (t + kRowWaves < t1) load_keys(t + kRowWaves);
+        if (MODE == kCap) {
+            tanh_all<4>(p);
+            p = p * a.cap2;
+        }
+        if (MODE != kPlain) {
+            const float far = (float)(range.at - (16 * t + 4 * g));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[r] = fmaf(-slope2, fabsf(far - (float)r), p[r]);
+        }
+        if (16 * t < from || 16 * t + 16 > to) {
+            // a value that is not finite must not meet the weight 0 of a row that does not
+            // see it: the key gets zeros, and a NaN for a score
+            int bad = 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float most_v = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                    if (c * NJ + j < a.D)
+                        most_v = __builtin_elementwise_maximum(most_v, __builtin_fabsf(vf[r][j]));
+                bad |= most_v < INFINITY ? 0 : 1 << r;
+            }
+#pragma unroll
+            for (int i = 1; i < 16; i *= 2) bad |= __shfl_xor(bad, i, 64);
+            const uint32_t span = range.hi - range.lo;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (bad >> r & 1) {
+                    p[r] = NAN;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) vf[r][j] = 0.0f;
+                }
+                p[r] = (uint32_t)(16 * t + 4 * g + r - range.lo) < span ? p[r] : -INFINITY;
+            }
+        }
+        float top = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), m);
+        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
         m = top;
-        l = l * old + p;
-        acc[0] = acc[0] * old + p * v[0];
-        acc[1] = acc[1] * old + p * v[1];
-    }
-    const bool any = range.hi > range.lo;
-    const float f = any ? 1.0f / l : 0.0f;
-    float* const out = a.out + query_offset(a, b, kv, r, a.ld_out);
-    if (lane < a.D) out[lane] = acc[0] * f;
-    if (lane + 64 < a.D) out[lane + 64] = acc[1] * f;
-    if (a.stats && lane == 0) {
-        float* const st = row_stats(a, b, kv, r);
-        st[0] = any ? m : 0.0f;
-        st[1] = l;
-    }
-}
-
-// P and dS of a row and a key; all lanes get them.
-__device__ __forceinline__ void weights(const MaskedArgs& a, const Scores& scores, int t,
-                                        const float (&q)[2], const float (&g)[2],
-                                        const float (&k)[2], const float (&v)[2], float lse,
-                                        float delta, float& p, float& ds) {
-    float inner;
-    const float u = scores.of(wave_sum(q[0] * k[0] + q[1] * k[1]), t, inner);
-    p = __builtin_amdgcn_exp2f(u - lse);
-    ds = p * (wave_sum(g[0] * v[0] + g[1] * v[1]) - delta) * inner * a.scale;
-}
-
-__device__ __forceinline__ void add_to(float* dst, const float (&x)[2], float beta, int lane, int D) {
-    if (lane < D) dst[lane] = beta != 0.0f ? x[0] + beta * dst[lane] : x[0];
-    if (lane + 64 < D) dst[lane + 64] = beta != 0.0f ? x[1] + beta * dst[lane + 64] : x[1];
-}
-
-__device__ __forceinline__ void row_start(const MaskedArgs& a, int b, int kv, int r,
-                                          const float (&g)[2], int lane, float& lse, float& delta) {
-    float o[2];
-    row2(o, a.o + query_offset(a, b, kv, r, a.ld_out), lane, a.D);
-    const float* const st = row_stats(a, b, kv, r);
-    lse = st[0] + __builtin_amdgcn_logf(st[1]);
-    delta = wave_sum(g[0] * o[0] + g[1] * o[1]);
-}
-
-// dq, a wave to a row.
-__global__ __launch_bounds__(256) void masked_dq_kernel(MaskedArgs a) {
-    const int lane = threadIdx.x & 63, R = a.Sq * a.G;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (int64_t)a.B * a.KV * R) return;
-    const int item = (int)(row / R), r = (int)(row - (int64_t)item * R);
-    const int b = item / a.KV, kv = item - b * a.KV;
-    const RowRange range = row_range(a, b, r / a.G);
-    const Scores scores(a, range, kv * a.G + r % a.G);
-    float q[2], g[2], acc[2] = {0.0f, 0.0f}, lse, delta;
-    row2(q, a.q + query_offset(a, b, kv, r, a.ld_q), lane, a.D);
-    row2(g, a.dout + query_offset(a, b, kv, r, a.ld_out), lane, a.D);
-    row_start(a, b, kv, r, g, lane, lse, delta);
-    for (int t = range.lo; t < range.hi; ++t) {
-        float k[2], v[2], p, ds;
-        const int64_t at = key_offset(a, b, kv, t);
-        row2(k, a.k + at, lane, a.D);
-        row2(v, a.v + at, lane, a.D);
-        weights(a, scores, t, q, g, k, v, lse, delta, p, ds);
-        acc[0] += ds * k[0];
-        acc[1] += ds * k[1];
-    }
-    add_to(a.dq + query_offset(a, b, kv, r, a.ld_q), acc, a.beta_q, lane, a.D);
-}
-
-// dk and dv, a wave to a key.
-__global__ __launch_bounds__(256) void masked_dkv_kernel(MaskedArgs a) {
-    const int lane = threadIdx.x & 63, R = a.Sq * a.G;
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= (int64_t)a.B * a.KV * a.Sk) return;
-    const int item = (int)(at / a.Sk), t = (int)(at - (int64_t)item * a.Sk);
-    const int b = item / a.KV, kv = item - b * a.KV;
-    const int64_t key = key_offset(a, b, kv, t);
-    float k[2] = {0.0f, 0.0f}, v[2] = {0.0f, 0.0f}, dk[2] = {0.0f, 0.0f}, dv[2] = {0.0f, 0.0f};
-    bool seen = false;
-    for (int r = 0; r < R; ++r) {
-        const RowRange range = row_range(a, b, r / a.G);
-        if (t < range.lo || t >= range.hi) continue;
-        if (!seen) {
-            row2(k, a.k + key, lane, a.D);
-            row2(v, a.v + key, lane, a.D);
-            seen = true;
-        }
-        const Scores scores(a, range, kv * a.G + r % a.G);
-        float q[2], g[2], lse, delta, p, ds;
-        row2(q, a.q + query_offset(a, b, kv, r, a.ld_q), lane, a.D);
-        row2(g, a.dout + query_offset(a, b, kv, r, a.ld_out), lane, a.D);
-        row_start(a, b, kv, r, g, lane, lse, delta);
-        weights(a, scores, t, q, g, k, v, lse, delta, p, ds);
+        l *= alpha;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            dk[e] += ds * q[e];
-            dv[e] += p * g[e];
+        for (int j = 0; j < NJ; ++j) acc[j] = acc[j] * alpha;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            p[r] = p[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[r] - m);
+            l += p[r];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[j] = mfma16(vf[r][j], p[r], acc[j]);
+        }
+        if (t + kRowWaves < t1) load_values(t + kRowWaves);
+    }
+    l = across_groups(l);
+    if (g == 0) {
+        tops[w][c] = m;
+        totals[w][c] = l;
+    }
+    __syncthreads();
+    float top = tops[0][c];
+#pragma unroll
+    for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, tops[i][c]);
+    const float f = Joined<32>::weight(m, l, top);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) sums[w][r * NJ + j][lane] = acc[j][r] * f;
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kRowWaves; ++i) {
+        const float of = Joined<32>::weight(tops[i][c], totals[i][c], top);
+        total += totals[i][c] * of;
+    }
+    __syncthreads();
+    if (!live) return;
+    // wave w adds the waves' register w: NJ neighbouring columns of row c
+    const bool whole = used == 1, none = total == 0.0f;
+    const float scale = !whole ? 1.0f : none ? 0.0f : 1.0f / total;
+    const int64_t at = ((int64_t)no * a.units + unit) * 16 + c;
+    float* dst = whole ? a.out + query_offset(a, b, kv, r0 + c, a.ld_out) : a.part + at * a.D;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRowWaves; ++i) v += sums[i][w * NJ + j][lane];
+        const int d = (4 * g + w) * NJ + j;
+        if (d < a.D) dst[d] = v * scale;
+    }
+    if (w == 0 && g == 0 && (!whole || a.stats)) {
+        float* st = whole ? row_stats(a, b, kv, r0 + c) : a.part_stats + 2 * at;
+        st[0] = whole && none ? 0.0f : top;
+        st[1] = total;
+    }
+}
+
+// Joins the parts of a row: GROUPS groups of LANES threads (four columns each) take even
+// shares of them and are added up in LDS.
+template <int LANES, int GROUPS>
+__global__ __launch_bounds__(256) void masked_join_kernel(MaskedArgs a) {
+    constexpr int ROWS = 256 / (LANES * GROUPS);  // of a workgroup
+    __shared__ f32x4 sums[ROWS][GROUPS][LANES];
+    __shared__ float tops[ROWS][GROUPS], totals[ROWS][GROUPS];
+    const int x = threadIdx.x % LANES, group = threadIdx.x / LANES % GROUPS;
+    const int in = threadIdx.x / (LANES * GROUPS), R = a.Sq * a.G;
+    const int64_t row = (int64_t)blockIdx.x * ROWS + in;
+    const bool there = row < (int64_t)a.B * a.KV * R;
+    const int item = there ? (int)(row / R) : 0, r = there ? (int)(row - (int64_t)item * R) : 0;
+    const int b = item / a.KV, live = max(0, min(4, a.D - 4 * x));
+    const int unit = item * ((R + a.unit_rows - 1) / a.unit_rows) + r / a.unit_rows;
+    const int parts = there ? a.counts[unit] : 1;
+    // a group that is past the rows, or whose row one workgroup took whole, is idle; the
+    // others may wait for each other
+    Joined<LANES> sum;
+    auto at = [&](int s) { return ((int64_t)s * a.units + unit) * a.unit_rows + r % a.unit_rows; };
+    if (parts > 1)
+        sum.add(parts * group / GROUPS, parts * (group + 1) / GROUPS, live,
+                [&](int s) { return a.part_stats + 2 * at(s); },
+                [&](int s) { return a.part + at(s) * a.D; });
+    if (GROUPS > 1) {
+        sums[in][group][x] = sum.v;
+        if (x == 0) {
+            tops[in][group] = sum.top;
+            totals[in][group] = sum.total;
+        }
+        __syncthreads();
+    }
+    if (parts == 1 || group != 0) return;
+    for (int i = 1; i < GROUPS; ++i) {
+        const float most = fmaxf(sum.top, tops[in][i]);
+        const float f = Joined<LANES>::weight(sum.top, sum.total, most),
+                    of = Joined<LANES>::weight(tops[in][i], totals[in][i], most);
+        sum.v = sum.v * f + sums[in][i][x] * of;
+        sum.total = sum.total * f + totals[in][i] * of;
+        sum.top = most;
+    }
+    const bool none = sum.total == 0.0f;
+    const float scale = none ? 0.0f : 1.0f / sum.total;
+    float* dst = a.out + query_offset(a, b, item - b * a.KV, r, a.ld_out) + 4 * x;
+    if (live == 4)
+        reinterpret_cast<Quad*>(dst)->v = sum.v * scale;
+    else
+        for (int e = 0; e < live; ++e) dst[e] = sum.v[e] * scale;
+    if (a.stats && x == 0) {
+        float* st = row_stats(a, b, item - b * a.KV, r);
+        st[0] = none ? 0.0f : sum.top;
+        st[1] = sum.total;
+    }
+}
+
+// Adds the parts of a gradient in order: dst = f * sum + beta * dst, D / 4 threads to a
+// row. KEYS: rows are keys, blockIdx.y is 0 for dk and 1 for dv.
+template <int D, bool KEYS>
+__global__ __launch_bounds__(256) void masked_sum_kernel(MaskedArgs a) {
+    constexpr int LANES = D / 4;
+    const int n = KEYS ? a.Sk : a.Sq * a.G, x = threadIdx.x % LANES;
+    const int64_t at = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const int64_t rows = (int64_t)a.B * a.KV * n;
+    if (at >= rows) return;
+    const int item = (int)(at / n), r = (int)(at - (int64_t)item * n);
+    const int b = item / a.KV, kv = item - b * a.KV;
+    const int unit = item * ((n + kCrossBackwardRows - 1) / kCrossBackwardRows) + r / kCrossBackwardRows;
+    const int parts = (KEYS ? a.counts : a.q_counts)[unit];
+    if (parts == 1) return;  // one workgroup took all of it
+    const bool second = KEYS && blockIdx.y == 1;
+    const float beta = KEYS ? a.beta_kv : a.beta_q, f = second ? 1.0f : a.scale;
+    const float* part = (KEYS ? (second ? a.dv_part : a.dk_part) : a.dq_part) + at * a.D + 4 * x;
+    float* dst = (KEYS ? (second ? a.dv : a.dk) + key_offset(a, b, kv, r)
+                       : a.dq + query_offset(a, b, kv, r, a.ld_q)) + 4 * x;
+    if (4 * x + 4 <= a.D) {
+        f32x4 v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int s = 0; s < parts; ++s)
+            v = v + reinterpret_cast<const Quad*>(part + s * rows * a.D)->v;
+        v = v * f;
+        Quad* const to = reinterpret_cast<Quad*>(dst);
+        if (beta != 0.0f) v = v + beta * to->v;
+        to->v = v;
+    } else {
+        for (int e = 0; 4 * x + e < a.D; ++e) {
+            float v = 0.0f;
+            for (int s = 0; s < parts; ++s) v += part[s * rows * a.D + e];
+            dst[e] = beta != 0.0f ? v * f + beta * dst[e] : v * f;
         }
     }
-    if (!seen && a.beta_kv == 1.0f) return;
-    add_to(a.dk + key, dk, a.beta_kv, lane, a.D);
-    add_to(a.dv + key, dv, a.beta_kv, lane, a.D);
+}
+
+template <int D>
+void launch_sums(const MaskedArgs& a, bool dq, bool dkv) {
+    constexpr int PER = 1024 / D;
+    const int64_t rows = (int64_t)a.B * a.KV * a.Sq * a.G, keys = (int64_t)a.B * a.KV * a.Sk;
+    if (dq)
+        hipLaunchKernelGGL((masked_sum_kernel<D, false>), dim3((unsigned)((rows + PER - 1) / PER)),
+                           dim3(256), 0, stream(), a);
+    if (dkv)
+        hipLaunchKernelGGL((masked_sum_kernel<D, true>), dim3((unsigned)((keys + PER - 1) / PER), 2),
+                           dim3(256), 0, stream(), a);
+}
+
+template <int D>
+void launch_join(const MaskedArgs& a, int64_t rows) {
+    constexpr int PER = 1024 / D;
+    hipLaunchKernelGGL((masked_join_kernel<D / 4, 1>), dim3((unsigned)((rows + PER - 1) / PER)),
+                       dim3(256), 0, stream(), a);
+}
+
+template <int NJ>
+void launch_rows(const MaskedArgs& a, unsigned blocks) {
+    auto kernel = a.cap2 > 0.0f ? masked_rows_fwd_kernel<NJ, kCap>
+                  : a.slopes    ? masked_rows_fwd_kernel<NJ, kBias>
+                                : masked_rows_fwd_kernel<NJ, kPlain>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * kRowWaves), 0, stream(), a);
 }
 
 int check(const char* what, const nrs_attention_mask* mask, int64_t batch, int64_t heads,
@@ -190,8 +307,11 @@ MaskedArgs arguments(const nrs_attention_mask* mask, int64_t batch, int64_t head
         a.key_begin = mask->key_begin;
         a.key_end = mask->key_end;
         a.slopes = mask->slopes;
-        a.cap = mask->cap;
     }
+    const float cap = mask ? mask->cap : 0.0f;
+    a.cap2 = cap * kLog2e;
+    // (taken in 64 bits, rounded once)
+    a.scale_own = (float)(cap > 0.0f ? (double)scale / cap : (double)scale * 1.4426950408889634);
     a.B = (int)batch;
     a.H = (int)heads;
     a.KV = (int)kv_heads;
@@ -227,8 +347,11 @@ int nrs_masked_attention_workspace(size_t* bytes, int64_t batch, int64_t heads, 
     if (int rc = nrs::cross_check_shape(what, batch, heads, kv_heads, seq_q, seq_k, d_head, ld, ld,
                                         ld))
         return rc;
-    (void)backward;
-    *bytes = 0;
+    const int cus = nrs::num_cus();
+    *bytes =
+        backward
+            ? nrs::plan_masked_backward(batch, heads, kv_heads, seq_q, seq_k, d_head, cus).bytes()
+            : nrs::plan_masked_forward(batch, heads, kv_heads, seq_q, seq_k, d_head, cus).bytes();
     return NRS_OK;
 }
 
@@ -245,8 +368,10 @@ int nrs_masked_attention_forward(float* out, float* stats, const float* q, const
     NRS_ARG_CHECK(out && q && ((k && v) || seq_k == 0), "%s: null pointer", what);
     NRS_REQUIRE_INIT();
     if (int rc = nrs::check_device(what)) return rc;
+    const auto plan = nrs::plan_masked_forward(batch, heads, kv_heads, seq_q, seq_k, d_head,
+                                               nrs::num_cus());
     float* scratch = nullptr;
-    if (int rc = nrs::call_scratch(&scratch, 0, work, work_bytes, what)) return rc;
+    if (int rc = nrs::call_scratch(&scratch, plan.bytes(), work, work_bytes, what)) return rc;
     auto a = nrs::arguments(mask, batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv,
                             ld_out, scale);
     a.q = q;
@@ -254,9 +379,32 @@ int nrs_masked_attention_forward(float* out, float* stats, const float* q, const
     a.v = v;
     a.out = out;
     a.stats = stats;
+    a.unit_rows = plan.unit_rows;
+    a.units = (int)plan.walk.units;
+    a.part_tiles = plan.walk.part;
+    a.parts = plan.walk.parts;
+    a.part = scratch;
+    a.part_stats = scratch + plan.part;
+    a.counts = reinterpret_cast<int32_t*>(scratch + plan.part + plan.stats);
+    const unsigned blocks = (unsigned)plan.blocks();
+    if (plan.tiles)
+        nrs::masked_tile_forward(a, blocks);
+    else
+        (a.D <= 16   ? nrs::launch_rows<1>
+         : a.D <= 32 ? nrs::launch_rows<2>
+         : a.D <= 64 ? nrs::launch_rows<4>
+                     : nrs::launch_rows<8>)(a, blocks);
+    NRS_LAUNCH_CHECK(what);
+    if (a.parts == 1) return NRS_OK;
     const int64_t rows = batch * heads * seq_q;
-    hipLaunchKernelGGL(nrs::masked_fwd_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0,
-                       nrs::stream(), a);
+    const int width = nrs::cross_row_width(a.D);
+    if (!plan.tiles)  // many parts of few rows
+        hipLaunchKernelGGL((nrs::masked_join_kernel<32, 8>), dim3((unsigned)rows), dim3(256), 0,
+                           nrs::stream(), a);
+    else
+        (width == 32   ? nrs::launch_join<32>
+         : width == 64 ? nrs::launch_join<64>
+                       : nrs::launch_join<128>)(a, rows);
     NRS_LAUNCH_CHECK(what);
     return NRS_OK;
 }
@@ -279,8 +427,10 @@ int nrs_masked_attention_backward(float* dq, float* dk, float* dv, const float* 
                   "%s: null pointer", what);
     NRS_REQUIRE_INIT();
     if (int rc = nrs::check_device(what)) return rc;
+    const auto plan = nrs::plan_masked_backward(batch, heads, kv_heads, seq_q, seq_k, d_head,
+                                                nrs::num_cus());
     float* scratch = nullptr;
-    if (int rc = nrs::call_scratch(&scratch, 0, work, work_bytes, what)) return rc;
+    if (int rc = nrs::call_scratch(&scratch, plan.bytes(), work, work_bytes, what)) return rc;
     auto a = nrs::arguments(mask, batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv,
                             ld_out, scale);
     a.q = q;
@@ -294,13 +444,35 @@ int nrs_masked_attention_backward(float* dq, float* dk, float* dv, const float* 
     a.dv = keys ? dv : nullptr;
     a.beta_q = beta_q;
     a.beta_kv = beta_kv;
-    const int64_t all_rows = batch * heads * seq_q, all_keys = batch * kv_heads * seq_k;
-    if (a.dq)
-        hipLaunchKernelGGL(nrs::masked_dq_kernel, dim3((unsigned)((all_rows + 3) / 4)), dim3(256),
-                           0, nrs::stream(), a);
-    if (a.dk)
-        hipLaunchKernelGGL(nrs::masked_dkv_kernel, dim3((unsigned)((all_keys + 3) / 4)), dim3(256),
-                           0, nrs::stream(), a);
+    a.q_units = (int)plan.q.units;
+    a.q_part_tiles = plan.q.part;
+    a.q_parts = plan.q.parts;
+    a.units = (int)plan.kv.units;
+    a.part_tiles = plan.kv.part;
+    a.parts = plan.kv.parts;
+    a.row_tiles = (int)plan.row_tiles;
+    float* next = scratch;
+    auto take = [&next](size_t words) {
+        float* const p = next;
+        next += words;
+        return p;
+    };
+    a.neg_lse = take(plan.rows);
+    a.neg_delta = a.neg_lse + batch * heads * seq_q;
+    a.ranges = reinterpret_cast<nrs::RowKeys*>(take(plan.ranges));
+    a.ends = reinterpret_cast<nrs::TileEnds*>(take(plan.ends));
+    a.dq_part = take(plan.q_part);
+    a.dk_part = take(plan.kv_part);
+    a.dv_part = take(plan.kv_part);
+    a.q_counts = reinterpret_cast<int32_t*>(take(plan.counts));
+    a.counts = a.q_counts + plan.q.units;
+    if (!a.dq && !a.dk) return NRS_OK;
+    nrs::masked_tile_backward(a);
+    NRS_LAUNCH_CHECK(what);
+    const int width = nrs::cross_row_width(a.D);
+    (width == 32   ? nrs::launch_sums<32>
+     : width == 64 ? nrs::launch_sums<64>
+                   : nrs::launch_sums<128>)(a, a.dq && a.q_parts > 1, a.dk && a.parts > 1);
     NRS_LAUNCH_CHECK(what);
     return NRS_OK;
 }

@@ -1,4 +1,6 @@
-// Arguments and device helpers shared by the masked attention kernels.
+// Arguments and device helpers shared by the masked attention kernels
+// (masked_attention.hip: few rows, joins and sums, entry points;
+// masked_attention_tile.hip: many rows, the backward).
 //
 // Rows are those of cross_attention.hpp: row r of an item (batch item, key head) is
 // query r / group of head kv_head * group + r % group. Every row sees an unbroken
@@ -7,46 +9,95 @@
 #pragma once
 
 #include "cross_attention.hpp"
+#include "masked_attention_plan.hpp"
 
 namespace nrs {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A row's keys and place, as the backward keeps them.
+struct __attribute__((aligned(16))) RowKeys {
+    int lo, hi, at, unused;
+};
+// Of the rows of a tile: all that any of them sees lies in least .. most - 1, and what
+// lies in from .. to - 1 is seen by each.
+struct __attribute__((aligned(16))) TileEnds {
+    int least, most, from, to;
+};
 
 struct MaskedArgs : CrossArgs {
     bool causal;
     const int32_t *q_start, *prefix_len;    // per batch item, or null
     const int32_t *key_begin, *key_end;     // per batch item and query, or null
     const float* slopes;                    // per head, or null
-    float cap;                              // 0: none
+    float scale_own;                        // of the rows' (or keys') operands
+    float cap2;                             // cap * log2(e)
+    // the forward's walk, or the backward's two
+    int units, part_tiles, parts, q_units, q_part_tiles, q_parts;
+    int row_tiles;
+    int32_t *counts, *q_counts;             // parts of each unit
+    RowKeys* ranges;                        // [batch][seq_q]
+    TileEnds* ends;                         // [batch][row_tiles]
 };
 
 // The keys that a row sees, lo .. hi - 1 (lo = hi: none), and where it stands among
-// them.
+// them for the bias: at its own position, or the nearest key if that is not among them.
+// The distance from there differs from the row's own by the same amount for all
+// of its keys, which changes no weight, and keeps the last bits of a far row's scores.
 struct RowRange {
-    int lo, hi;
-    int64_t at;
+    int lo, hi, at;
 };
 
 __device__ __forceinline__ RowRange row_range(const MaskedArgs& a, int b, int s) {
-    RowRange r;
-    r.at = (int64_t)(a.q_start ? a.q_start[b] : a.Sk - a.Sq) + s;
+    const int64_t at = (int64_t)(a.q_start ? a.q_start[b] : a.Sk - a.Sq) + s;
     const int64_t i = (int64_t)b * a.Sq + s;
-    int64_t hi = live_keys(a, b);
+    int hi = live_keys(a, b);
     if (a.causal) {
-        int64_t seen = r.at + 1;
+        int64_t seen = at + 1;
         if (a.prefix_len) seen = max(seen, (int64_t)a.prefix_len[b]);
-        hi = min(hi, seen);
+        hi = (int)min((int64_t)hi, seen);
     }
-    if (a.key_end) hi = min(hi, (int64_t)a.key_end[i]);
-    const int64_t lo = a.key_begin ? max(0, a.key_begin[i]) : 0;
-    r.lo = (int)lo;
-    r.hi = (int)max(lo, hi);
+    if (a.key_end) hi = min(hi, a.key_end[i]);
+    RowRange r;
+    r.lo = a.key_begin ? max(0, a.key_begin[i]) : 0;
+    r.hi = hi;
+    if (r.lo >= r.hi) r.lo = r.hi = 0;
+    r.at = (int)max((int64_t)r.lo, min((int64_t)r.hi - 1, at));
     return r;
 }
 
-// The distance to the nearest key of a row's range: biases are taken relative to
-// that key's, which changes every score of the row by the same amount, so that far
-// rows do not lose their scores' last bits in the size of the bias.
-__device__ __forceinline__ int64_t nearest(const RowRange& r) {
-    return r.at < r.lo ? r.lo - r.at : r.at >= r.hi ? r.at - (r.hi - 1) : 0;
+// y[i] = tanh(y[i]). tanh y = y + y z P(z), z = y^2, P of degree 4 for |y| up to 0.6,
+// where scores well inside their cap lie (the least largest relative error of that form:
+// 0.05 * 2^-24); 1 - 2 / (1 + e^(2 |y|)) past it, where a wave has such.
+template <int N, class V>
+__device__ __forceinline__ void tanh_all(V& y) {
+    float most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) most = fmaxf(most, fabsf(y[i]));
+    const bool far = __any(most > 0.6f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float x = y[i], z = x * x;
+        float p = fmaf(z, -0.00589516f, 0.02079597f);
+        p = fmaf(z, p, -0.05378383f);
+        p = fmaf(z, p, 0.13331924f);
+        p = fmaf(z, p, -0.33333298f);
+        float t = fmaf(x * z, p, x);
+        if (far) {
+            const float e = __builtin_amdgcn_exp2f(fabsf(x) * (2.0f * kLog2e));
+            const float big = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+            t = fabsf(x) > 0.6f ? copysignf(big, x) : t;
+        }
+        y[i] = t;
+    }
 }
+
+// What is added to a product to get a score, by what a call asks for.
+enum { kPlain = 0, kBias = 1, kCap = 2 };  // kCap: with a bias, too (of slope 0 if none)
+
+// The kernels of masked_attention_tile.hip.
+void masked_tile_forward(const MaskedArgs& a, unsigned blocks);
+// The rows' statistics and ranges, then what is asked for of dq and dk, dv.
+void masked_tile_backward(const MaskedArgs& a);
 
 }  // namespace nrs

@@ -1,0 +1,98 @@
+// Which kernels take a masked attention call, how long walks are cut into parts, and
+// the scratch that this needs: by the sizes alone. Host only and free of HIP.
+#pragma once
+
+#include "cross_attention_plan.hpp"
+
+namespace nrs {
+
+// A unit is an unbroken set of an item's rows (or keys, in the backward) that a
+// workgroup holds; its walk is the tiles of the other side that any of them sees.
+// How many these are, only the device knows. A walk is cut into parts of `part` tiles,
+// from its own first tile on, each a workgroup's; the grid has `parts` of them for
+// every unit, and those that a unit does not need end at once.
+struct MaskedWalk {
+    int64_t units = 0;
+    int part = 1, parts = 1;
+};
+
+// Parts no longer than `share` tiles (at least `least`) of walks of up to `tiles`.
+inline void cut_walk(MaskedWalk& w, int64_t tiles, int64_t share, int64_t least) {
+    const int64_t part = std::max<int64_t>(1, std::min(tiles, std::max(share, least)));
+    w.part = (int)part;
+    w.parts = (int)std::max<int64_t>(1, (tiles + part - 1) / part);
+}
+
+struct MaskedForwardPlan {
+    bool tiles;  // the kernel of many rows
+    int unit_rows;
+    MaskedWalk walk;
+    size_t part, stats, counts;  // scratch, in 4-byte words
+    size_t bytes() const { return 4 * (part + stats + counts); }
+    int64_t blocks() const { return walk.units * walk.parts; }
+};
+
+inline MaskedForwardPlan plan_masked_forward(int64_t batch, int64_t heads, int64_t kv_heads,
+                                             int64_t seq_q, int64_t seq_k, int64_t d_head,
+                                             int64_t cus) {
+    const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads;
+    MaskedForwardPlan p{R > kFewRows, 16, {}, 0, 0, 0};
+    if (items == 0 || R == 0) return p;
+    int64_t tiles, at_once;
+    if (p.tiles) {
+        // 256 rows to a workgroup when there are two such ones for every compute unit
+        p.unit_rows = items * ((R + 255) / 256) >= 2 * cus ? 256 : 128;
+        const int64_t keys = cross_tile_keys((int)d_head, p.unit_rows / 32);
+        tiles = (seq_k + keys - 1) / keys;
+        at_once = p.unit_rows == 128 && d_head <= 96 ? 2 * cus : cus;
+    } else {
+        tiles = (seq_k + 15) / 16;
+        at_once = (d_head > 64 ? 1 : d_head > 32 ? 3 : 6) * cus;
+    }
+    p.walk.units = items * ((R + p.unit_rows - 1) / p.unit_rows);
+    // half a workgroup's even share of the tiles of an unmasked call (a causal one has
+    // half as many): the longest part ends no later than the others' sum
+    cut_walk(p.walk, tiles, p.walk.units * tiles / (2 * at_once), 8);
+    if (p.walk.parts > 1) {
+        const int64_t rows = p.walk.parts * p.walk.units * p.unit_rows;
+        p.part = (size_t)((rows * d_head + 3) / 4 * 4);
+        p.stats = (size_t)(2 * rows);
+        p.counts = (size_t)p.walk.units;
+    }
+    return p;
+}
+
+struct MaskedBackwardPlan {
+    MaskedWalk q, kv;
+    int64_t row_tiles;  // tiles of rows that a walk of dk and dv meets, of an item
+    // scratch, in 4-byte words: rows' log sums and deltas, queries' ranges, tiles' ends,
+    // the gradients' parts and their counts
+    size_t rows, ranges, ends, q_part, kv_part, counts;
+    size_t bytes() const { return 4 * (rows + ranges + ends + q_part + 2 * kv_part + counts); }
+};
+
+inline MaskedBackwardPlan plan_masked_backward(int64_t batch, int64_t heads, int64_t kv_heads,
+                                               int64_t seq_q, int64_t seq_k, int64_t d_head,
+                                               int64_t cus) {
+    const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads;
+    MaskedBackwardPlan p{};
+    const int64_t tile = cross_tile_keys((int)d_head, 8), own = kCrossBackwardRows;
+    p.row_tiles = (R + tile - 1) / tile;
+    const int64_t key_tiles = (seq_k + tile - 1) / tile;
+    p.rows = (size_t)((2 * items * R + 3) / 4 * 4);
+    p.ranges = (size_t)(4 * batch * seq_q);
+    p.ends = (size_t)(4 * batch * p.row_tiles);
+    p.q.units = items * ((R + own - 1) / own);
+    p.kv.units = items * ((seq_k + own - 1) / own);
+    // A step of dq is three products a tile, one of dk and dv four. Asked for both
+    // gradients or not, the plan is that of both: each has the same bits by itself.
+    const int64_t even = (3 * p.q.units * key_tiles + 4 * p.kv.units * p.row_tiles) / cus;
+    cut_walk(p.q, key_tiles, even / 6, 8);
+    cut_walk(p.kv, p.row_tiles, even / 8, 8);
+    if (p.q.parts > 1) p.q_part = (size_t)((p.q.parts * items * R * d_head + 3) / 4 * 4);
+    if (p.kv.parts > 1) p.kv_part = (size_t)((p.kv.parts * items * seq_k * d_head + 3) / 4 * 4);
+    p.counts = (size_t)((p.q.units + p.kv.units + 3) / 4 * 4);
+    return p;
+}
+
+}  // namespace nrs
