@@ -120,12 +120,16 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_t
         k.template load<false>(a, a.k, a.ld_kv, b, kv, t * C::KT, n);
         v.template load<false>(a, a.v, a.ld_kv, b, kv, t * C::KT, n);
     };
+    // From the last tile down: in a causal call a row's nearest keys come first, whose
+    // scores a bias by distance makes the largest, and the reference stays
+    // near the maximum; from the first tile up, it lagged by up to 2^8, and the rounding
+    // of scores that far above it cost 0.9e-6 of the result in place of 0.2e-6.
     auto store = [&](int t) {
-        const int buf = (t - t0) & 1;
+        const int buf = (t1 - 1 - t) & 1;
         store_marked(k, a, lds[buf], marks[buf], t + 1);
         store_marked(v, a, lds[buf] + C::SET, marks[buf], t + 1);
     };
-    if (t0 < t1) load(t0);
+    if (t0 < t1) load(t1 - 1);
     const int s = live ? row - s_row * a.G : 0;
     const float slope2 = MODE != kPlain && a.slopes ? a.slopes[kv * a.G + s] * kLog2e : 0.0f;
     u32x4 qf[C::NS][3];
@@ -137,14 +141,14 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_t
     float m = 0.0f, l = 0.0f;
     bool fresh = true;  // no key seen yet
     if (t0 < t1) {
-        store(t0);
-        if (t0 + 1 < t1) load(t0 + 1);
+        store(t1 - 1);
+        if (t0 + 1 < t1) load(t1 - 2);
         __syncthreads();
     }
-    for (int t = t0; t < t1; ++t) {
-        const u32x4* const kl = lds[(t - t0) & 1];
+    for (int t = t1 - 1; t >= t0; --t) {
+        const u32x4* const kl = lds[(t1 - 1 - t) & 1];
         const u32x4* const vl = kl + C::SET;
-        const int* const mark = marks[(t - t0) & 1];
+        const int* const mark = marks[(t1 - 1 - t) & 1];
         const int k0 = t * C::KT;
         if (k0 < seen.most && k0 + C::KT > seen.least) {
             f32x16 p[C::NB];
@@ -209,11 +213,11 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_t
                     add_transposed<C>(acc, vl, kb, u, pieces, lane);
                 }
         }
-        if (t + 1 < t1) {
-            // the other buffer was last read in step t - 1, which every wave
+        if (t > t0) {
+            // the other buffer was last read in step t + 1, which every wave
             // had left before the barrier that ended it
-            store(t + 1);
-            if (t + 2 < t1) load(t + 2);
+            store(t - 1);
+            if (t - 1 > t0) load(t - 2);
             __syncthreads();
         }
     }
