@@ -436,8 +436,8 @@ int nrs_masked_attention_backward(float *dq, float *dk, float *dv, const float *
  * freq[j] (taken in 64 bits):
  *   (a, b) -> (a cos - b sin, b cos + a sin)
  * (a, b) are columns j and pairs + j of the head, or 2j and 2j + 1 if interleaved.
- * The other columns, and pairs whose axis is outside [0, axes), are copied. positions
- * [axes, rows] (any sign), freq [pairs], axis [pairs] (NULL: all 0) are on the device.
+ * The other columns are copied, and pairs whose axis is outside [0, axes) turned by zero.
+ * positions [axes, rows] (any sign), freq [pairs], axis [pairs] (NULL: all 0) are on the device.
  * The queries and keys of one projection are turned together as heads side by side.
  * out may be x, with the same stride; else they must not overlap. Strides are at most
  * 2^20 floats, rows 2^30, and rows * heads * ceil(d_head / 8) about 2^31.            */
