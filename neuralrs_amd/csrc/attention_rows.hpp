@@ -160,4 +160,23 @@ struct Joined {
     }
 };
 
+// The parts of row r of an item: their number (0: no key is seen by its unit) and where in rows
+// of `part` each one is.
+struct RowParts {
+    int n = 0, unit_rows, begun = 0, line = 0;  // the rows of part 0, and of one before part 1
+    __device__ __forceinline__ RowParts(const CrossArgs& a, int item, int r, bool any)
+        : unit_rows(a.unit_rows) {
+        if (!any) return;
+        const int units = (a.Sq * a.G + unit_rows - 1) / unit_rows, in_item = r / unit_rows;
+        const int unit = item * units + in_item, first = a.shares[2 * unit];
+        n = a.shares[2 * unit + 1] - first + 1;
+        const int in_unit = r - in_item * unit_rows;
+        begun = begun_slot(a, unit, first) * unit_rows + in_unit;
+        line = first * unit_rows + in_unit;
+    }
+    __device__ __forceinline__ int64_t at(int s) const {
+        return s == 0 ? begun : line + s * unit_rows;
+    }
+};
+
 }  // namespace nrs

@@ -149,25 +149,6 @@ __global__ __launch_bounds__(64 * kRowWaves) void cross_rows_fwd_kernel(CrossArg
                  part.slot(a));
 }
 
-// The parts of row r of an item: their number (0: no live keys) and where in rows
-// of `part` each one is.
-struct RowParts {
-    int n = 0, unit_rows, begun = 0, line = 0;  // the rows of part 0, and of one before part 1
-    __device__ __forceinline__ RowParts(const CrossArgs& a, int item, int b, int r)
-        : unit_rows(a.unit_rows) {
-        if (live_keys(a, b) == 0) return;
-        const int units = (a.Sq * a.G + unit_rows - 1) / unit_rows, in_item = r / unit_rows;
-        const int unit = item * units + in_item, first = a.shares[2 * unit];
-        n = a.shares[2 * unit + 1] - first + 1;
-        const int in_unit = r - in_item * unit_rows;
-        begun = begun_slot(a, unit, first) * unit_rows + in_unit;
-        line = first * unit_rows + in_unit;
-    }
-    __device__ __forceinline__ int64_t at(int s) const {
-        return s == 0 ? begun : line + s * unit_rows;
-    }
-};
-
 // Joins the parts of cross_rows_fwd_kernel, a workgroup to a row: eight groups of
 // 32 threads take an eighth of them each and are added up in LDS: 4.8 us for 64
 // rows of 17 parts, a launch and its round trips.
@@ -177,7 +158,7 @@ __global__ __launch_bounds__(256) void cross_rows_join_kernel(CrossArgs a) {
     const int x = threadIdx.x % 32, group = threadIdx.x / 32, R = a.Sq * a.G;
     const int item = blockIdx.x / R, r = blockIdx.x - item * R, b = item / a.KV;
     const int live = max(0, min(4, a.D - 4 * x));
-    const RowParts parts(a, item, b, r);
+    const RowParts parts(a, item, r, live_keys(a, b) > 0);
     if (parts.n == 1) return;  // one workgroup took all of the unit
     Joined<32> sum;
     sum.add(parts.n * group / 8, parts.n * (group + 1) / 8, live,
@@ -212,7 +193,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
     if (row >= (int64_t)a.B * a.KV * R) return;
     const int item = (int)(row / R), r = (int)(row - (int64_t)item * R), b = item / a.KV;
     const int live = max(0, min(4, a.D - 4 * x));
-    const RowParts parts(a, item, b, r);
+    const RowParts parts(a, item, r, live_keys(a, b) > 0);
     if (parts.n == 1) return;
     Joined<LANES> sum;
     sum.add(0, parts.n, live, [&](int s) { return a.part_stats + 2 * parts.at(s); },

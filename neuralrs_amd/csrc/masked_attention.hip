@@ -8,214 +8,359 @@
 namespace nrs {
 namespace {
 
+// All that any query of an item sees, least .. most - 1 (0 .. -1: nothing).
+struct Span {
+    int least, most;
+    __device__ __forceinline__ int first() const { return least / 16; }
+    __device__ __forceinline__ int tiles() const {
+        return most > 0 ? (most + 15) / 16 - least / 16 : 0;
+    }
+};
+
+__device__ __forceinline__ Span item_span(const MaskedArgs& a, int b) {
+    Span all{INT32_MAX, 0};
+    for (int s = 0; s < a.Sq; ++s) {
+        const RowRange r = row_range(a, b, s);
+        if (r.hi > 0) all.least = min(all.least, r.lo);
+        all.most = max(all.most, r.hi);
+    }
+    return all;
+}
+
+// A workgroup's part of the line of all items' tiles of 16 keys, as LinePart
+// (cross_attention.hpp): there an item's tiles are those of its length, here those that
+// any of its queries sees.
+template <int NT>
+struct SpanLine {
+    Span* spans;  // of all items, in shared memory
+    int b, base, p, end, per_item;
+    int sub, t0, t1, tiles;  // of the piece at hand: tiles t0 .. t1 - 1, from the span's first
+
+    // False if the part is empty. All NT threads call it; `scan` and `found` are shared.
+    __device__ __forceinline__ bool begin(const MaskedArgs& a, int per_item_, int (&scan)[NT / 64],
+                                          int (&found)[2]) {
+        per_item = per_item_;
+        const int t = threadIdx.x, lane = t & 63, w = t >> 6, each = (a.B + NT - 1) / NT;
+        int own = 0;
+        for (int i = t * each; i < min((t + 1) * each, a.B); ++i) {
+            spans[i] = item_span(a, i);
+            own += spans[i].tiles() * per_item;
+        }
+        int upto = own;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int v = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += v;
+        }
+        if (lane == 63) scan[w] = upto;
+        __syncthreads();
+        int at = upto - own, total = 0;
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) {
+            at += i < w ? scan[i] : 0;
+            total += scan[i];
+        }
+        // a tile to a workgroup at least, so that those that share a unit follow each other
+        const int parts = min(a.groups, total);
+        if ((int)blockIdx.x >= parts) return false;
+        p = (int)((int64_t)total * blockIdx.x / parts);
+        end = (int)((int64_t)total * (blockIdx.x + 1) / parts);
+        for (int i = t * each; i < min((t + 1) * each, a.B); ++i) {
+            const int n = spans[i].tiles() * per_item;
+            if (at <= p && p < at + n) {
+                found[0] = i;
+                found[1] = at;
+            }
+            at += n;
+        }
+        __syncthreads();
+        b = found[0];
+        base = found[1];
+        return true;
+    }
+    __device__ __forceinline__ bool next(const MaskedArgs& a) {
+        if (p >= end) return false;
+        for (;;) {  // (items that see nothing have no tiles)
+            tiles = __builtin_amdgcn_readfirstlane(spans[b].tiles());
+            if (p < base + tiles * per_item) break;
+            base += tiles * per_item;
+            ++b;
+        }
+        sub = (p - base) / tiles;
+        t0 = p - base - sub * tiles;
+        t1 = min(tiles, t0 + end - p);
+        p += t1 - t0;
+        const int unit = b * per_item + sub;
+        if (threadIdx.x == 0) {
+            if (t0 == 0) a.shares[2 * unit] = blockIdx.x;
+            if (t1 == tiles) a.shares[2 * unit + 1] = blockIdx.x;
+        }
+        return true;
+    }
+    // Where the piece's sums go: -1 if it is all of its unit.
+    __device__ __forceinline__ int64_t slot(const MaskedArgs& a) const {
+        if (t0 > 0) return blockIdx.x;
+        return t1 == tiles ? -1 : begun_slot(a, b * per_item + sub, blockIdx.x);
+    }
+};
+
 // Few rows (tokens being decoded): K and V stream from memory once, straight into
-// registers, as operands of v_mfma_f32_16x16x4_f32. A unit is 16 rows of an item, a
-// workgroup has a part of its keys, and its waves take turns at tiles of 16 keys, each
-// with its next tile on the way.
+// registers, as operands of v_mfma_f32_16x16x4_f32. A unit is 16 rows of an item; a
+// workgroup's waves take turns at tiles of 16 keys, each with its next tile on the way,
+// and are joined at the end.
+template <int NJ, int MODE>
+struct MaskedRows {
+    const MaskedArgs& a;
+    float (&sums)[kRowWaves][4 * NJ][64];
+    float (&tops)[kRowWaves][16];
+    float (&totals)[kRowWaves][16];
+
+    // Tiles t0 .. t1 - 1 of the rows from r0 on of (b, kv), whose item sees `span`: all of
+    // them (slot < 0) or a part.
+    __device__ __forceinline__ void run(int b, int kv, int r0, Span span, int t0, int t1,
+                                        int64_t slot) const {
+        const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+        const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int R = a.Sq * a.G, most = __builtin_amdgcn_readfirstlane(span.most);
+        f32x4 qf[NJ], acc[NJ], kf[NJ];
+        float vf[4][NJ];
+        auto load_keys = [&](int t) {
+            Rows<false>(a, a.k, b, kv, a.ld_kv, 16 * t, min(16, most - 16 * t))
+                .template along<NJ>(kf, c, g);
+        };
+        auto load_values = [&](int t) {
+            const Rows<false> vs(a, a.v, b, kv, a.ld_kv, 16 * t, min(16, most - 16 * t));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) vs.template across<NJ>(vf[r], 4 * g + r, c);
+        };
+        if (t0 + w < t1) {
+            load_keys(t0 + w);
+            load_values(t0 + w);
+        }
+        const bool live = r0 + c < R;
+        const int s_row = live ? (r0 + c) / a.G : 0;
+        RowRange range = row_range(a, b, s_row);
+        if (!live) range.lo = range.hi = range.at = 0;
+        // what all rows see
+        int from = !live ? 0 : range.hi > 0 ? range.lo : INT32_MAX, to = live ? range.hi : INT32_MAX;
+#pragma unroll
+        for (int i = 1; i < 16; i *= 2) {
+            from = max(from, __shfl_xor(from, i, 64));
+            to = min(to, __shfl_xor(to, i, 64));
+        }
+        const float slope2 = MODE != kPlain && a.slopes && live
+                                 ? a.slopes[kv * a.G + r0 + c - s_row * a.G] * kLog2e
+                                 : 0.0f;
+        Rows<true>(a, a.q, b, kv, a.ld_q, r0, min(16, R - r0)).template along<NJ>(qf, c, g);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            qf[j] = qf[j] * a.scale_own;
+            acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        float m = -INFINITY, l = 0.0f;
+        for (int t = t0 + w; t < t1; t += kRowWaves) {
+            f32x4 p = dot_rows<NJ>(kf, qf);
+            if (t + kRowWaves < t1) load_keys(t + kRowWaves);
+            if (MODE == kCap) {
+                tanh_all<4>(p);
+                p = p * a.cap2;
+            }
+            if (MODE != kPlain) {
+                const float far = (float)(range.at - (16 * t + 4 * g));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[r] = fmaf(-slope2, fabsf(far - (float)r), p[r]);
+            }
+            if (16 * t < from || 16 * t + 16 > to) {
+                // a value that is not finite must not meet the weight 0 of a row that does
+                // not see it: the key gets zeros, and a NaN for a score
+                int bad = 0;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float most_v = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+                        if (c * NJ + j < a.D)
+                            most_v = __builtin_elementwise_maximum(most_v, __builtin_fabsf(vf[r][j]));
+                    bad |= most_v < INFINITY ? 0 : 1 << r;
+                }
+#pragma unroll
+                for (int i = 1; i < 16; i *= 2) bad |= __shfl_xor(bad, i, 64);
+                const uint32_t keys = range.hi - range.lo;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (bad >> r & 1) {
+                        p[r] = NAN;
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) vf[r][j] = 0.0f;
+                    }
+                    p[r] = (uint32_t)(16 * t + 4 * g + r - range.lo) < keys ? p[r] : -INFINITY;
+                }
+            }
+            float top = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), m);
+            const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+            m = top;
+            l *= alpha;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[j] = acc[j] * alpha;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[r] = p[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[r] - m);
+                l += p[r];
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[j] = mfma16(vf[r][j], p[r], acc[j]);
+            }
+            if (t + kRowWaves < t1) load_values(t + kRowWaves);
+        }
+        l = across_groups(l);
+        if (g == 0) {
+            tops[w][c] = m;
+            totals[w][c] = l;
+        }
+        __syncthreads();
+        float top = tops[0][c];
+#pragma unroll
+        for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, tops[i][c]);
+        const float f = Joined<32>::weight(m, l, top);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) sums[w][r * NJ + j][lane] = acc[j][r] * f;
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRowWaves; ++i) {
+            const float of = Joined<32>::weight(tops[i][c], totals[i][c], top);
+            total += totals[i][c] * of;
+        }
+        __syncthreads();
+        if (live) {
+            // wave w adds the waves' register w: NJ neighbouring columns of row c
+            static_assert(kRowWaves == 4, "a register of an accumulator to each wave");
+            const bool whole = slot < 0, none = total == 0.0f;
+            const float scale = !whole ? 1.0f : none ? 0.0f : 1.0f / total;
+            const int64_t at = slot * a.unit_rows + c;
+            float* dst = whole ? a.out + query_offset(a, b, kv, r0 + c, a.ld_out) : a.part + at * a.D;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                float v = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kRowWaves; ++i) v += sums[i][w * NJ + j][lane];
+                const int d = (4 * g + w) * NJ + j;
+                if (d < a.D) dst[d] = v * scale;
+            }
+            if (w == 0 && g == 0 && (!whole || a.stats)) {
+                float* st = whole ? row_stats(a, b, kv, r0 + c) : a.part_stats + 2 * at;
+                st[0] = whole && none ? 0.0f : top;
+                st[1] = total;
+            }
+        }
+        __syncthreads();  // before the shared arrays serve the next unit
+    }
+};
+
 template <int NJ, int MODE>
 __global__ __launch_bounds__(64 * kRowWaves) void masked_rows_fwd_kernel(MaskedArgs a) {
-    static_assert(kRowWaves == 4, "a register of an accumulator to each wave");
     __shared__ float sums[kRowWaves][4 * NJ][64];
     __shared__ float tops[kRowWaves][16], totals[kRowWaves][16];
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int R = a.Sq * a.G, row_tiles = (R + 15) / 16;
-    const int unit = blockIdx.x % a.units, no = blockIdx.x / a.units;
-    const int item = unit / row_tiles, r0 = unit % row_tiles * 16;
-    const int b = item / a.KV, kv = item - b * a.KV;
-    const bool live = r0 + c < R;
-    const int s_row = live ? (r0 + c) / a.G : 0;
-    RowRange range = row_range(a, b, s_row);
-    if (!live) range.lo = range.hi = range.at = 0;
-    int least = live && range.hi > 0 ? range.lo : INT32_MAX, most = range.hi;
-    int from = !live ? 0 : range.hi > 0 ? range.lo : INT32_MAX, to = live ? range.hi : INT32_MAX;
-#pragma unroll
-    for (int i = 1; i < 16; i *= 2) {
-        least = min(least, __shfl_xor(least, i, 64));
-        most = max(most, __shfl_xor(most, i, 64));
-        from = max(from, __shfl_xor(from, i, 64));
-        to = min(to, __shfl_xor(to, i, 64));
+    __shared__ int scan[kRowWaves], found[2];
+    __shared__ Span spans[kMaxSharedBatch];
+    const MaskedRows<NJ, MODE> walk{a, sums, tops, totals};
+    const int row_tiles = (a.Sq * a.G + 15) / 16, per_item = a.KV * row_tiles;
+    if (a.groups == 0) {
+        const int unit = blockIdx.x, b = unit / per_item, sub = unit - b * per_item;
+        const Span span = item_span(a, b);
+        walk.run(b, sub / row_tiles, sub % row_tiles * 16, span, span.most > 0 ? span.first() : 0,
+                 span.most > 0 ? span.first() + span.tiles() : 0, -1);
+        return;
     }
-    least = __builtin_amdgcn_readfirstlane(least);
-    most = __builtin_amdgcn_readfirstlane(most);
-    const int first = most > 0 ? least / 16 : 0, last = (most + 15) / 16;
-    const int used = max(1, (last - first + a.part_tiles - 1) / a.part_tiles);
-    if (no >= used) return;
-    if (a.parts > 1 && no == 0 && threadIdx.x == 0) a.counts[unit] = used;
-    const int t0 = first + no * a.part_tiles, t1 = min(last, t0 + a.part_tiles);
-    f32x4 qf[NJ], acc[NJ], kf[NJ];
-    float vf[4][NJ];
-    auto load_keys = [&](int t) {
-        Rows<false>(a, a.k, b, kv, a.ld_kv, 16 * t, min(16, most - 16 * t))
-            .template along<NJ>(kf, c, g);
-    };
-    auto load_values = [&](int t) {
-        const Rows<false> vs(a, a.v, b, kv, a.ld_kv, 16 * t, min(16, most - 16 * t));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) vs.template across<NJ>(vf[r], 4 * g + r, c);
-    };
-    if (t0 + w < t1) {
-        load_keys(t0 + w);
-        load_values(t0 + w);
-    }
-    const float slope2 =
-        MODE != kPlain && a.slopes && live ? a.slopes[kv * a.G + r0 + c - s_row * a.G] * kLog2e : 0.0f;
-    Rows<true>(a, a.q, b, kv, a.ld_q, r0, min(16, R - r0)).template along<NJ>(qf, c, g);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        qf[j] = qf[j] * a.scale_own;
-        acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int t = t0 + w; t < t1; t += kRowWaves) {
-        f32x4 p = dot_rows<NJ>(kf, qf);
-        if (t + kRowWaves < t1) load_keys(t + kRowWaves);
-        if (MODE == kCap) {
-            tanh_all<4>(p);
-            p = p * a.cap2;
-        }
-        if (MODE != kPlain) {
-            const float far = (float)(range.at - (16 * t + 4 * g));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) p[r] = fmaf(-slope2, fabsf(far - (float)r), p[r]);
-        }
-        if (16 * t < from || 16 * t + 16 > to) {
-            // a value that is not finite must not meet the weight 0 of a row that does not
-            // see it: the key gets zeros, and a NaN for a score
-            int bad = 0;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float most_v = 0.0f;
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-                    if (c * NJ + j < a.D)
-                        most_v = __builtin_elementwise_maximum(most_v, __builtin_fabsf(vf[r][j]));
-                bad |= most_v < INFINITY ? 0 : 1 << r;
-            }
-#pragma unroll
-            for (int i = 1; i < 16; i *= 2) bad |= __shfl_xor(bad, i, 64);
-            const uint32_t span = range.hi - range.lo;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if (bad >> r & 1) {
-                    p[r] = NAN;
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) vf[r][j] = 0.0f;
-                }
-                p[r] = (uint32_t)(16 * t + 4 * g + r - range.lo) < span ? p[r] : -INFINITY;
-            }
-        }
-        float top = fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]));
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(fmaxf(top, __shfl_xor(top, 32, 64)), m);
-        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-        m = top;
-        l *= alpha;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[j] = acc[j] * alpha;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            p[r] = p[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[r] - m);
-            l += p[r];
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) acc[j] = mfma16(vf[r][j], p[r], acc[j]);
-        }
-        if (t + kRowWaves < t1) load_values(t + kRowWaves);
-    }
-    l = across_groups(l);
-    if (g == 0) {
-        tops[w][c] = m;
-        totals[w][c] = l;
-    }
-    __syncthreads();
-    float top = tops[0][c];
-#pragma unroll
-    for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, tops[i][c]);
-    const float f = Joined<32>::weight(m, l, top);
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) sums[w][r * NJ + j][lane] = acc[j][r] * f;
-    float total = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kRowWaves; ++i) {
-        const float of = Joined<32>::weight(tops[i][c], totals[i][c], top);
-        total += totals[i][c] * of;
-    }
-    __syncthreads();
-    if (!live) return;
-    // wave w adds the waves' register w: NJ neighbouring columns of row c
-    const bool whole = used == 1, none = total == 0.0f;
-    const float scale = !whole ? 1.0f : none ? 0.0f : 1.0f / total;
-    const int64_t at = ((int64_t)no * a.units + unit) * 16 + c;
-    float* dst = whole ? a.out + query_offset(a, b, kv, r0 + c, a.ld_out) : a.part + at * a.D;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        float v = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kRowWaves; ++i) v += sums[i][w * NJ + j][lane];
-        const int d = (4 * g + w) * NJ + j;
-        if (d < a.D) dst[d] = v * scale;
-    }
-    if (w == 0 && g == 0 && (!whole || a.stats)) {
-        float* st = whole ? row_stats(a, b, kv, r0 + c) : a.part_stats + 2 * at;
-        st[0] = whole && none ? 0.0f : top;
-        st[1] = total;
+    SpanLine<64 * kRowWaves> line{spans};
+    if (!line.begin(a, per_item, scan, found)) return;
+    while (line.next(a)) {
+        const Span span = spans[line.b];
+        walk.run(line.b, line.sub / row_tiles, line.sub % row_tiles * 16, span,
+                 span.first() + line.t0, span.first() + line.t1, line.slot(a));
     }
 }
 
-// Joins the parts of a row: GROUPS groups of LANES threads (four columns each) take even
-// shares of them and are added up in LDS.
-template <int LANES, int GROUPS>
-__global__ __launch_bounds__(256) void masked_join_kernel(MaskedArgs a) {
-    constexpr int ROWS = 256 / (LANES * GROUPS);  // of a workgroup
-    __shared__ f32x4 sums[ROWS][GROUPS][LANES];
-    __shared__ float tops[ROWS][GROUPS], totals[ROWS][GROUPS];
-    const int x = threadIdx.x % LANES, group = threadIdx.x / LANES % GROUPS;
-    const int in = threadIdx.x / (LANES * GROUPS), R = a.Sq * a.G;
-    const int64_t row = (int64_t)blockIdx.x * ROWS + in;
-    const bool there = row < (int64_t)a.B * a.KV * R;
-    const int item = there ? (int)(row / R) : 0, r = there ? (int)(row - (int64_t)item * R) : 0;
-    const int b = item / a.KV, live = max(0, min(4, a.D - 4 * x));
-    const int unit = item * ((R + a.unit_rows - 1) / a.unit_rows) + r / a.unit_rows;
-    const int parts = there ? a.counts[unit] : 1;
-    // a group that is past the rows, or whose row one workgroup took whole, is idle; the
-    // others may wait for each other
-    Joined<LANES> sum;
-    auto at = [&](int s) { return ((int64_t)s * a.units + unit) * a.unit_rows + r % a.unit_rows; };
-    if (parts > 1)
-        sum.add(parts * group / GROUPS, parts * (group + 1) / GROUPS, live,
-                [&](int s) { return a.part_stats + 2 * at(s); },
-                [&](int s) { return a.part + at(s) * a.D; });
-    if (GROUPS > 1) {
-        sums[in][group][x] = sum.v;
-        if (x == 0) {
-            tops[in][group] = sum.top;
-            totals[in][group] = sum.total;
-        }
-        __syncthreads();
+// The parts of a row of the kernel of many rows: their number, and where each is.
+struct WalkParts {
+    int n, unit, units, unit_rows, in_unit;
+    __device__ __forceinline__ WalkParts(const MaskedArgs& a, int item, int r)
+        : unit(item * ((a.Sq * a.G + a.unit_rows - 1) / a.unit_rows) + r / a.unit_rows),
+          units(a.units), unit_rows(a.unit_rows), in_unit(r % a.unit_rows) {
+        n = a.counts[unit];
     }
-    if (parts == 1 || group != 0) return;
-    for (int i = 1; i < GROUPS; ++i) {
-        const float most = fmaxf(sum.top, tops[in][i]);
-        const float f = Joined<LANES>::weight(sum.top, sum.total, most),
-                    of = Joined<LANES>::weight(tops[in][i], totals[in][i], most);
-        sum.v = sum.v * f + sums[in][i][x] * of;
-        sum.total = sum.total * f + totals[in][i] * of;
-        sum.top = most;
+    __device__ __forceinline__ int64_t at(int s) const {
+        return ((int64_t)s * units + unit) * unit_rows + in_unit;
     }
+};
+
+template <int LANES>
+__device__ __forceinline__ void store_joined(const MaskedArgs& a, const Joined<LANES>& sum, int item,
+                                             int r, int live) {
+    const int x = threadIdx.x % LANES, b = item / a.KV, kv = item - b * a.KV;
     const bool none = sum.total == 0.0f;
     const float scale = none ? 0.0f : 1.0f / sum.total;
-    float* dst = a.out + query_offset(a, b, item - b * a.KV, r, a.ld_out) + 4 * x;
+    float* dst = a.out + query_offset(a, b, kv, r, a.ld_out) + 4 * x;
     if (live == 4)
         reinterpret_cast<Quad*>(dst)->v = sum.v * scale;
     else
         for (int e = 0; e < live; ++e) dst[e] = sum.v[e] * scale;
     if (a.stats && x == 0) {
-        float* st = row_stats(a, b, item - b * a.KV, r);
+        float* st = row_stats(a, b, kv, r);
         st[0] = none ? 0.0f : sum.top;
         st[1] = sum.total;
     }
+}
+
+// Joins the parts of masked_rows_fwd_kernel, which may be many, a workgroup to a row:
+// eight groups of 32 threads take an eighth of them each and are added up in LDS.
+__global__ __launch_bounds__(256) void masked_rows_join_kernel(MaskedArgs a) {
+    __shared__ f32x4 sums[8][32];
+    __shared__ float tops[8], totals[8];
+    const int x = threadIdx.x % 32, group = threadIdx.x / 32, R = a.Sq * a.G;
+    const int item = blockIdx.x / R, r = blockIdx.x - item * R;
+    const int live = max(0, min(4, a.D - 4 * x));
+    const RowParts parts(a, item, r, item_span(a, item / a.KV).most > 0);
+    if (parts.n == 1) return;  // one workgroup took all of the unit
+    Joined<32> sum;
+    sum.add(parts.n * group / 8, parts.n * (group + 1) / 8, live,
+            [&](int s) { return a.part_stats + 2 * parts.at(s); },
+            [&](int s) { return a.part + parts.at(s) * a.D; });
+    sums[group][x] = sum.v;
+    if (x == 0) {
+        tops[group] = sum.top;
+        totals[group] = sum.total;
+    }
+    __syncthreads();
+    if (group != 0) return;
+    for (int i = 1; i < 8; ++i) {
+        const float most = fmaxf(sum.top, tops[i]);
+        const float f = Joined<32>::weight(sum.top, sum.total, most),
+                    of = Joined<32>::weight(tops[i], totals[i], most);
+        sum.v = sum.v * f + sums[i][x] * of;
+        sum.total = sum.total * f + totals[i] * of;
+        sum.top = most;
+    }
+    store_joined(a, sum, item, r, live);
+}
+
+// Joins the parts of masked_tile_fwd_kernel, which are few: D / 4 threads to a row.
+template <int D>
+__global__ __launch_bounds__(256) void masked_join_kernel(MaskedArgs a) {
+    constexpr int LANES = D / 4;
+    const int R = a.Sq * a.G, x = threadIdx.x % LANES;
+    const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    if (row >= (int64_t)a.B * a.KV * R) return;
+    const int item = (int)(row / R), r = (int)(row - (int64_t)item * R);
+    const int live = max(0, min(4, a.D - 4 * x));
+    const WalkParts parts(a, item, r);
+    if (parts.n == 1) return;
+    Joined<LANES> sum;
+    sum.add(0, parts.n, live, [&](int s) { return a.part_stats + 2 * parts.at(s); },
+            [&](int s) { return a.part + parts.at(s) * a.D; });
+    store_joined(a, sum, item, r, live);
 }
 
 // Adds the parts of a gradient in order: dst = f * sum + beta * dst, D / 4 threads to a
@@ -270,7 +415,7 @@ void launch_sums(const MaskedArgs& a, bool dq, bool dkv) {
 template <int D>
 void launch_join(const MaskedArgs& a, int64_t rows) {
     constexpr int PER = 1024 / D;
-    hipLaunchKernelGGL((masked_join_kernel<D / 4, 1>), dim3((unsigned)((rows + PER - 1) / PER)),
+    hipLaunchKernelGGL(masked_join_kernel<D>, dim3((unsigned)((rows + PER - 1) / PER)),
                        dim3(256), 0, stream(), a);
 }
 
@@ -383,28 +528,31 @@ int nrs_masked_attention_forward(float* out, float* stats, const float* q, const
     a.units = (int)plan.walk.units;
     a.part_tiles = plan.walk.part;
     a.parts = plan.walk.parts;
+    a.groups = plan.line.groups;
+    a.few_units = plan.line.few_units;
     a.part = scratch;
     a.part_stats = scratch + plan.part;
-    a.counts = reinterpret_cast<int32_t*>(scratch + plan.part + plan.stats);
+    a.shares = a.counts = reinterpret_cast<int32_t*>(scratch + plan.part + plan.stats);
     const unsigned blocks = (unsigned)plan.blocks();
-    if (plan.tiles)
+    const int64_t rows = batch * heads * seq_q;
+    if (plan.tiles) {
         nrs::masked_tile_forward(a, blocks);
-    else
+        NRS_LAUNCH_CHECK(what);
+        const int width = nrs::cross_row_width(a.D);
+        if (a.parts > 1)
+            (width == 32   ? nrs::launch_join<32>
+             : width == 64 ? nrs::launch_join<64>
+                           : nrs::launch_join<128>)(a, rows);
+    } else {
         (a.D <= 16   ? nrs::launch_rows<1>
          : a.D <= 32 ? nrs::launch_rows<2>
          : a.D <= 64 ? nrs::launch_rows<4>
                      : nrs::launch_rows<8>)(a, blocks);
-    NRS_LAUNCH_CHECK(what);
-    if (a.parts == 1) return NRS_OK;
-    const int64_t rows = batch * heads * seq_q;
-    const int width = nrs::cross_row_width(a.D);
-    if (!plan.tiles)  // many parts of few rows
-        hipLaunchKernelGGL((nrs::masked_join_kernel<32, 8>), dim3((unsigned)rows), dim3(256), 0,
-                           nrs::stream(), a);
-    else
-        (width == 32   ? nrs::launch_join<32>
-         : width == 64 ? nrs::launch_join<64>
-                       : nrs::launch_join<128>)(a, rows);
+        NRS_LAUNCH_CHECK(what);
+        if (a.groups > 0)
+            hipLaunchKernelGGL(nrs::masked_rows_join_kernel, dim3((unsigned)rows), dim3(256), 0,
+                               nrs::stream(), a);
+    }
     NRS_LAUNCH_CHECK(what);
     return NRS_OK;
 }

@@ -26,29 +26,32 @@ inline void cut_walk(MaskedWalk& w, int64_t tiles, int64_t share, int64_t least)
 struct MaskedForwardPlan {
     bool tiles;  // the kernel of many rows
     int unit_rows;
-    MaskedWalk walk;
-    size_t part, stats, counts;  // scratch, in 4-byte words
+    MaskedWalk walk;             // of many rows
+    CrossForwardPlan line;       // of few, whose tiles are shared as cross attention's are
+    size_t part, stats, counts;  // scratch, in 4-byte words (counts, or the line's shares)
     size_t bytes() const { return 4 * (part + stats + counts); }
-    int64_t blocks() const { return walk.units * walk.parts; }
+    int64_t blocks() const { return tiles ? walk.units * walk.parts : line.blocks; }
 };
 
 inline MaskedForwardPlan plan_masked_forward(int64_t batch, int64_t heads, int64_t kv_heads,
                                              int64_t seq_q, int64_t seq_k, int64_t d_head,
                                              int64_t cus) {
     const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads;
-    MaskedForwardPlan p{R > kFewRows, 16, {}, 0, 0, 0};
+    MaskedForwardPlan p{R > kFewRows, 16, {}, {}, 0, 0, 0};
     if (items == 0 || R == 0) return p;
-    int64_t tiles, at_once;
-    if (p.tiles) {
-        // 256 rows to a workgroup when there are two such ones for every compute unit
-        p.unit_rows = items * ((R + 255) / 256) >= 2 * cus ? 256 : 128;
-        const int64_t keys = cross_tile_keys((int)d_head, p.unit_rows / 32);
-        tiles = (seq_k + keys - 1) / keys;
-        at_once = p.unit_rows == 128 && d_head <= 96 ? 2 * cus : cus;
-    } else {
-        tiles = (seq_k + 15) / 16;
-        at_once = (d_head > 64 ? 1 : d_head > 32 ? 3 : 6) * cus;
+    if (!p.tiles) {
+        p.line = plan_cross_forward(batch, heads, kv_heads, seq_q, seq_k, d_head, cus);
+        p.unit_rows = p.line.unit_rows;
+        p.part = p.line.part;
+        p.stats = p.line.stats;
+        p.counts = p.line.shares;
+        return p;
     }
+    // 256 rows to a workgroup when there are two such ones for every compute unit
+    p.unit_rows = items * ((R + 255) / 256) >= 2 * cus ? 256 : 128;
+    const int64_t keys = cross_tile_keys((int)d_head, p.unit_rows / 32);
+    const int64_t tiles = (seq_k + keys - 1) / keys;
+    const int64_t at_once = p.unit_rows == 128 && d_head <= 96 ? 2 * cus : cus;
     p.walk.units = items * ((R + p.unit_rows - 1) / p.unit_rows);
     // half a workgroup's even share of the tiles of an unmasked call (a causal one has
     // half as many): the longest part ends no later than the others' sum
