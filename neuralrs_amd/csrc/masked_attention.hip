@@ -374,7 +374,7 @@ __global__ __launch_bounds__(256) void masked_sum_kernel(MaskedArgs a) {
     if (at >= rows) return;
     const int item = (int)(at / n), r = (int)(at - (int64_t)item * n);
     const int b = item / a.KV, kv = item - b * a.KV;
-    const int unit = item * ((n + kCrossBackwardRows - 1) / kCrossBackwardRows) + r / kCrossBackwardRows;
+    const int own = 16 * masked_backward_waves(a.D), unit = item * ((n + own - 1) / own) + r / own;
     const int parts = (KEYS ? a.counts : a.q_counts)[unit];
     if (parts == 1) return;  // one workgroup took all of it
     const bool second = KEYS && blockIdx.y == 1;

@@ -47,15 +47,23 @@ inline MaskedForwardPlan plan_masked_forward(int64_t batch, int64_t heads, int64
         p.counts = p.line.shares;
         return p;
     }
-    // 256 rows to a workgroup when there are two such ones for every compute unit
-    p.unit_rows = items * ((R + 255) / 256) >= 2 * cus ? 256 : 128;
+    // 256 rows to a workgroup when an unmasked call has 64 steps of such a one for every
+    // compute unit, else 128
+    const int64_t steps =
+        items * ((R + 255) / 256) * ((seq_k * cross_tile_width((int)d_head) + 4095) / 4096);
+    p.unit_rows = R > 128 && steps >= 64 * cus ? 256 : 128;
     const int64_t keys = cross_tile_keys((int)d_head, p.unit_rows / 32);
     const int64_t tiles = (seq_k + keys - 1) / keys;
     const int64_t at_once = p.unit_rows == 128 && d_head <= 96 ? 2 * cus : cus;
     p.walk.units = items * ((R + p.unit_rows - 1) / p.unit_rows);
-    // half a workgroup's even share of the tiles of an unmasked call (a causal one has
-    // half as many): the longest part ends no later than the others' sum
-    cut_walk(p.walk, tiles, p.walk.units * tiles / (2 * at_once), 8);
+    // The longest part is half a workgroup's even share of the tiles of an unmasked call (a
+    // causal one has half as many), so that it ends no later than the others' sum; the
+    // whole of it where units are more than the workgroups at once, as the longest begin
+    // first (4 x 3000 rows, 8 heads of 64, 384 on 256: 227 us, by halves 245; but 2 x 2000, 8 of
+    // 128, 256 on 256: 222 and 181); 1024 keys at least, which a join costs (4 x 1021, 16 of
+    // 64: whole walks 80 us, by halves of 512 keys 86).
+    cut_walk(p.walk, tiles, p.walk.units * tiles / (p.walk.units > at_once ? at_once : 2 * at_once),
+             1024 / keys);
     if (p.walk.parts > 1) {
         const int64_t rows = p.walk.parts * p.walk.units * p.unit_rows;
         p.part = (size_t)((rows * d_head + 3) / 4 * 4);
@@ -64,6 +72,9 @@ inline MaskedForwardPlan plan_masked_forward(int64_t batch, int64_t heads, int64
     }
     return p;
 }
+
+// Waves of a workgroup of the backward, 16 rows or keys each.
+constexpr int masked_backward_waves(int D) { return D > 96 ? 8 : 4; }
 
 struct MaskedBackwardPlan {
     MaskedWalk q, kv;
@@ -79,7 +90,9 @@ inline MaskedBackwardPlan plan_masked_backward(int64_t batch, int64_t heads, int
                                                int64_t cus) {
     const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads;
     MaskedBackwardPlan p{};
-    const int64_t tile = cross_tile_keys((int)d_head, 8), own = kCrossBackwardRows;
+    const int waves = masked_backward_waves((int)d_head);
+    const int64_t tile = cross_tile_keys((int)d_head, waves), own = 16 * waves;
+    const int64_t at_once = waves == 8 ? cus : 2 * cus;
     p.row_tiles = (R + tile - 1) / tile;
     const int64_t key_tiles = (seq_k + tile - 1) / tile;
     p.rows = (size_t)((2 * items * R + 3) / 4 * 4);
@@ -89,7 +102,7 @@ inline MaskedBackwardPlan plan_masked_backward(int64_t batch, int64_t heads, int
     p.kv.units = items * ((seq_k + own - 1) / own);
     // A step of dq is three products a tile, one of dk and dv four. Asked for both
     // gradients or not, the plan is that of both: each has the same bits by itself.
-    const int64_t even = (3 * p.q.units * key_tiles + 4 * p.kv.units * p.row_tiles) / cus;
+    const int64_t even = (3 * p.q.units * key_tiles + 4 * p.kv.units * p.row_tiles) / at_once;
     cut_walk(p.q, key_tiles, even / 6, 8);
     cut_walk(p.kv, p.row_tiles, even / 8, 8);
     if (p.q.parts > 1) p.q_part = (size_t)((p.q.parts * items * R * d_head + 3) / 4 * 4);

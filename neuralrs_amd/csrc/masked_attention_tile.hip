@@ -17,6 +17,21 @@ namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+// A wave's issue priority while it feeds the matrix cores, over that of the other wave on
+// its SIMD, which then takes the cycles between for its exponentials and splits (2 x 4000
+// rows of 16 heads of 128, training: 4198 us -> 3931; a prompt of 8192 rows of 32 heads:
+// 2818 -> 2730). ON: where that pays, not for heads up to 64 columns in the backward
+// (4 x 1021 of 16: 273 us -> 282) or a wave alone (a prompt of 2000: 152 -> 160).
+template <bool ON>
+__device__ __forceinline__ void priority(int level) {
+    if constexpr (ON) {
+        if (level)
+            __builtin_amdgcn_s_setprio(1);
+        else
+            __builtin_amdgcn_s_setprio(0);
+    }
+}
+
 // The least and the largest of 32 or 16 neighbouring lanes.
 template <int LANES>
 __device__ __forceinline__ int lanes_min(int x) {
@@ -152,6 +167,7 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_t
         const int k0 = t * C::KT;
         if (k0 < seen.most && k0 + C::KT > seen.least) {
             f32x16 p[C::NB];
+            priority<WAVES == 8>(1);
 #pragma unroll
             for (int kb = 0; kb < C::NB; ++kb) {
                 p[kb] = products<C>(kl, qf, kb, MODE == kCap ? all16(0.0f) : start, c, h);
@@ -162,6 +178,7 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_t
                 }
                 add_bias<MODE, 16>(p[kb], (float)(range.at - (k0 + kb * 32 + 4 * h)), slope2, place32);
             }
+            priority<WAVES == 8>(0);
             if (mark[C::KT] == t + 1) {
 #pragma unroll
                 for (int kb = 0; kb < C::NB; ++kb)
@@ -210,7 +227,9 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_t
                     }
                     u32x4 pieces[3];
                     split8(x, pieces);
+                    priority<WAVES == 8>(1);
                     add_transposed<C>(acc, vl, kb, u, pieces, lane);
+                    priority<WAVES == 8>(0);
                 }
         }
         if (t > t0) {
@@ -290,19 +309,19 @@ __global__ __launch_bounds__(256) void masked_prepare_kernel(MaskedArgs a, int r
 
 __device__ __forceinline__ constexpr int place16(int i) { return 16 * (i / 4) + i % 4; }
 
-// dq of 128 rows, 16 to a wave: P = 2^(score - lse), dS = P (v . dout - delta) and, with a
+// dq of a workgroup's rows, 16 to a wave: P = 2^(score - lse), dS = P (v . dout - delta) and, with a
 // cap, times 1 - tanh^2; dQ = scale * K^T dS.
-template <int D, bool FULL, int MODE>
-__device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, int (*marks)[TileCfg<D, 8>::KT + 1],
-                                               int (*shared_ends)[8], int block) {
-    using C = TileCfg<D, 8>;
+template <int D, int WAVES, bool FULL, int MODE>
+__device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, int (*marks)[TileCfg<D, WAVES>::KT + 1],
+                                               int (*shared_ends)[WAVES], int block) {
+    using C = TileCfg<D, WAVES>;
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int R = a.Sq * a.G, tiles = (R + 127) / 128, items = a.B * a.KV;
+    const int R = a.Sq * a.G, tiles = (R + 16 * WAVES - 1) / (16 * WAVES), items = a.B * a.KV;
     const int no = a.q_parts - 1 - block / a.q_units, place = block % a.q_units;
     const int item = place % items, tile = tiles - 1 - place / items;
     const int b = item / a.KV, kv = item - b * a.KV, unit = item * tiles + tile;
-    const int row = (tile * 8 + w) * 16 + c;
+    const int row = (tile * WAVES + w) * 16 + c;
     const bool live = row < R;
     const int s_row = live ? (int)fast_div((uint32_t)row, a.by_group) : 0;
     RowKeys range = a.ranges[(int64_t)b * a.Sq + s_row];
@@ -315,7 +334,7 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
     __syncthreads();
     int least = INT32_MAX, most = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < WAVES; ++i) {
         least = min(least, shared_ends[0][i]);
         most = max(most, shared_ends[1][i]);
     }
@@ -368,8 +387,10 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
                 s[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 dp[half] = f32x4{nd, nd, nd, nd};
             }
+            priority<(D > 64)>(1);
             products16<C, true>(s, kl, qf, kb, c, g);
             products16<C, false>(dp, kl + C::SET, gf, kb, c, g);
+            priority<(D > 64)>(0);
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = s[i / 4][i % 4];
@@ -400,7 +421,9 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
                 x[i] = __builtin_amdgcn_exp2f(x[i] + nl) * dp[i / 4][i % 4];
             u32x4 p[3];
             split8(x, p);
+            priority<(D > 64)>(1);
             add16<C>(acc, kl, kb, p, lane);
+            priority<(D > 64)>(0);
         }
         if (t + 1 < t1) {
             store(t + 1);
@@ -416,25 +439,25 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
         store16<C, FULL>(a.dq + query_offset(a, b, kv, row, a.ld_q), acc, a.scale, a.beta_q, a.D, g);
 }
 
-// dk and dv of 128 keys, 16 to a wave: the same P and dS with the rows met, dV = dO^T P,
+// dk and dv of a workgroup's keys, 16 to a wave: the same P and dS with the rows met, dV = dO^T P,
 // dK = scale * Q^T dS.
-template <int D, bool FULL, int MODE>
-__device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds, int (*marks)[TileCfg<D, 8>::KT + 1],
-                                                f32x4* starts, int (*shared_ends)[8], int block) {
-    using C = TileCfg<D, 8>;
+template <int D, int WAVES, bool FULL, int MODE>
+__device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds, int (*marks)[TileCfg<D, WAVES>::KT + 1],
+                                                f32x4* starts, int (*shared_ends)[WAVES], int block) {
+    using C = TileCfg<D, WAVES>;
     constexpr int ROWS = MODE == kPlain ? 4 : 6;  // -lse, -delta, lo, keys; place, slope
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int R = a.Sq * a.G, tiles = (a.Sk + 127) / 128, items = a.B * a.KV;
+    const int R = a.Sq * a.G, tiles = (a.Sk + 16 * WAVES - 1) / (16 * WAVES), items = a.B * a.KV;
     const int no = a.parts - 1 - block / a.units, place = block % a.units;
     const int item = place % items, tile = place / items;
     const int b = item / a.KV, kv = item - b * a.KV, unit = item * tiles + tile;
-    const int key0 = (tile * 8 + w) * 16, key = key0 + c;
+    const int key0 = (tile * WAVES + w) * 16, key = key0 + c;
     // the tiles of rows of which any sees a key of the workgroup
     const TileEnds* const ends = a.ends + (int64_t)b * a.row_tiles;
     int first = INT32_MAX, last = 0;
-    for (int t = threadIdx.x; t < a.row_tiles; t += 512)
-        if (ends[t].least < (tile + 1) * 128 && ends[t].most > tile * 128) {
+    for (int t = threadIdx.x; t < a.row_tiles; t += C::NT)
+        if (ends[t].least < (tile + 1) * 16 * WAVES && ends[t].most > tile * 16 * WAVES) {
             first = min(first, t);
             last = t + 1;
         }
@@ -446,7 +469,7 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < WAVES; ++i) {
         first = min(first, shared_ends[0][i]);
         last = max(last, shared_ends[1][i]);
     }
@@ -489,7 +512,7 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
             to[2 * C::KT] = __builtin_bit_cast(float, range.lo);
             to[3 * C::KT] = __builtin_bit_cast(float, range.hi - range.lo);
             if (MODE != kPlain) {
-                to[4 * C::KT] = (float)(range.at - tile * 128);
+                to[4 * C::KT] = (float)(range.at - tile * 16 * WAVES);
                 to[5 * C::KT] = slope * kLog2e;
             }
         }
@@ -524,8 +547,10 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
                     s[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                     dp[half] = st[C::KT / 4 + 4 * half];
                 }
+                priority<(D > 64)>(1);
                 products16<C, true>(s, ql, kf, rb, c, g);
                 products16<C, false>(dp, ql + C::SET, vf, rb, c, g);
+                priority<(D > 64)>(0);
                 float x[8], y[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -541,7 +566,7 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
                     }
                 }
                 if (MODE != kPlain) {
-                    const float place_key = (float)(key - tile * 128);
+                    const float place_key = (float)(key - tile * 16 * WAVES);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const f32x4 at = st[4 * C::KT / 4 + 4 * half], by = st[5 * C::KT / 4 + 4 * half];
@@ -581,9 +606,13 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
                 }
                 u32x4 p[3];
                 split8(x, p);
+                priority<(D > 64)>(1);
                 add16<C>(acc_v, ql + C::SET, rb, p, lane);
+                priority<(D > 64)>(0);
                 split8(y, p);
+                priority<(D > 64)>(1);
                 add16<C>(acc_k, ql, rb, p, lane);
+                priority<(D > 64)>(0);
             }
         }
         if (t + 1 < t1) {
@@ -608,18 +637,18 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
 
 // One launch for both: they need nothing of each other, and the workgroups of one fill
 // the compute units that the other leaves idle (the longer walks begin first).
-template <int D, bool FULL, int MODE>
-__global__ __launch_bounds__(512, 2) void masked_tile_bwd_kernel(MaskedArgs a) {
-    using C = TileCfg<D, 8>;
+template <int D, int WAVES, bool FULL, int MODE>
+__global__ __launch_bounds__(64 * WAVES, 2) void masked_tile_bwd_kernel(MaskedArgs a) {
+    using C = TileCfg<D, WAVES>;
     __shared__ u32x4 lds[4 * C::SET];
     __shared__ f32x4 starts[2 * (MODE == kPlain ? 4 : 6) * C::KT / 4];
-    __shared__ int marks[2][C::KT + 1], ends[2][8];
+    __shared__ int marks[2][C::KT + 1], ends[2][WAVES];
     for (int i = threadIdx.x; i < 2 * (C::KT + 1); i += C::NT) marks[0][i] = 0;
     const int kv_blocks = gridDim.x - a.q_blocks;
     if ((int)blockIdx.x >= kv_blocks)
-        masked_dq_walk<D, FULL, MODE>(a, lds, marks, ends, blockIdx.x - kv_blocks);
+        masked_dq_walk<D, WAVES, FULL, MODE>(a, lds, marks, ends, blockIdx.x - kv_blocks);
     else
-        masked_dkv_walk<D, FULL, MODE>(a, lds, marks, starts, ends, blockIdx.x);
+        masked_dkv_walk<D, WAVES, FULL, MODE>(a, lds, marks, starts, ends, blockIdx.x);
 }
 
 int mode_of(const MaskedArgs& a) { return a.cap2 > 0.0f ? kCap : a.slopes ? kBias : kPlain; }
@@ -633,9 +662,10 @@ void launch_forward(const MaskedArgs& a, unsigned blocks) {
 
 template <int D, int MODE>
 void launch_backward(const MaskedArgs& a, unsigned blocks) {
-    auto kernel = a.D == D ? masked_tile_bwd_kernel<D, true, MODE>
-                           : masked_tile_bwd_kernel<D, false, MODE>;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(512), 0, stream(), a);
+    constexpr int WAVES = masked_backward_waves(D);
+    auto kernel = a.D == D ? masked_tile_bwd_kernel<D, WAVES, true, MODE>
+                           : masked_tile_bwd_kernel<D, WAVES, false, MODE>;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(64 * WAVES), 0, stream(), a);
 }
 
 template <int D>
@@ -658,7 +688,7 @@ void backward(MaskedArgs a) {
         constexpr int WIDE = cross_row_width(D), PER = 1024 / WIDE;
         const int64_t row_blocks = (rows + PER - 1) / PER,
                       end_blocks = ((int64_t)a.B * a.row_tiles + 7) / 8;
-        hipLaunchKernelGGL((masked_prepare_kernel<WIDE, TileCfg<D, 8>::KT>),
+        hipLaunchKernelGGL((masked_prepare_kernel<WIDE, TileCfg<D, masked_backward_waves(D)>::KT>),
                            dim3((unsigned)(row_blocks + end_blocks)), dim3(256), 0, stream(), a,
                            (int)row_blocks);
     }
