@@ -614,6 +614,42 @@ void cross_entropy_backward(const NodeRef& pred, const NodeRef& target) {
           "cuda ce: backward launch failed");
 }
 
+namespace {
+// The pass of distillation and distillation_backward.
+float distill(const NodeRef& pred, const Teacher& teacher, bool backward) {
+    const auto [rows, vocab] = batch_classes(pred);
+    GpuBuffers& p = gpu_of(pred, "distillation: logits not on GPU");
+    GpuBuffers& t = gpu_of(teacher.top, "distillation: teacher not on GPU");
+    const size_t k = rows > 0 ? product(teacher.top->shape) / rows : 0;
+    if (product(teacher.top->shape) != rows * k || !teacher.ids || teacher.ids->len() != rows * k)
+        throw Panic("distillation: teacher's logits and ids must be [rows, k]");
+    if (teacher.labels && teacher.labels->len() != rows)
+        throw Panic("distillation: one label per row");
+    const int32_t* labels = teacher.labels ? teacher.labels->ptr() : nullptr;
+    DeviceBuffer row_loss(rows, false);
+    if (backward)
+        check(nrs_distill_backward(p.grad->write_target(), row_loss.ptr(), nullptr, p.data.ptr(),
+                                   t.data.ptr(), teacher.ids->ptr(), labels, rows, vocab, k, vocab,
+                                   teacher.temperature, teacher.hard),
+              "distillation: backward launch failed");
+    else
+        check(nrs_distill_forward(row_loss.ptr(), p.data.ptr(), t.data.ptr(), teacher.ids->ptr(),
+                                  labels, rows, vocab, k, vocab, teacher.temperature, teacher.hard),
+              "distillation: forward launch failed");
+    float total = 0.0f;
+    for (float v : row_loss.to_host()) total += v;
+    return total / (float)rows;
+}
+}  // namespace
+
+float distillation(const NodeRef& pred, const Teacher& teacher) {
+    return distill(pred, teacher, false);
+}
+
+float distillation_backward(const NodeRef& pred, const Teacher& teacher) {
+    return distill(pred, teacher, true);
+}
+
 }  // namespace loss
 
 // ---------------------------------------------------------------------- nn
@@ -1267,6 +1303,141 @@ NodeRef MultiHeadAttention::forward_cross(const NodeRef& x, const NodeRef& memor
     const NodeRef heads = fused_cross_attention(q, kv[0], kv[1], key_len, batch, num_heads,
                                                 num_heads, seq_q, seq_k, d_model / num_heads);
     return graph::reshape(graph::matmul(heads, w_o), {batch, seq_q, d_model});
+}
+
+// The fused node of masked_attention and forward_masked, in any leading shape as
+// fused_cross_attention's.
+static NodeRef fused_masked_attention(const NodeRef& q, const NodeRef& k, const NodeRef& v,
+                                      const AttentionMask& mask, size_t batch, size_t heads,
+                                      size_t kv_heads, size_t seq_q, size_t seq_k, size_t d) {
+    GpuBuffers& qg = gpu_of(q, "masked attention: q not on GPU");
+    GpuBuffers& kg = gpu_of(k, "masked attention: k not on GPU");
+    GpuBuffers& vg = gpu_of(v, "masked attention: v not on GPU");
+    for (const IntsRef& per_item : {mask.q_start, mask.key_len, mask.prefix_len})
+        if (per_item && per_item->len() != batch)
+            throw Panic("masked attention: q_start, key_len and prefix_len have one number per item");
+    for (const IntsRef& per_query : {mask.key_begin, mask.key_end})
+        if (per_query && per_query->len() != batch * seq_q)
+            throw Panic("masked attention: key_begin and key_end have one number per query");
+    if (mask.slopes && product(mask.slopes->shape) != heads)
+        throw Panic("masked attention: one slope per head");
+    // (made anew for each call: the arrays are the mask's, which the closure keeps)
+    auto plain = [](const AttentionMask& m) {
+        auto ints = [](const IntsRef& x) { return x ? x->ptr() : nullptr; };
+        nrs_attention_mask a{};
+        a.causal = m.causal;
+        a.q_start = ints(m.q_start);
+        a.key_len = ints(m.key_len);
+        a.prefix_len = ints(m.prefix_len);
+        a.key_begin = ints(m.key_begin);
+        a.key_end = ints(m.key_end);
+        a.slopes =
+            m.slopes ? gpu_of(m.slopes, "masked attention: slopes not on GPU").data.ptr() : nullptr;
+        a.cap = m.cap;
+        return a;
+    };
+    const size_t ld_q = heads * d, ld_kv = kv_heads * d;
+    const float scale = 1.0f / std::sqrt(static_cast<float>(d));
+    const size_t q_len = batch * seq_q * ld_q, kv_len = batch * seq_k * ld_kv;
+    DeviceBuffer out(q_len, false);
+    auto stats = std::make_shared<DeviceBuffer>(batch * heads * seq_q * 2, false);
+    const nrs_attention_mask m = plain(mask);
+    check(nrs_masked_attention_forward(out.ptr(), stats->ptr(), qg.data.ptr(), kg.data.ptr(),
+                                       vg.data.ptr(), &m, batch, heads, kv_heads, seq_q, seq_k, d,
+                                       ld_q, ld_kv, ld_q, scale, nullptr, 0),
+          "masked attention: launch failed");
+    NodeRef node = make_output(q->shape, {q, k, v}, std::move(out));
+    Node* self = node.get();
+    node->backward_fn = [grad = node->gpu->grad, self, q, k, v, mask, plain, stats, q_len, kv_len,
+                         batch, heads, kv_heads, seq_q, seq_k, d, ld_q, ld_kv,
+                         scale](const std::vector<float>&) {
+        GpuBuffers& qg = gpu_of(q, "masked attention bwd: q not on GPU");
+        GpuBuffers& kg = gpu_of(k, "masked attention bwd: k not on GPU");
+        GpuBuffers& vg = gpu_of(v, "masked attention bwd: v not on GPU");
+        const nrs_attention_mask m = plain(mask);
+        auto run = [&](float* dq, float* dk, float* dv, float beta_q, float beta_kv) {
+            check(nrs_masked_attention_backward(
+                      dq, dk, dv, grad->ptr(), self->gpu->data.ptr(), qg.data.ptr(),
+                      kg.data.ptr(), vg.data.ptr(), stats->ptr(), &m, batch, heads, kv_heads,
+                      seq_q, seq_k, d, ld_q, ld_kv, ld_q, scale, beta_q, beta_kv, nullptr, 0),
+                  "masked attention bwd: launch");
+        };
+        if (qg.grad != kg.grad && kg.grad != vg.grad && qg.grad != vg.grad) {
+            const float beta_kv = joint_beta({kg.grad.get(), vg.grad.get()});
+            float beta_q = 1.0f;
+            float* dq = qg.grad->acc_target(beta_q);
+            run(dq, kg.grad->write_target(), vg.grad->write_target(), beta_q, beta_kv);
+            return;
+        }
+        // q, k or v are one node: the gradients go to temporaries, then add up
+        DeviceBuffer tq(q_len, false), tk(kv_len, false), tv(kv_len, false);
+        run(tq.ptr(), tk.ptr(), tv.ptr(), 0.0f, 0.0f);
+        accumulate_into(*qg.grad, tq.ptr(), q_len);
+        accumulate_into(*kg.grad, tk.ptr(), kv_len);
+        accumulate_into(*vg.grad, tv.ptr(), kv_len);
+    };
+    return node;
+}
+
+NodeRef masked_attention(const NodeRef& q, const NodeRef& k, const NodeRef& v, size_t heads,
+                         size_t kv_heads, const AttentionMask& mask) {
+    if (q->shape.size() != 3 || k->shape.size() != 3)
+        throw Panic("masked attention: q and k must be [batch, seq, width]");
+    const size_t batch = q->shape[0], width = q->shape[2];
+    if (heads == 0 || kv_heads == 0 || width % heads != 0)
+        throw Panic("masked attention: width % heads != 0");
+    const size_t d = width / heads;
+    if (k->shape[0] != batch || k->shape[2] != kv_heads * d || v->shape != k->shape)
+        throw Panic("masked attention: shape mismatch");
+    return fused_masked_attention(q, k, v, mask, batch, heads, kv_heads, q->shape[1], k->shape[1],
+                                  d);
+}
+
+NodeRef rotary(const NodeRef& x, size_t heads, const Rotary& turn) {
+    GpuBuffers& xg = gpu_of(x, "rotary: input not on GPU");
+    GpuBuffers& fg = gpu_of(turn.freq, "rotary: frequencies not on GPU");
+    if (x->shape.empty() || heads == 0 || x->shape.back() % heads != 0)
+        throw Panic("rotary: width % heads != 0");
+    const size_t width = x->shape.back(), d = width / heads;
+    const size_t rows = width > 0 ? product(x->shape) / width : 0;
+    const size_t pairs = product(turn.freq->shape);
+    if (!turn.positions || rows == 0 || turn.positions->len() == 0 ||
+        turn.positions->len() % rows != 0)
+        throw Panic("rotary: one position per row and axis");
+    if (turn.axis && turn.axis->len() != pairs) throw Panic("rotary: one axis per pair");
+    const size_t axes = turn.positions->len() / rows;
+    DeviceBuffer out(rows * width, false);
+    check(nrs_rotary_forward(out.ptr(), xg.data.ptr(), turn.positions->ptr(), fg.data.ptr(),
+                             turn.axis ? turn.axis->ptr() : nullptr, rows, heads, d, pairs, axes,
+                             width, width, turn.interleaved),
+          "rotary: launch failed");
+    NodeRef node = make_output(x->shape, {x}, std::move(out));
+    node->backward_fn = [grad = node->gpu->grad, x, turn, rows, heads, d, pairs, axes,
+                         width](const std::vector<float>&) {
+        float beta = 1.0f;
+        float* gx = gpu_of(x, "rotary bwd: input not on GPU").grad->acc_target(beta);
+        check(nrs_rotary_backward(gx, grad->ptr(), turn.positions->ptr(),
+                                  gpu_of(turn.freq, "rotary bwd: frequencies not on GPU").data.ptr(),
+                                  turn.axis ? turn.axis->ptr() : nullptr, rows, heads, d, pairs,
+                                  axes, width, width, turn.interleaved, beta),
+              "rotary bwd: launch");
+    };
+    return node;
+}
+
+NodeRef MultiHeadAttention::forward_masked(const NodeRef& x, const AttentionMask& mask,
+                                           const Rotary* turn) const {
+    if (x->shape.size() != 3) throw Panic("multihead: x must be [batch, seq, d_model]");
+    if (num_heads == 0 || d_model % num_heads != 0) throw Panic("multihead: d_model % heads != 0");
+    const size_t batch = x->shape[0], seq = x->shape[1];
+    if (x->shape[2] != d_model) throw Panic("multihead: input width is not d_model");
+    const std::vector<NodeRef> qkv =
+        matmul_shared_lhs(reshape_view(x, {batch * seq, d_model}), {w_q, w_k, w_v});
+    const NodeRef q = turn ? rotary(qkv[0], num_heads, *turn) : qkv[0];
+    const NodeRef k = turn ? rotary(qkv[1], num_heads, *turn) : qkv[1];
+    const NodeRef heads = fused_masked_attention(q, k, qkv[2], mask, batch, num_heads, num_heads,
+                                                 seq, seq, d_model / num_heads);
+    return graph::reshape(graph::matmul(heads, w_o), {batch, seq, d_model});
 }
 
 NodeRef Embedding::forward(const IntsRef& ids, std::vector<size_t> shape) const {

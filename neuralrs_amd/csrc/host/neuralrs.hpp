@@ -12,7 +12,7 @@
 //          concat_cols, scaled_softmax}
 //                                        src/cuda/graph/*.rs
 //   nn::{conv2d, maxpool2d, Linear, attention, attention_batch, layernorm,
-//        cross_attention, Embedding, dropout, Dropout,
+//        cross_attention, Embedding, dropout, Dropout, masked_attention, rotary,
 //        SelfAttention, MultiHeadAttention, TransformerBlock}
 //                                        src/cuda/nn/*.rs
 // Rc<RefCell<Node>> becomes std::shared_ptr<Node>; a panic ("cuda matmul: lhs
@@ -228,6 +228,22 @@ float cross_entropy(const NodeRef& pred, const NodeRef& target);
 // src/cuda/loss/cross_entropy.rs:100-127: writes (softmax - target) / batch
 // into the logits' gradient; backward_graph then propagates it.
 void cross_entropy_backward(const NodeRef& pred, const NodeRef& target);
+
+// What a student's logits [rows, vocab] learn from (nrs_distill_forward): a teacher's
+// k largest logits of each row with their tokens, at a temperature, and the rows'
+// labels with the weight `hard`. Ids outside the vocabulary, -1 say, are left out.
+struct Teacher {
+    NodeRef top;     // [rows, k], no gradient flows to it
+    IntsRef ids;     // rows * k
+    IntsRef labels;  // rows; null when hard is 0
+    float temperature = 1.0f;
+    float hard = 0.0f;
+};
+// The loss averaged over the rows, as cross_entropy's.
+float distillation(const NodeRef& pred, const Teacher& teacher);
+// Writes that mean's gradient into the logits' gradient, as cross_entropy_backward, and
+// returns the mean from the same pass.
+float distillation_backward(const NodeRef& pred, const Teacher& teacher);
 }  // namespace loss
 
 namespace nn {
@@ -276,6 +292,32 @@ NodeRef layernorm(const NodeRef& input, const NodeRef& gamma, const NodeRef& bet
 // once and calls this with those nodes.
 NodeRef cross_attention(const NodeRef& q, const NodeRef& k, const NodeRef& v, size_t heads,
                         size_t kv_heads, const IntsRef& key_len = nullptr);
+
+// What the queries of a decoder's self-attention see and how scores change
+// (nrs_attention_mask); arrays that are not given hide nothing and add nothing.
+struct AttentionMask {
+    bool causal = true;
+    IntsRef q_start, key_len, prefix_len;  // per batch item
+    IntsRef key_begin, key_end;            // per batch item and query
+    NodeRef slopes;                        // [heads], constants: no gradient
+    float cap = 0.0f;
+};
+// softmax of the visible scores times v, for every head: shapes as cross_attention. With
+// a cache, k and v hold all its keys and the queries are the last ones, or from
+// mask.q_start on. One fused node.
+NodeRef masked_attention(const NodeRef& q, const NodeRef& k, const NodeRef& v, size_t heads,
+                         size_t kv_heads, const AttentionMask& mask);
+
+// Positions of the rows (batch * seq of them) along each axis, the frequency and axis
+// of every pair of a head's columns (nrs_rotary_forward).
+struct Rotary {
+    IntsRef positions;  // axes * rows
+    NodeRef freq;       // [pairs], constants: no gradient
+    IntsRef axis;       // pairs; null: one axis
+    bool interleaved = false;
+};
+// x [.., heads * d] with each head's pairs turned.
+NodeRef rotary(const NodeRef& x, size_t heads, const Rotary& turn);
 
 // The reference's embedding layer (src/cuda/nn/embedding): resident table
 // [vocab, dim]; the rows of `ids`, times scale (sqrt(dim) in a Transformer). An
@@ -348,6 +390,11 @@ struct MultiHeadAttention {
     // the memory anew, to keys and values of their own, at every call.
     NodeRef forward_cross(const NodeRef& x, const NodeRef& memory,
                           const IntsRef& key_len = nullptr) const;
+    // A decoder's self-attention, x [batch, seq, d_model] (no counterpart in the
+    // reference, whose attention has no mask): what the mask hides is not seen, and
+    // queries and keys are turned by `turn` if it is given. Heads of at most 128.
+    NodeRef forward_masked(const NodeRef& x, const AttentionMask& mask,
+                           const Rotary* turn = nullptr) const;
 };
 
 // src/cuda/nn/transformer_block.rs:9-45: post-norm block, x + MHA(x) -> norm1
