@@ -387,7 +387,8 @@ int nrs_cross_attention_backward(float *dq, float *dk, float *dv, const float *d
  * It sees key t when t < key_len[b], key_begin[b, s] <= t < key_end[b, s] and, if
  * causal, t <= i or t < prefix_len[b]; a mask that is not given hides nothing. So
  * key_begin, the first token of each token's document, keeps packed documents apart;
- * with key_end it says any range. Every range is cut to 0 .. seq_k - 1.
+ * with key_end it says any range. Every range is cut to 0 .. seq_k - 1. With a cap,
+ * scale / cap * q and its products with k have to be below 2^127 in magnitude, too.
  *   Values of keys that a row does not see, infinite and NaN ones among them, do not
  * change its results or gradients; keys that no row of an item sees get a zero gradient
  * (written as zeros with beta_kv 0, left as they are with 1). A row that sees a key with

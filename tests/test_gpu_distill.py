@@ -120,7 +120,7 @@ CASES = [
     # rows, vocab, k
     (1, 1, 1), (2, 2, 1), (3, 5, 5), (7, 64, 8), (5, 1000, 16), (4, 2047, 3), (3, 2048, 33),
     (2, 2049, 256), (9, 8000, 64), (2, 30001, 1000), (1, 70000, 1024), (300, 257, 20), (1, 160000, 7),
-    (3, 40003, 100), (2, 131075, 12),
+    (3, 40003, 100), (2, 131075, 12), (2, 1500, 1024), (70, 33000, 5), (1, 8193, 1),
 ]
 
 

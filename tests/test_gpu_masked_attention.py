@@ -296,3 +296,48 @@ def test_nothing_to_do(hip):
     mark = hip.DeviceBuffer.from_host(np.full(32, MARK))
     hip.masked_attention_forward(mark, None, mark, None, None, None, 2, 1, 1, 2, 0, 8, 8, 8, 8, 1.0)
     assert np.all(mark.to_host() == 0)
+
+
+@pytest.mark.parametrize("shape", [(2, 4, 2, 100, 0, 32), (2, 4, 2, 0, 100, 32), (2, 4, 2, 0, 100, 128),
+                                   (1, 2, 1, 0, 0, 64)], ids=str)
+def test_no_rows_or_no_keys(hip, shape):
+    check(hip, Problem(*shape, seed=18), beta_kv=0.5)
+    check(hip, Problem(*shape, seed=18), beta_q=1.0, beta_kv=1.0)
+
+
+def test_many_items_of_a_token(hip):
+    """More items than share one line of tiles."""
+    check(hip, Problem(1500, 2, 1, 1, 60, 16, q_start=np.arange(1500) % 60, seed=19), gradients=False)
+
+
+def test_many_short_items(hip):
+    check(hip, Problem(300, 2, 2, 7, 7, 8, key_len=np.arange(300) % 8, seed=20))
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_long_walks_in_parts(hip, d):
+    """Few units over long ranges: forward and backward walks in several parts, of which
+    some rows (and keys) have one."""
+    p = Problem(1, 1, 1, 2100, 2100, d, seed=21, key_begin=np.where(np.arange(2100) % 700 < 650, 0, 1900))
+    check(hip, p)
+    check(hip, Problem(1, 2, 1, 600, 4000, d, seed=22, slopes=True, prefix_len=[3800]))
+
+
+@pytest.mark.parametrize("magnitude", [1e-12, 1e-3, 30.0])
+def test_magnitudes(hip, magnitude):
+    check(hip, Problem(1, 2, 2, 60, 60, 32, seed=23, magnitude=magnitude, cap=5.0))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+def test_scales(hip, scale):
+    p = Problem(1, 2, 2, 60, 60, 32, seed=24, slopes=True)
+    p.scale = np.float32(scale)
+    check(hip, p)
+    p = Problem(1, 2, 2, 3, 60, 32, seed=24, cap=1.0)
+    p.scale = np.float32(scale)
+    check(hip, p, gradients=False)
+
+
+def test_a_group_of_many_heads(hip):
+    check(hip, Problem(1, 112, 1, 9, 40, 24, seed=25, cap=3.0))
+    check(hip, Problem(2, 33, 1, 1, 200, 24, seed=26, slopes=True))
