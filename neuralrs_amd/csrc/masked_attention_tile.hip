@@ -176,7 +176,9 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_t
 #pragma unroll
                     for (int i = 0; i < 16; ++i) p[kb][i] = fmaf(a.cap2, p[kb][i], -m);
                 }
-                add_bias<MODE, 16>(p[kb], (float)(range.at - (k0 + kb * 32 + 4 * h)), slope2, place32);
+                if (MODE != kCap || a.slopes)
+                    add_bias<MODE, 16>(p[kb], (float)(range.at - (k0 + kb * 32 + 4 * h)), slope2,
+                                       place32);
             }
             priority<WAVES == 8>(0);
             if (mark[C::KT] == t + 1) {
@@ -307,6 +309,36 @@ __global__ __launch_bounds__(256) void masked_prepare_kernel(MaskedArgs a, int r
     if ((threadIdx.x & 31) == 0) a.ends[no] = all;
 }
 
+// out = met . own^T of block kb of a tile, the small products of the pieces in a sum of
+// their own: rounded as products16's closer form, which reads the large ones' operand a
+// second time.
+template <class C>
+__device__ __forceinline__ void close16(f32x4 (&out)[2], const u32x4* set,
+                                        const u32x4 (&own)[C::D / 32][3], int kb, int c, int g) {
+    f32x4 small[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+        out[half] = small[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < C::D / 32; ++s) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            u32x4 met[3];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) met[p] = piece16<C>(set, kb * 32 + 16 * half, s, p, c, g);
+            f32x4& o = small[half];
+            o = mfma16(met[2], own[s][0], o);
+            o = mfma16(met[1], own[s][1], o);
+            o = mfma16(met[0], own[s][2], o);
+            o = mfma16(met[1], own[s][0], o);
+            o = mfma16(met[0], own[s][1], o);
+            out[half] = mfma16(met[0], own[s][0], out[half]);
+        }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) out[half] = out[half] + small[half];
+}
+
 __device__ __forceinline__ constexpr int place16(int i) { return 16 * (i / 4) + i % 4; }
 
 // dq of a workgroup's rows, 16 to a wave: P = 2^(score - lse), dS = P (v . dout - delta) and, with a
@@ -383,12 +415,9 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
             if (k0 >= seen.most || k0 + 32 <= seen.least) continue;
             f32x4 s[2], dp[2];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                s[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                dp[half] = f32x4{nd, nd, nd, nd};
-            }
+            for (int half = 0; half < 2; ++half) dp[half] = f32x4{nd, nd, nd, nd};
             priority<(D > 64)>(1);
-            products16<C, true>(s, kl, qf, kb, c, g);
+            close16<C>(s, kl, qf, kb, c, g);
             products16<C, false>(dp, kl + C::SET, gf, kb, c, g);
             priority<(D > 64)>(0);
             float x[8];
@@ -402,7 +431,8 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
                     x[i] *= a.cap2;
                 }
             }
-            add_bias<MODE, 8>(x, (float)(range.at - (k0 + 4 * g)), slope2, place16);
+            if (MODE != kCap || a.slopes)
+                add_bias<MODE, 8>(x, (float)(range.at - (k0 + 4 * g)), slope2, place16);
             if (marked) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -543,12 +573,9 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
                 const f32x4* const st = starts + (buf * ROWS * C::KT + rb * 32) / 4 + g;
                 f32x4 s[2], dp[2];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    s[half] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    dp[half] = st[C::KT / 4 + 4 * half];
-                }
+                for (int half = 0; half < 2; ++half) dp[half] = st[C::KT / 4 + 4 * half];
                 priority<(D > 64)>(1);
-                products16<C, true>(s, ql, kf, rb, c, g);
+                close16<C>(s, ql, kf, rb, c, g);
                 products16<C, false>(dp, ql + C::SET, vf, rb, c, g);
                 priority<(D > 64)>(0);
                 float x[8], y[8];
@@ -565,7 +592,7 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
                         x[i] *= a.cap2;
                     }
                 }
-                if (MODE != kPlain) {
+                if (MODE == kBias || (MODE == kCap && a.slopes)) {
                     const float place_key = (float)(key - tile * 16 * WAVES);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
