@@ -41,6 +41,14 @@ inline MaskedForwardPlan plan_masked_forward(int64_t batch, int64_t heads, int64
     if (items == 0 || R == 0) return p;
     if (!p.tiles) {
         p.line = plan_cross_forward(batch, heads, kv_heads, seq_q, seq_k, d_head, cus);
+        // Up to 384 keys (six tiles to a wave) the join costs more than the shares save: 8
+        // requests of 300 keys, 8 heads of 32, 15.7 us shared and 9.4 like this, one of 256
+        // keys, 8 of 64, 14.5 and 11.0; 512 keys 14.7 and 16.6.
+        if (seq_k <= 384 && p.line.groups > 0) {
+            p.line.groups = 0;
+            p.line.blocks = items * ((R + 15) / 16);
+            p.line.part = p.line.stats = p.line.shares = 0;
+        }
         p.unit_rows = p.line.unit_rows;
         p.part = p.line.part;
         p.stats = p.line.stats;
