@@ -90,8 +90,13 @@ __device__ __forceinline__ void add_bias(V& s, float far, float slope2, O o) {
 
 __device__ __forceinline__ constexpr int place32(int i) { return 8 * (i / 4) + i % 4; }
 
+// (narrow heads leave room for three: 2 x 1500 rows, 16 heads of 32, 51 us, with two 59)
+constexpr int forward_waves_per_simd(int D, int waves) {
+    return D <= 32 && waves == 4 ? 3 : waves_per_simd(D, waves);
+}
+
 template <int D, int WAVES, bool FULL, int MODE>
-__global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_tile_fwd_kernel(
+__global__ __launch_bounds__(64 * WAVES, forward_waves_per_simd(D, WAVES)) void masked_tile_fwd_kernel(
     MaskedArgs a) {
     using C = TileCfg<D, WAVES>;
     __shared__ u32x4 lds[2][2 * C::SET];
@@ -150,7 +155,7 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_t
     u32x4 qf[C::NS][3];
     own_pieces<C, FULL>(qf, a, a.q + (live ? query_offset(a, b, kv, row, a.ld_q) : 0), live, h,
                         a.scale_own);
-    f32x16 acc[C::NJ], start = all16(0.0f);  // start: -m, where the scores start
+    f32x16 acc[C::NJ];
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) acc[j] = all16(0.0f);
     float m = 0.0f, l = 0.0f;
@@ -170,11 +175,14 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_t
             priority<WAVES == 8>(1);
 #pragma unroll
             for (int kb = 0; kb < C::NB; ++kb) {
-                p[kb] = products<C>(kl, qf, kb, MODE == kCap ? all16(0.0f) : start, c, h);
+                // (from zero, not from -m: 16 registers less, which wide heads spilled)
+                p[kb] = products<C>(kl, qf, kb, all16(0.0f), c, h);
                 if (MODE == kCap) {
                     tanh_all<16>(p[kb]);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) p[kb][i] = fmaf(a.cap2, p[kb][i], -m);
+                } else {
+                    p[kb] = p[kb] - m;
                 }
                 if (MODE != kCap || a.slopes)
                     add_bias<MODE, 16>(p[kb], (float)(range.at - (k0 + kb * 32 + 4 * h)), slope2,
@@ -211,7 +219,6 @@ __global__ __launch_bounds__(64 * WAVES, waves_per_simd(D, WAVES)) void masked_t
                 m += shift;
                 l *= alpha;
                 fresh = fresh && !begins;
-                start = all16(-m);
 #pragma unroll
                 for (int kb = 0; kb < C::NB; ++kb) p[kb] = p[kb] - shift;
 #pragma unroll
