@@ -458,11 +458,13 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
                     if (mark[kb * 32 + 4 * g + place16(i)] == t + 1) x[i] = NAN;
             }
             if (k0 < seen.from || k0 + 32 > seen.to) {
+                // (both: a hidden value may be as large as to make its product infinite)
                 const uint32_t span = range.hi - range.lo;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint32_t at = k0 + 4 * g - range.lo + place16(i);
-                    x[i] = at < span ? x[i] : -INFINITY;
+                    const bool sees = k0 + 4 * g - range.lo + place16(i) < span;
+                    x[i] = sees ? x[i] : -INFINITY;
+                    dp[i / 4][i % 4] = sees ? dp[i / 4][i % 4] : 0.0f;
                 }
             }
 #pragma unroll

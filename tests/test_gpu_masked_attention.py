@@ -341,3 +341,36 @@ def test_scales(hip, scale):
 def test_a_group_of_many_heads(hip):
     check(hip, Problem(1, 112, 1, 9, 40, 24, seed=25, cap=3.0))
     check(hip, Problem(2, 33, 1, 1, 200, 24, seed=26, slopes=True))
+
+
+@pytest.mark.parametrize("extra", [dict(), dict(cap=2.0), dict(cap=2.0, slopes=True), dict(slopes=True)],
+                         ids=str)
+@pytest.mark.parametrize("sq,d", [(150, 32), (150, 96), (150, 128), (600, 64), (9, 64)])
+def test_hidden_magnitudes(hip, sq, d, extra):
+    """Finite values whose products overflow, in a document of their own: the other
+    document's results and gradients keep their bits."""
+    sk, firsts = 150 if sq < 150 else sq, [0, sq // 2]
+    begin, end = (np.array(x) for x in documents(sq, firsts))
+    cut = sk - sq + firsts[1]  # the second document's first key
+    p = Problem(1, 2, 1, sq, sk, d, causal=False, seed=27, key_begin=np.where(begin > 0, cut, 0),
+                key_end=np.where(begin > 0, sk, cut), **extra)
+    clean = run(hip, p)
+    rng = np.random.default_rng(5)
+    for x, at in ((p.q, firsts[1]), (p.dout, firsts[1]), (p.k, cut), (p.v, cut)):
+        x[at:] = rng.choice([-1.6e38, 1.6e38], x[at:].shape)
+    got = run(hip, p)
+    for i, at in ((0, firsts[1]), (1, firsts[1]), (2, cut), (3, cut)):
+        assert np.array_equal(got[i][:at], clean[i][:at]), ["out", "dq", "dk", "dv"][i]
+
+
+@pytest.mark.parametrize("bad", BAD, ids=str)
+@pytest.mark.parametrize("d", [32, 128])
+def test_a_row_that_sees_nothing_has_no_gradient(hip, d, bad):
+    """Whatever its own numbers are."""
+    p = Problem(1, 2, 2, 150, 150, d, key_begin=np.where(np.arange(150) % 3 == 0, 200, 0), seed=28)
+    clean = run(hip, p)
+    p.q[::3] = p.dout[::3] = bad
+    got = run(hip, p)
+    for x, was in zip(got, clean):
+        assert np.array_equal(x, was)
+    assert np.all(got[0][::3] == 0) and np.all(got[1][::3] == 0)
