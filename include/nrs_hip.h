@@ -389,6 +389,7 @@ int nrs_cross_attention_backward(float *dq, float *dk, float *dv, const float *d
  * key_begin, the first token of each token's document, keeps packed documents apart;
  * with key_end it says any range. Every range is cut to 0 .. seq_k - 1. With a cap,
  * scale / cap * q and its products with k have to be below 2^127 in magnitude, too.
+ * In stats a row's bias is less that of the nearest key of its range.
  *   Values of keys that a row does not see, infinite and NaN ones among them, do not
  * change its results or gradients; keys that no row of an item sees get a zero gradient
  * (written as zeros with beta_kv 0, left as they are with 1). A row that sees a key with
@@ -401,7 +402,7 @@ typedef struct nrs_attention_mask {
     const int32_t *prefix_len; /* device [batch]; NULL: 0 (needs causal)             */
     const int32_t *key_begin;  /* device [batch * seq_q]; NULL: 0                    */
     const int32_t *key_end;    /* device [batch * seq_q]; NULL: seq_k                */
-    const float *slopes;       /* device [heads], finite and 0 or more; NULL: 0      */
+    const float *slopes;       /* device [heads], 0 or more, below 2^127; NULL: 0    */
     float cap;                 /* of the scores; 0: none                             */
 } nrs_attention_mask;
 int nrs_masked_attention_supported(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
@@ -420,7 +421,8 @@ int nrs_masked_attention_forward(float *out, float *stats, const float *q, const
  *   dS = P * (dout . v^T - dout . out) * (1 - tanh^2 where capped) * scale,
  *   dq = beta_q * dq + dS . k,  dk = beta_kv * dk + dS^T . q,
  *   dv = beta_kv * dv + P^T . dout.
- * The slopes are constants: they get no gradient.                            */
+ * A row that sees no key gets a zero gradient, whatever dout is there, and the slopes,
+ * which are constants, none.                                                 */
 int nrs_masked_attention_backward(float *dq, float *dk, float *dv, const float *dout,
                                   const float *out, const float *q, const float *k, const float *v,
                                   const float *stats, const nrs_attention_mask *mask,
@@ -509,8 +511,9 @@ int nrs_dropout_backward(float *gin, const float *grad, int64_t n, float p, uint
  * labels [rows] (may be NULL when hard is 0). A teacher token whose id is outside
  * [0, vocab), -1 say, is left out, and a token named twice has the sum of both weights.
  * A row without teacher tokens, or with teacher logits of minus infinity alone, has the
- * second part alone; one whose label is outside [0, vocab), the first alone. Logits may be minus
- * infinity, but not all of a row.                                               */
+ * second part alone; one whose label is outside [0, vocab), the first alone; and one with
+ * neither has no loss and no gradient, whatever its logits are. Logits may be minus
+ * infinity, but not all of another row.                                          */
 int nrs_distill_forward(float *row_loss, const float *logits, const float *top,
                         const int32_t *top_ids, const int32_t *labels, int64_t rows, int64_t vocab,
                         int64_t k, int64_t ld, float temperature, float hard);

@@ -435,13 +435,16 @@ void launch_rows(const MaskedArgs& a, unsigned blocks) {
 
 int check(const char* what, const nrs_attention_mask* mask, int64_t batch, int64_t heads,
           int64_t kv_heads, int64_t seq_q, int64_t seq_k, int64_t d_head, int64_t ld_q,
-          int64_t ld_kv, int64_t ld_out) {
+          int64_t ld_kv, int64_t ld_out, float scale) {
     if (int rc = cross_check_shape(what, batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q,
                                    ld_kv, ld_out))
         return rc;
     if (!mask) return NRS_OK;
-    NRS_ARG_CHECK(mask->cap >= 0.0f && std::isfinite(mask->cap),
-                  "%s: cap must be 0 (none) or a positive number, is %g", what, (double)mask->cap);
+    NRS_ARG_CHECK(mask->cap >= 0.0f && std::isfinite(mask->cap * kLog2e),
+                  "%s: cap must be 0 (none) or a positive number below 2^127, is %g", what,
+                  (double)mask->cap);
+    NRS_ARG_CHECK(mask->cap == 0.0f || std::isfinite((float)((double)scale / mask->cap)),
+                  "%s: scale / cap is %g / %g", what, (double)scale, (double)mask->cap);
     NRS_ARG_CHECK(mask->causal || !mask->prefix_len, "%s: a prefix without a causal mask", what);
     return NRS_OK;
 }
@@ -513,7 +516,7 @@ int nrs_masked_attention_forward(float* out, float* stats, const float* q, const
                                  float scale, void* work, size_t work_bytes) {
     const char* what = "masked attention forward";
     if (int rc = nrs::check(what, mask, batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv,
-                            ld_out))
+                            ld_out, scale))
         return rc;
     if (batch == 0 || seq_q == 0) return NRS_OK;
     NRS_ARG_CHECK(out && q && ((k && v) || seq_k == 0), "%s: null pointer", what);
@@ -572,7 +575,7 @@ int nrs_masked_attention_backward(float* dq, float* dk, float* dv, const float* 
                                   void* work, size_t work_bytes) {
     const char* what = "masked attention backward";
     if (int rc = nrs::check(what, mask, batch, heads, kv_heads, seq_q, seq_k, d_head, ld_q, ld_kv,
-                            ld_out))
+                            ld_out, scale))
         return rc;
     NRS_ARG_CHECK((dk == nullptr) == (dv == nullptr), "%s: dk and dv go together", what);
     if (batch == 0) return NRS_OK;

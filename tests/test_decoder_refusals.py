@@ -46,6 +46,16 @@ def test_masks(mask, why):
         _abi.masked_attention_backward(*[P] * 9, m, *GOOD.values(), 1.0)
 
 
+@pytest.mark.parametrize("cap,scale", [(3e38, 1.0), (1e-39, 1.0), (1.0, math.inf), (1.0, math.nan),
+                                       (1e-30, 1e10)])
+def test_caps_that_floats_do_not_hold(cap, scale):
+    m = _abi.attention_mask(cap=cap)
+    with pytest.raises(_abi.NrsError, match="cap"):
+        _abi.masked_attention_forward(P, P, P, P, P, m, *GOOD.values(), scale)
+    with pytest.raises(_abi.NrsError, match="cap"):
+        _abi.masked_attention_backward(*[P] * 9, m, *GOOD.values(), scale)
+
+
 @pytest.mark.parametrize("null", [0, 2, 3, 4])
 def test_masked_attention_forward_nulls(null):
     args = [P, P, P, P, P, None]
