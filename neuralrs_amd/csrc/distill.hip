@@ -225,6 +225,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void distill_kernel(DistillArgs a) {
     const float of_soft = taught ? w * (1.0f - a.hard) * a.temperature : 0.0f;
     const float of_one = labelled ? w * a.hard : 0.0f;
     const float by_soft = of_soft / soft, by_one = of_one / one;
+    // (padding may hold any numbers: a row that learns from nothing gets zeros)
+    const bool learns = taught || labelled;
     auto dense = [&](float x) {
         // one exponential serves both where they are the same
         const float e = __builtin_amdgcn_exp2f((x - m[0]) * by_t);
@@ -243,7 +245,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void distill_kernel(DistillArgs a) {
     auto mine = [&](int64_t run) { return (uint32_t)run % (uint32_t)a.shares == (uint32_t)share; };
     auto put = [&](int64_t i, f32x4 x) {
         if (i >= quads) return;
-        x = dense4(x);
+        x = learns ? dense4(x) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (WAVES <= 8) {
             reinterpret_cast<Quad*>(g + 4 * i)->v = x;
         } else {  // past the caches, which hold what is read again (1021 x 128003: 259 us if not)
@@ -254,7 +256,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void distill_kernel(DistillArgs a) {
 #pragma unroll
     for (int n = 0; n < QUADS; ++n)
         if (mine(n)) put(t + n * kThreads, held[n]);
-    if (has_tail && mine(quads / kThreads)) g[4 * quads + t] = dense(tail);
+    if (has_tail && mine(quads / kThreads)) g[4 * quads + t] = learns ? dense(tail) : 0.0f;
     for (int64_t run = QUADS; run * kThreads < quads; run += kAhead) {
         f32x4 x[kAhead];
 #pragma unroll
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void distill_kernel(DistillArgs a) {
     if (a.k > 0) {
 #pragma unroll
         for (int n = 0; n < kOwn; ++n)
-            if (first[n] && mine(id[n] / 4 / kThreads))
+            if (learns && first[n] && mine(id[n] / 4 / kThreads))
                 g[id[n]] = dense(own_z[n]) - of_soft * p[n] -
                            (labelled && id[n] == label ? of_one : 0.0f);
     }
@@ -311,7 +313,8 @@ int check(const char* what, const float* logits, const float* top, const int32_t
     NRS_ARG_CHECK(k <= kMaxTop, "%s: k is %lld, at most %d are taken", what, (long long)k, kMaxTop);
     NRS_ARG_CHECK(ld >= vocab, "%s: row stride %lld is shorter than the vocabulary of %lld", what,
                   (long long)ld, (long long)vocab);
-    // a row is a workgroup of 512 threads, of fewer than 2^32 in all
+    // a row is a workgroup of 512 threads, of fewer than 2^32 in all (1024 past 32768
+    // columns, of which no memory holds 2^22 rows)
     NRS_ARG_CHECK(rows < (int64_t(1) << 23) && ld < (int64_t(1) << 31),
                   "%s: more than 2^23 - 1 rows or 2^31 - 1 columns (rows %lld, stride %lld)", what,
                   (long long)rows, (long long)ld);

@@ -266,3 +266,24 @@ def test_the_same_call_has_the_same_bits(hip):
     a = check(hip, logits, 9001, top, ids, labels, 2.0, 0.3)
     b = check(hip, logits, 9001, top, ids, labels, 2.0, 0.3)
     assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf], ids=str)
+@pytest.mark.parametrize("rows,vocab", [(4, 1003), (300, 35), (3, 140001)])
+def test_rows_that_learn_from_nothing(hip, rows, vocab, bad):
+    """Padding: no teacher token and no label, and anything in the logits, none finite
+    among it."""
+    logits, top, ids, labels = make(rows, vocab, 5, seed=13)
+    ids[1], labels[1] = -1, -1
+    top[2], labels[2] = -np.inf, vocab
+    logits[1:3] = bad
+    up = hip.DeviceBuffer.from_host
+    for grad in (hip.DeviceBuffer(rows * vocab), None):
+        z, loss = up(logits), hip.DeviceBuffer(rows)
+        into = grad or z
+        hip.distill_backward(into, loss, None, z, up(top), up(ids, np.int32), up(labels, np.int32),
+                             rows, vocab, 5, vocab, temperature=2.0, hard=0.5)
+        got = into.to_host((rows, vocab))
+        assert np.all(loss.to_host()[1:3] == 0) and np.all(got[1:3] == 0)
+        assert np.isfinite(loss.to_host()).all() and np.isfinite(got).all()
+        assert np.any(got[0] != 0)
