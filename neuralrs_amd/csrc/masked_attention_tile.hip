@@ -58,14 +58,20 @@ __device__ __forceinline__ int lanes_max(int x) {
     return x;
 }
 
-// TileEnds of the ranges that LANES lanes hold, LIVE of them rows.
+// The same in scalar registers: for all lanes alike.
+__device__ __forceinline__ TileEnds uniform(TileEnds x) {
+    return TileEnds{__builtin_amdgcn_readfirstlane(x.least), __builtin_amdgcn_readfirstlane(x.most),
+                    __builtin_amdgcn_readfirstlane(x.from), __builtin_amdgcn_readfirstlane(x.to)};
+}
+
+// TileEnds of the ranges of a wave's rows, which every LANES of its lanes hold, LIVE of them rows.
 template <int LANES>
 __device__ __forceinline__ TileEnds ends_of(int lo, int hi, bool live) {
     const bool any = hi > lo;
-    return TileEnds{lanes_min<LANES>(live && any ? lo : INT32_MAX),
-                    lanes_max<LANES>(live && any ? hi : 0),
-                    lanes_max<LANES>(!live ? 0 : any ? lo : INT32_MAX),
-                    lanes_min<LANES>(!live ? INT32_MAX : any ? hi : 0)};
+    return uniform(TileEnds{lanes_min<LANES>(live && any ? lo : INT32_MAX),
+                            lanes_max<LANES>(live && any ? hi : 0),
+                            lanes_max<LANES>(!live ? 0 : any ? lo : INT32_MAX),
+                            lanes_min<LANES>(!live ? INT32_MAX : any ? hi : 0)});
 }
 
 // A tile's way into LDS, with the rows of it that hold a NaN, an infinity or a magnitude
@@ -201,7 +207,7 @@ __global__ __launch_bounds__(64 * WAVES, forward_waves_per_simd(D, WAVES)) void 
                                        place32);
             }
             priority<WAVES == 8>(0);
-            if (mark[C::KT] == t + 1) {
+            if (__builtin_amdgcn_readfirstlane(mark[C::KT]) == t + 1) {
 #pragma unroll
                 for (int kb = 0; kb < C::NB; ++kb)
 #pragma unroll
@@ -427,7 +433,7 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
     for (int t = t0; t < t1; ++t) {
         const u32x4* const kl = lds + ((t - t0) & 1) * 2 * C::SET;
         const int* const mark = marks[(t - t0) & 1];
-        const bool marked = mark[C::KT] == t + 1;
+        const bool marked = __builtin_amdgcn_readfirstlane(mark[C::KT]) == t + 1;
 #pragma unroll
         for (int kb = 0; kb < C::NB; ++kb) {
             const int k0 = t * C::KT + kb * 32;
@@ -577,7 +583,7 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
     for (int j = 0; j < D / 16; ++j) acc_k[j] = acc_v[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     TileEnds seen{};
     if (t0 < t1) {
-        seen = next;
+        seen = uniform(next);
         store(t0);
         if (t0 + 1 < t1) load(t0 + 1);
         __syncthreads();
@@ -587,7 +593,7 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
         const u32x4* const ql = lds + buf * 2 * C::SET;
         const int* const mark = marks[buf];
         if (seen.least < key0 + 16 && seen.most > key0) {
-            const bool marked = mark[C::KT] == t + 1;
+            const bool marked = __builtin_amdgcn_readfirstlane(mark[C::KT]) == t + 1;
             const bool part = key0 < seen.from || key0 + 16 > seen.to;
 #pragma unroll
             for (int rb = 0; rb < C::NB; ++rb) {
@@ -664,7 +670,7 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
             }
         }
         if (t + 1 < t1) {
-            seen = next;
+            seen = uniform(next);
             store(t + 1);
             if (t + 2 < t1) load(t + 2);
             __syncthreads();
