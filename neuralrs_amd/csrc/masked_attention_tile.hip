@@ -44,6 +44,19 @@ __device__ __forceinline__ void priority(int level) {
     }
 }
 
+// The same in the backward. Up to 64 columns three waves share a SIMD, if the parts of a
+// step keep their order: an operand that is asked for before its part has its turn would take
+// the registers of the third (4 x 1021 rows of 16 heads of 64, both directions: two waves 267 us,
+// three in any order 264 and, with documents and a bias, of which 50 registers spill, 160 for
+// 146, three like this 254 and 138).
+template <int D>
+__device__ __forceinline__ void phase(int level) {
+    if constexpr (D > 64)
+        priority<true>(level);
+    else
+        __builtin_amdgcn_sched_barrier(0);
+}
+
 // The least and the largest of 32 or 16 neighbouring lanes.
 template <int LANES>
 __device__ __forceinline__ int lanes_min(int x) {
@@ -108,7 +121,9 @@ __device__ __forceinline__ void add_bias(V& s, float far, float slope2, O o) {
 
 __device__ __forceinline__ constexpr int place32(int i) { return 8 * (i / 4) + i % 4; }
 
-// (narrow heads leave room for three: 2 x 1500 rows, 16 heads of 32, 51 us, with two 59)
+// (narrow heads leave room for three: 2 x 1500 rows, 16 heads of 32, 51 us, with two 59; with
+// 64 columns few calls have that many workgroups, and a wave has fewer registers: 8000
+// rows of 2 heads 129 us, with two 143, but 4 x 1021 of 16 heads 81 and 78)
 constexpr int forward_waves_per_simd(int D, int waves) {
     return D <= 32 && waves == 4 ? 3 : waves_per_simd(D, waves);
 }
@@ -441,10 +456,10 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
             f32x4 s[2], dp[2];
 #pragma unroll
             for (int half = 0; half < 2; ++half) dp[half] = f32x4{nd, nd, nd, nd};
-            priority<(D > 64)>(1);
+            phase<D>(1);
             close16<C>(s, kl, qf, kb, c, g);
             products16<C, false>(dp, kl + C::SET, gf, kb, c, g);
-            priority<(D > 64)>(0);
+            phase<D>(0);
             float x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = s[i / 4][i % 4];
@@ -478,9 +493,9 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
                 x[i] = __builtin_amdgcn_exp2f(x[i] + nl) * dp[i / 4][i % 4];
             u32x4 p[3];
             split8(x, p);
-            priority<(D > 64)>(1);
+            phase<D>(1);
             add16<C>(acc, kl, kb, p, lane);
-            priority<(D > 64)>(0);
+            phase<D>(0);
         }
         if (t + 1 < t1) {
             store(t + 1);
@@ -601,10 +616,10 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
                 f32x4 s[2], dp[2];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) dp[half] = st[C::KT / 4 + 4 * half];
-                priority<(D > 64)>(1);
+                phase<D>(1);
                 close16<C>(s, ql, kf, rb, c, g);
                 products16<C, false>(dp, ql + C::SET, vf, rb, c, g);
-                priority<(D > 64)>(0);
+                phase<D>(0);
                 float x[8], y[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -660,13 +675,13 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
                 }
                 u32x4 p[3];
                 split8(x, p);
-                priority<(D > 64)>(1);
+                phase<D>(1);
                 add16<C>(acc_v, ql + C::SET, rb, p, lane);
-                priority<(D > 64)>(0);
+                phase<D>(0);
                 split8(y, p);
-                priority<(D > 64)>(1);
+                phase<D>(1);
                 add16<C>(acc_k, ql, rb, p, lane);
-                priority<(D > 64)>(0);
+                phase<D>(0);
             }
         }
         if (t + 1 < t1) {
@@ -692,7 +707,7 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
 // One launch for both: they need nothing of each other, and the workgroups of one fill
 // the compute units that the other leaves idle (the longer walks begin first).
 template <int D, int WAVES, bool FULL, int MODE>
-__global__ __launch_bounds__(64 * WAVES, 2) void masked_tile_bwd_kernel(MaskedArgs a) {
+__global__ __launch_bounds__(64 * WAVES, D <= 64 ? 3 : 2) void masked_tile_bwd_kernel(MaskedArgs a) {
     using C = TileCfg<D, WAVES>;
     __shared__ u32x4 lds[4 * C::SET];
     __shared__ f32x4 starts[2 * (MODE == kPlain ? 4 : 6) * C::KT / 4];
