@@ -9,16 +9,16 @@
 // and marked, and whoever sees it gets a NaN in place of the score.
 //
 // What bounds it is that a wave's steps (operands from LDS, matrix instructions,
-// exponentials and splits) follow one another and two waves to a SIMD hide a part of it: in the
-// three largest launches below matrix instructions run 60%, 51% and 46% of the time that
-// a compute unit has work, vector instructions issue 36%, 41% and 44%, LDS is busy 27%, 23% and
-// 37%. Splitting the met side costs 5 to 10% (measured by leaving it out), so tiles split
+// exponentials and splits) follow one another, and two waves to a SIMD hide a part of it: in
+// the last three launches below matrix instructions run 53%, 46% and 63% of the time that a
+// compute unit has work, vector instructions issue 43%, 44% and 38%, LDS is busy 24%, 37% and
+// 28%. Splitting the met side costs 5 to 10% (measured by leaving it out), so tiles split
 // beforehand would not pay for the pass that makes them.
-//   32 x 128 rows, 8 heads of 32, causal         forward 10.5 us, backward 17.4
-//   4 x 1021, 16 of 64, documents, bias          48 and 99: walks of 7 tiles, their beginnings
-//   2 x 4000, 16 of 128 on 4, prefix, cap        821 (170 TFLOP/s of what is seen) and 2770 (126;
-//                                                176 with the two products it repeats)
-//   8192, 32 of 128 on 8, causal, forward        2627 (209)
+//   32 x 128 rows, 8 heads of 32, causal       forward 10.5 us, backward 17.4 to 18.1
+//   4 x 1021, 16 of 64, documents, bias        48 and 87: walks of 7 tiles, their beginnings
+//   2 x 4000, 16 of 128 on 4, prefix, cap      834 (167 TFLOP/s of what is seen), backward 2762
+//                                              (126; 176 with the two products it repeats)
+//   8192, 32 of 128 on 8, causal, forward      2625 (209)
 #include <algorithm>
 
 #include "attention_tile.hpp"
