@@ -513,7 +513,8 @@ int nrs_dropout_backward(float *gin, const float *grad, int64_t n, float p, uint
  * A row without teacher tokens, or with teacher logits of minus infinity alone, has the
  * second part alone; one whose label is outside [0, vocab), the first alone; and one with
  * neither has no loss and no gradient, whatever its logits are. Logits may be minus
- * infinity, but not all of another row.                                          */
+ * infinity, but not all of another row. A NaN among a row's teacher logits, those of ids
+ * that are left out apart, gives NaN for its loss and its tokens' gradients (hard 1: none). */
 int nrs_distill_forward(float *row_loss, const float *logits, const float *top,
                         const int32_t *top_ids, const int32_t *labels, int64_t rows, int64_t vocab,
                         int64_t k, int64_t ld, float temperature, float hard);

@@ -63,6 +63,12 @@ struct Add {
 struct Max {
     __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };
+// (NaN if either is)
+struct MaxOrNan {
+    __device__ __forceinline__ float operator()(float a, float b) const {
+        return __builtin_elementwise_maximum(a, b);
+    }
+};
 
 __device__ __forceinline__ float most_of(f32x4 z) {
     return fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
@@ -145,12 +151,13 @@ __global__ __launch_bounds__(64 * WAVES, 4) void distill_kernel(DistillArgs a) {
                 top[n] = -INFINITY;
             }
             own_z[n] = id[n] >= 0 ? z[id[n]] : 0.0f;
-            most[0] = fmaxf(most[0], top[n]);
+            most[0] = MaxOrNan()(most[0], top[n]);
         }
-        all_threads(most, part, Max());
+        // (a teacher of NaN alone has a weight, too, which is not the absence of one)
+        all_threads(most, part, MaxOrNan());
 #pragma unroll
         for (int n = 0; n < kOwn; ++n)
-            if (most[0] > -INFINITY) mass[0] += __builtin_amdgcn_exp2f((top[n] - most[0]) * by_t);
+            if (most[0] != -INFINITY) mass[0] += __builtin_amdgcn_exp2f((top[n] - most[0]) * by_t);
         if (GRAD)  // the barrier of the sum stands between this and the look at `repeated`
 #pragma unroll
             for (int n = 0; n < kOwn; ++n) {
@@ -166,7 +173,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void distill_kernel(DistillArgs a) {
             }
         all_threads(mass, part, Add());
     }
-    const bool taught = a.hard < 1.0f && most[0] > -INFINITY;
+    const bool taught = a.hard < 1.0f && most[0] != -INFINITY;
 
     // the row's maximum and sums
     Sums<TWO> s;

@@ -287,3 +287,41 @@ def test_rows_that_learn_from_nothing(hip, rows, vocab, bad):
         assert np.all(loss.to_host()[1:3] == 0) and np.all(got[1:3] == 0)
         assert np.isfinite(loss.to_host()).all() and np.isfinite(got).all()
         assert np.any(got[0] != 0)
+
+
+@pytest.mark.parametrize("hard", [0.0, 0.4, 1.0])
+@pytest.mark.parametrize("rows,vocab,k", [(6, 500, 7), (6, 9001, 300), (300, 2100, 2), (6, 40001, 5)])
+def test_a_teacher_that_is_not_a_number(hip, rows, vocab, k, hard):
+    """NaN in a teacher's logits, in all of them too, comes out in the row's loss and in
+    its tokens' gradients, wherever the teacher has a weight; a NaN beside an id that is
+    left out is left out with it."""
+    logits, top, ids, labels = make(rows, vocab, k, seed=17, ragged=False)
+    labels[:5] = [3, -1, -1, 5, vocab]
+    ids[3, k // 2:] = -1
+    up = hip.DeviceBuffer.from_host
+
+    def run():
+        loss, grad = hip.DeviceBuffer(rows), hip.DeviceBuffer(rows * vocab)
+        args = (up(logits), up(top), up(ids, np.int32), up(labels, np.int32), rows, vocab, k, vocab)
+        hip.distill_backward(grad, loss, None, *args, temperature=2.0, hard=hard)
+        alone = hip.DeviceBuffer(rows)
+        hip.distill_forward(alone, *args, temperature=2.0, hard=hard)
+        assert np.array_equal(alone.to_host(), loss.to_host(), equal_nan=True)
+        return loss.to_host(), grad.to_host((rows, vocab))
+
+    was_loss, was = run()
+    assert np.isfinite(was_loss).all() and np.isfinite(was).all()
+    top[1] = np.nan
+    top[2, k // 2] = np.nan
+    top[3, k // 2:] = np.nan
+    top[4], top[4, k - 1] = -np.inf, np.nan
+    loss, grad = run()
+    bad = [1, 2, 4] if hard < 1.0 else []
+    assert np.isnan(loss[bad]).all()
+    other = np.ones((rows, vocab), bool)
+    for r in bad:
+        assert np.isnan(grad[r, ids[r]]).all()
+        other[r, ids[r]] = False
+    assert np.array_equal(grad[other], was[other])
+    rest = np.setdiff1d(np.arange(rows), bad)
+    assert np.array_equal(loss[rest], was_loss[rest])
