@@ -387,9 +387,10 @@ int nrs_cross_attention_backward(float *dq, float *dk, float *dv, const float *d
  * It sees key t when t < key_len[b], key_begin[b, s] <= t < key_end[b, s] and, if
  * causal, t <= i or t < prefix_len[b]; a mask that is not given hides nothing. So
  * key_begin, the first token of each token's document, keeps packed documents apart;
- * with key_end it says any range. Every range is cut to 0 .. seq_k - 1. With a cap,
- * scale / cap * q and its products with k have to be below 2^127 in magnitude, too.
- * In stats a row's bias is less that of the nearest key of its range.
+ * with key_end it says any range. Every range is cut to 0 .. seq_k - 1. In stats a
+ * row's bias is less that of the nearest key of its range. Whatever the cap, scale *
+ * log2(e) * q, its products with k and, in the backward, scale * log2(e) * k have to
+ * be below 2^127 in magnitude.
  *   Values of keys that a row does not see, infinite and NaN ones among them, do not
  * change its results or gradients; keys that no row of an item sees get a zero gradient
  * (written as zeros with beta_kv 0, left as they are with 1). A row that sees a key with
@@ -403,7 +404,7 @@ typedef struct nrs_attention_mask {
     const int32_t *key_begin;  /* device [batch * seq_q]; NULL: 0                    */
     const int32_t *key_end;    /* device [batch * seq_q]; NULL: seq_k                */
     const float *slopes;       /* device [heads], 0 or more, below 2^127; NULL: 0    */
-    float cap;                 /* of the scores; 0: none                             */
+    float cap;                 /* of the scores, 2^-126 to 2^127; 0: none            */
 } nrs_attention_mask;
 int nrs_masked_attention_supported(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
                                    int64_t seq_k, int64_t d_head, int64_t ld_q, int64_t ld_kv,

@@ -167,10 +167,7 @@ struct MaskedRows {
         for (int t = t0 + w; t < t1; t += kRowWaves) {
             f32x4 p = dot_rows<NJ>(kf, qf);
             if (t + kRowWaves < t1) load_keys(t + kRowWaves);
-            if (MODE == kCap) {
-                tanh_all<4>(p);
-                p = p * a.cap2;
-            }
+            if (MODE == kCap) cap_scores<4>(p, a.cap2, a.by_cap, 0.0f);
             if (MODE != kPlain) {
                 const float far = (float)(range.at - (16 * t + 4 * g));
 #pragma unroll
@@ -440,8 +437,9 @@ int check(const char* what, const nrs_attention_mask* mask, int64_t batch, int64
                                    ld_kv, ld_out))
         return rc;
     if (!mask) return NRS_OK;
-    NRS_ARG_CHECK(mask->cap >= 0.0f && std::isfinite(mask->cap * kLog2e),
-                  "%s: cap must be 0 (none) or a positive number below 2^127, is %g", what,
+    // (the reciprocal of a smaller one is past the largest float)
+    NRS_ARG_CHECK(mask->cap == 0.0f || (mask->cap >= 0x1p-126f && std::isfinite(mask->cap * kLog2e)),
+                  "%s: cap must be 0 (none) or a number from 2^-126 to below 2^127, is %g", what,
                   (double)mask->cap);
     NRS_ARG_CHECK(mask->cap == 0.0f || std::isfinite((float)((double)scale / mask->cap)),
                   "%s: scale / cap is %g / %g", what, (double)scale, (double)mask->cap);
@@ -462,10 +460,11 @@ MaskedArgs arguments(const nrs_attention_mask* mask, int64_t batch, int64_t head
         a.key_end = mask->key_end;
         a.slopes = mask->slopes;
     }
-    const float cap = mask ? mask->cap : 0.0f;
-    a.cap2 = cap * kLog2e;
     // (taken in 64 bits, rounded once)
-    a.scale_own = (float)(cap > 0.0f ? (double)scale / cap : (double)scale * 1.4426950408889634);
+    const double log2e = 1.4426950408889634, cap2 = (mask ? mask->cap : 0.0f) * log2e;
+    a.scale_own = (float)(scale * log2e);
+    a.cap2 = (float)cap2;
+    a.by_cap = cap2 > 0.0 ? (float)(1.0 / cap2) : 0.0f;
     a.B = (int)batch;
     a.H = (int)heads;
     a.KV = (int)kv_heads;

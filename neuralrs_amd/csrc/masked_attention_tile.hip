@@ -111,7 +111,7 @@ __device__ __forceinline__ void store_marked(Stage<C, FULL>& x, const CrossArgs&
 }
 
 // Turns products into scores in base 2: those of the rows' 32 (or 2 x 4) places o(i)
-// past `far`, the distance of place 0. The products of kCap have scale / cap in them.
+// past `far`, the distance of place 0.
 template <int MODE, int N, class V, class O>
 __device__ __forceinline__ void add_bias(V& s, float far, float slope2, O o) {
     if (MODE == kPlain) return;
@@ -210,13 +210,10 @@ __global__ __launch_bounds__(64 * WAVES, forward_waves_per_simd(D, WAVES)) void 
             for (int kb = 0; kb < C::NB; ++kb) {
                 // (from zero, not from -m: 16 registers less, which wide heads spilled)
                 p[kb] = products<C>(kl, qf, kb, all16(0.0f), c, h);
-                if (MODE == kCap) {
-                    tanh_all<16>(p[kb]);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) p[kb][i] = fmaf(a.cap2, p[kb][i], -m);
-                } else {
+                if (MODE == kCap)
+                    cap_scores<16>(p[kb], a.cap2, a.by_cap, m);
+                else
                     p[kb] = p[kb] - m;
-                }
                 if (MODE != kCap || a.slopes)
                     add_bias<MODE, 16>(p[kb], (float)(range.at - (k0 + kb * 32 + 4 * h)), slope2,
                                        place32);
@@ -460,17 +457,13 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
             close16<C>(s, kl, qf, kb, c, g);
             products16<C, false>(dp, kl + C::SET, gf, kb, c, g);
             phase<D>(0);
-            float x[8];
+            float x[8], y[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = s[i / 4][i % 4];
-            if (MODE == kCap) {
-                tanh_all<8>(x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    dp[i / 4][i % 4] *= fmaf(-x[i], x[i], 1.0f);
-                    x[i] *= a.cap2;
-                }
+            for (int i = 0; i < 8; ++i) {
+                x[i] = s[i / 4][i % 4];
+                y[i] = dp[i / 4][i % 4];
             }
+            if (MODE == kCap) cap_scores_and_slopes(x, y, a.cap2, a.by_cap);
             if (MODE != kCap || a.slopes)
                 add_bias<MODE, 8>(x, (float)(range.at - (k0 + 4 * g)), slope2, place16);
             if (marked) {
@@ -485,12 +478,11 @@ __device__ __forceinline__ void masked_dq_walk(const MaskedArgs& a, u32x4* lds, 
                 for (int i = 0; i < 8; ++i) {
                     const bool sees = k0 + 4 * g - range.lo + place16(i) < span;
                     x[i] = sees ? x[i] : -INFINITY;
-                    dp[i / 4][i % 4] = sees ? dp[i / 4][i % 4] : 0.0f;
+                    y[i] = sees ? y[i] : 0.0f;
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[i] = __builtin_amdgcn_exp2f(x[i] + nl) * dp[i / 4][i % 4];
+            for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] + nl) * y[i];
             u32x4 p[3];
             split8(x, p);
             phase<D>(1);
@@ -626,14 +618,7 @@ __device__ __forceinline__ void masked_dkv_walk(const MaskedArgs& a, u32x4* lds,
                     x[i] = s[i / 4][i % 4];
                     y[i] = dp[i / 4][i % 4];
                 }
-                if (MODE == kCap) {
-                    tanh_all<8>(x);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        y[i] *= fmaf(-x[i], x[i], 1.0f);
-                        x[i] *= a.cap2;
-                    }
-                }
+                if (MODE == kCap) cap_scores_and_slopes(x, y, a.cap2, a.by_cap);
                 if (MODE == kBias || (MODE == kCap && a.slopes)) {
                     const float place_key = (float)(key - tile * 16 * WAVES);
 #pragma unroll

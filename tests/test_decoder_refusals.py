@@ -56,6 +56,16 @@ def test_caps_that_floats_do_not_hold(cap, scale):
         _abi.masked_attention_backward(*[P] * 9, m, *GOOD.values(), scale)
 
 
+@pytest.mark.parametrize("cap", [1e-45, 1e-39, 1.17e-38])
+def test_caps_without_a_reciprocal(cap):
+    """Below 2^-126, whatever the scale."""
+    m = _abi.attention_mask(cap=cap)
+    with pytest.raises(_abi.NrsError, match="2\\^-126"):
+        _abi.masked_attention_forward(P, P, P, P, P, m, *GOOD.values(), 1e-10)
+    with pytest.raises(_abi.NrsError, match="2\\^-126"):
+        _abi.masked_attention_backward(*[P] * 9, m, *GOOD.values(), 1e-10)
+
+
 @pytest.mark.parametrize("null", [0, 2, 3, 4])
 def test_masked_attention_forward_nulls(null):
     args = [P, P, P, P, P, None]
