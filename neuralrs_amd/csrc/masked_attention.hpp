@@ -101,8 +101,10 @@ __device__ __forceinline__ void cap_scores(V& s, float cap2, float by_cap, float
     }
 }
 
-// The same from 0, and d[i] *= 1 - tanh^2. (A branch for each score: the backward's kernels
-// spill the registers that two loops take, 16384 rows of a head of 64 1499 us in place of 1222.)
+// The same from 0, and d[i] *= 1 - tanh^2: past 0.6 that is 4 e / (1 + e)^2, e = e^(-2 |y|),
+// which has all its bits where 1 - tanh^2 cancels (near 8 caps 3 bits are left of that). (A
+// branch for each score: the backward's kernels spill the registers that two loops take,
+// 16384 rows of a head of 64 1499 us in place of 1222.)
 template <int N>
 __device__ __forceinline__ void cap_scores_and_slopes(float (&s)[N], float (&d)[N], float cap2,
                                                       float by_cap) {
@@ -113,16 +115,17 @@ __device__ __forceinline__ void cap_scores_and_slopes(float (&s)[N], float (&d)[
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const float x = s[i], y = x * by_cap, p = tanh_by_y(y);
-        float t = y * p;
+        const float t = y * p;
+        float slope = fmaf(-t, t, 1.0f);
         s[i] = x * p;
         if (far) {
-            const float e = __builtin_amdgcn_exp2f(fabsf(y) * (2.0f * kLog2e));
-            const float big = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+            const float e = __builtin_amdgcn_exp2f(fabsf(y) * (-2.0f * kLog2e));
+            const float r = __builtin_amdgcn_rcpf(1.0f + e), er = e * r;
             const bool past = fabsf(y) > 0.6f;
-            t = past ? big : t;
-            s[i] = past ? copysignf(cap2, x) * big : s[i];
+            s[i] = past ? copysignf(cap2, x) * fmaf(-2.0f, er, 1.0f) : s[i];
+            slope = past ? 4.0f * er * r : slope;
         }
-        d[i] *= fmaf(-t, t, 1.0f);
+        d[i] *= slope;
     }
 }
 
