@@ -168,3 +168,31 @@ def test_positions_past_2_31_floats(hip):
     assert np.all(np.abs(got - want[0]) <= tol[0])
     x.free()
     hip.call("nrs_empty_cache")
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf], ids=str)
+def test_bad_numbers_stay_in_their_pair(hip, bad, interleaved):
+    """Turned by angles that are not zero: the other pairs of the row, of its heads and of
+    other rows, and the columns that are not turned, keep their bits; both ways."""
+    case = (5, 2, 22, 10, 2)  # two columns of a head are copied
+    x, pos, freq, axis = inputs(*case, seed=8)
+    pos[pos == 0] = 1
+    clean, dirty = x.copy(), x.copy()
+    partner = lambda c: (c // 2 * 2 + 1 - c % 2) if interleaved else (c + 10) % 20
+    hit = np.zeros(x.shape, bool)
+    for row, head, c in ((1, 0, 2), (2, 1, 13), (2, 0, 0), (4, 1, 19), (3, 0, 9)):
+        dirty[row, head * 22 + c] = bad
+        hit[row, [head * 22 + c, head * 22 + partner(c)]] = True
+    dirty[0, 21] = bad  # copied: alone
+    hit[0, 21] = True
+    _, dpos, dfreq, daxis = upload(hip, x, pos, freq, axis)
+    for turn in (hip.rotary_forward, hip.rotary_backward):
+        got = []
+        for a in (clean, dirty):
+            out = hip.DeviceBuffer(a.size)
+            turn(out, upload(hip, a)[0], dpos, dfreq, daxis, *case, 44, 44, interleaved=interleaved)
+            got.append(out.to_host(a.shape))
+        assert np.isfinite(got[0]).all()
+        assert np.array_equal(got[0][~hit], got[1][~hit])
+        assert not np.isfinite(got[1][hit]).any()
