@@ -242,7 +242,8 @@ struct Teacher {
 // The loss averaged over the rows, as cross_entropy's.
 float distillation(const NodeRef& pred, const Teacher& teacher);
 // Writes that mean's gradient into the logits' gradient, as cross_entropy_backward, and
-// returns the mean from the same pass.
+// returns the mean from the same pass, for which it waits for the device.
+// (nrs_distill_backward does not, and takes weights of the rows.)
 float distillation_backward(const NodeRef& pred, const Teacher& teacher);
 }  // namespace loss
 
@@ -392,7 +393,8 @@ struct MultiHeadAttention {
                           const IntsRef& key_len = nullptr) const;
     // A decoder's self-attention, x [batch, seq, d_model] (no counterpart in the
     // reference, whose attention has no mask): what the mask hides is not seen, and
-    // queries and keys are turned by `turn` if it is given. Heads of at most 128.
+    // queries and keys are turned by `turn` if it is given. Heads of at most 128, as many
+    // key heads, no cache: those are masked_attention's.
     NodeRef forward_masked(const NodeRef& x, const AttentionMask& mask,
                            const Rotary* turn = nullptr) const;
 };

@@ -111,8 +111,8 @@ struct SpanLine {
 // Few rows (tokens being decoded): K and V stream from memory once, straight into
 // registers, as operands of v_mfma_f32_16x16x4_f32. A unit is 16 rows of an item; a
 // workgroup's waves take turns at tiles of 16 keys, each with its next tile on the way,
-// and are joined at the end. 4 x 16384 keys and fewer, 8 key heads of 128, 4 rows each: 78
-// us, 4.6 TB/s; 32 items of up to 1500 keys, 8 heads of 64, a row each: 29 us, 3.9 TB/s,
+// and are joined at the end. 4 x 16384 keys and fewer, 8 key heads of 128, 4 rows each, capped:
+// 76 us, 4.7 TB/s; 32 items of up to 1500 keys, 8 heads of 64, a row each: 29 us, 3.9 TB/s,
 // where a wave sees five tiles behind the lengths' and the rows' own round trips.
 template <int NJ, int MODE>
 struct MaskedRows {

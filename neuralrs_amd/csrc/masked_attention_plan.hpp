@@ -37,6 +37,8 @@ inline MaskedForwardPlan plan_masked_forward(int64_t batch, int64_t heads, int64
                                              int64_t seq_q, int64_t seq_k, int64_t d_head,
                                              int64_t cus) {
     const int64_t R = seq_q * (heads / kv_heads), items = batch * kv_heads;
+    // (kFewRows is where cross attention's kernels are level, whose few rows' walk this is;
+    // masked attention's own two were not timed against each other)
     MaskedForwardPlan p{R > kFewRows, 16, {}, {}, 0, 0, 0};
     if (items == 0 || R == 0) return p;
     if (!p.tiles) {
@@ -69,7 +71,10 @@ inline MaskedForwardPlan plan_masked_forward(int64_t batch, int64_t heads, int64
     // whole of it where units are more than the workgroups at once, as the longest begin
     // first (4 x 3000 rows, 8 heads of 64, 384 on 256: 227 us, by halves 245; but 2 x 2000, 8 of
     // 128, 256 on 256: 222 and 181); 1024 keys at least, which a join costs (4 x 1021, 16 of
-    // 64: whole walks 80 us, by halves of 512 keys 86).
+    // 64, 512 units on 512: whole walks 80 us, by halves of 512 keys 86; where units are few,
+    // nothing shorter was timed). At once are two workgroups to a compute unit, also up to
+    // 32 columns, where three have room: by three 8000 rows, 8 heads of 32, take 222 us in place
+    // of 261, but 4 x 3000 134 in place of 127.
     cut_walk(p.walk, tiles, p.walk.units * tiles / (p.walk.units > at_once ? at_once : 2 * at_once),
              1024 / keys);
     if (p.walk.parts > 1) {
@@ -100,6 +105,9 @@ inline MaskedBackwardPlan plan_masked_backward(int64_t batch, int64_t heads, int
     MaskedBackwardPlan p{};
     const int waves = masked_backward_waves((int)d_head);
     const int64_t tile = cross_tile_keys((int)d_head, waves), own = 16 * waves;
+    // (two workgroups of four waves to a compute unit, also up to 64 columns, where three have
+    // room: by three 2 x 3000 rows, 8 heads of 32, take 288 us in place of 276, 16384 rows of a
+    // head of 64 1051 in place of 1086, 4 x 1021 of 16 the same 251)
     const int64_t at_once = waves == 8 ? cus : 2 * cus;
     p.row_tiles = (R + tile - 1) / tile;
     const int64_t key_tiles = (seq_k + tile - 1) / tile;

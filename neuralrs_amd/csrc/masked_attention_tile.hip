@@ -10,15 +10,15 @@
 //
 // What bounds it is that a wave's steps (operands from LDS, matrix instructions,
 // exponentials and splits) follow one another, and two waves to a SIMD hide a part of it: in
-// the last three launches below matrix instructions run 53%, 46% and 63% of the time that a
-// compute unit has work, vector instructions issue 43%, 44% and 38%, LDS is busy 24%, 37% and
+// the last three launches below matrix instructions run 55%, 47% and 63% of the time that a
+// compute unit has work, vector instructions issue 43%, 40% and 38%, LDS is busy 25%, 38% and
 // 28%. Splitting the met side costs 5 to 10% (measured by leaving it out), so tiles split
 // beforehand would not pay for the pass that makes them.
 //   32 x 128 rows, 8 heads of 32, causal       forward 10.5 us, backward 17.4 to 18.1
 //   4 x 1021, 16 of 64, documents, bias        48 and 87: walks of 7 tiles, their beginnings
-//   2 x 4000, 16 of 128 on 4, prefix, cap      834 (167 TFLOP/s of what is seen), backward 2762
-//                                              (126; 176 with the two products it repeats)
-//   8192, 32 of 128 on 8, causal, forward      2625 (209)
+//   2 x 4000, 16 of 128 on 4, prefix, cap      769 (181 TFLOP/s of what is seen), backward 2682
+//                                              (130; 181 with the two products it repeats)
+//   8192, 32 of 128 on 8, causal, forward      2526 (217)
 #include <algorithm>
 
 #include "attention_tile.hpp"
@@ -48,7 +48,8 @@ __device__ __forceinline__ void priority(int level) {
 // step keep their order: an operand that is asked for before its part has its turn would take
 // the registers of the third (4 x 1021 rows of 16 heads of 64, both directions: two waves 267 us,
 // three in any order 264 and, with documents and a bias, of which 50 registers spill, 160 for
-// 146, three like this 254 and 138).
+// 146, three like this 254 and 138; with a cap 14 registers spill like this, 280 us, and two
+// waves take 292, 16384 rows of one head 1218 and 1300).
 template <int D>
 __device__ __forceinline__ void phase(int level) {
     if constexpr (D > 64)
